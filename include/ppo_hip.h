@@ -734,6 +734,117 @@ int ppo_lstm_unpack_grads_norm(const ppo_lstm_grad_problem* problems, const int3
 int ppo_gru_unpack_grads_norm(const ppo_lstm_grad_problem* problems, const int32_t* groups, int32_t count,
                               double* norm_partials, ppo_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Token policies.  No counterpart in the reference, whose policies are Gaussian (rsl_rl/modules/distribution.py): what a
+ * policy over a vocabulary of tokens needs beside the entry points above.  The element types are fp32, bf16 and fp16;
+ * arithmetic is fp32 and a result is rounded once, to nearest even, when it is stored.  Rows are row-major with a leading
+ * dimension in elements; pointers are aligned to their element.  A token outside [0, vocab) is no token.
+ * ------------------------------------------------------------------------------------------------------------------ */
+enum { PPO_TYPE_F32 = 0, PPO_TYPE_BF16 = 1, PPO_TYPE_F16 = 2 };
+enum { PPO_TOKENS_I64 = 0, PPO_TOKENS_I32 = 1 };
+
+/* Embedding lookup with scaling:   dst[i, :] = scale * src[tokens[i], :]   (zeros where tokens[i] is no token), with src
+ * the table [vocab, dim], dst [count, dim] of the same type; accumulate is not read.
+ * Its gradient:   dst[v, :] = scale * sum over tokens[i] = v of src[i, :]   with src the outputs' gradient [count, dim], dst
+ * the table's gradient [vocab, dim], fp32 or of src's type.  Each row is summed in fp32 in an order that depends on the
+ * tokens alone (the tokens are sorted first, stably), so the same call gives the same bits.  accumulate = 0 writes every
+ * row, zeros where no token names it; otherwise the sum is added to the row and rows without tokens are left alone.
+ * count may be 0; count < 2^31, vocab < 2^31. */
+typedef struct ppo_embedding_args {
+  const void* tokens;
+  const void* src;
+  int64_t ld_src;
+  void* dst;
+  int64_t ld_dst;
+  int64_t count;
+  int64_t vocab;
+  int32_t dim;
+  int32_t token_type; /* PPO_TOKENS_* */
+  int32_t src_type;   /* PPO_TYPE_* */
+  int32_t dst_type;
+  float scale;
+  int32_t accumulate;
+} ppo_embedding_args;
+int ppo_embedding_fwd(const ppo_embedding_args* args, ppo_stream_t stream);
+size_t ppo_embedding_bwd_workspace_bytes(int64_t count, int64_t vocab, int32_t dim);
+int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+
+/* Log-probabilities and the clipped policy loss of tokens.  Row r with z = logits[r, :] / temperature and t = tokens[r]:
+ *   lp = z_t - log sum_j exp(z_j);   p_j = exp(z_j - log sum exp z);   H = -sum_j p_j log p_j   (0 where p_j is 0);
+ *   ratio = exp(lp - old_logp);   s = max(-A ratio, -A min(max(ratio, 1 - clip_low), 1 + clip_high));
+ *   d = ref_logp - lp;   k = exp(d) - d - 1   (the estimate of KL(policy || reference) that is never negative);
+ *   loss = sum_r (s + kl_coef k - entropy_coef H) / N;
+ *   d_logits[r, j] = (g ([j = t] - p_j) + entropy_coef p_j (log p_j + H)) / (N temperature),
+ *   g = (-A ratio where that is the larger branch, else 0) + kl_coef (1 - exp(d)).
+ * A row counts where mask[r] is not 0 (mask NULL: everywhere) and its token is one; N is the number of rows that count, or
+ * denom where that is positive (rows of several calls that share one mean).  A row that does not count is not read: its
+ * logp, entropy and d_logits are 0.  Logits of -inf have probability 0; a row that holds nothing else has no distribution
+ * and gives 0 too, though it counts in N.  If no row counts, everything is 0.
+ * ppo_token_log_probs writes logp and entropy (either may be NULL).  ppo_token_ppo_loss writes also stats[8] = loss,
+ * mean s, mean k, mean H, the share of rows whose ratio the range clips, mean old_logp - lp, N, 0 (each mean over N) and
+ * d_logits, of the logits' type (NULL: not wanted); d_logits may be logits itself.  ref_logp NULL: no KL term.  The sums
+ * over rows are fp64 in a fixed order. */
+typedef struct ppo_token_loss_args {
+  const void* logits; /* [rows, vocab] */
+  int64_t ld_logits;
+  const void* tokens;
+  const uint8_t* mask;
+  const float* old_logp;
+  const float* ref_logp;
+  const float* advantages;
+  void* d_logits; /* [rows, vocab] */
+  int64_t ld_d_logits;
+  float* logp;
+  float* entropy;
+  float* stats;
+  int64_t rows;
+  int64_t vocab;
+  double clip_low, clip_high;
+  double kl_coef;
+  double entropy_coef;
+  double temperature;
+  double denom;
+  int32_t type;       /* PPO_TYPE_* */
+  int32_t token_type; /* PPO_TOKENS_* */
+} ppo_token_loss_args;
+size_t ppo_token_loss_workspace_bytes(int64_t rows, int64_t vocab);
+int ppo_token_log_probs(const ppo_token_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+int ppo_token_ppo_loss(const ppo_token_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+
+/* AdamW over a list of tensors, with the clip by their global norm (torch.nn.utils.clip_grad_norm_ over all of them; the
+ * gradients themselves are left as they are):
+ *   total = ||all gradients||_2 (fp64);   c = min(1, max_norm / (total + 1e-6))   (max_norm <= 0: no clip, c = 1);
+ *   g' = c g;   m = m + (1-b1) (g' - m);   v = v b2 + ((1-b2) g') g';
+ *   p = p fl(1 - lr weight_decay) + ((-lr/bc1) m) / (sqrt(v)/bc2_sqrt + eps),
+ * in ppo_adam_step's fp32 operation order; lr and weight_decay are each tensor's.  param is fp32 or bf16.  A bf16 param may
+ * have an fp32 master: p is then the master, and param its rounding; without one p is param itself, rounded once a step.
+ * States in 32 bits are fp32 [count]; in 8 bits, each 256 consecutive elements (the last block may be shorter) share one fp32
+ * scale per state: m = sign(q) m_scale (|q| / 127)^2 with q int8, v = v_scale (q / 255)^4 with q uint8; the scale is the
+ * block's largest |m| (v), q is rounded to nearest, and q >= 1 where v > 0 (a second moment rounded to zero would leave its
+ * parameter a step of m / eps).  All zeros are the zero state.  norm_out (NULL: not wanted): total, c.  Tensors of count 0
+ * are allowed. */
+typedef struct ppo_adamw_tensor {
+  void* param;
+  const void* grad;
+  float* master;     /* NULL: none */
+  void* exp_avg;     /* fp32, or int8 */
+  void* exp_avg_sq;  /* fp32, or uint8 */
+  float* m_scale;    /* [ceil(count / 256)], 8-bit states only */
+  float* v_scale;
+  int64_t count;
+  double lr;
+  double weight_decay;
+  int32_t param_type; /* PPO_TYPE_F32 or PPO_TYPE_BF16 */
+  int32_t grad_type;
+  int32_t state_bits; /* 32 or 8 */
+  int32_t reserved;
+} ppo_adamw_tensor;
+#define PPO_ADAMW_BLOCK 256
+size_t ppo_adamw_workspace_bytes(const ppo_adamw_tensor* tensors, int32_t count);
+int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, double max_norm, double beta1, double beta2, double eps,
+                   double bc1, double bc2_sqrt, float* norm_out, void* workspace, size_t workspace_bytes,
+                   ppo_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

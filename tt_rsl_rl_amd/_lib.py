@@ -197,6 +197,35 @@ class MlpProblem(C.Structure):
                 ("num_layers", i32), ("activation", i32)]
 
 
+# token policies
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+TOKENS_I64, TOKENS_I32 = 0, 1
+ADAMW_BLOCK = 256  # elements that share a scale where AdamW's states are held in 8 bits
+
+
+class EmbeddingArgs(C.Structure):
+    _fields_ = [("tokens", vp), ("src", vp), ("ld_src", i64), ("dst", vp), ("ld_dst", i64), ("count", i64), ("vocab", i64),
+                ("dim", i32), ("token_type", i32), ("src_type", i32), ("dst_type", i32), ("scale", C.c_float),
+                ("accumulate", i32)]
+
+
+class TokenLossArgs(C.Structure):
+    _fields_ = [("logits", vp), ("ld_logits", i64), ("tokens", vp), ("mask", vp), ("old_logp", vp), ("ref_logp", vp),
+                ("advantages", vp), ("d_logits", vp), ("ld_d_logits", i64), ("logp", vp), ("entropy", vp), ("stats", vp),
+                ("rows", i64), ("vocab", i64), ("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_coef", C.c_double),
+                ("entropy_coef", C.c_double), ("temperature", C.c_double), ("denom", C.c_double), ("type", i32),
+                ("token_type", i32)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", vp), ("grad", vp), ("master", vp), ("exp_avg", vp), ("exp_avg_sq", vp), ("m_scale", vp),
+                ("v_scale", vp), ("count", i64), ("lr", C.c_double), ("weight_decay", C.c_double), ("param_type", i32),
+                ("grad_type", i32), ("state_bits", i32), ("reserved", i32)]
+
+
+ADAMW_TENSOR = struct.Struct("@PPPPPPPqddiiii")  # one AdamwTensor, packed by hand
+assert ADAMW_TENSOR.size == C.sizeof(AdamwTensor)
+
 # (name, restype, argtypes)
 _SIGNATURES = [
     ("ppo_last_error", C.c_char_p, []),
@@ -282,6 +311,15 @@ _SIGNATURES = [
     ("ppo_optim_step", C.c_int, [f32p, f32p, f32p, f32p, C.c_void_p, i32, C.c_double, C.POINTER(OptimConfig),
                                  C.c_double, C.c_double, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
                                  i32, C.c_void_p]),
+    ("ppo_embedding_fwd", C.c_int, [C.POINTER(EmbeddingArgs), vp]),
+    ("ppo_embedding_bwd_workspace_bytes", C.c_size_t, [i64, i64, i32]),
+    ("ppo_embedding_bwd", C.c_int, [C.POINTER(EmbeddingArgs), vp, C.c_size_t, vp]),
+    ("ppo_token_loss_workspace_bytes", C.c_size_t, [i64, i64]),
+    ("ppo_token_log_probs", C.c_int, [C.POINTER(TokenLossArgs), vp, C.c_size_t, vp]),
+    ("ppo_token_ppo_loss", C.c_int, [C.POINTER(TokenLossArgs), vp, C.c_size_t, vp]),
+    ("ppo_adamw_workspace_bytes", C.c_size_t, [vp, i32]),
+    ("ppo_adamw_step", C.c_int, [vp, i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp,
+                                 C.c_size_t, vp]),
 ]
 
 EXPORTED_SYMBOLS = [name for name, _, _ in _SIGNATURES]

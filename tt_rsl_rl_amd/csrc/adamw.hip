@@ -1,0 +1,367 @@
+// AdamW over a list of tensors (ppo_adamw_step): clip by the global norm, then the update, states in 32 or in 8 bits.
+//
+//   1. sums of squares of the gradients, fp64, one partial per block;
+//   2. one block adds the partials in order: total and the clip coefficient (both left out without a clip);
+//   3. the update, chunks of a tensor per block.
+// The tensors' addresses travel as kernel arguments, kMaxTensors to a launch, so nothing about a call is kept on the device.
+// The element update is optim.hip's, torch's fp32 operation order with contraction disabled.
+//
+// States in 8 bits: 256 consecutive elements share an fp32 scale per state; m = +-scale (|q| / 127)^2, v = scale (q / 255)^4.
+// The powers place codes densely near zero, as the magnitudes lie: the smallest m but zero is 6e-5 of the block's largest, the
+// smallest sqrt(v) 1.5e-5 of it.  A wave owns a block of elements, four per lane, so the new scale is one wave reduction.
+//
+// Bound by memory: 28 bytes per fp32 parameter with fp32 states, and the gradient once more for the norm.
+#include "elem.hpp"
+
+#pragma clang fp contract(off)
+
+namespace ppo {
+namespace {
+
+constexpr int kAdamwThreads = 256, kPer = 4;
+constexpr int kChunk = kAdamwThreads * kPer;  // elements a block takes at a time
+constexpr int kMaxTensors = 48, kMaxGrads = 160;
+constexpr int kNormBlocks = 1024;  // of one norm launch
+static_assert(kChunk % PPO_ADAMW_BLOCK == 0 && PPO_ADAMW_BLOCK == kWave * kPer, "a wave owns a scale's block");
+
+struct NormTable {
+  const void* grad[kMaxGrads];
+  int64_t count[kMaxGrads];
+  int32_t first[kMaxGrads + 1];  // chunks before the tensor
+  int32_t tensors;
+};
+static_assert(sizeof(NormTable) <= 3800, "kernel arguments");
+
+struct Tensor {
+  void* param;
+  const void* grad;
+  float* master;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  int32_t count4;  // unused low bits of the count are in tail
+  int32_t tail;
+  float neg_step, decay;
+};
+
+struct UpdateTable {
+  Tensor t[kMaxTensors];
+  int32_t first[kMaxTensors + 1];
+  int32_t tensors;
+};
+static_assert(sizeof(UpdateTable) <= 3800, "kernel arguments");
+
+struct Scalars {
+  float w1, b2, c2, eps, bc2_sqrt;
+};
+
+// The tensor of a chunk: the last one whose first chunk is not behind it.
+template <int N>
+__device__ __forceinline__ int tensor_of(const int32_t (&first)[N], int tensors, int chunk) {
+  int lo = 0, hi = tensors;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= chunk) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ double block_sum(double x, double* red) {
+  for (int d = kWave / 2; d > 0; d >>= 1) x += __shfl_down(x, d, kWave);
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = x;
+  __syncthreads();
+  double s = 0.0;
+  for (int w = 0; w < kAdamwThreads / kWave; ++w) s += red[w];
+  __syncthreads();
+  return s;
+}
+
+// Four elements from p, those past n as zeros.
+template <class T>
+__device__ __forceinline__ void load4(const T* p, int n, float (&x)[kPer]) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= kPer) {
+    const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = static_cast<float>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = i < n ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, int n, const float (&x)[kPer]) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= kPer) {
+    vec v;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = static_cast<T>(x[i]);
+    *reinterpret_cast<vec*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i < n) p[i] = static_cast<T>(x[i]);
+  }
+}
+
+template <class G>
+__global__ __launch_bounds__(kAdamwThreads) void adamw_norm_kernel(const NormTable t, int chunks, double* __restrict__ partial) {
+  __shared__ double red[kAdamwThreads / kWave];
+  double sum = 0.0;
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int k = tensor_of(t.first, t.tensors, c);
+    const int64_t i = static_cast<int64_t>(c - t.first[k]) * kChunk + threadIdx.x * kPer;
+    const int n = static_cast<int>(min<int64_t>(kPer, t.count[k] - i));
+    if (n <= 0) continue;
+    float g[kPer];
+    load4(static_cast<const G*>(t.grad[k]) + i, n, g);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += static_cast<double>(g[e]) * static_cast<double>(g[e]);
+  }
+  sum = block_sum(sum, red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+// coef[0] = the clip coefficient
+__global__ __launch_bounds__(kAdamwThreads) void adamw_clip_kernel(const double* __restrict__ partial, int partials, float max_norm,
+                                                                   float* __restrict__ coef, float* __restrict__ norm_out) {
+  __shared__ double red[kAdamwThreads / kWave];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < partials; i += kAdamwThreads) sum += partial[i];
+  sum = block_sum(sum, red);
+  if (threadIdx.x != 0) return;
+  const float total = static_cast<float>(sqrt(sum));
+  float c = 1.0f;
+  if (max_norm > 0.0f) {
+    c = max_norm / (total + 1e-6f);
+    c = c > 1.0f ? 1.0f : c;  // (NaN stays)
+  }
+  coef[0] = c;
+  if (norm_out != nullptr) {
+    norm_out[0] = total;
+    norm_out[1] = c;
+  }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int d = kWave / 2; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, kWave));
+  return x;
+}
+
+// A block's new scale: the largest of its values (none negative); NaN where one is not finite, so that the block does not
+// come back as if it were.
+__device__ __forceinline__ float block_scale(const float (&x)[kPer]) {
+  float s = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    s = fmaxf(s, x[i]);
+    bad |= !(x[i] < INFINITY);
+  }
+  s = wave_max(s);
+  return __ballot(bad) != 0 ? __builtin_nanf("") : s;
+}
+
+template <class P, class G, bool MASTER, bool BITS8>
+__global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const UpdateTable t, const Scalars s,
+                                                                     const float* __restrict__ coef) {
+  const int k = tensor_of(t.first, t.tensors, blockIdx.x);
+  const Tensor& q = t.t[k];
+  const int64_t count = static_cast<int64_t>(q.count4) * 4 + q.tail;
+  const int64_t i = static_cast<int64_t>(static_cast<int>(blockIdx.x) - t.first[k]) * kChunk + threadIdx.x * kPer;
+  const int n = static_cast<int>(max<int64_t>(0, min<int64_t>(kPer, count - i)));
+  if (!BITS8 && n == 0) return;
+  const float c = coef != nullptr ? *coef : 1.0f;
+  float g[kPer], p[kPer], m[kPer], v[kPer];
+  load4(static_cast<const G*>(q.grad) + i, n, g);
+  if constexpr (MASTER) load4(q.master + i, n, p);
+  else load4(static_cast<const P*>(q.param) + i, n, p);
+  const int64_t block = i / PPO_ADAMW_BLOCK;
+  if constexpr (BITS8) {
+    const bool some = block * PPO_ADAMW_BLOCK < count;  // (of the wave's block)
+    const float ms = some ? q.m_scale[block] : 0.0f, vs = some ? q.v_scale[block] : 0.0f;
+    load4(static_cast<const int8_t*>(q.m) + i, n, m);
+    load4(static_cast<const uint8_t*>(q.v) + i, n, v);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const float a = fabsf(m[e]) * (1.0f / 127.0f), b = v[e] * (1.0f / 255.0f);
+      m[e] = (m[e] < 0.0f ? -ms : ms) * (a * a);
+      const float b2 = b * b;
+      v[e] = vs * (b2 * b2);
+    }
+  } else {
+    load4(static_cast<const float*>(q.m) + i, n, m);
+    load4(static_cast<const float*>(q.v) + i, n, v);
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const float d = g[e] * c;
+    m[e] = m[e] + s.w1 * (d - m[e]);
+    v[e] = v[e] * s.b2;
+    v[e] = v[e] + (s.c2 * d) * d;
+    p[e] = p[e] * q.decay;
+    p[e] = p[e] + (q.neg_step * m[e]) / (sqrtf(v[e]) / s.bc2_sqrt + s.eps);
+  }
+  if constexpr (BITS8) {
+    // elements past the end hold zeros: g, m and v
+    float am[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) am[e] = fabsf(m[e]);
+    const float ms = block_scale(am), vs = block_scale(v);
+    float qm[kPer], qv[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const float a = rintf(sqrtf(am[e] / (ms > 0.0f ? ms : 1.0f)) * 127.0f);
+      qm[e] = copysignf(fminf(fmaxf(a, 0.0f), 127.0f), m[e]);
+      float b = rintf(sqrtf(sqrtf(v[e] / (vs > 0.0f ? vs : 1.0f))) * 255.0f);
+      b = fminf(fmaxf(b, 0.0f), 255.0f);
+      qv[e] = v[e] > 0.0f ? fmaxf(b, 1.0f) : b;
+    }
+    if (n == 0) return;
+    store4(static_cast<int8_t*>(q.m) + i, n, qm);
+    store4(static_cast<uint8_t*>(q.v) + i, n, qv);
+    if (threadIdx.x % kWave == 0) {
+      q.m_scale[block] = ms;
+      q.v_scale[block] = vs;
+    }
+  } else {
+    store4(static_cast<float*>(q.m) + i, n, m);
+    store4(static_cast<float*>(q.v) + i, n, v);
+  }
+  if constexpr (MASTER) store4(q.master + i, n, p);
+  store4(static_cast<P*>(q.param) + i, n, p);
+}
+
+int64_t chunks_of(const ppo_adamw_tensor& t) { return ceil_div(t.count, kChunk); }
+
+int64_t norm_partials(const ppo_adamw_tensor* tensors, int32_t count) {
+  // a bound: each launch writes at most kNormBlocks, and there is one per kMaxGrads tensors of a type
+  return static_cast<int64_t>(kNormBlocks) * (count / kMaxGrads + 2);
+}
+
+template <class P, class G, bool MASTER>
+void launch_update(bool bits8, int chunks, hipStream_t st, const UpdateTable& t, const Scalars& s, const float* coef) {
+  if (bits8)
+    hipLaunchKernelGGL((adamw_update_kernel<P, G, MASTER, true>), dim3(chunks), dim3(kAdamwThreads), 0, st, t, s, coef);
+  else
+    hipLaunchKernelGGL((adamw_update_kernel<P, G, MASTER, false>), dim3(chunks), dim3(kAdamwThreads), 0, st, t, s, coef);
+}
+
+// The kinds a launch holds together: bit 0 bf16 param, bit 1 bf16 gradient, bit 2 master, bit 3 8-bit states.
+int kind_of(const ppo_adamw_tensor& t) {
+  return (t.param_type == PPO_TYPE_BF16 ? 1 : 0) | (t.grad_type == PPO_TYPE_BF16 ? 2 : 0) | (t.master != nullptr ? 4 : 0) |
+         (t.state_bits == 8 ? 8 : 0);
+}
+
+}  // namespace
+}  // namespace ppo
+
+using namespace ppo;
+
+extern "C" size_t ppo_adamw_workspace_bytes(const ppo_adamw_tensor* tensors, int32_t count) {
+  if (tensors == nullptr || count < 1) return 0;
+  return 256 + sizeof(double) * static_cast<size_t>(norm_partials(tensors, count));
+}
+
+extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, double max_norm, double beta1, double beta2,
+                              double eps, double bc1, double bc2_sqrt, float* norm_out, void* workspace,
+                              size_t workspace_bytes, ppo_stream_t stream) {
+  PPO_REQUIRE(tensors != nullptr && count >= 1, "ppo_adamw_step: %d tensors", count);
+  PPO_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0, "ppo_adamw_step: beta1=%g beta2=%g eps=%g",
+              beta1, beta2, eps);
+  PPO_REQUIRE(bc1 > 0.0 && bc2_sqrt > 0.0, "ppo_adamw_step: bias corrections must be positive");
+  for (int i = 0; i < count; ++i) {
+    const ppo_adamw_tensor& t = tensors[i];
+    PPO_REQUIRE(t.count >= 0 && t.count < (int64_t{1} << 33), "ppo_adamw_step: tensor %d holds %lld elements", i, (long long)t.count);
+    PPO_REQUIRE((t.param_type == PPO_TYPE_F32 || t.param_type == PPO_TYPE_BF16) &&
+                    (t.grad_type == PPO_TYPE_F32 || t.grad_type == PPO_TYPE_BF16),
+                "ppo_adamw_step: tensor %d: param_type=%d grad_type=%d", i, t.param_type, t.grad_type);
+    PPO_REQUIRE(t.state_bits == 32 || t.state_bits == 8, "ppo_adamw_step: tensor %d: state_bits=%d", i, t.state_bits);
+    PPO_REQUIRE(t.master == nullptr || t.param_type == PPO_TYPE_BF16, "ppo_adamw_step: tensor %d: a master of an fp32 param", i);
+    PPO_REQUIRE(t.param_type == PPO_TYPE_BF16 || t.grad_type == PPO_TYPE_F32, "ppo_adamw_step: tensor %d: a bf16 gradient of an fp32 param", i);
+    PPO_REQUIRE(t.count == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq &&
+                                 (t.state_bits == 32 || (t.m_scale && t.v_scale))),
+                "ppo_adamw_step: tensor %d: null pointer", i);
+    PPO_REQUIRE(reinterpret_cast<uintptr_t>(t.param) % type_size(t.param_type) == 0 &&
+                    reinterpret_cast<uintptr_t>(t.grad) % type_size(t.grad_type) == 0 &&
+                    reinterpret_cast<uintptr_t>(t.master) % 4 == 0 && reinterpret_cast<uintptr_t>(t.m_scale) % 4 == 0 &&
+                    reinterpret_cast<uintptr_t>(t.v_scale) % 4 == 0 &&
+                    (t.state_bits == 8 || (reinterpret_cast<uintptr_t>(t.exp_avg) % 4 == 0 &&
+                                           reinterpret_cast<uintptr_t>(t.exp_avg_sq) % 4 == 0)),
+                "ppo_adamw_step: tensor %d: pointers must be aligned to their elements", i);
+  }
+  const bool norm = max_norm > 0.0 || norm_out != nullptr;
+  const size_t need = ppo_adamw_workspace_bytes(tensors, count);
+  PPO_REQUIRE(!norm || (workspace != nullptr && workspace_bytes >= need), "ppo_adamw_step: workspace too small (%zu < %zu)",
+              workspace_bytes, need);
+  PPO_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "ppo_adamw_step: the workspace must be 8-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  float* coef = nullptr;
+  if (norm) {
+    coef = static_cast<float*>(workspace);
+    double* partial = reinterpret_cast<double*>(static_cast<char*>(workspace) + 256);
+    int partials = 0;
+    for (int type : {PPO_TYPE_F32, PPO_TYPE_BF16}) {
+      int i = 0;
+      while (i < count) {
+        NormTable t{};
+        int64_t chunks = 0;
+        for (; i < count && t.tensors < kMaxGrads; ++i) {
+          if (tensors[i].grad_type != type || tensors[i].count == 0) continue;
+          t.grad[t.tensors] = tensors[i].grad;
+          t.count[t.tensors] = tensors[i].count;
+          t.first[t.tensors++] = static_cast<int32_t>(chunks);
+          chunks += chunks_of(tensors[i]);
+          PPO_REQUIRE(chunks < INT32_MAX, "ppo_adamw_step: too many parameters");
+        }
+        if (t.tensors == 0) break;
+        t.first[t.tensors] = static_cast<int32_t>(chunks);
+        const int blocks = static_cast<int>(std::min<int64_t>(chunks, kNormBlocks));
+        if (type == PPO_TYPE_F32)
+          hipLaunchKernelGGL(adamw_norm_kernel<float>, dim3(blocks), dim3(kAdamwThreads), 0, st, t, static_cast<int>(chunks), partial + partials);
+        else
+          hipLaunchKernelGGL(adamw_norm_kernel<__bf16>, dim3(blocks), dim3(kAdamwThreads), 0, st, t, static_cast<int>(chunks), partial + partials);
+        if (int rc = check_launch("adamw_norm_kernel")) return rc;
+        partials += blocks;
+      }
+    }
+    hipLaunchKernelGGL(adamw_clip_kernel, dim3(1), dim3(kAdamwThreads), 0, st, partial, partials, static_cast<float>(max_norm), coef, norm_out);
+    if (int rc = check_launch("adamw_clip_kernel")) return rc;
+  }
+  const Scalars s{static_cast<float>(1.0 - beta1), static_cast<float>(beta2), static_cast<float>(1.0 - beta2),
+                  static_cast<float>(eps), static_cast<float>(bc2_sqrt)};
+  for (int kind = 0; kind < 16; ++kind) {
+    int i = 0;
+    while (i < count) {
+      UpdateTable t{};
+      int64_t chunks = 0;
+      for (; i < count && t.tensors < kMaxTensors; ++i) {
+        const ppo_adamw_tensor& a = tensors[i];
+        if (kind_of(a) != kind || a.count == 0) continue;
+        Tensor& b = t.t[t.tensors];
+        b = Tensor{a.param, a.grad, a.master, a.exp_avg, a.exp_avg_sq, a.m_scale, a.v_scale,
+                   static_cast<int32_t>(a.count / 4), static_cast<int32_t>(a.count % 4),
+                   static_cast<float>(-(a.lr / bc1)), static_cast<float>(1.0 - a.lr * a.weight_decay)};
+        t.first[t.tensors++] = static_cast<int32_t>(chunks);
+        chunks += chunks_of(a);
+        PPO_REQUIRE(chunks < INT32_MAX, "ppo_adamw_step: too many parameters");
+      }
+      if (t.tensors == 0) break;
+      t.first[t.tensors] = static_cast<int32_t>(chunks);
+      const bool bits8 = kind & 8;
+      switch (kind & 7) {
+        case 0: launch_update<float, float, false>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
+        case 1: launch_update<__bf16, float, false>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
+        case 3: launch_update<__bf16, __bf16, false>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
+        case 5: launch_update<__bf16, float, true>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
+        case 7: launch_update<__bf16, __bf16, true>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
+        default: return fail(PPO_EINVAL, "ppo_adamw_step: kind %d", kind);
+      }
+      if (int rc = check_launch("adamw_update_kernel")) return rc;
+    }
+  }
+  return PPO_OK;
+}

@@ -1,0 +1,51 @@
+// Element types of the token operators (embedding.hip, token_loss.hip, adamw.hip): fp32, bf16 and fp16 in memory, fp32 in
+// registers.  A rounding to 16 bits is to nearest even (gfx950's converts), once, at a store.
+#pragma once
+
+#include "common.hpp"
+
+namespace ppo {
+
+constexpr int kTypes = 3;
+__host__ __device__ constexpr int type_size(int type) { return type == PPO_TYPE_F32 ? 4 : 2; }
+inline bool type_ok(int type) { return type >= 0 && type < kTypes; }
+
+template <class T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte piece
+
+// A 16-byte piece that need not lie on a 16-byte boundary (rows of an odd width): gfx950 loads and stores it in one
+// instruction all the same, at one more cache line per wave.
+template <class T>
+struct Piece {
+  typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+template <class T>
+__device__ __forceinline__ typename Piece<T>::type load_piece(const T* p) {
+  return *reinterpret_cast<const typename Piece<T>::type*>(p);
+}
+
+template <class T>
+__device__ __forceinline__ void store_piece(T* p, const float (&x)[kVec<T>]) {
+  typename Piece<T>::type v;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) v[i] = static_cast<T>(x[i]);
+  *reinterpret_cast<typename Piece<T>::type*>(p) = v;
+}
+
+// Tokens are int64 or int32; anything outside [0, vocab) is no token (-1).
+__device__ __forceinline__ int64_t token_at(const void* tokens, int type, int64_t i, int64_t vocab) {
+  const int64_t t = type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(tokens)[i]
+                                           : static_cast<int64_t>(static_cast<const int32_t*>(tokens)[i]);
+  return t >= 0 && t < vocab ? t : -1;
+}
+
+// f(T()) for the element type of `type`.
+template <class F>
+void with_type(int type, F&& f) {
+  if (type == PPO_TYPE_F32) f(float());
+  else if (type == PPO_TYPE_BF16) f(static_cast<__bf16>(0.0f));
+  else f(static_cast<_Float16>(0.0f));
+}
+
+}  // namespace ppo

@@ -8,6 +8,7 @@ on a GPU are rejected.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -1037,3 +1038,222 @@ def lstm_unpack_grads(items: list[tuple], gru: bool = False, norm: tuple | None 
             import ctypes
             grp = (ctypes.c_int32 * len(part))(*norm[1][i:i + L.MAX_LSTM_PROBLEMS])
             L.call(name + "_norm", L.array(L.LstmGradProblem, part), grp, len(part), norm[0].data_ptr(), _stream())
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# token policies: embedding, log-probabilities and the clipped policy loss, AdamW over many tensors
+# ----------------------------------------------------------------------------------------------------------------------
+
+ELEMENT_TYPES = {torch.float32: L.TYPE_F32, torch.bfloat16: L.TYPE_BF16, torch.float16: L.TYPE_F16}
+TOKEN_TYPES = {torch.int64: L.TOKENS_I64, torch.int32: L.TOKENS_I32}
+
+
+def _current_gpu(name: str, *tensors: torch.Tensor | None) -> int:
+    """The current GPU's index; every tensor must be on it: the kernels are enqueued on its current stream."""
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"{name}: GPU tensors only (no CPU path exists)")
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: tensors must be on the current GPU ({dev}), got one on {t.device}")
+    return dev
+
+
+def _element_type(t: torch.Tensor, name: str) -> int:
+    code = ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _matrix(t: torch.Tensor, name: str) -> int:
+    """Leading dimension of a [rows, columns] view of unit column stride whose rows do not overlap."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix, got shape {tuple(t.shape)}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        raise ValueError(f"{name} must have unit column stride and rows apart, got strides {t.stride()}")
+    return max(t.stride(0), cols) if rows > 1 else cols
+
+
+def _vector(t: torch.Tensor | None, name: str, n: int, dtype: torch.dtype) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} of {n} elements, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _tokens(tokens: torch.Tensor, name: str) -> int:
+    code = TOKEN_TYPES.get(tokens.dtype)
+    if code is None or not tokens.is_contiguous():
+        raise ValueError(f"{name}: tokens must be contiguous int64 or int32, got {tokens.dtype} {tuple(tokens.shape)}")
+    return code
+
+
+def _scratch(ws: Workspace | None, device: torch.device, nbytes: int) -> torch.Tensor:
+    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device) if ws is None else ws.get(nbytes)
+
+
+def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor, scale: float = 1.0) -> None:
+    """out[i] = scale * table[tokens[i]]; zeros where a token is outside [0, vocab) (padding).  tokens: int64 or int32,
+    contiguous, of any shape; table [vocab, dim] and out [tokens.numel(), dim] of one type, float32, bfloat16 or float16,
+    row-major views."""
+    dev = _current_gpu("embedding_fwd", tokens, table, out)
+    token_type, elem = _tokens(tokens, "embedding_fwd"), _element_type(table, "embedding_fwd: table")
+    ld_src, ld_dst = _matrix(table, "table"), _matrix(out, "out")
+    n, (vocab, dim) = tokens.numel(), table.shape
+    if out.dtype != table.dtype or tuple(out.shape) != (n, dim):
+        raise ValueError(f"embedding_fwd: out must be {table.dtype} [{n}, {dim}], got {out.dtype} {tuple(out.shape)}")
+    args = L.EmbeddingArgs(tokens.data_ptr(), table.data_ptr(), ld_src, out.data_ptr(), ld_dst, n, vocab, dim, token_type,
+                           elem, elem, float(scale), 0)
+    L.call("ppo_embedding_fwd", C_ref(args), _raw_stream(dev))
+
+
+def embedding_bwd(tokens: torch.Tensor, d_out: torch.Tensor, d_table: torch.Tensor, scale: float = 1.0,
+                  accumulate: bool = False, ws: Workspace | None = None) -> None:
+    """d_table[v] = scale * the sum of d_out's rows whose token is v (zeros where none is; with accumulate the sum is added
+    and rows without tokens are left as they are).  d_out [tokens.numel(), dim]; d_table [vocab, dim] of d_out's type or
+    float32.  The sums are fp32, in an order that depends on the tokens alone: the same call gives the same bits."""
+    dev = _current_gpu("embedding_bwd", tokens, d_out, d_table)
+    token_type = _tokens(tokens, "embedding_bwd")
+    src_type, dst_type = _element_type(d_out, "embedding_bwd: d_out"), _element_type(d_table, "embedding_bwd: d_table")
+    ld_src, ld_dst = _matrix(d_out, "d_out"), _matrix(d_table, "d_table")
+    n, (vocab, dim) = tokens.numel(), d_table.shape
+    if tuple(d_out.shape) != (n, dim):
+        raise ValueError(f"embedding_bwd: d_out must be [{n}, {dim}], got {tuple(d_out.shape)}")
+    nbytes = L.load().ppo_embedding_bwd_workspace_bytes(n, vocab, dim)
+    buf = _scratch(ws, d_table.device, nbytes)
+    args = L.EmbeddingArgs(tokens.data_ptr(), d_out.data_ptr(), ld_src, d_table.data_ptr(), ld_dst, n, vocab, dim, token_type,
+                           src_type, dst_type, float(scale), int(accumulate))
+    L.call("ppo_embedding_bwd", C_ref(args), buf.data_ptr(), buf.numel(), _raw_stream(dev))
+
+
+def _token_args(name: str, logits, tokens, logp, entropy, mask, temperature) -> tuple["L.TokenLossArgs", int]:
+    dev = _current_gpu(name, logits, tokens, logp, entropy, mask)
+    ld = _matrix(logits, f"{name}: logits")
+    rows, vocab = logits.shape
+    elem, token_type = _element_type(logits, f"{name}: logits"), _tokens(tokens, name)
+    if tokens.numel() != rows:
+        raise ValueError(f"{name}: {tokens.numel()} tokens for {rows} rows of logits")
+    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != rows or not mask.is_contiguous()):
+        raise ValueError(f"{name}: mask must be contiguous bool or uint8 of {rows} elements, got {mask.dtype} {tuple(mask.shape)}")
+    return L.TokenLossArgs(logits=logits.data_ptr(), ld_logits=ld, tokens=tokens.data_ptr(), mask=_ptr(mask),
+                           logp=_vector(logp, f"{name}: logp", rows, torch.float32),
+                           entropy=_vector(entropy, f"{name}: entropy", rows, torch.float32), rows=rows, vocab=vocab,
+                           temperature=float(temperature), type=elem, token_type=token_type), dev
+
+
+def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor | None, entropy: torch.Tensor | None = None,
+                    mask: torch.Tensor | None = None, temperature: float = 1.0, ws: Workspace | None = None) -> None:
+    """logp[r] = the log-probability of tokens[r] under softmax(logits[r] / temperature), entropy[r] that distribution's
+    entropy (float32, either may be None).  logits [rows, vocab] float32, bfloat16 or float16.  Rows whose mask (bool or
+    uint8) is 0 or whose token is outside [0, vocab) are not read and give 0."""
+    args, dev = _token_args("token_log_probs", logits, tokens, logp, entropy, mask, temperature)
+    nbytes = L.load().ppo_token_loss_workspace_bytes(args.rows, args.vocab)
+    buf = _scratch(ws, logits.device, nbytes)
+    L.call("ppo_token_log_probs", C_ref(args), buf.data_ptr(), buf.numel(), _raw_stream(dev))
+
+
+def token_ppo_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
+                   d_logits: torch.Tensor | None, stats: torch.Tensor, ref_logp: torch.Tensor | None = None,
+                   logp: torch.Tensor | None = None, entropy: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                   clip_param: float | tuple[float, float] = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                   temperature: float = 1.0, denom: float | None = None, ws: Workspace | None = None) -> None:
+    """The clipped policy loss of tokens and its gradient: the mean over the rows that count (mask, as token_log_probs) of
+    max(-A ratio, -A clip(ratio)) + kl_coef KL(policy || reference) - entropy_coef H, with ratio = exp(logp - old_logp) held
+    to [1 - clip, 1 + clip] (a pair: its low and high width) and the KL estimated as exp(d) - d - 1, d = ref_logp - logp.
+    stats[8] float32 = loss, surrogate, KL, entropy, the share of clipped rows, mean old_logp - logp, rows, 0.
+    d_logits: like logits (may be logits itself), or None.  denom: divides the sums instead of the number of rows that
+    count, for calls that share one mean."""
+    args, dev = _token_args("token_ppo_loss", logits, tokens, logp, entropy, mask, temperature)
+    _current_gpu("token_ppo_loss", old_logp, advantages, ref_logp, d_logits, stats)
+    rows = args.rows
+    args.old_logp = _vector(old_logp, "token_ppo_loss: old_logp", rows, torch.float32)
+    args.advantages = _vector(advantages, "token_ppo_loss: advantages", rows, torch.float32)
+    args.ref_logp = _vector(ref_logp, "token_ppo_loss: ref_logp", rows, torch.float32)
+    args.stats = _vector(stats, "token_ppo_loss: stats", 8, torch.float32)
+    if d_logits is not None:
+        if d_logits.dtype != logits.dtype or d_logits.shape != logits.shape:
+            raise ValueError(f"token_ppo_loss: d_logits must be {logits.dtype} {tuple(logits.shape)}, got {d_logits.dtype} "
+                             f"{tuple(d_logits.shape)}")
+        args.d_logits, args.ld_d_logits = d_logits.data_ptr(), _matrix(d_logits, "token_ppo_loss: d_logits")
+    args.clip_low, args.clip_high = clip_param if isinstance(clip_param, (tuple, list)) else (clip_param, clip_param)
+    args.kl_coef, args.entropy_coef = float(kl_coef), float(entropy_coef)
+    if denom is not None:
+        if not denom > 0:
+            raise ValueError(f"token_ppo_loss: denom must be positive, got {denom}")
+        args.denom = float(denom)
+    nbytes = L.load().ppo_token_loss_workspace_bytes(rows, args.vocab)
+    buf = _scratch(ws, logits.device, nbytes)
+    L.call("ppo_token_ppo_loss", C_ref(args), buf.data_ptr(), buf.numel(), _raw_stream(dev))
+
+
+def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step: int, lr, beta1: float = 0.9,
+               beta2: float = 0.999, eps: float = 1e-8, weight_decay=1e-2, max_grad_norm: float | None = None,
+               masters: list | None = None, scales: tuple[list, list] | None = None, norm_out: torch.Tensor | None = None,
+               ws: Workspace | None = None) -> None:
+    """One AdamW step over a list of contiguous tensors, in place, their gradients clipped by their common norm first
+    (max_grad_norm; the gradients themselves are left as they are).  params: float32, or bfloat16 with (masters) or without
+    a float32 master each, in which case the master is stepped and the parameter is its rounding; grads: float32, or
+    bfloat16 for a bfloat16 parameter; exp_avg / exp_avg_sq: float32, or int8 / uint8 with scales = (lists of) float32
+    [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  lr, weight_decay: one value, or one per tensor.
+    step counts from 1.  norm_out: float32 [2] for the norm and the clip coefficient."""
+    n = len(params)
+    lists = [("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)]
+    lists += [("masters", masters)] if masters is not None else []
+    lists += [("scales", scales[0]), ("scales", scales[1])] if scales is not None else []
+    lists += [("lr", lr)] if isinstance(lr, (list, tuple)) else []
+    lists += [("weight_decay", weight_decay)] if isinstance(weight_decay, (list, tuple)) else []
+    for name, v in lists:
+        if len(v) != n:
+            raise ValueError(f"adamw_step: {len(v)} {name} for {n} params")
+    if step < 1:
+        raise ValueError(f"adamw_step: step={step} (the first is 1)")
+    if max_grad_norm is not None and not max_grad_norm > 0:
+        raise ValueError(f"adamw_step: max_grad_norm={max_grad_norm}")
+    if n == 0:
+        return
+    dev = _current_gpu("adamw_step", params[0], norm_out)
+    f32, bf16 = torch.float32, torch.bfloat16
+    items = []
+    for i in range(n):
+        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
+        count, bits = p.numel(), 32
+        master = ms = vs = None
+        tensors = (p, g, m, v)
+        if masters is not None and masters[i] is not None:
+            master = masters[i]
+            tensors += (master,)
+            if master.dtype != f32 or p.dtype != bf16:
+                raise ValueError(f"adamw_step: masters[{i}] must be float32 of a bfloat16 parameter")
+        for t in tensors:
+            if t.get_device() != dev or t.numel() != count or not t.is_contiguous():
+                raise ValueError(f"adamw_step: tensor {i} must be contiguous, of {count} elements, on GPU {dev}: got "
+                                 f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
+        if (p.dtype != f32 and p.dtype != bf16) or (g.dtype != f32 and g.dtype != p.dtype):
+            raise ValueError(f"adamw_step: tensor {i}: parameter {p.dtype}, gradient {g.dtype}")
+        if m.dtype != f32 or v.dtype != f32:
+            if m.dtype != torch.int8 or v.dtype != torch.uint8 or scales is None:
+                raise ValueError(f"adamw_step: tensor {i}: states {m.dtype}, {v.dtype} (float32, or int8 and uint8 with scales)")
+            bits, blocks = 8, -(-count // L.ADAMW_BLOCK)
+            ms, vs = scales[0][i], scales[1][i]
+            for t in (ms, vs):
+                if t.get_device() != dev or t.dtype != f32 or t.numel() != blocks or not t.is_contiguous():
+                    raise ValueError(f"adamw_step: scales of tensor {i} must be contiguous float32 of {blocks} elements")
+        items.append(L.ADAMW_TENSOR.pack(
+            p.data_ptr(), g.data_ptr(), 0 if master is None else master.data_ptr(), m.data_ptr(), v.data_ptr(),
+            0 if ms is None else ms.data_ptr(), 0 if vs is None else vs.data_ptr(), count,
+            lr[i] if isinstance(lr, (list, tuple)) else lr,
+            weight_decay[i] if isinstance(weight_decay, (list, tuple)) else weight_decay,
+            L.TYPE_F32 if p.dtype == f32 else L.TYPE_BF16, L.TYPE_F32 if g.dtype == f32 else L.TYPE_BF16, bits, 0))
+    packed = b"".join(items)
+    buf = None
+    if max_grad_norm is not None or norm_out is not None:
+        if norm_out is not None:
+            _vector(norm_out, "adamw_step: norm_out", 2, f32)
+        buf = _scratch(ws, params[0].device, L.load().ppo_adamw_workspace_bytes(packed, n))
+    L.call("ppo_adamw_step", packed, n, float(max_grad_norm or 0.0), float(beta1), float(beta2), float(eps),
+           1.0 - beta1**step, math.sqrt(1.0 - beta2**step), _ptr(norm_out), _ptr(buf), 0 if buf is None else buf.numel(),
+           _raw_stream(dev))
