@@ -20,9 +20,47 @@ struct Piece {
   typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
+// A piece as it lies in memory, four registers whatever the type, for values that are kept and converted where they are used.
+// (An array: element reads of a vector through a reference are miscompiled, all of them to the first element.)
+struct RawPiece {
+  uint32_t w[4];
+};
+
+template <class T>
+__device__ __forceinline__ float element(const RawPiece& r, int e) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(float, r.w[e]);
+  } else {
+    const uint32_t w = r.w[e / 2];
+    if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(float, e % 2 != 0 ? w & 0xffff0000u : w << 16);
+    else return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(e % 2 != 0 ? w >> 16 : w)));
+  }
+}
+
+// Makes element e -inf.
+template <class T>
+__device__ __forceinline__ void make_neg_inf(RawPiece& r, int e) {
+  if constexpr (sizeof(T) == 4) {
+    r.w[e] = 0xff800000u;
+  } else {
+    const uint32_t bits = __is_same(T, __bf16) ? 0xff80u : 0xfc00u;
+    r.w[e / 2] = e % 2 != 0 ? (r.w[e / 2] & 0xffffu) | bits << 16 : (r.w[e / 2] & 0xffff0000u) | bits;
+  }
+}
+
+// The compiler forgets what it knows of the piece, once `done` is computed: otherwise it keeps the converted values of one
+// pass for the next, or puts the pass off, at two or more registers for each of the piece's.
+__device__ __forceinline__ void forget(RawPiece& r, float& done) { asm volatile("" : "+v"(r.w[0]), "+v"(r.w[1]), "+v"(r.w[2]), "+v"(r.w[3]), "+v"(done)); }
+__device__ __forceinline__ void forget(int& x) { asm volatile("" : "+v"(x)); }
+
 template <class T>
 __device__ __forceinline__ typename Piece<T>::type load_piece(const T* p) {
   return *reinterpret_cast<const typename Piece<T>::type*>(p);
+}
+
+template <class T>
+__device__ __forceinline__ RawPiece load_raw(const T* p) {
+  return __builtin_bit_cast(RawPiece, load_piece(p));
 }
 
 template <class T>

@@ -1,13 +1,17 @@
 // Token log-probabilities and the clipped policy loss with a KL term, forward and gradient (ppo_token_log_probs,
 // ppo_token_ppo_loss): the categorical counterpart of loss.hip's Gaussian head.
 //
-// With c = log2(e) / temperature, m = max_j x_j and t_j = c (x_j - m) (the difference first: where every logit is the type's
-// lowest value c m alone would overflow):
+// With c = log2(e) / temperature, m = max_j x_j and t_j = c x_j - c m:
 //   S = sum_j 2^t_j,  E = sum_j 2^t_j t_j,  lp = ln2 (t_token - log2 S),  H = ln2 (log2 S - E / S),
-//   p_j = 2^w_j with w_j = t_j - log2 S,  d_logits_j = p_j (a + b w_j) + [j = token] g k,
-//   k = 1 / (N temperature),  a = k (entropy_coef H - g),  b = k entropy_coef ln2.
-// A logit of -inf has 2^t = 0 exactly; its t and w are raised to kFloor, where 2^kFloor is 0 too, so that 0 t stays 0.
-// Bound by memory: the logits once in, their gradient once out.
+//   d_logits_j = 2^t_j (A + B t_j) + [j = token] g k,
+//   k = 1 / (N temperature),  B = k entropy_coef ln2 / S,  A = k (entropy_coef H - g) / S - B log2 S
+// (p_j = 2^t_j / S and log p_j = ln2 (t_j - log2 S) put into the header's formula; t_j is one fused multiply-add, so the
+// rounding of c m is the same in every term and cancels).  A logit of -inf has 2^t = 0 exactly; where t itself is a factor it
+// is raised to kFloor, 2^kFloor being 0 too, so that 0 t stays 0.
+//
+// Bound by memory: the logits once in, their gradient once out.  So a row is read once and stays in registers between its
+// sums and its gradient (token_row_kernel); only rows too wide for that are read twice (token_wide_kernel).  Each wave
+// takes its own maximum and sums, and the waves' (m, S, E) are joined after the one barrier of a row.
 #include "elem.hpp"
 
 namespace ppo {
@@ -15,18 +19,21 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kFloor = -1000.0f;
-constexpr int kThreads = 256;
-constexpr int kTerms = 5;  // per row: s, k, H, clipped, old_logp - lp
+// sums over rows per row: s, k, H, clipped, old_logp - lp, counts, (2 unused)
+constexpr int kTerms = 6, kTermStride = 8;
+constexpr int kCountRows = 2048;  // up to so many rows each block counts them itself: one launch less
+constexpr int kStatsThreads = 1024;
 
 struct LossKernelArgs {
   ppo_token_loss_args a;
-  float* inv_n;   // 1 / N (0: no row counts)
-  float* n;
-  float* terms;   // [kTerms][rows]
+  float* inv_n;   // 1 / N of token_count_kernel, where that ran
+  float* terms;   // [rows][kTermStride]
+  int32_t count;  // 1: the block counts the rows, 2: inv_n holds 1 / N, 0: given_inv_n does
+  float given_inv_n;
   float c, inv_temp, clip_lo, clip_hi, kl_coef, entropy_coef;
 };
 
-__device__ __forceinline__ bool counts(const ppo_token_loss_args& a, int64_t r, int64_t& tok) {
+__device__ __forceinline__ bool row_counts(const ppo_token_loss_args& a, int64_t r, int64_t& tok) {
   tok = -1;
   if (a.mask != nullptr && a.mask[r] == 0) return false;
   tok = token_at(a.tokens, a.token_type, r, a.vocab);
@@ -39,135 +46,331 @@ __device__ __forceinline__ R wave_sum(R x) {
   return x;
 }
 
-__global__ __launch_bounds__(1024) void token_count_kernel(const LossKernelArgs q) {
-  __shared__ int32_t part[1024 / kWave];
-  int32_t n = 0;
-  int64_t tok;
-  for (int64_t r = threadIdx.x; r < q.a.rows; r += 1024) n += counts(q.a, r, tok) ? 1 : 0;
-  n = wave_sum(n);
-  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = n;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int64_t all = 0;
-    for (int w = 0; w < 1024 / kWave; ++w) all += part[w];
-    const double d = q.a.denom > 0.0 ? q.a.denom : static_cast<double>(all);
-    *q.n = static_cast<float>(d);
-    *q.inv_n = all > 0 ? static_cast<float>(1.0 / d) : 0.0f;
-  }
-}
-
-// Sum (or maximum) over the block, in every thread.
-template <class F>
-__device__ __forceinline__ float block_reduce(float x, float* scratch, F&& f) {
-  for (int d = kWave / 2; d > 0; d >>= 1) x = f(x, __shfl_xor(x, d, kWave));
-  if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = x;
-  __syncthreads();
-  x = scratch[0];
-  for (int w = 1; w < kThreads / kWave; ++w) x = f(x, scratch[w]);
-  __syncthreads();
+__device__ __forceinline__ float wave_max(float x) {
+  for (int d = kWave / 2; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, kWave));
   return x;
 }
 
-// The row's scalars once S and E are known; writes logp, entropy and the loss terms. Returns g (the derivative by lp).
-struct RowScalars {
-  float log2_s, h, g;
+__device__ __forceinline__ int32_t rows_counted(const LossKernelArgs& q, int first, int step) {
+  int32_t n = 0;
+  int64_t tok;
+  for (int64_t r = first; r < q.a.rows; r += step) n += row_counts(q.a, r, tok) ? 1 : 0;
+  return n;
+}
+
+__global__ __launch_bounds__(kStatsThreads) void token_count_kernel(const LossKernelArgs q) {
+  __shared__ int32_t part[kStatsThreads / kWave];
+  const int32_t n = wave_sum(rows_counted(q, threadIdx.x, kStatsThreads));
+  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int32_t all = 0;
+    for (int w = 0; w < kStatsThreads / kWave; ++w) all += part[w];
+    *q.inv_n = all > 0 ? static_cast<float>(1.0 / all) : 0.0f;
+  }
+}
+
+// c, or where c m would not be finite a power of two that keeps it so: floats as large as that lie so far apart that
+// 2^t is 1 for the maximum itself and 0 for anything below it with either.
+__device__ __forceinline__ float scale_for(float m, float c) { return fabsf(m * c) < 1e30f ? c : 0x1p-20f; }
+
+struct RowSums {
+  float m, s, e;
 };
 
-__device__ __forceinline__ RowScalars row_scalars(const LossKernelArgs& q, int64_t r, float t_tok, float s, float e, bool loss,
-                                                  bool write) {
-  RowScalars o;
-  o.log2_s = log2f(s);
-  const float lp = kLn2 * (t_tok - o.log2_s);
-  o.h = kLn2 * (o.log2_s - e / s);
-  o.g = 0.0f;
-  if (write && q.a.logp != nullptr) q.a.logp[r] = lp;
-  if (write && q.a.entropy != nullptr) q.a.entropy[r] = o.h;
-  if (!loss) return o;
-  const float old = q.a.old_logp[r], adv = q.a.advantages[r];
-  const float ratio = expf(lp - old);
-  const float clipped = fminf(fmaxf(ratio, q.clip_lo), q.clip_hi);
-  const float first = -adv * ratio, second = -adv * clipped;
-  float kl = 0.0f;
-  o.g = first >= second ? first : first < second ? 0.0f : first + second;  // (NaN goes on)
-  if (q.a.ref_logp != nullptr) {
-    const float d = q.a.ref_logp[r] - lp, x = expf(d);
-    kl = x - d - 1.0f;
-    o.g += q.kl_coef * (1.0f - x);
-  }
-  if (write) {
-    const int64_t n = q.a.rows;
-    q.terms[r] = first != first || second != second ? first + second : fmaxf(first, second);
-    q.terms[n + r] = kl;
-    q.terms[2 * n + r] = o.h;
-    q.terms[3 * n + r] = ratio != clipped ? 1.0f : 0.0f;
-    q.terms[4 * n + r] = old - lp;
-  }
+// The sums of one part of a row next to those of another.
+__device__ __forceinline__ RowSums join(const RowSums& u, const RowSums& v, float c) {
+#pragma clang fp contract(off)
+  RowSums o;  // (no fused multiply-add: the same bits whichever part comes first)
+  o.m = fmaxf(u.m, v.m);
+  const float ce = scale_for(o.m, c);
+  const float du = u.m == o.m ? 0.0f : fmaxf((u.m - o.m) * ce, kFloor), dv = v.m == o.m ? 0.0f : fmaxf((v.m - o.m) * ce, kFloor);
+  const float fu = __builtin_amdgcn_exp2f(du), fv = __builtin_amdgcn_exp2f(dv);
+  o.s = u.s * fu + v.s * fv;
+  o.e = (u.e + u.s * du) * fu + (v.e + v.s * dv) * fv;
   return o;
 }
 
-__device__ __forceinline__ void row_zeros(const LossKernelArgs& q, int64_t r, bool loss) {
-  if (q.a.logp != nullptr) q.a.logp[r] = 0.0f;
-  if (q.a.entropy != nullptr) q.a.entropy[r] = 0.0f;
-  if (loss)
-    for (int i = 0; i < kTerms; ++i) q.terms[i * q.a.rows + r] = 0.0f;
+__device__ __forceinline__ RowSums join_lanes(const RowSums& u, int d, float c) {
+  return join(u, RowSums{__shfl_xor(u.m, d, kWave), __shfl_xor(u.s, d, kWave), __shfl_xor(u.e, d, kWave)}, c);
 }
 
-// One block per row, the row read three times: its maximum, its sums, its gradient.
+template <int WAVES>
+struct RowShared {
+  RowSums sums[WAVES];
+  int32_t count[WAVES];
+};
+
+// What a row's gradient needs once its sums are known: t = fma(x, c, -mc), d = 2^t (a + b t), + at at the token.
+struct RowCoefs {
+  float c, mc, a, b, at;
+  bool live;
+};
+
+// Joins the waves' sums (the row's only barrier) and writes logp, entropy and the loss terms.
+template <int NT, bool LOSS>
+__device__ __forceinline__ RowCoefs finish_row(const LossKernelArgs& q, int64_t r, RowSums mine, float x_tok, int32_t counted,
+                                               RowShared<NT / kWave>& sh) {
+  constexpr int WAVES = NT / kWave;
+  if constexpr (WAVES > 1) {
+    if (threadIdx.x % kWave == 0) {
+      sh.sums[threadIdx.x / kWave] = mine;
+      if (LOSS) sh.count[threadIdx.x / kWave] = counted;
+    }
+    __syncthreads();
+    mine = sh.sums[threadIdx.x % WAVES];
+    counted = LOSS ? sh.count[threadIdx.x % WAVES] : 0;
+#pragma unroll
+    for (int d = WAVES / 2; d > 0; d >>= 1) {
+      mine = join_lanes(mine, d, q.c);
+      if (LOSS) counted += __shfl_xor(counted, d, kWave);
+    }
+  }
+  RowCoefs o;
+  o.live = mine.m > -INFINITY || mine.s != mine.s;  // nothing but -inf: no distribution (a NaN goes on)
+  o.c = scale_for(mine.m, q.c);
+  o.mc = mine.m * o.c;
+  o.a = o.b = o.at = 0.0f;
+  float lp = 0.0f, h = 0.0f, log2_s = 0.0f;
+  if (o.live) {
+    log2_s = log2f(mine.s);
+    lp = kLn2 * ((x_tok - mine.m) * q.c - log2_s);
+    h = kLn2 * (log2_s - mine.e / mine.s);
+  }
+  const bool write = threadIdx.x == 0;
+  if (write && q.a.logp != nullptr) q.a.logp[r] = lp;
+  if (write && q.a.entropy != nullptr) q.a.entropy[r] = h;
+  if (!LOSS) return o;
+  float term[kTerms] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 1.0f};
+  if (o.live) {
+    const float old = q.a.old_logp[r], adv = q.a.advantages[r];
+    const float ratio = expf(lp - old);
+    const float clipped = fminf(fmaxf(ratio, q.clip_lo), q.clip_hi);
+    const float first = -adv * ratio, second = -adv * clipped;
+    float g = first >= second ? first : first < second ? 0.0f : first + second;  // (NaN goes on)
+    term[0] = first != first || second != second ? first + second : fmaxf(first, second);
+    if (q.a.ref_logp != nullptr) {
+      const float d = q.a.ref_logp[r] - lp, x = expf(d);
+      term[1] = x - d - 1.0f;
+      g += q.kl_coef * (1.0f - x);
+    }
+    term[2] = h;
+    term[3] = ratio != clipped ? 1.0f : 0.0f;
+    term[4] = old - lp;
+    const float inv_n = q.count == 1 ? 1.0f / static_cast<float>(counted) : q.count == 2 ? *q.inv_n : q.given_inv_n;
+    const float k = inv_n * q.inv_temp, inv_s = 1.0f / mine.s;
+    o.b = k * q.entropy_coef * kLn2 * inv_s;
+    o.a = k * (q.entropy_coef * h - g) * inv_s - o.b * log2_s;
+    o.at = k * g;
+  }
+  if (write)
+#pragma unroll
+    for (int i = 0; i < kTerms; ++i) q.terms[r * kTermStride + i] = term[i];
+  return o;
+}
+
+// A row that does not count, or has no distribution: its gradient is zero.
+template <class T, int NT>
+__device__ __forceinline__ void zero_gradient(T* dx, int64_t vocab) {
+  constexpr int V = kVec<T>;
+  const float zero[V] = {};
+  for (int64_t j = threadIdx.x * V; j < vocab; j += NT * V) {
+    if (j + V <= vocab) store_piece(dx + j, zero);
+    else
+      for (int64_t i = j; i < vocab; ++i) dx[i] = static_cast<T>(0.0f);
+  }
+}
+
+template <bool LOSS>
+__device__ __forceinline__ void skip_row(const LossKernelArgs& q, int64_t r) {
+  if (threadIdx.x != 0) return;
+  if (q.a.logp != nullptr) q.a.logp[r] = 0.0f;
+  if (q.a.entropy != nullptr) q.a.entropy[r] = 0.0f;
+  if (LOSS)
+    for (int i = 0; i < kTerms; ++i) q.terms[r * kTermStride + i] = 0.0f;
+}
+
+__device__ __forceinline__ float gradient_of(float x, const RowCoefs& o) {
+  const float t = fmaxf(fmaf(x, o.c, -o.mc), kFloor);
+  return exp2f(t) * fmaf(o.b, t, o.a);
+}
+
+// One block of NT threads per row, K 16-byte pieces of it in each thread's registers (NT K V >= vocab >= V): piece k of
+// thread i is the (k NT + i)-th.  The last piece of a row whose width is no multiple of V is read from V columns before the
+// end; what it shares with the piece before it, and pieces past the end, become -inf, which adds nothing to a sum.
+template <class T, int NT, int K, bool LOSS>
+__global__ __launch_bounds__(NT) void token_row_kernel(const LossKernelArgs q) {
+  constexpr int V = kVec<T>;
+  __shared__ RowShared<NT / kWave> sh;
+  const ppo_token_loss_args& a = q.a;
+  const int64_t r = blockIdx.x;
+  const int vocab = static_cast<int>(a.vocab);
+  const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
+  T* dx = LOSS && a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
+  int64_t tok;
+  if (!row_counts(a, r, tok)) {
+    skip_row<LOSS>(q, r);
+    if (dx != nullptr) zero_gradient<T, NT>(dx, vocab);
+    return;
+  }
+  // of piece k: its first column, and whether the wave's pieces lie inside the row, partly or not at all (wave-uniform)
+  const int wave_first = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave * kWave);
+  int tid = threadIdx.x;
+  auto column = [&](int k) { return (k * NT + tid) * V; };
+  auto whole = [&](int k) { return (k * NT + wave_first + kWave) * V <= vocab; };
+  auto some = [&](int k) { return (k * NT + wave_first) * V < vocab; };
+  auto offset = [&](int j) { return static_cast<uint32_t>(j) * static_cast<uint32_t>(sizeof(T)); };  // 32 bits, of a uniform base
+  RawPiece raw[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) raw[k] = load_raw(reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + offset(min(column(k), vocab - V))));
+  const float x_tok = static_cast<float>(x[tok]);
+  const int32_t counted = LOSS && q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x, NT)) : 0;
+  forget(tid);  // (the columns are computed again where they are needed, not kept)
+  RowSums mine{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (!whole(k)) {
+      const int skip = column(k) - min(column(k), vocab - V);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < skip) make_neg_inf<T>(raw[k], e);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) mine.m = fmaxf(mine.m, element<T>(raw[k], e));
+    forget(raw[k], mine.m);
+    __builtin_amdgcn_sched_barrier(0);  // one piece at a time: its converted values are gone before the next one's
+  }
+  mine.m = wave_max(mine.m);
+  {
+    const float c = scale_for(mine.m, q.c), mc = mine.m > -INFINITY ? mine.m * c : 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (some(k)) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float t = fmaf(element<T>(raw[k], e), c, -mc), p = __builtin_amdgcn_exp2f(t);
+          mine.s += p;
+          mine.e = fmaf(p, fmaxf(t, kFloor), mine.e);
+        }
+      }
+      forget(raw[k], mine.s);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  mine.s = wave_sum(mine.s);
+  mine.e = wave_sum(mine.e);
+  const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh);
+  if (dx == nullptr) return;
+  if (!o.live) {
+    zero_gradient<T, NT>(dx, vocab);
+    return;
+  }
+  forget(tid);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (some(k)) {
+      const int at = min(column(k), vocab - V);
+      float d[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float t = fmaxf(fmaf(element<T>(raw[k], e), o.c, -o.mc), kFloor);
+        d[e] = __builtin_amdgcn_exp2f(t) * fmaf(o.b, t, o.a);
+      }
+      const uint32_t hit = static_cast<uint32_t>(static_cast<int>(tok) - at);
+      if (hit < V)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (static_cast<uint32_t>(e) == hit) d[e] += o.at;
+      if (whole(k)) {
+        store_piece(reinterpret_cast<T*>(reinterpret_cast<char*>(dx) + offset(at)), d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e >= column(k) - at) dx[at + e] = static_cast<T>(d[e]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Rows of any width: the sums in one pass, each thread rescaling its own when its maximum grows, the gradient in another.
+constexpr int kWideThreads = 1024;
+
 template <class T, bool LOSS>
-__global__ __launch_bounds__(kThreads) void token_row_kernel(const LossKernelArgs q) {
-  __shared__ float scratch[kThreads / kWave];
+__global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKernelArgs q) {
+  constexpr int V = kVec<T>, NT = kWideThreads;
+  __shared__ RowShared<NT / kWave> sh;
   const ppo_token_loss_args& a = q.a;
   const int64_t r = blockIdx.x;
   const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
   T* dx = LOSS && a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
   int64_t tok;
-  bool live = counts(a, r, tok);
-  float m = -INFINITY;
-  if (live) {
-    for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) m = fmaxf(m, static_cast<float>(x[j]));
-    m = block_reduce(m, scratch, [](float u, float v) { return fmaxf(u, v); });
-    // -inf throughout (a NaN among them still goes on): no distribution
-    if (m == -INFINITY) {
-      float nan = 0.0f;
-      for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) nan += x[j] != x[j] ? 1.0f : 0.0f;
-      live = block_reduce(nan, scratch, [](float u, float v) { return u + v; }) > 0.0f;
-    }
-  }
-  if (!live) {
-    if (threadIdx.x == 0) row_zeros(q, r, LOSS);
-    if (dx != nullptr)
-      for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) dx[j] = static_cast<T>(0.0f);
+  if (!row_counts(a, r, tok)) {
+    skip_row<LOSS>(q, r);
+    if (dx != nullptr) zero_gradient<T, NT>(dx, a.vocab);
     return;
   }
-  float s = 0.0f, e = 0.0f;
-  for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) {
-    const float t = (static_cast<float>(x[j]) - m) * q.c, p = exp2f(t);
-    s += p;
-    e = fmaf(p, fmaxf(t, kFloor), e);
+  auto load = [&](int64_t j, float (&v)[V]) {
+    if (j + V <= a.vocab) {
+      const auto p = load_piece(x + j);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = static_cast<float>(p[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = j + e < a.vocab ? static_cast<float>(x[j + e]) : -INFINITY;
+    }
+  };
+  const float x_tok = static_cast<float>(x[tok]);
+  const int32_t counted = LOSS && q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x, NT)) : 0;
+  RowSums mine{-INFINITY, 0.0f, 0.0f};
+  for (int64_t j = threadIdx.x * V; j < a.vocab; j += NT * V) {
+    float v[V];
+    load(j, v);
+    RowSums part{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < V; ++e) part.m = fmaxf(part.m, v[e]);
+    const float m = fmaxf(part.m, mine.m);
+    if (m > mine.m) mine = join(mine, RowSums{m, 0.0f, 0.0f}, q.c);
+    const float c = scale_for(m, q.c), mc = m > -INFINITY ? m * c : 0.0f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float t = fmaf(v[e], c, -mc), p = exp2f(t);
+      mine.s += p;
+      mine.e = fmaf(p, fmaxf(t, kFloor), mine.e);
+    }
   }
-  s = block_reduce(s, scratch, [](float u, float v) { return u + v; });
-  e = block_reduce(e, scratch, [](float u, float v) { return u + v; });
-  const float t_tok = (static_cast<float>(x[tok]) - m) * q.c;
-  const RowScalars o = row_scalars(q, r, t_tok, s, e, LOSS, threadIdx.x == 0);
+  for (int d = kWave / 2; d > 0; d >>= 1)
+    mine = join_lanes(mine, d, q.c);
+  const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh);
   if (dx == nullptr) return;
-  const float k = *q.inv_n * q.inv_temp;
-  const float ca = k * (q.entropy_coef * o.h - o.g), cb = k * q.entropy_coef * kLn2, ct = k * o.g;
-  __syncthreads();  // x[tok] has been read by every thread: d_logits may be the logits
-  for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) {
-    const float w = fmaxf((static_cast<float>(x[j]) - m) * q.c - o.log2_s, kFloor);
-    float d = exp2f(w) * fmaf(cb, w, ca);
-    if (j == tok) d += ct;
-    dx[j] = static_cast<T>(d);
+  if (!o.live) {
+    zero_gradient<T, NT>(dx, a.vocab);
+    return;
+  }
+  for (int64_t j = threadIdx.x * V; j < a.vocab; j += NT * V) {
+    float v[V];
+    load(j, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[e] = gradient_of(v[e], o);
+      if (j + e == tok) v[e] += o.at;
+    }
+    if (j + V <= a.vocab) store_piece(dx + j, v);
+    else
+      for (int e = 0; e < V; ++e)
+        if (j + e < a.vocab) dx[j + e] = static_cast<T>(v[e]);
   }
 }
 
 // The means over rows, fp64 sums in a fixed order.
-__global__ __launch_bounds__(1024) void token_stats_kernel(const LossKernelArgs q) {
-  __shared__ double part[kTerms][1024 / kWave];
+__global__ __launch_bounds__(kStatsThreads) void token_stats_kernel(const LossKernelArgs q) {
+  __shared__ double part[kTerms][kStatsThreads / kWave];
   double sum[kTerms] = {};
-  for (int64_t r = threadIdx.x; r < q.a.rows; r += 1024)
-#pragma unroll
-    for (int i = 0; i < kTerms; ++i) sum[i] += static_cast<double>(q.terms[i * q.a.rows + r]);
+  for (int64_t r = threadIdx.x; r < q.a.rows; r += kStatsThreads) {
+    const float4* t = reinterpret_cast<const float4*>(q.terms + r * kTermStride);
+    const float4 u = t[0], v = t[1];
+    sum[0] += u.x, sum[1] += u.y, sum[2] += u.z, sum[3] += u.w, sum[4] += v.x, sum[5] += v.y;
+  }
 #pragma unroll
   for (int i = 0; i < kTerms; ++i) {
     const double x = wave_sum(sum[i]);
@@ -175,21 +378,36 @@ __global__ __launch_bounds__(1024) void token_stats_kernel(const LossKernelArgs 
   }
   __syncthreads();
   if (threadIdx.x != 0) return;
-  const double inv = *q.inv_n > 0.0f ? 1.0 / static_cast<double>(*q.n) : 0.0;
-  double mean[kTerms];
   for (int i = 0; i < kTerms; ++i) {
-    double x = 0.0;
-    for (int w = 0; w < 1024 / kWave; ++w) x += part[i][w];
-    mean[i] = x * inv;
+    sum[i] = 0.0;
+    for (int w = 0; w < kStatsThreads / kWave; ++w) sum[i] += part[i][w];
   }
-  q.a.stats[0] = static_cast<float>(mean[0] + q.a.kl_coef * mean[1] - q.a.entropy_coef * mean[2]);
-  for (int i = 0; i < kTerms; ++i) q.a.stats[1 + i] = static_cast<float>(mean[i]);
-  q.a.stats[6] = *q.n;
+  const double n = q.a.denom > 0.0 ? q.a.denom : sum[5], inv = sum[5] > 0.0 ? 1.0 / n : 0.0;
+  for (int i = 0; i < 5; ++i) q.a.stats[1 + i] = static_cast<float>(sum[i] * inv);
+  q.a.stats[0] = static_cast<float>((sum[0] + q.a.kl_coef * sum[1] - q.a.entropy_coef * sum[2]) * inv);
+  q.a.stats[6] = static_cast<float>(n);
   q.a.stats[7] = 0.0f;
 }
 
+template <class T, bool LOSS>
+void launch_rows(const LossKernelArgs& q, hipStream_t st) {
+  const int64_t pieces = ceil_div(q.a.vocab, kVec<T>);
+  const dim3 grid(static_cast<uint32_t>(q.a.rows));
+#define PPO_ROWS(NT, K) hipLaunchKernelGGL((token_row_kernel<T, NT, K, LOSS>), grid, dim3(NT), 0, st, q)
+  if (q.a.vocab < kVec<T> || pieces > 16 * 1024)
+    hipLaunchKernelGGL((token_wide_kernel<T, LOSS>), grid, dim3(kWideThreads), 0, st, q);
+  else if (pieces <= 64) PPO_ROWS(64, 1);
+  else if (pieces <= 256) PPO_ROWS(64, 4);
+  else if (pieces <= 1024) PPO_ROWS(256, 4);
+  else if (pieces <= 2048) PPO_ROWS(256, 8);
+  else if (pieces <= 4096) PPO_ROWS(256, 16);
+  else if (pieces <= 8192) PPO_ROWS(512, 16);
+  else PPO_ROWS(1024, 16);
+#undef PPO_ROWS
+}
+
 size_t workspace_for(int64_t rows) {
-  return (64 + static_cast<size_t>(kTerms) * static_cast<size_t>(rows)) * sizeof(float);
+  return (64 + static_cast<size_t>(kTermStride) * static_cast<size_t>(rows)) * sizeof(float);
 }
 
 int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream,
@@ -200,7 +418,7 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
               (long long)a.rows, (long long)a.vocab);
   PPO_REQUIRE(type_ok(a.type), "%s: type=%d", who, a.type);
   PPO_REQUIRE(a.token_type == PPO_TOKENS_I64 || a.token_type == PPO_TOKENS_I32, "%s: token_type=%d", who, a.token_type);
-  PPO_REQUIRE(a.temperature > 0.0 && a.temperature < 1e30, "%s: temperature=%g", who, a.temperature);
+  PPO_REQUIRE(a.temperature >= 1e-6 && a.temperature <= 1e6, "%s: temperature=%g", who, a.temperature);
   PPO_REQUIRE(a.ld_logits >= a.vocab && (!loss || a.d_logits == nullptr || a.ld_d_logits >= a.vocab),
               "%s: leading dimensions below vocab=%lld", who, (long long)a.vocab);
   PPO_REQUIRE(a.rows == 0 || (a.logits != nullptr && a.tokens != nullptr), "%s: null pointer", who);
@@ -214,7 +432,7 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
     PPO_REQUIRE(a.clip_low >= 0.0 && a.clip_high >= 0.0, "%s: clip range %g, %g", who, a.clip_low, a.clip_high);
     PPO_REQUIRE(a.denom >= 0.0 && a.denom < 1e30, "%s: denom=%g", who, a.denom);
     const size_t need = workspace_for(a.rows);
-    PPO_REQUIRE(workspace != nullptr && workspace_bytes >= need, "%s: workspace too small (%zu < %zu)", who,
+    PPO_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= need, "%s: workspace too small or not 16-byte aligned (%zu < %zu)", who,
                 workspace_bytes, need);
     PPO_REQUIRE(a.d_logits != a.logits || a.ld_d_logits == a.ld_logits, "%s: in place needs the same rows", who);
   } else if (a.rows == 0 || (a.logp == nullptr && a.entropy == nullptr)) {
@@ -224,31 +442,31 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
   LossKernelArgs q{};
   q.a = a;
   q.inv_n = static_cast<float*>(workspace);
-  q.n = q.inv_n + 1;
   q.terms = q.inv_n + 64;
+  q.count = !loss || a.denom > 0.0 ? 0 : a.rows <= kCountRows ? 1 : 2;
+  q.given_inv_n = a.denom > 0.0 ? static_cast<float>(1.0 / a.denom) : 0.0f;
   q.inv_temp = static_cast<float>(1.0 / a.temperature);
   q.c = static_cast<float>(1.4426950408889634 / a.temperature);
   q.clip_lo = static_cast<float>(1.0 - a.clip_low);
   q.clip_hi = static_cast<float>(1.0 + a.clip_high);
   q.kl_coef = static_cast<float>(a.kl_coef);
   q.entropy_coef = static_cast<float>(a.entropy_coef);
-  if (loss) {
-    hipLaunchKernelGGL(token_count_kernel, dim3(1), dim3(1024), 0, st, q);
+  if (q.count == 2) {
+    hipLaunchKernelGGL(token_count_kernel, dim3(1), dim3(kStatsThreads), 0, st, q);
     if (int rc = check_launch("token_count_kernel")) return rc;
   }
   if (a.rows > 0) {
     int rc = PPO_OK;
     with_type(a.type, [&](auto t) {
       using T = decltype(t);
-      const dim3 grid(static_cast<uint32_t>(a.rows));
-      if (loss) hipLaunchKernelGGL((token_row_kernel<T, true>), grid, dim3(kThreads), 0, st, q);
-      else hipLaunchKernelGGL((token_row_kernel<T, false>), grid, dim3(kThreads), 0, st, q);
+      if (loss) launch_rows<T, true>(q, st);
+      else launch_rows<T, false>(q, st);
       rc = check_launch("token_row_kernel");
     });
     if (rc != PPO_OK) return rc;
   }
   if (!loss) return PPO_OK;
-  hipLaunchKernelGGL(token_stats_kernel, dim3(1), dim3(1024), 0, st, q);
+  hipLaunchKernelGGL(token_stats_kernel, dim3(1), dim3(kStatsThreads), 0, st, q);
   return check_launch("token_stats_kernel");
 }
 
