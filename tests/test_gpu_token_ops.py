@@ -192,6 +192,7 @@ def _loss_error(x, vocab, temperature):
     return U * (4 * top / math.log(2) + vocab / 256 + 64)
 
 
+MANY = [(129, 7), (130, 600), (129, 3001), (131, 9000), (129, 20001), (130, 40000), (129, 70001), (129, 131072), (129, 140001)]
 SHAPES = [(1, 1), (1, 2), (2, 5), (3, 64), (5, 1000), (64, 257), (9, 4096), (4, 32000), (3, 50021), (2, 131072), (300, 77)]
 
 
@@ -231,6 +232,19 @@ def test_token_loss(cuda, dtype, masked, banned, rows, vocab):
                        entropy_coef=ent, temperature=T)
     _inside(s2[:6], want["stats"], size * e + 2 * U * want["stats"].abs(), "stats without gradient")
     ops.token_log_probs(d(x), d(tok), lp2, temperature=T)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", MANY)
+def test_token_loss_of_many_rows(cuda, dtype, rows, vocab):
+    """More rows than a row each is worth cutting into parts."""
+    test_token_loss(cuda, dtype, 0.6, True, rows, vocab)
+
+
+@pytest.mark.parametrize("rows", [2049, 5000])
+def test_token_loss_counts_many_rows(cuda, rows):
+    """So many rows that a launch of its own counts them."""
+    test_token_loss(cuda, F32, 0.4, False, rows, 30)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -21,7 +21,7 @@ namespace {
 constexpr int kAdamwThreads = 256, kPer = 4;
 constexpr int kChunk = kAdamwThreads * kPer;  // elements a block takes at a time
 constexpr int kMaxTensors = 48, kMaxGrads = 160;
-constexpr int kNormBlocks = 1024;  // of one norm launch
+constexpr int kNormChunk = 8 * kChunk, kNormBlocks = 2048;  // elements a block's loads have in flight, blocks of one norm launch
 static_assert(kChunk % PPO_ADAMW_BLOCK == 0 && PPO_ADAMW_BLOCK == kWave * kPer, "a wave owns a scale's block");
 
 struct NormTable {
@@ -53,7 +53,7 @@ struct UpdateTable {
 static_assert(sizeof(UpdateTable) <= 3800, "kernel arguments");
 
 struct Scalars {
-  float w1, b2, c2, eps, bc2_sqrt;
+  float w1, b2, c2, eps, bc2_sqrt, inv_bc2_sqrt;
 };
 
 // The tensor of a chunk: the last one whose first chunk is not behind it.
@@ -109,20 +109,35 @@ __device__ __forceinline__ void store4(T* p, int n, const float (&x)[kPer]) {
 
 template <class G>
 __global__ __launch_bounds__(kAdamwThreads) void adamw_norm_kernel(const NormTable t, int chunks, double* __restrict__ partial) {
+  constexpr int V = kVec<G>, K = kNormChunk / (kAdamwThreads * V);
   __shared__ double red[kAdamwThreads / kWave];
-  double sum = 0.0;
+  double sum[4] = {};
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const int k = tensor_of(t.first, t.tensors, c);
-    const int64_t i = static_cast<int64_t>(c - t.first[k]) * kChunk + threadIdx.x * kPer;
-    const int n = static_cast<int>(min<int64_t>(kPer, t.count[k] - i));
-    if (n <= 0) continue;
-    float g[kPer];
-    load4(static_cast<const G*>(t.grad[k]) + i, n, g);
+    const G* g = static_cast<const G*>(t.grad[k]);
+    const int64_t from = static_cast<int64_t>(c - t.first[k]) * kNormChunk;
+    const int left = static_cast<int>(min<int64_t>(kNormChunk, t.count[k] - from));
+    g += from;
+    if (left == kNormChunk) {
+      RawPiece x[K];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) sum += static_cast<double>(g[e]) * static_cast<double>(g[e]);
+      for (int i = 0; i < K; ++i) x[i] = load_raw(g + (i * kAdamwThreads + static_cast<int>(threadIdx.x)) * V);
+#pragma unroll
+      for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const double d = element<G>(x[i], e);
+          sum[e % 4] = fma(d, d, sum[e % 4]);
+        }
+    } else {
+      for (int i = threadIdx.x; i < left; i += kAdamwThreads) {
+        const double d = static_cast<float>(g[i]);
+        sum[0] = fma(d, d, sum[0]);
+      }
+    }
   }
-  sum = block_sum(sum, red);
-  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+  const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = all;
 }
 
 // coef[0] = the clip coefficient
@@ -165,6 +180,39 @@ __device__ __forceinline__ float block_scale(const float (&x)[kPer]) {
   return __ballot(bad) != 0 ? __builtin_nanf("") : s;
 }
 
+// The codes of a block's four values: round(127 sqrt(x / scale)) and round(255 sqrt(sqrt(x / scale))), with every operation
+// correctly rounded, so that they are what any implementation in this order gives.  Correctly rounded quotients and roots take
+// ten instructions each and bound the kernel (250 M parameters: 1,026 us against 740 that memory takes), so they are computed
+// from the hardware's reciprocal and root first (one unit in the last place each).  Those differ by less than 127 * 4e-7 and
+// 255 * 5e-7 codes; only where a value lies that near the middle between two codes, twice as near for safety, the wave
+// computes it the long way.
+template <bool SECOND>
+__device__ __forceinline__ void codes(const float (&x)[kPer], float scale, float (&q)[kPer]) {
+  constexpr float kTop = SECOND ? 255.0f : 127.0f, kNear = SECOND ? 2.6e-4f : 1.1e-4f;
+  const bool plain = scale > 1e-30f;  // (the reciprocal of less may not be finite; NaN takes the long way too)
+  bool near = !plain;
+  const float inv = __builtin_amdgcn_rcpf(plain ? scale : 1.0f);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    float r = __builtin_amdgcn_sqrtf(x[e] * inv);
+    if (SECOND) r = __builtin_amdgcn_sqrtf(r);
+    r *= kTop;
+    q[e] = rintf(r);
+    near |= fabsf(r - q[e]) > 0.5f - kNear;
+  }
+  if (__ballot(near) != 0) {
+    const float by = scale > 0.0f ? scale : 1.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      float r = sqrtf(x[e] / by);
+      if (SECOND) r = sqrtf(r);
+      q[e] = rintf(r * kTop);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) q[e] = fminf(fmaxf(q[e], 0.0f), kTop);  // (NaN becomes 0)
+}
+
 template <class P, class G, bool MASTER, bool BITS8>
 __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const UpdateTable t, const Scalars s,
                                                                      const float* __restrict__ coef) {
@@ -203,7 +251,10 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
     v[e] = v[e] * s.b2;
     v[e] = v[e] + (s.c2 * d) * d;
     p[e] = p[e] * q.decay;
-    p[e] = p[e] + (q.neg_step * m[e]) / (sqrtf(v[e]) / s.bc2_sqrt + s.eps);
+    if (BITS8 && s.eps >= 1e-16f)  // beside the states' rounding the last bit of the step does not count
+      p[e] = p[e] + (q.neg_step * m[e]) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * s.inv_bc2_sqrt + s.eps);
+    else
+      p[e] = p[e] + (q.neg_step * m[e]) / (sqrtf(v[e]) / s.bc2_sqrt + s.eps);
   }
   if constexpr (BITS8) {
     // elements past the end hold zeros: g, m and v
@@ -212,13 +263,12 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
     for (int e = 0; e < kPer; ++e) am[e] = fabsf(m[e]);
     const float ms = block_scale(am), vs = block_scale(v);
     float qm[kPer], qv[kPer];
+    codes<false>(am, ms, qm);
+    codes<true>(v, vs, qv);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const float a = rintf(sqrtf(am[e] / (ms > 0.0f ? ms : 1.0f)) * 127.0f);
-      qm[e] = copysignf(fminf(fmaxf(a, 0.0f), 127.0f), m[e]);
-      float b = rintf(sqrtf(sqrtf(v[e] / (vs > 0.0f ? vs : 1.0f))) * 255.0f);
-      b = fminf(fmaxf(b, 0.0f), 255.0f);
-      qv[e] = v[e] > 0.0f ? fmaxf(b, 1.0f) : b;
+      qm[e] = copysignf(qm[e], m[e]);
+      if (v[e] > 0.0f) qv[e] = fmaxf(qv[e], 1.0f);
     }
     if (n == 0) return;
     store4(static_cast<int8_t*>(q.m) + i, n, qm);
@@ -314,7 +364,7 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
           t.grad[t.tensors] = tensors[i].grad;
           t.count[t.tensors] = tensors[i].count;
           t.first[t.tensors++] = static_cast<int32_t>(chunks);
-          chunks += chunks_of(tensors[i]);
+          chunks += ceil_div(tensors[i].count, kNormChunk);
           PPO_REQUIRE(chunks < INT32_MAX, "ppo_adamw_step: too many parameters");
         }
         if (t.tensors == 0) break;
@@ -332,7 +382,7 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
     if (int rc = check_launch("adamw_clip_kernel")) return rc;
   }
   const Scalars s{static_cast<float>(1.0 - beta1), static_cast<float>(beta2), static_cast<float>(1.0 - beta2),
-                  static_cast<float>(eps), static_cast<float>(bc2_sqrt)};
+                  static_cast<float>(eps), static_cast<float>(bc2_sqrt), static_cast<float>(1.0 / bc2_sqrt)};
   for (int kind = 0; kind < 16; ++kind) {
     int i = 0;
     while (i < count) {

@@ -53,6 +53,9 @@ __device__ __forceinline__ void make_neg_inf(RawPiece& r, int e) {
 __device__ __forceinline__ void forget(RawPiece& r, float& done) { asm volatile("" : "+v"(r.w[0]), "+v"(r.w[1]), "+v"(r.w[2]), "+v"(r.w[3]), "+v"(done)); }
 __device__ __forceinline__ void forget(int& x) { asm volatile("" : "+v"(x)); }
 
+// A loaded value that has to have arrived here: what follows may overwrite where it came from.
+__device__ __forceinline__ void arrived(float& x) { asm volatile("" : "+v"(x)); }
+
 template <class T>
 __device__ __forceinline__ typename Piece<T>::type load_piece(const T* p) {
   return *reinterpret_cast<const typename Piece<T>::type*>(p);

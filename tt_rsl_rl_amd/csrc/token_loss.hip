@@ -53,8 +53,17 @@ __device__ __forceinline__ float wave_max(float x) {
 
 __device__ __forceinline__ int32_t rows_counted(const LossKernelArgs& q, int first, int step) {
   int32_t n = 0;
-  int64_t tok;
-  for (int64_t r = first; r < q.a.rows; r += step) n += row_counts(q.a, r, tok) ? 1 : 0;
+  for (int64_t r = first; r < q.a.rows; r += 4 * step) {
+    bool in[4];  // four rows' loads in flight
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = min(r + u * step, q.a.rows - 1);
+      const bool kept = q.a.mask == nullptr || q.a.mask[i] != 0;
+      in[u] = (token_at(q.a.tokens, q.a.token_type, i, q.a.vocab) >= 0) & kept & (r + u * step < q.a.rows);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) n += in[u] ? 1 : 0;
+  }
   return n;
 }
 
@@ -110,7 +119,7 @@ struct RowCoefs {
 // Joins the waves' sums (the row's only barrier) and writes logp, entropy and the loss terms.
 template <int NT, bool LOSS>
 __device__ __forceinline__ RowCoefs finish_row(const LossKernelArgs& q, int64_t r, RowSums mine, float x_tok, int32_t counted,
-                                               RowShared<NT / kWave>& sh) {
+                                               RowShared<NT / kWave>& sh, bool write) {
   constexpr int WAVES = NT / kWave;
   if constexpr (WAVES > 1) {
     if (threadIdx.x % kWave == 0) {
@@ -137,7 +146,6 @@ __device__ __forceinline__ RowCoefs finish_row(const LossKernelArgs& q, int64_t 
     lp = kLn2 * ((x_tok - mine.m) * q.c - log2_s);
     h = kLn2 * (log2_s - mine.e / mine.s);
   }
-  const bool write = threadIdx.x == 0;
   if (write && q.a.logp != nullptr) q.a.logp[r] = lp;
   if (write && q.a.entropy != nullptr) q.a.entropy[r] = h;
   if (!LOSS) return o;
@@ -171,10 +179,10 @@ __device__ __forceinline__ RowCoefs finish_row(const LossKernelArgs& q, int64_t 
 
 // A row that does not count, or has no distribution: its gradient is zero.
 template <class T, int NT>
-__device__ __forceinline__ void zero_gradient(T* dx, int64_t vocab) {
+__device__ __forceinline__ void zero_gradient(T* dx, int64_t first, int64_t vocab) {
   constexpr int V = kVec<T>;
   const float zero[V] = {};
-  for (int64_t j = threadIdx.x * V; j < vocab; j += NT * V) {
+  for (int64_t j = first + threadIdx.x * V; j < vocab; j += NT * V) {
     if (j + V <= vocab) store_piece(dx + j, zero);
     else
       for (int64_t i = j; i < vocab; ++i) dx[i] = static_cast<T>(0.0f);
@@ -192,57 +200,52 @@ __device__ __forceinline__ void skip_row(const LossKernelArgs& q, int64_t r) {
 
 __device__ __forceinline__ float gradient_of(float x, const RowCoefs& o) {
   const float t = fmaxf(fmaf(x, o.c, -o.mc), kFloor);
-  return exp2f(t) * fmaf(o.b, t, o.a);
+  return __builtin_amdgcn_exp2f(t) * fmaf(o.b, t, o.a);
 }
 
-// One block of NT threads per row, K 16-byte pieces of it in each thread's registers (NT K V >= vocab >= V): piece k of
-// thread i is the (k NT + i)-th.  The last piece of a row whose width is no multiple of V is read from V columns before the
-// end; what it shares with the piece before it, and pieces past the end, become -inf, which adds nothing to a sum.
-template <class T, int NT, int K, bool LOSS>
-__global__ __launch_bounds__(NT) void token_row_kernel(const LossKernelArgs q) {
-  constexpr int V = kVec<T>;
-  __shared__ RowShared<NT / kWave> sh;
-  const ppo_token_loss_args& a = q.a;
-  const int64_t r = blockIdx.x;
-  const int vocab = static_cast<int>(a.vocab);
-  const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
-  T* dx = LOSS && a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
-  int64_t tok;
-  if (!row_counts(a, r, tok)) {
-    skip_row<LOSS>(q, r);
-    if (dx != nullptr) zero_gradient<T, NT>(dx, vocab);
-    return;
-  }
-  // of piece k: its first column, and whether the wave's pieces lie inside the row, partly or not at all (wave-uniform)
-  const int wave_first = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave * kWave);
-  int tid = threadIdx.x;
-  auto column = [&](int k) { return (k * NT + tid) * V; };
-  auto whole = [&](int k) { return (k * NT + wave_first + kWave) * V <= vocab; };
-  auto some = [&](int k) { return (k * NT + wave_first) * V < vocab; };
-  auto offset = [&](int j) { return static_cast<uint32_t>(j) * static_cast<uint32_t>(sizeof(T)); };  // 32 bits, of a uniform base
+// 16-byte pieces of a row in the registers of NT threads, K each: piece k of thread i holds the columns from
+// first + (k NT + i) V on (vocab >= V).  The last piece of a row whose width is no multiple of V is read from V columns before
+// the end; what it shares with the piece before it, and pieces past the end, become -inf, which adds nothing to a sum.
+template <class T, int NT, int K>
+struct RowPieces {
+  static constexpr int V = kVec<T>;
   RawPiece raw[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) raw[k] = load_raw(reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + offset(min(column(k), vocab - V))));
-  const float x_tok = static_cast<float>(x[tok]);
-  const int32_t counted = LOSS && q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x, NT)) : 0;
-  forget(tid);  // (the columns are computed again where they are needed, not kept)
-  RowSums mine{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (!whole(k)) {
-      const int skip = column(k) - min(column(k), vocab - V);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (e < skip) make_neg_inf<T>(raw[k], e);
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) mine.m = fmaxf(mine.m, element<T>(raw[k], e));
-    forget(raw[k], mine.m);
-    __builtin_amdgcn_sched_barrier(0);  // one piece at a time: its converted values are gone before the next one's
+  int vocab, first, tid, wave;
+
+  __device__ __forceinline__ RowPieces(int vocab_, int first_) : vocab(vocab_), first(first_), tid(threadIdx.x) {
+    wave = __builtin_amdgcn_readfirstlane(tid / kWave * kWave);
   }
-  mine.m = wave_max(mine.m);
-  {
-    const float c = scale_for(mine.m, q.c), mc = mine.m > -INFINITY ? mine.m * c : 0.0f;
+  __device__ __forceinline__ int column(int k) const { return first + (k * NT + tid) * V; }
+  // whether the wave's pieces lie inside the row, partly or not at all: the same for its lanes
+  __device__ __forceinline__ bool whole(int k) const { return first + (k * NT + wave + kWave) * V <= vocab; }
+  __device__ __forceinline__ bool some(int k) const { return first + (k * NT + wave) * V < vocab; }
+  __device__ __forceinline__ uint32_t offset(int j) const { return static_cast<uint32_t>(j) * static_cast<uint32_t>(sizeof(T)); }
+
+  __device__ __forceinline__ void load(const T* x) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)  // a uniform base and 32 bits of offset
+      raw[k] = load_raw(reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + offset(min(column(k), vocab - V))));
+  }
+
+  // The wave's maximum and sums.
+  __device__ __forceinline__ RowSums sums(float scale) {
+    RowSums mine{-INFINITY, 0.0f, 0.0f};
+    forget(tid);  // (columns are computed again where they are needed, not kept)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!whole(k)) {
+        const int skip = column(k) - min(column(k), vocab - V);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e < skip) make_neg_inf<T>(raw[k], e);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) mine.m = fmaxf(mine.m, element<T>(raw[k], e));
+      forget(raw[k], mine.m);
+      __builtin_amdgcn_sched_barrier(0);  // one piece at a time: its converted values are gone before the next one's
+    }
+    mine.m = wave_max(mine.m);
+    const float c = scale_for(mine.m, scale), mc = mine.m > -INFINITY ? mine.m * c : 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (some(k)) {
@@ -256,41 +259,142 @@ __global__ __launch_bounds__(NT) void token_row_kernel(const LossKernelArgs q) {
       forget(raw[k], mine.s);
       __builtin_amdgcn_sched_barrier(0);
     }
+    mine.s = wave_sum(mine.s);
+    mine.e = wave_sum(mine.e);
+    return mine;
   }
-  mine.s = wave_sum(mine.s);
-  mine.e = wave_sum(mine.e);
-  const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh);
-  if (dx == nullptr) return;
-  if (!o.live) {
-    zero_gradient<T, NT>(dx, vocab);
+
+  __device__ __forceinline__ void gradient(T* dx, int tok, const RowCoefs& o) {
+    forget(tid);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (some(k)) {
+        const int at = min(column(k), vocab - V);
+        float d[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] = gradient_of(element<T>(raw[k], e), o);
+        const uint32_t hit = static_cast<uint32_t>(tok - at);
+        if (hit < V)
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (static_cast<uint32_t>(e) == hit) d[e] += o.at;
+        if (whole(k)) {
+          store_piece(reinterpret_cast<T*>(reinterpret_cast<char*>(dx) + offset(at)), d);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (e >= column(k) - at) dx[at + e] = static_cast<T>(d[e]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+// One block of NT threads per row, the whole row in its registers (NT K V >= vocab).
+template <class T, int NT, int K, bool LOSS>
+__global__ __launch_bounds__(NT) void token_row_kernel(const LossKernelArgs q) {
+  __shared__ RowShared<NT / kWave> sh;
+  const ppo_token_loss_args& a = q.a;
+  const int64_t r = blockIdx.x;
+  const int vocab = static_cast<int>(a.vocab);
+  const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
+  T* dx = LOSS && a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
+  int64_t tok;
+  if (!row_counts(a, r, tok)) {
+    skip_row<LOSS>(q, r);
+    if (dx != nullptr) zero_gradient<T, NT>(dx, 0, vocab);
     return;
   }
-  forget(tid);
+  RowPieces<T, NT, K> row(vocab, 0);
+  row.load(x);
+  float x_tok = static_cast<float>(x[tok]);
+  const int32_t counted = LOSS && q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x, NT)) : 0;
+  const RowSums mine = row.sums(q.c);
+  arrived(x_tok);
+  const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh, threadIdx.x == 0);
+  if (dx == nullptr) return;
+  if (o.live) row.gradient(dx, static_cast<int>(tok), o);
+  else zero_gradient<T, NT>(dx, 0, vocab);
+}
+
+// A few wide rows, which one compute unit each would leave waiting for its arithmetic (131,072 bf16 logits: 10.9 us): a row
+// is cut into parts of kPartThreads kPartPieces pieces, a block each.  token_part_kernel leaves a part's sums; then
+// token_joined_kernel's one wave per row joins them, or each block of token_part_gradient_kernel does before it reads its part
+// again.
+constexpr int kPartThreads = 256, kPartPieces = 4, kMaxParts = kWave;
+constexpr int64_t kSplitRows = 128, kSplitPieces = 2 * kPartThreads * kPartPieces;
+
+struct RowPart {
+  RowSums sums;
+  float x_tok;  // of part 0 (d_logits may be the logits, so nobody reads it later)
+};
+
+template <class T>
+__global__ __launch_bounds__(kPartThreads) void token_part_kernel(const LossKernelArgs q, RowPart* __restrict__ parts) {
+  __shared__ RowSums sh[kPartThreads / kWave];
+  const ppo_token_loss_args& a = q.a;
+  const int64_t r = blockIdx.y;
+  int64_t tok;
+  if (!row_counts(a, r, tok)) return;
+  const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
+  RowPieces<T, kPartThreads, kPartPieces> row(static_cast<int>(a.vocab), blockIdx.x * (kPartThreads * kPartPieces * kVec<T>));
+  row.load(x);
+  const float x_tok = blockIdx.x == 0 ? static_cast<float>(x[tok]) : 0.0f;
+  RowSums mine = row.sums(q.c);
+  if (threadIdx.x % kWave == 0) sh[threadIdx.x / kWave] = mine;
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  mine = sh[threadIdx.x % (kPartThreads / kWave)];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (some(k)) {
-      const int at = min(column(k), vocab - V);
-      float d[V];
+  for (int d = kPartThreads / kWave / 2; d > 0; d >>= 1) mine = join_lanes(mine, d, q.c);
+  if (threadIdx.x == 0) parts[r * gridDim.x + blockIdx.x] = RowPart{mine, x_tok};
+}
+
+// The parts of a row joined, in every lane.
+__device__ __forceinline__ RowSums join_parts(const RowPart* parts, int n, float c) {
+  const int lane = threadIdx.x % kWave;
+  RowSums mine = lane < n ? parts[lane].sums : RowSums{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float t = fmaxf(fmaf(element<T>(raw[k], e), o.c, -o.mc), kFloor);
-        d[e] = __builtin_amdgcn_exp2f(t) * fmaf(o.b, t, o.a);
-      }
-      const uint32_t hit = static_cast<uint32_t>(static_cast<int>(tok) - at);
-      if (hit < V)
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (static_cast<uint32_t>(e) == hit) d[e] += o.at;
-      if (whole(k)) {
-        store_piece(reinterpret_cast<T*>(reinterpret_cast<char*>(dx) + offset(at)), d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (e >= column(k) - at) dx[at + e] = static_cast<T>(d[e]);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
+  for (int d = kWave / 2; d > 0; d >>= 1) mine = join_lanes(mine, d, c);
+  return mine;
+}
+
+__global__ __launch_bounds__(kWave) void token_joined_kernel(const LossKernelArgs q, const RowPart* __restrict__ parts, int n) {
+  __shared__ RowShared<1> sh;
+  const int64_t r = blockIdx.x;
+  int64_t tok;
+  if (!row_counts(q.a, r, tok)) {
+    skip_row<false>(q, r);
+    return;
   }
+  finish_row<kWave, false>(q, r, join_parts(parts + r * n, n, q.c), parts[r * n].x_tok, 0, sh, threadIdx.x == 0);
+}
+
+template <class T>
+__global__ __launch_bounds__(kPartThreads) void token_part_gradient_kernel(const LossKernelArgs q, const RowPart* __restrict__ parts) {
+  constexpr int kPart = kPartThreads * kPartPieces * kVec<T>;
+  __shared__ RowShared<1> sh;
+  const ppo_token_loss_args& a = q.a;
+  const int64_t r = blockIdx.y;
+  const int vocab = static_cast<int>(a.vocab), first = blockIdx.x * kPart, n = gridDim.x;
+  const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
+  T* dx = a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
+  if (dx == nullptr && first > 0) return;
+  int64_t tok;
+  if (!row_counts(a, r, tok)) {
+    if (first == 0) skip_row<true>(q, r);
+    if (dx != nullptr) zero_gradient<T, kPartThreads>(dx, first, min(first + kPart, vocab));
+    return;
+  }
+  RowPieces<T, kPartThreads, kPartPieces> row(vocab, first);
+  if (dx != nullptr) row.load(x);
+  const int32_t counted = q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x % kWave, kWave)) : 0;
+  const RowCoefs o = finish_row<kWave, true>(q, r, join_parts(parts + r * n, n, q.c), parts[r * n].x_tok, counted, sh,
+                                             first == 0 && threadIdx.x == 0);
+  if (dx == nullptr) return;
+  if (o.live) row.gradient(dx, static_cast<int>(tok), o);
+  else zero_gradient<T, kPartThreads>(dx, first, min(first + kPart, vocab));
 }
 
 // Rows of any width: the sums in one pass, each thread rescaling its own when its maximum grows, the gradient in another.
@@ -307,7 +411,7 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
   int64_t tok;
   if (!row_counts(a, r, tok)) {
     skip_row<LOSS>(q, r);
-    if (dx != nullptr) zero_gradient<T, NT>(dx, a.vocab);
+    if (dx != nullptr) zero_gradient<T, NT>(dx, 0, a.vocab);
     return;
   }
   auto load = [&](int64_t j, float (&v)[V]) {
@@ -320,7 +424,7 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
       for (int e = 0; e < V; ++e) v[e] = j + e < a.vocab ? static_cast<float>(x[j + e]) : -INFINITY;
     }
   };
-  const float x_tok = static_cast<float>(x[tok]);
+  float x_tok = static_cast<float>(x[tok]);
   const int32_t counted = LOSS && q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x, NT)) : 0;
   RowSums mine{-INFINITY, 0.0f, 0.0f};
   for (int64_t j = threadIdx.x * V; j < a.vocab; j += NT * V) {
@@ -334,17 +438,18 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
     const float c = scale_for(m, q.c), mc = m > -INFINITY ? m * c : 0.0f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float t = fmaf(v[e], c, -mc), p = exp2f(t);
+      const float t = fmaf(v[e], c, -mc), p = __builtin_amdgcn_exp2f(t);
       mine.s += p;
       mine.e = fmaf(p, fmaxf(t, kFloor), mine.e);
     }
   }
   for (int d = kWave / 2; d > 0; d >>= 1)
     mine = join_lanes(mine, d, q.c);
-  const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh);
+  arrived(x_tok);
+  const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh, threadIdx.x == 0);
   if (dx == nullptr) return;
   if (!o.live) {
-    zero_gradient<T, NT>(dx, a.vocab);
+    zero_gradient<T, NT>(dx, 0, a.vocab);
     return;
   }
   for (int64_t j = threadIdx.x * V; j < a.vocab; j += NT * V) {
@@ -366,6 +471,7 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
 __global__ __launch_bounds__(kStatsThreads) void token_stats_kernel(const LossKernelArgs q) {
   __shared__ double part[kTerms][kStatsThreads / kWave];
   double sum[kTerms] = {};
+#pragma unroll 4
   for (int64_t r = threadIdx.x; r < q.a.rows; r += kStatsThreads) {
     const float4* t = reinterpret_cast<const float4*>(q.terms + r * kTermStride);
     const float4 u = t[0], v = t[1];
@@ -390,9 +496,18 @@ __global__ __launch_bounds__(kStatsThreads) void token_stats_kernel(const LossKe
 }
 
 template <class T, bool LOSS>
-void launch_rows(const LossKernelArgs& q, hipStream_t st) {
+int launch_rows(const LossKernelArgs& q, RowPart* parts, hipStream_t st) {
   const int64_t pieces = ceil_div(q.a.vocab, kVec<T>);
   const dim3 grid(static_cast<uint32_t>(q.a.rows));
+  const int64_t n = ceil_div(pieces, kPartThreads * kPartPieces);
+  if (q.a.rows <= kSplitRows && pieces >= kSplitPieces && n <= kMaxParts) {
+    const dim3 split(static_cast<uint32_t>(n), static_cast<uint32_t>(q.a.rows));
+    hipLaunchKernelGGL(token_part_kernel<T>, split, dim3(kPartThreads), 0, st, q, parts);
+    if (int rc = check_launch("token_part_kernel")) return rc;
+    if (LOSS) hipLaunchKernelGGL(token_part_gradient_kernel<T>, split, dim3(kPartThreads), 0, st, q, parts);
+    else hipLaunchKernelGGL(token_joined_kernel, grid, dim3(kWave), 0, st, q, parts, static_cast<int>(n));
+    return check_launch("token_part_gradient_kernel");
+  }
 #define PPO_ROWS(NT, K) hipLaunchKernelGGL((token_row_kernel<T, NT, K, LOSS>), grid, dim3(NT), 0, st, q)
   if (q.a.vocab < kVec<T> || pieces > 16 * 1024)
     hipLaunchKernelGGL((token_wide_kernel<T, LOSS>), grid, dim3(kWideThreads), 0, st, q);
@@ -404,10 +519,19 @@ void launch_rows(const LossKernelArgs& q, hipStream_t st) {
   else if (pieces <= 8192) PPO_ROWS(512, 16);
   else PPO_ROWS(1024, 16);
 #undef PPO_ROWS
+  return check_launch("token_row_kernel");
 }
 
-size_t workspace_for(int64_t rows) {
-  return (64 + static_cast<size_t>(kTermStride) * static_cast<size_t>(rows)) * sizeof(float);
+struct Layout {
+  size_t terms, parts, bytes;
+};
+
+Layout workspace_for(int64_t rows) {
+  Layout l;
+  l.terms = 256;
+  l.parts = l.terms + static_cast<size_t>(rows) * kTermStride * sizeof(float);
+  l.bytes = l.parts + (rows <= kSplitRows ? static_cast<size_t>(rows) * kMaxParts * sizeof(RowPart) : 0);
+  return l;
 }
 
 int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream,
@@ -431,18 +555,19 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
                 "%s: null pointer", who);
     PPO_REQUIRE(a.clip_low >= 0.0 && a.clip_high >= 0.0, "%s: clip range %g, %g", who, a.clip_low, a.clip_high);
     PPO_REQUIRE(a.denom >= 0.0 && a.denom < 1e30, "%s: denom=%g", who, a.denom);
-    const size_t need = workspace_for(a.rows);
-    PPO_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= need, "%s: workspace too small or not 16-byte aligned (%zu < %zu)", who,
-                workspace_bytes, need);
     PPO_REQUIRE(a.d_logits != a.logits || a.ld_d_logits == a.ld_logits, "%s: in place needs the same rows", who);
   } else if (a.rows == 0 || (a.logp == nullptr && a.entropy == nullptr)) {
     return PPO_OK;
   }
+  const Layout l = workspace_for(a.rows);
+  PPO_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= l.bytes,
+              "%s: workspace too small or not 16-byte aligned (%zu < %zu)", who, workspace_bytes, l.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
   LossKernelArgs q{};
   q.a = a;
   q.inv_n = static_cast<float*>(workspace);
-  q.terms = q.inv_n + 64;
+  q.terms = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.terms);
+  RowPart* parts = reinterpret_cast<RowPart*>(static_cast<char*>(workspace) + l.parts);
   q.count = !loss || a.denom > 0.0 ? 0 : a.rows <= kCountRows ? 1 : 2;
   q.given_inv_n = a.denom > 0.0 ? static_cast<float>(1.0 / a.denom) : 0.0f;
   q.inv_temp = static_cast<float>(1.0 / a.temperature);
@@ -459,9 +584,7 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
     int rc = PPO_OK;
     with_type(a.type, [&](auto t) {
       using T = decltype(t);
-      if (loss) launch_rows<T, true>(q, st);
-      else launch_rows<T, false>(q, st);
-      rc = check_launch("token_row_kernel");
+      rc = loss ? launch_rows<T, true>(q, parts, st) : launch_rows<T, false>(q, parts, st);
     });
     if (rc != PPO_OK) return rc;
   }
@@ -477,7 +600,7 @@ using namespace ppo;
 
 extern "C" size_t ppo_token_loss_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || rows >= INT32_MAX || vocab < 1 || vocab >= INT32_MAX) return 0;
-  return workspace_for(rows);
+  return workspace_for(rows).bytes;
 }
 
 extern "C" int ppo_token_log_probs(const ppo_token_loss_args* args, void* workspace, size_t workspace_bytes,

@@ -1217,37 +1217,34 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step:
         return
     dev = _current_gpu("adamw_step", params[0], norm_out)
     f32, bf16 = torch.float32, torch.bfloat16
-    items = []
-    for i in range(n):
-        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
-        count, bits = p.numel(), 32
-        master = ms = vs = None
-        tensors = (p, g, m, v)
+    each_lr, each_wd = isinstance(lr, (list, tuple)), isinstance(weight_decay, (list, tuple))
+    pack, items = L.ADAMW_TENSOR.pack, []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avg, exp_avg_sq)):
+        count, ptype, gtype, bits = p.numel(), p.dtype, g.dtype, 32
+        master = ms = vs = 0
+        if not (p.get_device() == g.get_device() == m.get_device() == v.get_device() == dev and p.is_contiguous() and
+                g.is_contiguous() and m.is_contiguous() and v.is_contiguous() and
+                g.numel() == m.numel() == v.numel() == count):
+            raise ValueError(f"adamw_step: parameter {i}, its gradient and states must be contiguous, of one size, on GPU {dev}: "
+                             f"got {[(tuple(t.shape), t.stride(), str(t.device)) for t in (p, g, m, v)]}")
+        if (ptype != f32 and ptype != bf16) or (gtype != f32 and gtype != ptype):
+            raise ValueError(f"adamw_step: tensor {i}: parameter {ptype}, gradient {gtype}")
         if masters is not None and masters[i] is not None:
-            master = masters[i]
-            tensors += (master,)
-            if master.dtype != f32 or p.dtype != bf16:
-                raise ValueError(f"adamw_step: masters[{i}] must be float32 of a bfloat16 parameter")
-        for t in tensors:
-            if t.get_device() != dev or t.numel() != count or not t.is_contiguous():
-                raise ValueError(f"adamw_step: tensor {i} must be contiguous, of {count} elements, on GPU {dev}: got "
-                                 f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
-        if (p.dtype != f32 and p.dtype != bf16) or (g.dtype != f32 and g.dtype != p.dtype):
-            raise ValueError(f"adamw_step: tensor {i}: parameter {p.dtype}, gradient {g.dtype}")
+            t = masters[i]
+            if t.dtype != f32 or ptype != bf16 or t.get_device() != dev or t.numel() != count or not t.is_contiguous():
+                raise ValueError(f"adamw_step: masters[{i}] must be contiguous float32 of a bfloat16 parameter's size")
+            master = t.data_ptr()
         if m.dtype != f32 or v.dtype != f32:
             if m.dtype != torch.int8 or v.dtype != torch.uint8 or scales is None:
                 raise ValueError(f"adamw_step: tensor {i}: states {m.dtype}, {v.dtype} (float32, or int8 and uint8 with scales)")
             bits, blocks = 8, -(-count // L.ADAMW_BLOCK)
-            ms, vs = scales[0][i], scales[1][i]
-            for t in (ms, vs):
+            for t in (scales[0][i], scales[1][i]):
                 if t.get_device() != dev or t.dtype != f32 or t.numel() != blocks or not t.is_contiguous():
                     raise ValueError(f"adamw_step: scales of tensor {i} must be contiguous float32 of {blocks} elements")
-        items.append(L.ADAMW_TENSOR.pack(
-            p.data_ptr(), g.data_ptr(), 0 if master is None else master.data_ptr(), m.data_ptr(), v.data_ptr(),
-            0 if ms is None else ms.data_ptr(), 0 if vs is None else vs.data_ptr(), count,
-            lr[i] if isinstance(lr, (list, tuple)) else lr,
-            weight_decay[i] if isinstance(weight_decay, (list, tuple)) else weight_decay,
-            L.TYPE_F32 if p.dtype == f32 else L.TYPE_BF16, L.TYPE_F32 if g.dtype == f32 else L.TYPE_BF16, bits, 0))
+            ms, vs = scales[0][i].data_ptr(), scales[1][i].data_ptr()
+        items.append(pack(p.data_ptr(), g.data_ptr(), master, m.data_ptr(), v.data_ptr(), ms, vs, count,
+                          lr[i] if each_lr else lr, weight_decay[i] if each_wd else weight_decay,
+                          L.TYPE_F32 if ptype == f32 else L.TYPE_BF16, L.TYPE_F32 if gtype == f32 else L.TYPE_BF16, bits, 0))
     packed = b"".join(items)
     buf = None
     if max_grad_norm is not None or norm_out is not None:
