@@ -22,7 +22,7 @@ constexpr float kFloor = -1000.0f;
 // sums over rows per row: s, k, H, clipped, old_logp - lp, counts, (2 unused)
 constexpr int kTerms = 6, kTermStride = 8;
 constexpr int kCountRows = 2048;  // up to so many rows each block counts them itself: one launch less
-constexpr int kStatsThreads = 1024;
+constexpr int kCountThreads = 1024;
 
 struct LossKernelArgs {
   ppo_token_loss_args a;
@@ -67,14 +67,14 @@ __device__ __forceinline__ int32_t rows_counted(const LossKernelArgs& q, int fir
   return n;
 }
 
-__global__ __launch_bounds__(kStatsThreads) void token_count_kernel(const LossKernelArgs q) {
-  __shared__ int32_t part[kStatsThreads / kWave];
-  const int32_t n = wave_sum(rows_counted(q, threadIdx.x, kStatsThreads));
+__global__ __launch_bounds__(kCountThreads) void token_count_kernel(const LossKernelArgs q) {
+  __shared__ int32_t part[kCountThreads / kWave];
+  const int32_t n = wave_sum(rows_counted(q, threadIdx.x, kCountThreads));
   if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = n;
   __syncthreads();
   if (threadIdx.x == 0) {
     int32_t all = 0;
-    for (int w = 0; w < kStatsThreads / kWave; ++w) all += part[w];
+    for (int w = 0; w < kCountThreads / kWave; ++w) all += part[w];
     *q.inv_n = all > 0 ? static_cast<float>(1.0 / all) : 0.0f;
   }
 }
@@ -110,7 +110,41 @@ struct RowShared {
   int32_t count[WAVES];
 };
 
-// What a row's gradient needs once its sums are known: t = fma(x, c, -mc), d = 2^t (a + b t), + at at the token.
+// What a row contributes: logp, H, log2 S, the derivative g by logp, and the terms of the means.
+struct RowTerms {
+  float lp, h, log2_s, g;
+  float term[kTerms];
+  bool live;  // (nothing but -inf: no distribution; a NaN goes on)
+};
+
+template <bool LOSS>
+__device__ __forceinline__ RowTerms row_terms(const LossKernelArgs& q, int64_t r, const RowSums& sums, float x_tok) {
+  RowTerms o{};
+  o.term[5] = 1.0f;
+  o.live = sums.m > -INFINITY || sums.s != sums.s;
+  if (!o.live) return o;
+  o.log2_s = log2f(sums.s);
+  o.lp = kLn2 * ((x_tok - sums.m) * q.c - o.log2_s);
+  o.h = kLn2 * (o.log2_s - sums.e / sums.s);
+  if (!LOSS) return o;
+  const float old = q.a.old_logp[r], adv = q.a.advantages[r];
+  const float ratio = expf(o.lp - old);
+  const float clipped = fminf(fmaxf(ratio, q.clip_lo), q.clip_hi);
+  const float first = -adv * ratio, second = -adv * clipped;
+  o.g = first >= second ? first : first < second ? 0.0f : first + second;  // (NaN goes on)
+  o.term[0] = first != first || second != second ? first + second : fmaxf(first, second);
+  if (q.a.ref_logp != nullptr) {
+    const float d = q.a.ref_logp[r] - o.lp, x = expf(d);
+    o.term[1] = x - d - 1.0f;
+    o.g += q.kl_coef * (1.0f - x);
+  }
+  o.term[2] = o.h;
+  o.term[3] = ratio != clipped ? 1.0f : 0.0f;
+  o.term[4] = old - o.lp;
+  return o;
+}
+
+// What its gradient needs: t = fma(x, c, -mc), d = 2^t (a + b t), + at at the token.
 struct RowCoefs {
   float c, mc, a, b, at;
   bool live;
@@ -135,45 +169,23 @@ __device__ __forceinline__ RowCoefs finish_row(const LossKernelArgs& q, int64_t 
       if (LOSS) counted += __shfl_xor(counted, d, kWave);
     }
   }
-  RowCoefs o;
-  o.live = mine.m > -INFINITY || mine.s != mine.s;  // nothing but -inf: no distribution (a NaN goes on)
-  o.c = scale_for(mine.m, q.c);
-  o.mc = mine.m * o.c;
-  o.a = o.b = o.at = 0.0f;
-  float lp = 0.0f, h = 0.0f, log2_s = 0.0f;
-  if (o.live) {
-    log2_s = log2f(mine.s);
-    lp = kLn2 * ((x_tok - mine.m) * q.c - log2_s);
-    h = kLn2 * (log2_s - mine.e / mine.s);
+  const RowTerms u = row_terms<LOSS>(q, r, mine, x_tok);
+  if (write) {
+    if (q.a.logp != nullptr) q.a.logp[r] = u.lp;
+    if (q.a.entropy != nullptr) q.a.entropy[r] = u.h;
+    if (LOSS)
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) q.terms[r * kTermStride + i] = u.term[i];
   }
-  if (write && q.a.logp != nullptr) q.a.logp[r] = lp;
-  if (write && q.a.entropy != nullptr) q.a.entropy[r] = h;
-  if (!LOSS) return o;
-  float term[kTerms] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 1.0f};
-  if (o.live) {
-    const float old = q.a.old_logp[r], adv = q.a.advantages[r];
-    const float ratio = expf(lp - old);
-    const float clipped = fminf(fmaxf(ratio, q.clip_lo), q.clip_hi);
-    const float first = -adv * ratio, second = -adv * clipped;
-    float g = first >= second ? first : first < second ? 0.0f : first + second;  // (NaN goes on)
-    term[0] = first != first || second != second ? first + second : fmaxf(first, second);
-    if (q.a.ref_logp != nullptr) {
-      const float d = q.a.ref_logp[r] - lp, x = expf(d);
-      term[1] = x - d - 1.0f;
-      g += q.kl_coef * (1.0f - x);
-    }
-    term[2] = h;
-    term[3] = ratio != clipped ? 1.0f : 0.0f;
-    term[4] = old - lp;
+  RowCoefs o{scale_for(mine.m, q.c), 0.0f, 0.0f, 0.0f, 0.0f, u.live};
+  o.mc = mine.m * o.c;
+  if (LOSS && u.live) {
     const float inv_n = q.count == 1 ? 1.0f / static_cast<float>(counted) : q.count == 2 ? *q.inv_n : q.given_inv_n;
     const float k = inv_n * q.inv_temp, inv_s = 1.0f / mine.s;
     o.b = k * q.entropy_coef * kLn2 * inv_s;
-    o.a = k * (q.entropy_coef * h - g) * inv_s - o.b * log2_s;
-    o.at = k * g;
+    o.a = k * (q.entropy_coef * u.h - u.g) * inv_s - o.b * u.log2_s;
+    o.at = k * u.g;
   }
-  if (write)
-#pragma unroll
-    for (int i = 0; i < kTerms; ++i) q.terms[r * kTermStride + i] = term[i];
   return o;
 }
 
@@ -293,7 +305,7 @@ struct RowPieces {
 
 // One block of NT threads per row, the whole row in its registers (NT K V >= vocab).
 template <class T, int NT, int K, bool LOSS>
-__global__ __launch_bounds__(NT) void token_row_kernel(const LossKernelArgs q) {
+__global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void token_row_kernel(const LossKernelArgs q) {
   __shared__ RowShared<NT / kWave> sh;
   const ppo_token_loss_args& a = q.a;
   const int64_t r = blockIdx.x;
@@ -318,12 +330,52 @@ __global__ __launch_bounds__(NT) void token_row_kernel(const LossKernelArgs q) {
   else zero_gradient<T, NT>(dx, 0, vocab);
 }
 
-// A few wide rows, which one compute unit each would leave waiting for its arithmetic (131,072 bf16 logits: 10.9 us): a row
-// is cut into parts of kPartThreads kPartPieces pieces, a block each.  token_part_kernel leaves a part's sums; then
-// token_joined_kernel's one wave per row joins them, or each block of token_part_gradient_kernel does before it reads its part
-// again.
+// The means from their sums; the same lane of the first wave holds the sum of the same term.
+__device__ __forceinline__ void write_stats(const LossKernelArgs& q, double sum) {
+  const double rows = __shfl(sum, 5, kWave), n = q.a.denom > 0.0 ? q.a.denom : rows, inv = rows > 0.0 ? 1.0 / n : 0.0;
+  const double s = __shfl(sum, 0, kWave), k = __shfl(sum, 1, kWave), h = __shfl(sum, 2, kWave);
+  if (threadIdx.x < 5) q.a.stats[1 + threadIdx.x] = static_cast<float>(sum * inv);
+  if (threadIdx.x == 5) q.a.stats[0] = static_cast<float>((s + q.a.kl_coef * k - q.a.entropy_coef * h) * inv);
+  if (threadIdx.x == 6) q.a.stats[6] = static_cast<float>(n);
+  if (threadIdx.x == 7) q.a.stats[7] = 0.0f;
+}
+
+// The means over rows, fp64 sums in a fixed order.
+template <int NT>
+__global__ __launch_bounds__(NT) void token_stats_kernel(const LossKernelArgs q) {
+  constexpr int WAVES = NT / kWave;
+  __shared__ double part[kTerms][WAVES];
+  double sum[kTerms] = {};
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < q.a.rows; r += NT) {
+    const float4* t = reinterpret_cast<const float4*>(q.terms + r * kTermStride);
+    const float4 u = t[0], v = t[1];
+    sum[0] += u.x, sum[1] += u.y, sum[2] += u.z, sum[3] += u.w, sum[4] += v.x, sum[5] += v.y;
+  }
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < kTerms; ++i) sum[i] += __shfl_xor(sum[i], d, kWave);
+  if (threadIdx.x % kWave == 0)
+#pragma unroll
+    for (int i = 0; i < kTerms; ++i) part[i][threadIdx.x / kWave] = sum[i];
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  double all = 0.0;  // lane i: term i
+  if (threadIdx.x < kTerms)
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all += part[threadIdx.x][w];
+  write_stats(q, all);
+}
+
+// A few wide rows, which one compute unit each would leave waiting for its arithmetic: a row is cut into parts of
+// kPartThreads kPartPieces pieces, a block each.  token_part_kernel leaves a part's sums; then token_joined_kernel's one wave
+// per row joins them, or each block of token_part_gradient_kernel does before it reads its part again, and one more block the
+// means of all rows.  Worth it (us a call, in one kernel -> in parts) for the loss of up to kSplitLossRows = a wave's lanes of rows
+// from 40,000 logits on (8 x 50,021 bf16 18.8 -> 15.0, 64 x 131,072 27.0 -> 19.7; 8 x 32,000 fp32 13.5 -> 14.3), for log-probabilities
+// of up to kSplitRows from 65,536 on (8 x 131,072 bf16 10.8 -> 9.3, 257 23.3 -> 16.2, 512 fp32 42.8 -> 43.0; 8 x 50,021 8.5 -> 9.4).
 constexpr int kPartThreads = 256, kPartPieces = 4, kMaxParts = kWave;
-constexpr int64_t kSplitRows = 128, kSplitPieces = 2 * kPartThreads * kPartPieces;
+constexpr int64_t kSplitRows = 256, kSplitVocab = 65536, kSplitLossRows = kWave, kSplitLossVocab = 40000;
 
 struct RowPart {
   RowSums sums;
@@ -371,6 +423,27 @@ __global__ __launch_bounds__(kWave) void token_joined_kernel(const LossKernelArg
   finish_row<kWave, false>(q, r, join_parts(parts + r * n, n, q.c), parts[r * n].x_tok, 0, sh, threadIdx.x == 0);
 }
 
+// The means, a lane per row (rows <= kSplitLossRows).
+__device__ __forceinline__ void part_stats(const LossKernelArgs& q, const RowPart* parts, int n) {
+  const int64_t r = threadIdx.x;
+  int64_t tok;
+  RowTerms u{};
+  if (r < q.a.rows && row_counts(q.a, r, tok)) {
+    const RowPart* row = parts + r * n;
+    RowSums sums = row[0].sums;
+#pragma unroll 4
+    for (int i = 1; i < n; ++i) sums = join(sums, row[i].sums, q.c);
+    u = row_terms<true>(q, r, sums, row[0].x_tok);
+  }
+  double mine = 0.0;  // lane i: term i
+#pragma unroll
+  for (int i = 0; i < kTerms; ++i) {
+    const double x = wave_sum(static_cast<double>(u.term[i]));
+    if (static_cast<int>(threadIdx.x) == i) mine = x;
+  }
+  write_stats(q, mine);
+}
+
 template <class T>
 __global__ __launch_bounds__(kPartThreads) void token_part_gradient_kernel(const LossKernelArgs q, const RowPart* __restrict__ parts) {
   constexpr int kPart = kPartThreads * kPartPieces * kVec<T>;
@@ -378,6 +451,10 @@ __global__ __launch_bounds__(kPartThreads) void token_part_gradient_kernel(const
   const ppo_token_loss_args& a = q.a;
   const int64_t r = blockIdx.y;
   const int vocab = static_cast<int>(a.vocab), first = blockIdx.x * kPart, n = gridDim.x;
+  if (r == a.rows) {
+    if (first == 0 && threadIdx.x < kWave) part_stats(q, parts, n);
+    return;
+  }
   const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
   T* dx = a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
   if (dx == nullptr && first > 0) return;
@@ -467,59 +544,39 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
   }
 }
 
-// The means over rows, fp64 sums in a fixed order.
-__global__ __launch_bounds__(kStatsThreads) void token_stats_kernel(const LossKernelArgs q) {
-  __shared__ double part[kTerms][kStatsThreads / kWave];
-  double sum[kTerms] = {};
-#pragma unroll 4
-  for (int64_t r = threadIdx.x; r < q.a.rows; r += kStatsThreads) {
-    const float4* t = reinterpret_cast<const float4*>(q.terms + r * kTermStride);
-    const float4 u = t[0], v = t[1];
-    sum[0] += u.x, sum[1] += u.y, sum[2] += u.z, sum[3] += u.w, sum[4] += v.x, sum[5] += v.y;
-  }
-#pragma unroll
-  for (int i = 0; i < kTerms; ++i) {
-    const double x = wave_sum(sum[i]);
-    if (threadIdx.x % kWave == 0) part[i][threadIdx.x / kWave] = x;
-  }
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int i = 0; i < kTerms; ++i) {
-    sum[i] = 0.0;
-    for (int w = 0; w < kStatsThreads / kWave; ++w) sum[i] += part[i][w];
-  }
-  const double n = q.a.denom > 0.0 ? q.a.denom : sum[5], inv = sum[5] > 0.0 ? 1.0 / n : 0.0;
-  for (int i = 0; i < 5; ++i) q.a.stats[1 + i] = static_cast<float>(sum[i] * inv);
-  q.a.stats[0] = static_cast<float>((sum[0] + q.a.kl_coef * sum[1] - q.a.entropy_coef * sum[2]) * inv);
-  q.a.stats[6] = static_cast<float>(n);
-  q.a.stats[7] = 0.0f;
-}
-
 template <class T, bool LOSS>
 int launch_rows(const LossKernelArgs& q, RowPart* parts, hipStream_t st) {
-  const int64_t pieces = ceil_div(q.a.vocab, kVec<T>);
-  const dim3 grid(static_cast<uint32_t>(q.a.rows));
-  const int64_t n = ceil_div(pieces, kPartThreads * kPartPieces);
-  if (q.a.rows <= kSplitRows && pieces >= kSplitPieces && n <= kMaxParts) {
-    const dim3 split(static_cast<uint32_t>(n), static_cast<uint32_t>(q.a.rows));
+  const int64_t rows = q.a.rows, vocab = q.a.vocab, pieces = ceil_div(vocab, kVec<T>), n = ceil_div(pieces, kPartThreads * kPartPieces);
+  const dim3 grid(static_cast<uint32_t>(rows));
+  if (rows <= (LOSS ? kSplitLossRows : kSplitRows) && vocab >= (LOSS ? kSplitLossVocab : kSplitVocab) && n <= kMaxParts) {
+    const dim3 split(static_cast<uint32_t>(n), static_cast<uint32_t>(rows));
     hipLaunchKernelGGL(token_part_kernel<T>, split, dim3(kPartThreads), 0, st, q, parts);
     if (int rc = check_launch("token_part_kernel")) return rc;
-    if (LOSS) hipLaunchKernelGGL(token_part_gradient_kernel<T>, split, dim3(kPartThreads), 0, st, q, parts);
-    else hipLaunchKernelGGL(token_joined_kernel, grid, dim3(kWave), 0, st, q, parts, static_cast<int>(n));
-    return check_launch("token_part_gradient_kernel");
+    if (LOSS) {
+      hipLaunchKernelGGL(token_part_gradient_kernel<T>, dim3(split.x, split.y + 1), dim3(kPartThreads), 0, st, q, parts);
+      return check_launch("token_part_gradient_kernel");
+    }
+    hipLaunchKernelGGL(token_joined_kernel, grid, dim3(kWave), 0, st, q, parts, static_cast<int>(n));
+    return check_launch("token_joined_kernel");
   }
+  // As few threads to a row as hold it, so that a compute unit has several rows in different phases.
 #define PPO_ROWS(NT, K) hipLaunchKernelGGL((token_row_kernel<T, NT, K, LOSS>), grid, dim3(NT), 0, st, q)
-  if (q.a.vocab < kVec<T> || pieces > 16 * 1024)
+  if (vocab < kVec<T> || pieces > 1024 * 16)
     hipLaunchKernelGGL((token_wide_kernel<T, LOSS>), grid, dim3(kWideThreads), 0, st, q);
   else if (pieces <= 64) PPO_ROWS(64, 1);
-  else if (pieces <= 256) PPO_ROWS(64, 4);
-  else if (pieces <= 1024) PPO_ROWS(256, 4);
-  else if (pieces <= 2048) PPO_ROWS(256, 8);
-  else if (pieces <= 4096) PPO_ROWS(256, 16);
-  else if (pieces <= 8192) PPO_ROWS(512, 16);
+  else if (pieces <= 64 * 4) PPO_ROWS(64, 4);
+  else if (pieces <= 256 * 4) PPO_ROWS(256, 4);
+  else if (pieces <= 256 * 8) PPO_ROWS(256, 8);
+  else if (pieces <= 256 * 16) PPO_ROWS(256, 16);
+  else if (pieces <= 512 * 16) PPO_ROWS(512, 16);
+  else if (pieces <= 512 * 25) PPO_ROWS(512, 25);
   else PPO_ROWS(1024, 16);
 #undef PPO_ROWS
-  return check_launch("token_row_kernel");
+  if (int rc = check_launch("token_row_kernel")) return rc;
+  if (!LOSS) return PPO_OK;
+  if (rows <= 1024) hipLaunchKernelGGL(token_stats_kernel<256>, dim3(1), dim3(256), 0, st, q);
+  else hipLaunchKernelGGL(token_stats_kernel<1024>, dim3(1), dim3(1024), 0, st, q);
+  return check_launch("token_stats_kernel");
 }
 
 struct Layout {
@@ -577,7 +634,7 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
   q.kl_coef = static_cast<float>(a.kl_coef);
   q.entropy_coef = static_cast<float>(a.entropy_coef);
   if (q.count == 2) {
-    hipLaunchKernelGGL(token_count_kernel, dim3(1), dim3(kStatsThreads), 0, st, q);
+    hipLaunchKernelGGL(token_count_kernel, dim3(1), dim3(kCountThreads), 0, st, q);
     if (int rc = check_launch("token_count_kernel")) return rc;
   }
   if (a.rows > 0) {
@@ -586,10 +643,9 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
       using T = decltype(t);
       rc = loss ? launch_rows<T, true>(q, parts, st) : launch_rows<T, false>(q, parts, st);
     });
-    if (rc != PPO_OK) return rc;
+    return rc;
   }
-  if (!loss) return PPO_OK;
-  hipLaunchKernelGGL(token_stats_kernel, dim3(1), dim3(kStatsThreads), 0, st, q);
+  hipLaunchKernelGGL(token_stats_kernel<256>, dim3(1), dim3(256), 0, st, q);  // no rows: zeros
   return check_launch("token_stats_kernel");
 }
 

@@ -1048,15 +1048,15 @@ ELEMENT_TYPES = {torch.float32: L.TYPE_F32, torch.bfloat16: L.TYPE_BF16, torch.f
 TOKEN_TYPES = {torch.int64: L.TOKENS_I64, torch.int32: L.TOKENS_I32}
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _current_gpu(name: str, *tensors: torch.Tensor | None) -> int:
     """The current GPU's index; every tensor must be on it: the kernels are enqueued on its current stream."""
+    dev = _get_device() if tensors[0].is_cuda else -1
     for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise ValueError(f"{name}: GPU tensors only (no CPU path exists)")
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{name}: tensors must be on the current GPU ({dev}), got one on {t.device}")
+        if t is not None and (t.get_device() != dev or dev < 0):
+            raise ValueError(f"{name}: tensors must be on the current GPU ({dev}), got one on {t.device} (no CPU path exists)")
     return dev
 
 
@@ -1067,19 +1067,22 @@ def _element_type(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _matrix(t: torch.Tensor, name: str) -> int:
-    """Leading dimension of a [rows, columns] view of unit column stride whose rows do not overlap."""
+def _matrix(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """Rows, columns and leading dimension of a view of unit column stride whose rows do not overlap."""
     if t.dim() != 2:
         raise ValueError(f"{name} must be a matrix, got shape {tuple(t.shape)}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+    if t.is_contiguous():
+        return rows, cols, cols
+    ld, unit = t.stride()
+    if cols > 1 and unit != 1 or rows > 1 and ld < cols:
         raise ValueError(f"{name} must have unit column stride and rows apart, got strides {t.stride()}")
-    return max(t.stride(0), cols) if rows > 1 else cols
+    return rows, cols, ld if rows > 1 else cols
 
 
-def _vector(t: torch.Tensor | None, name: str, n: int, dtype: torch.dtype) -> int | None:
+def _vector(t: torch.Tensor | None, name: str, n: int, dtype: torch.dtype = torch.float32) -> int:
     if t is None:
-        return None
+        return 0
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {dtype} of {n} elements, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
@@ -1102,13 +1105,12 @@ def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor, 
     row-major views."""
     dev = _current_gpu("embedding_fwd", tokens, table, out)
     token_type, elem = _tokens(tokens, "embedding_fwd"), _element_type(table, "embedding_fwd: table")
-    ld_src, ld_dst = _matrix(table, "table"), _matrix(out, "out")
-    n, (vocab, dim) = tokens.numel(), table.shape
-    if out.dtype != table.dtype or tuple(out.shape) != (n, dim):
-        raise ValueError(f"embedding_fwd: out must be {table.dtype} [{n}, {dim}], got {out.dtype} {tuple(out.shape)}")
-    args = L.EmbeddingArgs(tokens.data_ptr(), table.data_ptr(), ld_src, out.data_ptr(), ld_dst, n, vocab, dim, token_type,
-                           elem, elem, float(scale), 0)
-    L.call("ppo_embedding_fwd", C_ref(args), _raw_stream(dev))
+    vocab, dim, ld_src = _matrix(table, "table")
+    rows, cols, ld_dst = _matrix(out, "out")
+    if out.dtype != table.dtype or rows != tokens.numel() or cols != dim:
+        raise ValueError(f"embedding_fwd: out must be {table.dtype} [{tokens.numel()}, {dim}], got {out.dtype} {tuple(out.shape)}")
+    L.call("ppo_embedding_fwd", L.EMBEDDING_ARGS.pack(tokens.data_ptr(), table.data_ptr(), ld_src, out.data_ptr(), ld_dst, rows,
+                                                      vocab, dim, token_type, elem, elem, scale, 0), _raw_stream(dev))
 
 
 def embedding_bwd(tokens: torch.Tensor, d_out: torch.Tensor, d_table: torch.Tensor, scale: float = 1.0,
@@ -1119,30 +1121,27 @@ def embedding_bwd(tokens: torch.Tensor, d_out: torch.Tensor, d_table: torch.Tens
     dev = _current_gpu("embedding_bwd", tokens, d_out, d_table)
     token_type = _tokens(tokens, "embedding_bwd")
     src_type, dst_type = _element_type(d_out, "embedding_bwd: d_out"), _element_type(d_table, "embedding_bwd: d_table")
-    ld_src, ld_dst = _matrix(d_out, "d_out"), _matrix(d_table, "d_table")
-    n, (vocab, dim) = tokens.numel(), d_table.shape
-    if tuple(d_out.shape) != (n, dim):
-        raise ValueError(f"embedding_bwd: d_out must be [{n}, {dim}], got {tuple(d_out.shape)}")
-    nbytes = L.load().ppo_embedding_bwd_workspace_bytes(n, vocab, dim)
-    buf = _scratch(ws, d_table.device, nbytes)
-    args = L.EmbeddingArgs(tokens.data_ptr(), d_out.data_ptr(), ld_src, d_table.data_ptr(), ld_dst, n, vocab, dim, token_type,
-                           src_type, dst_type, float(scale), int(accumulate))
-    L.call("ppo_embedding_bwd", C_ref(args), buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    n, cols, ld_src = _matrix(d_out, "d_out")
+    vocab, dim, ld_dst = _matrix(d_table, "d_table")
+    if n != tokens.numel() or cols != dim:
+        raise ValueError(f"embedding_bwd: d_out must be [{tokens.numel()}, {dim}], got {tuple(d_out.shape)}")
+    buf = _scratch(ws, d_table.device, L.load().ppo_embedding_bwd_workspace_bytes(n, vocab, dim))
+    L.call("ppo_embedding_bwd", L.EMBEDDING_ARGS.pack(tokens.data_ptr(), d_out.data_ptr(), ld_src, d_table.data_ptr(), ld_dst, n,
+                                                      vocab, dim, token_type, src_type, dst_type, scale, bool(accumulate)),
+           buf.data_ptr(), buf.numel(), _raw_stream(dev))
 
 
-def _token_args(name: str, logits, tokens, logp, entropy, mask, temperature) -> tuple["L.TokenLossArgs", int]:
-    dev = _current_gpu(name, logits, tokens, logp, entropy, mask)
-    ld = _matrix(logits, f"{name}: logits")
-    rows, vocab = logits.shape
-    elem, token_type = _element_type(logits, f"{name}: logits"), _tokens(tokens, name)
+def _logits_of(name: str, logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None) -> tuple:
+    """(rows, vocab, leading dimension, element type, token type, mask pointer), checked."""
+    rows, vocab, ld = _matrix(logits, f"{name}: logits")
     if tokens.numel() != rows:
         raise ValueError(f"{name}: {tokens.numel()} tokens for {rows} rows of logits")
-    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != rows or not mask.is_contiguous()):
-        raise ValueError(f"{name}: mask must be contiguous bool or uint8 of {rows} elements, got {mask.dtype} {tuple(mask.shape)}")
-    return L.TokenLossArgs(logits=logits.data_ptr(), ld_logits=ld, tokens=tokens.data_ptr(), mask=_ptr(mask),
-                           logp=_vector(logp, f"{name}: logp", rows, torch.float32),
-                           entropy=_vector(entropy, f"{name}: entropy", rows, torch.float32), rows=rows, vocab=vocab,
-                           temperature=float(temperature), type=elem, token_type=token_type), dev
+    kept = 0
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != rows or not mask.is_contiguous():
+            raise ValueError(f"{name}: mask must be contiguous bool or uint8 of {rows} elements, got {mask.dtype} {tuple(mask.shape)}")
+        kept = mask.data_ptr()
+    return rows, vocab, ld, _element_type(logits, f"{name}: logits"), _tokens(tokens, name), kept
 
 
 def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor | None, entropy: torch.Tensor | None = None,
@@ -1150,10 +1149,14 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, logp: torch.Tens
     """logp[r] = the log-probability of tokens[r] under softmax(logits[r] / temperature), entropy[r] that distribution's
     entropy (float32, either may be None).  logits [rows, vocab] float32, bfloat16 or float16.  Rows whose mask (bool or
     uint8) is 0 or whose token is outside [0, vocab) are not read and give 0."""
-    args, dev = _token_args("token_log_probs", logits, tokens, logp, entropy, mask, temperature)
-    nbytes = L.load().ppo_token_loss_workspace_bytes(args.rows, args.vocab)
-    buf = _scratch(ws, logits.device, nbytes)
-    L.call("ppo_token_log_probs", C_ref(args), buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    name = "token_log_probs"
+    dev = _current_gpu(name, logits, tokens, logp, entropy, mask)
+    rows, vocab, ld, elem, token_type, kept = _logits_of(name, logits, tokens, mask)
+    args = L.TOKEN_LOSS_ARGS.pack(logits.data_ptr(), ld, tokens.data_ptr(), kept, 0, 0, 0, 0, 0, _vector(logp, f"{name}: logp", rows),
+                                  _vector(entropy, f"{name}: entropy", rows), 0, rows, vocab, 0.0, 0.0, 0.0, 0.0, temperature, 0.0,
+                                  elem, token_type)
+    buf = _scratch(ws, logits.device, L.load().ppo_token_loss_workspace_bytes(rows, vocab))
+    L.call("ppo_token_log_probs", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
 
 
 def token_ppo_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
@@ -1167,27 +1170,25 @@ def token_ppo_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.T
     stats[8] float32 = loss, surrogate, KL, entropy, the share of clipped rows, mean old_logp - logp, rows, 0.
     d_logits: like logits (may be logits itself), or None.  denom: divides the sums instead of the number of rows that
     count, for calls that share one mean."""
-    args, dev = _token_args("token_ppo_loss", logits, tokens, logp, entropy, mask, temperature)
-    _current_gpu("token_ppo_loss", old_logp, advantages, ref_logp, d_logits, stats)
-    rows = args.rows
-    args.old_logp = _vector(old_logp, "token_ppo_loss: old_logp", rows, torch.float32)
-    args.advantages = _vector(advantages, "token_ppo_loss: advantages", rows, torch.float32)
-    args.ref_logp = _vector(ref_logp, "token_ppo_loss: ref_logp", rows, torch.float32)
-    args.stats = _vector(stats, "token_ppo_loss: stats", 8, torch.float32)
+    name = "token_ppo_loss"
+    dev = _current_gpu(name, logits, tokens, old_logp, advantages, ref_logp, d_logits, stats, logp, entropy, mask)
+    rows, vocab, ld, elem, token_type, kept = _logits_of(name, logits, tokens, mask)
+    d_ptr = d_ld = 0
     if d_logits is not None:
         if d_logits.dtype != logits.dtype or d_logits.shape != logits.shape:
-            raise ValueError(f"token_ppo_loss: d_logits must be {logits.dtype} {tuple(logits.shape)}, got {d_logits.dtype} "
+            raise ValueError(f"{name}: d_logits must be {logits.dtype} {tuple(logits.shape)}, got {d_logits.dtype} "
                              f"{tuple(d_logits.shape)}")
-        args.d_logits, args.ld_d_logits = d_logits.data_ptr(), _matrix(d_logits, "token_ppo_loss: d_logits")
-    args.clip_low, args.clip_high = clip_param if isinstance(clip_param, (tuple, list)) else (clip_param, clip_param)
-    args.kl_coef, args.entropy_coef = float(kl_coef), float(entropy_coef)
-    if denom is not None:
-        if not denom > 0:
-            raise ValueError(f"token_ppo_loss: denom must be positive, got {denom}")
-        args.denom = float(denom)
-    nbytes = L.load().ppo_token_loss_workspace_bytes(rows, args.vocab)
-    buf = _scratch(ws, logits.device, nbytes)
-    L.call("ppo_token_ppo_loss", C_ref(args), buf.data_ptr(), buf.numel(), _raw_stream(dev))
+        d_ptr, d_ld = d_logits.data_ptr(), _matrix(d_logits, f"{name}: d_logits")[2]
+    if denom is not None and not denom > 0:
+        raise ValueError(f"{name}: denom must be positive, got {denom}")
+    low, high = clip_param if isinstance(clip_param, (tuple, list)) else (clip_param, clip_param)
+    args = L.TOKEN_LOSS_ARGS.pack(
+        logits.data_ptr(), ld, tokens.data_ptr(), kept, _vector(old_logp, f"{name}: old_logp", rows),
+        _vector(ref_logp, f"{name}: ref_logp", rows), _vector(advantages, f"{name}: advantages", rows), d_ptr, d_ld,
+        _vector(logp, f"{name}: logp", rows), _vector(entropy, f"{name}: entropy", rows), _vector(stats, f"{name}: stats", 8), rows,
+        vocab, low, high, kl_coef, entropy_coef, temperature, 0.0 if denom is None else denom, elem, token_type)
+    buf = _scratch(ws, logits.device, L.load().ppo_token_loss_workspace_bytes(rows, vocab))
+    L.call("ppo_token_ppo_loss", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
 
 
 def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step: int, lr, beta1: float = 0.9,
@@ -1201,13 +1202,11 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step:
     [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  lr, weight_decay: one value, or one per tensor.
     step counts from 1.  norm_out: float32 [2] for the norm and the clip coefficient."""
     n = len(params)
-    lists = [("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)]
-    lists += [("masters", masters)] if masters is not None else []
-    lists += [("scales", scales[0]), ("scales", scales[1])] if scales is not None else []
-    lists += [("lr", lr)] if isinstance(lr, (list, tuple)) else []
-    lists += [("weight_decay", weight_decay)] if isinstance(weight_decay, (list, tuple)) else []
-    for name, v in lists:
-        if len(v) != n:
+    each_lr, each_wd = isinstance(lr, (list, tuple)), isinstance(weight_decay, (list, tuple))
+    for name, v in (("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("masters", masters),
+                    ("scales", scales and scales[0]), ("scales", scales and scales[1]), ("lr", lr if each_lr else None),
+                    ("weight_decay", weight_decay if each_wd else None)):
+        if v is not None and len(v) != n:
             raise ValueError(f"adamw_step: {len(v)} {name} for {n} params")
     if step < 1:
         raise ValueError(f"adamw_step: step={step} (the first is 1)")
@@ -1216,40 +1215,42 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step:
     if n == 0:
         return
     dev = _current_gpu("adamw_step", params[0], norm_out)
-    f32, bf16 = torch.float32, torch.bfloat16
-    each_lr, each_wd = isinstance(lr, (list, tuple)), isinstance(weight_decay, (list, tuple))
-    pack, items = L.ADAMW_TENSOR.pack, []
+    T, f32, bf16 = torch.Tensor, torch.float32, torch.bfloat16
+    counts = [t.numel() for t in params]
+    columns = []  # each list's pointers, in AdamwTensor's order, checked (through map: a call of Python's own per tensor costs more than the check)
+    for name, ts, sizes in (("params", params, counts), ("grads", grads, counts), ("masters", masters, counts),
+                            ("exp_avg", exp_avg, counts), ("exp_avg_sq", exp_avg_sq, counts), ("scales", scales and scales[0], None), ("scales", scales and scales[1], None)):
+        if ts is None:
+            columns.append([0] * n)
+            continue
+        if name == "masters" and None in ts or sizes is None:  # lists that need not hold a tensor for each parameter
+            columns.append([0 if t is None else t.data_ptr() for t in ts])
+            sizes = sizes or [-(-c // L.ADAMW_BLOCK) for c in counts]
+            ts, sizes = zip(*[(t, c) for t, c in zip(ts, sizes) if t is not None]) if any(t is not None for t in ts) else ((), ())
+        else:
+            columns.append(list(map(T.data_ptr, ts)))
+        if not (all(map(T.is_contiguous, ts)) and set(map(T.get_device, ts)) <= {dev} and list(map(T.numel, ts)) == list(sizes)):
+            raise ValueError(f"adamw_step: {name} must be contiguous tensors of the parameters' sizes (scales: a value for each "
+                             f"{L.ADAMW_BLOCK} elements) on GPU {dev}, got {[(tuple(t.shape), t.stride(), str(t.device)) for t in ts]}")
+    kinds = []
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avg, exp_avg_sq)):
-        count, ptype, gtype, bits = p.numel(), p.dtype, g.dtype, 32
-        master = ms = vs = 0
-        if not (p.get_device() == g.get_device() == m.get_device() == v.get_device() == dev and p.is_contiguous() and
-                g.is_contiguous() and m.is_contiguous() and v.is_contiguous() and
-                g.numel() == m.numel() == v.numel() == count):
-            raise ValueError(f"adamw_step: parameter {i}, its gradient and states must be contiguous, of one size, on GPU {dev}: "
-                             f"got {[(tuple(t.shape), t.stride(), str(t.device)) for t in (p, g, m, v)]}")
+        ptype, gtype, mtype, vtype = p.dtype, g.dtype, m.dtype, v.dtype
         if (ptype != f32 and ptype != bf16) or (gtype != f32 and gtype != ptype):
             raise ValueError(f"adamw_step: tensor {i}: parameter {ptype}, gradient {gtype}")
-        if masters is not None and masters[i] is not None:
-            t = masters[i]
-            if t.dtype != f32 or ptype != bf16 or t.get_device() != dev or t.numel() != count or not t.is_contiguous():
-                raise ValueError(f"adamw_step: masters[{i}] must be contiguous float32 of a bfloat16 parameter's size")
-            master = t.data_ptr()
-        if m.dtype != f32 or v.dtype != f32:
-            if m.dtype != torch.int8 or v.dtype != torch.uint8 or scales is None:
-                raise ValueError(f"adamw_step: tensor {i}: states {m.dtype}, {v.dtype} (float32, or int8 and uint8 with scales)")
-            bits, blocks = 8, -(-count // L.ADAMW_BLOCK)
-            for t in (scales[0][i], scales[1][i]):
-                if t.get_device() != dev or t.dtype != f32 or t.numel() != blocks or not t.is_contiguous():
-                    raise ValueError(f"adamw_step: scales of tensor {i} must be contiguous float32 of {blocks} elements")
-            ms, vs = scales[0][i].data_ptr(), scales[1][i].data_ptr()
-        items.append(pack(p.data_ptr(), g.data_ptr(), master, m.data_ptr(), v.data_ptr(), ms, vs, count,
-                          lr[i] if each_lr else lr, weight_decay[i] if each_wd else weight_decay,
-                          L.TYPE_F32 if ptype == f32 else L.TYPE_BF16, L.TYPE_F32 if gtype == f32 else L.TYPE_BF16, bits, 0))
-    packed = b"".join(items)
+        if columns[2][i] and (masters[i].dtype != f32 or ptype != bf16):
+            raise ValueError(f"adamw_step: masters[{i}] must be float32, of a bfloat16 parameter")
+        bits = 32
+        if mtype != f32 or vtype != f32:
+            bits = 8
+            if (mtype != torch.int8 or vtype != torch.uint8 or scales is None or scales[0][i] is None or scales[1][i] is None
+                    or scales[0][i].dtype != f32 or scales[1][i].dtype != f32):
+                raise ValueError(f"adamw_step: tensor {i}: states {mtype}, {vtype} (float32, or int8 and uint8 with float32 scales)")
+        kinds.append((L.TYPE_F32 if ptype == f32 else L.TYPE_BF16, L.TYPE_F32 if gtype == f32 else L.TYPE_BF16, bits, 0))
+    packed = b"".join(map(L.ADAMW_TENSOR.pack, *columns, counts, lr if each_lr else [lr] * n,
+                          weight_decay if each_wd else [weight_decay] * n, *zip(*kinds)))
     buf = None
     if max_grad_norm is not None or norm_out is not None:
-        if norm_out is not None:
-            _vector(norm_out, "adamw_step: norm_out", 2, f32)
+        _vector(norm_out, "adamw_step: norm_out", 2)
         buf = _scratch(ws, params[0].device, L.load().ppo_adamw_workspace_bytes(packed, n))
     L.call("ppo_adamw_step", packed, n, float(max_grad_norm or 0.0), float(beta1), float(beta2), float(eps),
            1.0 - beta1**step, math.sqrt(1.0 - beta2**step), _ptr(norm_out), _ptr(buf), 0 if buf is None else buf.numel(),
