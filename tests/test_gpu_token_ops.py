@@ -120,6 +120,25 @@ def test_embedding_gradient(cuda, dtype, out, count, vocab, dim):
     assert torch.equal(got, again), "the same call gives the same bits"
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dim,most", [(24, 2000), (1100, 6000), (1100, 60000), (4100, 40000)])
+def test_embedding_gradient_of_runs(cuda, dim, most, accumulate):
+    """Tokens that occur 0, 1, 7, 8, 9, ... times, so that runs of the sorted tokens end on, before and behind every boundary the
+    kernels cut them at; small whole numbers, whose sums are exact in fp32."""
+    ops, g = _ops(), _gen(dim + most)
+    lens = torch.tensor([0, 1, 2, 3, 7, 8, 9, 10, 15, 16, 17, 23, 24, 25, 31, 32, 33, 39, 40, 41, 64, 300, 900])
+    lens = lens[torch.randint(0, len(lens), (4000,), generator=g)]
+    lens = lens[: int((lens.cumsum(0) <= most).sum())]
+    tok = torch.repeat_interleave(torch.arange(len(lens)), lens)
+    tok = tok[torch.randperm(len(tok), generator=g)]
+    d = torch.randint(-3, 4, (len(tok), dim), generator=g).to(BF16)
+    start = torch.randint(-3, 4, (len(lens), dim), generator=g).float()
+    got = start.to(cuda)
+    ops.embedding_bwd(tok.to(cuda), d.to(cuda), got, scale=2.0, accumulate=accumulate)
+    want = torch.zeros(len(lens), dim).index_add(0, tok, d.float()) * 2.0 + (start if accumulate else 0.0)
+    assert torch.equal(got.cpu(), want)
+
+
 @pytest.mark.parametrize("count,vocab,dim,out", [(1, 4, 3, F32), (700, 90, 37, BF16), (9001, 40, 130, F32)])
 def test_embedding_gradient_accumulates(cuda, count, vocab, dim, out):
     ops = _ops()

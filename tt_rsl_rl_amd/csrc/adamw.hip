@@ -79,11 +79,14 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
 }
 
 // Four elements from p, those past n as zeros.
-template <class T>
+template <bool STREAM, class T>
 __device__ __forceinline__ void load4(const T* p, int n, float (&x)[kPer]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   if (n >= kPer) {
-    const vec v = *reinterpret_cast<const vec*>(p);
+    const vec* q = reinterpret_cast<const vec*>(p);
+    vec v;
+    if constexpr (STREAM) v = __builtin_nontemporal_load(q);
+    else v = *q;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = static_cast<float>(v[i]);
   } else {
@@ -92,14 +95,15 @@ __device__ __forceinline__ void load4(const T* p, int n, float (&x)[kPer]) {
   }
 }
 
-template <class T>
+template <bool STREAM, class T>
 __device__ __forceinline__ void store4(T* p, int n, const float (&x)[kPer]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   if (n >= kPer) {
     vec v;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[i] = static_cast<T>(x[i]);
-    *reinterpret_cast<vec*>(p) = v;
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+    else *reinterpret_cast<vec*>(p) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
@@ -213,7 +217,7 @@ __device__ __forceinline__ void codes(const float (&x)[kPer], float scale, float
   for (int e = 0; e < kPer; ++e) q[e] = fminf(fmaxf(q[e], 0.0f), kTop);  // (NaN becomes 0)
 }
 
-template <class P, class G, bool MASTER, bool BITS8>
+template <class P, class G, bool MASTER, bool BITS8, bool STREAM>
 __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const UpdateTable t, const Scalars s,
                                                                      const float* __restrict__ coef) {
   const int k = tensor_of(t.first, t.tensors, blockIdx.x);
@@ -224,15 +228,15 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
   if (!BITS8 && n == 0) return;
   const float c = coef != nullptr ? *coef : 1.0f;
   float g[kPer], p[kPer], m[kPer], v[kPer];
-  load4(static_cast<const G*>(q.grad) + i, n, g);
-  if constexpr (MASTER) load4(q.master + i, n, p);
-  else load4(static_cast<const P*>(q.param) + i, n, p);
+  load4<STREAM>(static_cast<const G*>(q.grad) + i, n, g);
+  if constexpr (MASTER) load4<STREAM>(q.master + i, n, p);
+  else load4<STREAM>(static_cast<const P*>(q.param) + i, n, p);
   const int64_t block = i / PPO_ADAMW_BLOCK;
   if constexpr (BITS8) {
     const bool some = block * PPO_ADAMW_BLOCK < count;  // (of the wave's block)
     const float ms = some ? q.m_scale[block] : 0.0f, vs = some ? q.v_scale[block] : 0.0f;
-    load4(static_cast<const int8_t*>(q.m) + i, n, m);
-    load4(static_cast<const uint8_t*>(q.v) + i, n, v);
+    load4<STREAM>(static_cast<const int8_t*>(q.m) + i, n, m);
+    load4<STREAM>(static_cast<const uint8_t*>(q.v) + i, n, v);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const float a = fabsf(m[e]) * (1.0f / 127.0f), b = v[e] * (1.0f / 255.0f);
@@ -241,8 +245,8 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
       v[e] = vs * (b2 * b2);
     }
   } else {
-    load4(static_cast<const float*>(q.m) + i, n, m);
-    load4(static_cast<const float*>(q.v) + i, n, v);
+    load4<STREAM>(static_cast<const float*>(q.m) + i, n, m);
+    load4<STREAM>(static_cast<const float*>(q.v) + i, n, v);
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
@@ -271,18 +275,18 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
       if (v[e] > 0.0f) qv[e] = fmaxf(qv[e], 1.0f);
     }
     if (n == 0) return;
-    store4(static_cast<int8_t*>(q.m) + i, n, qm);
-    store4(static_cast<uint8_t*>(q.v) + i, n, qv);
+    store4<STREAM>(static_cast<int8_t*>(q.m) + i, n, qm);
+    store4<STREAM>(static_cast<uint8_t*>(q.v) + i, n, qv);
     if (threadIdx.x % kWave == 0) {
       q.m_scale[block] = ms;
       q.v_scale[block] = vs;
     }
   } else {
-    store4(static_cast<float*>(q.m) + i, n, m);
-    store4(static_cast<float*>(q.v) + i, n, v);
+    store4<STREAM>(static_cast<float*>(q.m) + i, n, m);
+    store4<STREAM>(static_cast<float*>(q.v) + i, n, v);
   }
-  if constexpr (MASTER) store4(q.master + i, n, p);
-  store4(static_cast<P*>(q.param) + i, n, p);
+  if constexpr (MASTER) store4<STREAM>(q.master + i, n, p);
+  store4<STREAM>(static_cast<P*>(q.param) + i, n, p);
 }
 
 int64_t chunks_of(const ppo_adamw_tensor& t) { return ceil_div(t.count, kChunk); }
@@ -293,11 +297,14 @@ int64_t norm_partials(const ppo_adamw_tensor* tensors, int32_t count) {
 }
 
 template <class P, class G, bool MASTER>
-void launch_update(bool bits8, int chunks, hipStream_t st, const UpdateTable& t, const Scalars& s, const float* coef) {
-  if (bits8)
-    hipLaunchKernelGGL((adamw_update_kernel<P, G, MASTER, true>), dim3(chunks), dim3(kAdamwThreads), 0, st, t, s, coef);
-  else
-    hipLaunchKernelGGL((adamw_update_kernel<P, G, MASTER, false>), dim3(chunks), dim3(kAdamwThreads), 0, st, t, s, coef);
+void launch_update(bool bits8, bool stream, int chunks, hipStream_t st, const UpdateTable& t, const Scalars& s, const float* coef) {
+#define PPO_UPDATE(BITS8, STREAM) \
+  hipLaunchKernelGGL((adamw_update_kernel<P, G, MASTER, BITS8, STREAM>), dim3(chunks), dim3(kAdamwThreads), 0, st, t, s, coef)
+  if (bits8 && stream) PPO_UPDATE(true, true);
+  else if (bits8) PPO_UPDATE(true, false);
+  else if (stream) PPO_UPDATE(false, true);
+  else PPO_UPDATE(false, false);
+#undef PPO_UPDATE
 }
 
 // The kinds a launch holds together: bit 0 bf16 param, bit 1 bf16 gradient, bit 2 master, bit 3 8-bit states.
@@ -383,6 +390,12 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
   }
   const Scalars s{static_cast<float>(1.0 - beta1), static_cast<float>(beta2), static_cast<float>(1.0 - beta2),
                   static_cast<float>(eps), static_cast<float>(bc2_sqrt), static_cast<float>(1.0 / bc2_sqrt)};
+  int64_t bytes = 0;
+  for (int i = 0; i < count; ++i) {
+    const ppo_adamw_tensor& t = tensors[i];
+    bytes += t.count * (type_size(t.param_type) + type_size(t.grad_type) + (t.master ? 4 : 0) + (t.state_bits == 8 ? 2 : 8));
+  }
+  const bool past_cache = bytes > kCacheBytes;
   for (int kind = 0; kind < 16; ++kind) {
     int i = 0;
     while (i < count) {
@@ -403,11 +416,11 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
       t.first[t.tensors] = static_cast<int32_t>(chunks);
       const bool bits8 = kind & 8;
       switch (kind & 7) {
-        case 0: launch_update<float, float, false>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
-        case 1: launch_update<__bf16, float, false>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
-        case 3: launch_update<__bf16, __bf16, false>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
-        case 5: launch_update<__bf16, float, true>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
-        case 7: launch_update<__bf16, __bf16, true>(bits8, static_cast<int>(chunks), st, t, s, coef); break;
+        case 0: launch_update<float, float, false>(bits8, past_cache, static_cast<int>(chunks), st, t, s, coef); break;
+        case 1: launch_update<__bf16, float, false>(bits8, past_cache, static_cast<int>(chunks), st, t, s, coef); break;
+        case 3: launch_update<__bf16, __bf16, false>(bits8, past_cache, static_cast<int>(chunks), st, t, s, coef); break;
+        case 5: launch_update<__bf16, float, true>(bits8, past_cache, static_cast<int>(chunks), st, t, s, coef); break;
+        case 7: launch_update<__bf16, __bf16, true>(bits8, past_cache, static_cast<int>(chunks), st, t, s, coef); break;
         default: return fail(PPO_EINVAL, "ppo_adamw_step: kind %d", kind);
       }
       if (int rc = check_launch("adamw_update_kernel")) return rc;

@@ -60,15 +60,17 @@ __global__ __launch_bounds__(kFwdThreads) void embedding_fwd_kernel(const ppo_em
 
 // ---- the sort ----
 
-// Items of a tile lie as wave, round, lane: each wave owns ROUNDS * 64 consecutive ones.  Up to kOneTile tokens are sorted
-// by one block in one launch; more go in tiles of kTile, two launches for each 9 bits of the token.
+// Up to kRankMax tokens find their places by comparing each with all (rank_kernel, one launch); more are sorted in tiles of
+// kTile, two launches for each 9 bits of the token.  A tile's items lie as wave, round, lane: each wave owns kRounds * 64
+// consecutive ones.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr int kTileRounds = 4, kTile = kTileRounds * kSortThreads, kOneRounds = 8, kOneTile = kOneRounds * kSortThreads;
+constexpr int kRounds = 4, kTile = kRounds * kSortThreads;
+constexpr int64_t kRankMax = 12288;  // (gradients of 12,000 tokens 34 us so, 39 by the other; of 16,384 45 and 39)
 constexpr int kMaxBits = 9, kMaxDigits = 1 << kMaxBits;
 
 struct SortPlan {
   int passes, bits;  // digits of `bits` bits, `passes` of them
-  int tiles;
+  int tiles;         // 0: by rank_kernel
   int digits() const { return 1 << bits; }
 };
 
@@ -78,7 +80,7 @@ SortPlan sort_plan(int64_t count, int64_t vocab) {
   SortPlan p;
   p.passes = static_cast<int>(ceil_div(need, kMaxBits));
   p.bits = static_cast<int>(ceil_div(need, p.passes));
-  p.tiles = count == 0 ? 0 : count <= kOneTile ? 1 : static_cast<int>(ceil_div(count, kTile));
+  p.tiles = count <= kRankMax ? 0 : static_cast<int>(ceil_div(count, kTile));
   return p;
 }
 
@@ -91,27 +93,35 @@ struct Fill {
   char* dst;
   int64_t rows, row_bytes, ld_bytes;
   int64_t first;  // blocks of earlier launches
+  bool stream;    // (kCacheBytes)
 };
 
-__device__ __forceinline__ void store_zeros(char* p, int64_t bytes, int lane, int lanes) {
+__device__ __forceinline__ void store_zeros(char* p, int64_t bytes, int lane, int lanes, bool stream) {
   // from an address of the element's alignment on; the ends by 2 bytes
   const int64_t head = min<int64_t>(bytes, -reinterpret_cast<intptr_t>(p) & 15);
   const int64_t pieces = (bytes - head) / 16, tail = head + pieces * 16;
-  for (int64_t i = lane; i < pieces; i += lanes) *reinterpret_cast<float4*>(p + head + 16 * i) = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  typedef float vec __attribute__((ext_vector_type(4)));
+  vec* q = reinterpret_cast<vec*>(p + head);
+  const vec zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (stream)
+    for (int64_t i = lane; i < pieces; i += lanes) __builtin_nontemporal_store(zero, q + i);
+  else
+    for (int64_t i = lane; i < pieces; i += lanes) q[i] = zero;
   for (int64_t i = 2 * lane; i < head; i += 2 * lanes) *reinterpret_cast<uint16_t*>(p + i) = 0;
   for (int64_t i = tail + 2 * lane; i < bytes; i += 2 * lanes) *reinterpret_cast<uint16_t*>(p + i) = 0;
 }
 
+template <int NT>
 __device__ __forceinline__ void fill_block(const Fill& f, int64_t block) {
   block += f.first;
   if (f.ld_bytes == f.row_bytes) {
     const int64_t from = block * kFillBytes;
-    store_zeros(f.dst + from, min<int64_t>(kFillBytes, f.rows * f.row_bytes - from), threadIdx.x, kSortThreads);
+    store_zeros(f.dst + from, min<int64_t>(kFillBytes, f.rows * f.row_bytes - from), threadIdx.x, NT, f.stream);
     return;
   }
   const int64_t per = max<int64_t>(1, kFillBytes / f.row_bytes), end = min<int64_t>(f.rows, (block + 1) * per);
-  for (int64_t r = block * per + threadIdx.x / kWave; r < end; r += kSortWaves)  // a wave per row
-    store_zeros(f.dst + r * f.ld_bytes, f.row_bytes, threadIdx.x % kWave, kWave);
+  for (int64_t r = block * per + threadIdx.x / kWave; r < end; r += NT / kWave)  // a wave per row
+    store_zeros(f.dst + r * f.ld_bytes, f.row_bytes, threadIdx.x % kWave, kWave, f.stream);
 }
 
 int64_t fill_blocks(const Fill& f) {
@@ -124,34 +134,107 @@ __device__ __forceinline__ uint32_t key_at(const ppo_embedding_args& a, int64_t 
   return static_cast<uint32_t>(t < 0 ? a.vocab : t);
 }
 
-template <int ROUNDS>
+// A block of kRankOwn tokens counts, for each of them, the tokens that come before it in the sorted order: smaller ones, and
+// equal ones of a smaller index.  Its waves take 64 of the others at a time, one per lane, and compare them with the own
+// tokens, which lie in scalar registers: two instructions each.  The loop is kept short and rolled: as straight-line code of
+// ten KB, and with a scalar count of each comparison's bits, it took 14 us for 5,003 tokens, most of it fetching instructions.
+// The time goes with count^2, but a sort of as many tokens in one block's LDS leaves the other compute units idle (16 us).
+constexpr int kRankThreads = 256, kRankWaves = kRankThreads / kWave, kRankOwn = 16;
+static_assert(4 * kRankOwn == kWave, "the reduction's exchanges");
+static_assert(kWave % kRankOwn == 0, "a block's tokens lie in one group of 64");
+
+template <class K>  // the tokens' type
+__global__ __launch_bounds__(kRankThreads) void rank_kernel(const ppo_embedding_args a, uint32_t* __restrict__ keys,
+                                                            uint32_t* __restrict__ idx, int blocks, const Fill fill) {
+  __shared__ uint32_t part[kRankWaves][kRankOwn];
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    fill_block<kRankThreads>(fill, static_cast<int>(blockIdx.x) - blocks);
+    return;
+  }
+  const int n = static_cast<int>(a.count), groups = (n + kWave - 1) / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int i0 = blockIdx.x * kRankOwn, group = i0 / kWave;
+  const K* tokens = static_cast<const K*>(a.tokens);
+  auto load = [&](int g) { return tokens[min(g * kWave + lane, n - 1)]; };
+  auto key_of = [&](K token, int g) {  // (past the end: before nothing)
+    return g * kWave + lane >= n ? INT32_MAX : static_cast<int>(token >= 0 && token < a.vocab ? token : a.vocab);
+  };
+  const int ours = key_of(load(group), group);
+  int own[kRankOwn];
+  uint32_t before[kRankOwn];
+#pragma unroll
+  for (int t = 0; t < kRankOwn; ++t) {
+    own[t] = __builtin_amdgcn_readlane(ours, i0 % kWave + t);
+    before[t] = 0;
+  }
+  if (wave == group % kRankWaves) {  // the own group: by index where equal
+#pragma unroll
+    for (int t = 0; t < kRankOwn; ++t) before[t] = ours < own[t] + (lane < i0 % kWave + t ? 1 : 0) ? 1 : 0;
+  }
+  // four groups' loads ahead of the comparisons (tokens as they are: a key made of one would wait for it)
+  K next[4];
+#pragma unroll
+  for (int f = 0; f < 4; ++f) next[f] = load(wave + f * kRankWaves);
+#pragma unroll 1
+  for (int g0 = wave; g0 < groups; g0 += 4 * kRankWaves)
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const int g = g0 + f * kRankWaves;
+      const int key = key_of(next[f], g);
+      const int theirs = g < group ? key - 1 : g > group ? key : INT32_MAX;  // (x <= y as x - 1 < y)
+      next[f] = load(g + 4 * kRankWaves);
+#pragma unroll
+      for (int t = 0; t < kRankOwn; ++t) before[t] += theirs < own[t] ? 1 : 0;
+    }
+  // the lanes' counts: with each exchange a lane keeps half of the tokens, until it holds one of them over 4 lanes
+#pragma unroll
+  for (int d = kWave / 2, half = kRankOwn / 2; half > 0; d /= 2, half /= 2)
+#pragma unroll
+    for (int t = 0; t < half; ++t) {
+      const uint32_t send = lane & d ? before[t] : before[t + half], keep = lane & d ? before[t + half] : before[t];
+      before[t] = keep + __shfl_xor(send, d, kWave);
+    }
+  before[0] += __shfl_xor(before[0], 2, kWave);
+  before[0] += __shfl_xor(before[0], 1, kWave);
+  if (lane % 4 == 0) part[wave][lane / 4] = before[0];
+  __syncthreads();
+  if (threadIdx.x >= kRankOwn || i0 + lane >= n) return;
+  uint32_t to = 0;
+  int key = 0;
+#pragma unroll
+  for (int w = 0; w < kRankWaves; ++w) to += part[w][lane];
+#pragma unroll
+  for (int t = 0; t < kRankOwn; ++t) key = lane == t ? own[t] : key;
+  keys[to] = key;
+  idx[to] = i0 + lane;
+}
+
 __device__ __forceinline__ int item_in_tile(int round) {
-  return (threadIdx.x / kWave) * (ROUNDS * kWave) + round * kWave + (threadIdx.x & (kWave - 1));
+  return (threadIdx.x / kWave) * (kRounds * kWave) + round * kWave + (threadIdx.x & (kWave - 1));
 }
 
 // Stable ranks of a tile's digits: rank[r] counts the items of the same digit before this one in its wave, and
 // counts[wave][digit] becomes how many the wave holds.  counts is zero on entry.  The lanes of a digit find each other by a
 // ballot per bit.
-template <int ROUNDS>
-__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[ROUNDS], const bool (&in)[ROUNDS], int bits,
-                                           uint32_t* counts, uint32_t (&rank)[ROUNDS]) {
+__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[kRounds], const bool (&in)[kRounds], int bits,
+                                           uint32_t* counts, uint32_t (&rank)[kRounds]) {
   uint32_t* mine = counts + (threadIdx.x / kWave) * kMaxDigits;
   const uint64_t below = (uint64_t{1} << (threadIdx.x & (kWave - 1))) - 1;
-  uint64_t same[ROUNDS];
+  uint64_t same[kRounds];
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) same[r] = __ballot(in[r]);
+  for (int r = 0; r < kRounds; ++r) same[r] = __ballot(in[r]);
 #pragma unroll
   for (int b = 0; b < kMaxBits; ++b)
     if (b < bits) {
 #pragma unroll
-      for (int r = 0; r < ROUNDS; ++r) {
+      for (int r = 0; r < kRounds; ++r) {
         const bool set = (digit[r] >> b) & 1;
         const uint64_t m = __ballot(set);
         same[r] &= set ? m : ~m;
       }
     }
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
+  for (int r = 0; r < kRounds; ++r) {
     const uint32_t before = __popcll(same[r] & below);
     const uint32_t base = in[r] ? mine[digit[r]] : 0;
     rank[r] = base + before;
@@ -199,82 +282,26 @@ __device__ __forceinline__ void clear_counts(uint32_t* counts) {
   for (int i = 0; i < kSortWaves * kMaxDigits / kSortThreads; ++i) counts[i * kSortThreads + threadIdx.x] = 0;
 }
 
-// Up to kOneTile tokens: all passes in one block.
-__global__ __launch_bounds__(kSortThreads) void sort_tile_kernel(const ppo_embedding_args a, int passes, int bits,
-                                                                 uint32_t* __restrict__ keys, uint32_t* __restrict__ idx,
-                                                                 const Fill fill) {
-  constexpr int ROUNDS = kOneRounds;
-  __shared__ uint32_t counts[kSortWaves * kMaxDigits], s_key[kOneTile], start[kMaxDigits], scratch[kSortWaves];
-  __shared__ uint16_t s_idx[kOneTile];
-  static_assert(kOneTile <= 1 << 16, "16-bit indices");
-  if (blockIdx.x > 0) {
-    fill_block(fill, blockIdx.x - 1);
-    return;
-  }
-  const int n = static_cast<int>(a.count);
-  uint32_t key[ROUNDS], from[ROUNDS], digit[ROUNDS], rank[ROUNDS];
-  bool in[ROUNDS];
-#pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int i = item_in_tile<ROUNDS>(r);
-    in[r] = i < n;
-    key[r] = in[r] ? key_at(a, i) : 0;
-    from[r] = i;
-  }
-  for (int p = 0; p < passes; ++p) {
-    clear_counts(counts);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) digit[r] = (key[r] >> (p * bits)) & ((1u << bits) - 1);
-    wave_ranks(digit, in, bits, counts, rank);
-    __syncthreads();
-    const uint32_t total = digit_totals(counts, 1 << bits);
-    const uint32_t first = exclusive_sum(total, scratch);
-    if (threadIdx.x < kMaxDigits) start[threadIdx.x] = first;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)
-      if (in[r]) {
-        const uint32_t to = start[digit[r]] + counts[(threadIdx.x / kWave) * kMaxDigits + digit[r]] + rank[r];
-        s_key[to] = key[r];
-        s_idx[to] = static_cast<uint16_t>(from[r]);
-      }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)
-      if (in[r]) {
-        key[r] = s_key[item_in_tile<ROUNDS>(r)];
-        from[r] = s_idx[item_in_tile<ROUNDS>(r)];
-      }
-  }
-#pragma unroll
-  for (int r = 0; r < ROUNDS; ++r)
-    if (in[r]) {
-      keys[item_in_tile<ROUNDS>(r)] = key[r];
-      idx[item_in_tile<ROUNDS>(r)] = from[r];
-    }
-}
-
 // One pass over several tiles: how many items of each digit a tile holds, hist[tile][digit]; then every item to its place.
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const ppo_embedding_args a, int shift, int bits, int tiles,
                                                                   const uint32_t* __restrict__ keys,
                                                                   uint32_t* __restrict__ hist, const Fill fill) {
   __shared__ uint32_t count[kMaxDigits];
   if (static_cast<int>(blockIdx.x) >= tiles) {
-    fill_block(fill, static_cast<int>(blockIdx.x) - tiles);
+    fill_block<kSortThreads>(fill, static_cast<int>(blockIdx.x) - tiles);
     return;
   }
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
-  uint32_t key[kTileRounds];
+  uint32_t key[kRounds];
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
+  for (int r = 0; r < kRounds; ++r) {
     const int64_t i = base + r * kSortThreads + threadIdx.x;
     key[r] = i < a.count ? (keys != nullptr ? keys[i] : key_at(a, i)) : 0;
   }
   if (threadIdx.x < kMaxDigits) count[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r)
+  for (int r = 0; r < kRounds; ++r)
     if (base + r * kSortThreads + threadIdx.x < a.count) atomicAdd(&count[(key[r] >> shift) & ((1u << bits) - 1)], 1u);
   __syncthreads();
   if (static_cast<int>(threadIdx.x) < (1 << bits)) hist[(static_cast<int64_t>(blockIdx.x) << bits) + threadIdx.x] = count[threadIdx.x];
@@ -288,16 +315,16 @@ __global__ __launch_bounds__(kSortThreads) void sort_move_kernel(const ppo_embed
                                                                  const Fill fill) {
   __shared__ uint32_t counts[kSortWaves * kMaxDigits], start[kMaxDigits], scratch[kSortWaves];
   if (static_cast<int>(blockIdx.x) >= tiles) {
-    fill_block(fill, static_cast<int>(blockIdx.x) - tiles);
+    fill_block<kSortThreads>(fill, static_cast<int>(blockIdx.x) - tiles);
     return;
   }
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
-  uint32_t key[kTileRounds], from[kTileRounds], digit[kTileRounds], rank[kTileRounds];
-  bool in[kTileRounds];
+  uint32_t key[kRounds], from[kRounds], digit[kRounds], rank[kRounds];
+  bool in[kRounds];
   clear_counts(counts);
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    const int64_t i = base + item_in_tile<kTileRounds>(r);
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = base + item_in_tile(r);
     in[r] = i < a.count;
     key[r] = in[r] ? (keys_in != nullptr ? keys_in[i] : key_at(a, i)) : 0;
     from[r] = in[r] ? (idx_in != nullptr ? idx_in[i] : static_cast<uint32_t>(i)) : 0;
@@ -321,7 +348,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_move_kernel(const ppo_embed
   if (threadIdx.x < kMaxDigits) start[threadIdx.x] = first + earlier;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r)
+  for (int r = 0; r < kRounds; ++r)
     if (in[r]) {
       const uint32_t to = start[digit[r]] + counts[(threadIdx.x / kWave) * kMaxDigits + digit[r]] + rank[r];
       keys[to] = key[r];
@@ -329,14 +356,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_move_kernel(const ppo_embed
     }
 }
 
-__global__ __launch_bounds__(kSortThreads) void fill_kernel(const Fill fill) { fill_block(fill, blockIdx.x); }
-
 // ---- the sums ----
 
-// The sorted positions are cut into units; a wave sums a unit's rows over 64 16-byte pieces of columns.  A run of
-// one token inside a unit is stored at once; the parts of a run that crosses units go to `partial` ([units][2][dim]: the
-// part of a run that began earlier, and of the one that goes on) and are joined by join_kernel in the units' order.
-constexpr int kFlight = 8;  // rows' loads in flight per wave
+// The sorted positions are cut into units; a wave sums a unit's rows over 64 16-byte pieces of columns.  A run of one token
+// that crosses into the next unit by at most kReach rows is finished where it began, and the next unit starts behind it.  A run
+// that goes on further leaves its parts in `partial` ([units][2][dim]: of the run that came into the unit, of the one that goes
+// out), joined by embedding_join_kernel in the units' order.
+constexpr int kFlight = 8;                    // rows' loads a wave issues together; it has two such groups in flight
+constexpr uint32_t kReach = 8, kMaxUnit = 48;  // (a unit, what it reaches and one more position fit a wave's lanes)
+static_assert(kMaxUnit + kReach < kWave, "a unit's keys, one per lane");
 
 struct SumArgs {
   ppo_embedding_args e;
@@ -344,8 +372,9 @@ struct SumArgs {
   const uint32_t* idx;
   float* partial;
   int64_t ld_partial;  // a multiple of 4
-  uint32_t unit;       // positions
+  uint32_t unit;       // positions, kReach to kMaxUnit
   uint32_t units;
+  uint32_t columns;    // waves side by side on a row
 };
 
 // sum[i] is column c + i of the row; columns from c0 on are this lane's.
@@ -377,23 +406,42 @@ __device__ __forceinline__ void store_sum(T* row, int c0, int c, int dim, const 
 template <class T, class O>
 __global__ __launch_bounds__(kWave) void embedding_sum_kernel(const SumArgs s) {
   constexpr int V = kVec<T>;
+  constexpr uint32_t kNone = 0xffffffffu;  // no key
   const ppo_embedding_args& a = s.e;
-  const int lane = threadIdx.x;
-  const uint32_t n = static_cast<uint32_t>(a.count);
+  const uint32_t lane = threadIdx.x, n = static_cast<uint32_t>(a.count);
+  const uint32_t unit = blockIdx.x / s.columns, column = blockIdx.x % s.columns, begin = unit * s.unit;  // a row's parts at about one time
+  // each lane a position's key and index, from the unit's first on
+  const uint32_t at = begin + lane;
+  const uint32_t keys = at < n ? s.keys[at] : kNone, idx = at < n ? s.idx[at] : 0;
+  const uint32_t before = begin > 0 ? s.keys[begin - 1] : kNone;
+  auto key_of = [&](uint32_t i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(keys), static_cast<int>(i))); };
+  auto run_from = [&](uint32_t i, uint32_t key) {  // how many positions from the i-th on hold the key
+    const uint64_t other = __ballot(keys != key) >> i;
+    return other == 0 ? kWave - i : static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(other)) - 1);
+  };
+  uint32_t first = 0, last = min(s.unit, n - begin);  // the positions this wave sums, from `begin` on
+  bool head = false, tail = false;                    // the first run came in, the last one goes on
+  if (begin > 0) {
+    first = run_from(0, before);
+    head = first > kReach;
+    if (head) first = 0;
+  }
+  const uint32_t more = last < s.unit ? 0 : run_from(last, key_of(last - 1));
+  tail = more > kReach;
+  if (!tail) last += more;
+  if (first >= last) return;  // the unit before has taken all of it
+
   O* out = static_cast<O*>(a.dst);
-  const int c0 = (blockIdx.y * kWave + lane) * V;
-  if (c0 >= a.dim) return;
+  const int c0 = static_cast<int>(column * kWave + lane) * V;
   const bool whole = a.dim >= V;
   const int c = whole ? min(c0, a.dim - V) : 0;  // an odd row's last piece is read from V columns before its end
   const T* src = static_cast<const T*>(a.src);
-  const uint32_t begin = blockIdx.x * s.unit, end = min(begin + s.unit, n);
-  uint32_t cur = s.keys[begin];
-  bool head = begin > 0 && s.keys[begin - 1] == cur;  // the run began in an earlier unit
+  uint32_t cur = key_of(first);
   float sum[V] = {};
-  auto flush = [&](bool tail) {
+  auto flush = [&](bool part) {
     if (cur < a.vocab) {
-      if (head || tail)
-        store_sum<V>(s.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (head ? 0 : 1)) * s.ld_partial, c0, c, a.dim, sum, 1.0f, false);
+      if (part)
+        store_sum<V>(s.partial + (static_cast<int64_t>(unit) * 2 + (head ? 0 : 1)) * s.ld_partial, c0, c, a.dim, sum, 1.0f, false);
       else
         store_sum<V>(out + static_cast<int64_t>(cur) * a.ld_dst, c0, c, a.dim, sum, a.scale, a.accumulate != 0);
     }
@@ -401,80 +449,122 @@ __global__ __launch_bounds__(kWave) void embedding_sum_kernel(const SumArgs s) {
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
   };
-  for (uint32_t p = begin; p < end; p += kFlight) {
+  struct Group {
     typename Piece<T>::type x[kFlight];
-    uint32_t key[kFlight];
+  };
+  auto load = [&](Group& g, uint32_t p) {
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
-      const uint32_t q = min(p + u, end - 1);
-      key[u] = s.keys[q];
-      const T* row = src + static_cast<int64_t>(s.idx[q]) * a.ld_src;
+      const int64_t i = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(idx), static_cast<int>(min(p + u, last - 1))));
+      const T* row = src + i * a.ld_src;
       if (whole) {
-        x[u] = load_piece(row + c);
+        g.x[u] = load_piece<true>(row + c);  // (read once)
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[u][i] = i < a.dim ? row[i] : static_cast<T>(0.0f);
+        for (int e = 0; e < V; ++e) g.x[u][e] = e < a.dim ? row[e] : static_cast<T>(0.0f);
       }
     }
+  };
+  auto add = [&](const Group& g, uint32_t p) {
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
-      if (p + u >= end) break;
-      if (key[u] != cur) {
-        flush(false);
-        cur = key[u];
+      if (p + u >= last) break;
+      const uint32_t key = key_of(p + u);
+      if (key != cur) {
+        flush(head);
+        cur = key;
       }
+      const typename Piece<T>::type x = g.x[u];
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += static_cast<float>(x[u][i]);
+      for (int i = 0; i < V; ++i) sum[i] += static_cast<float>(x[i]);
     }
+  };
+  // the next group's loads go out before this one's sums and their stores, whose completion they then need not wait for
+  Group even, odd;
+  load(even, first);
+  for (uint32_t p = first; p < last; p += 2 * kFlight) {
+    if (p + kFlight < last) load(odd, p + kFlight);
+    add(even, p);
+    if (p + 2 * kFlight < last) load(even, p + 2 * kFlight);
+    if (p + kFlight < last) add(odd, p + kFlight);
   }
-  flush(end < n && s.keys[end] == cur);
+  flush(head || tail);
 }
 
-// A run that crosses units: the block of the unit where it begins adds the parts of the units it goes on in, each wave a
-// consecutive share of them, and the waves' sums in order.
-constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave, kJoinColumns = 4 * kWave;
+// The runs that go on past a unit by more than kReach: a wave per unit adds the parts of those that begin there, unless there
+// are so many that the block's waves share them (at most one such run can begin in a block's units).
+constexpr int kJoinWaves = 16, kJoinThreads = kJoinWaves * kWave, kJoinColumns = 4 * kWave;
+constexpr uint32_t kJoinAlone = 16;
 
 template <class O>
 __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(const SumArgs s) {
   __shared__ float4 part[kJoinWaves][kWave];
+  __shared__ uint32_t shared_unit, shared_more;
   const ppo_embedding_args& a = s.e;
-  const uint32_t n = static_cast<uint32_t>(a.count), u = blockIdx.x;
-  const uint32_t begin = u * s.unit, end = min(begin + s.unit, n);
-  if (end >= n) return;
-  const uint32_t key = s.keys[end - 1];
-  if (s.keys[end] != key || key >= a.vocab) return;                           // the last run ends with the unit
-  if (s.keys[begin] == key && begin > 0 && s.keys[begin - 1] == key) return;  // it began in an earlier one
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  uint32_t more = 0;  // units after this one that begin with the same token
-  while (true) {
-    const uint32_t w = u + 1 + more + lane;
-    const uint64_t m = __ballot(w < s.units && s.keys[static_cast<int64_t>(min(w, s.units - 1)) * s.unit] == key);
-    more += m == ~uint64_t{0} ? kWave : __ffsll(static_cast<unsigned long long>(~m)) - 1;
-    if (m != ~uint64_t{0}) break;
+  const uint32_t n = static_cast<uint32_t>(a.count), lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t u = blockIdx.x * kJoinWaves + wave;
+  // whether a run goes on past the boundary before position b: the position kReach behind it still holds its key
+  auto crosses = [&](uint64_t b, uint32_t key) { return b + kReach < n && s.keys[b + kReach] == key; };
+  const uint64_t begin = static_cast<uint64_t>(u) * s.unit, end = begin + s.unit;
+  uint32_t key = 0, more = 0;  // the units that the run goes on in
+  if (end + kReach < n) {
+    key = s.keys[end - 1];
+    const uint32_t behind = s.keys[end + kReach], before = begin > 0 ? s.keys[begin - 1] : ~0u;
+    if (behind == key && key < a.vocab && before != key) {
+      // 64 boundaries at once; of a longer run every 64th first
+      auto leading = [&](uint32_t from, uint32_t step) {
+        const uint64_t m = __ballot(crosses(end + static_cast<uint64_t>(from + lane * step) * s.unit, key));
+        return m == ~uint64_t{0} ? static_cast<uint32_t>(kWave) : static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(~m)) - 1);
+      };
+      more = leading(0, 1);
+      if (more == kWave) {
+        uint32_t far = 0;
+        for (uint32_t k = kWave; k == kWave; far += k) k = leading(far * kWave, kWave);
+        more = (far - 1) * kWave;
+        more += leading(more, 1);
+      }
+    }
   }
-  const int c = (blockIdx.y * kWave + lane) * 4;
-  float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (c < a.dim) {
-    auto add = [&](const float4& x) { sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w; };
-    if (wave == 0) add(*reinterpret_cast<const float4*>(s.partial + (static_cast<int64_t>(u) * 2 + 1) * s.ld_partial + c));
-    const uint32_t share = (more + kJoinWaves - 1) / kJoinWaves, last = min(more, (wave + 1) * share);
+  const int c = (blockIdx.y * kWave + static_cast<int>(lane)) * 4;
+  auto sum_of = [&](uint32_t unit, uint32_t from, uint32_t to) {  // the parts of units unit + from .. unit + to - 1
+    float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < a.dim) {
 #pragma unroll 8
-    for (uint32_t i = wave * share; i < last; ++i)
-      add(*reinterpret_cast<const float4*>(s.partial + static_cast<int64_t>(u + 1 + i) * 2 * s.ld_partial + c));
-  }
-  part[wave][lane] = sum;
+      for (uint32_t i = from; i < to; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(s.partial + (static_cast<int64_t>(unit + i) * 2 + (i == 0 ? 1 : 0)) * s.ld_partial + c);
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+      }
+    }
+    return sum;
+  };
+  auto store = [&](uint32_t row, const float4& sum) {
+    const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+    O* to = static_cast<O*>(a.dst) + static_cast<int64_t>(row) * a.ld_dst + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < a.dim) to[i] = static_cast<O>(a.accumulate ? static_cast<float>(to[i]) + a.scale * x[i] : a.scale * x[i]);
+  };
+  if (threadIdx.x == 0) shared_more = 0;
   __syncthreads();
-  if (wave > 0 || c >= a.dim) return;
-  float x[4] = {};
-#pragma unroll
-  for (int w = 0; w < kJoinWaves; ++w) {
-    const float4 y = part[w][lane];
-    x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+  if (more > kJoinAlone && lane == 0) {
+    shared_unit = u;
+    shared_more = more;
   }
-  O* to = static_cast<O*>(a.dst) + static_cast<int64_t>(key) * a.ld_dst + c;
+  if (more > 0 && more <= kJoinAlone) store(key, sum_of(u, 0, more + 1));
+  __syncthreads();
+  const uint32_t all = shared_more + 1;
+  if (all == 1) return;
+  const uint32_t share = (all + kJoinWaves - 1) / kJoinWaves;
+  part[wave][lane] = sum_of(shared_unit, min(all, wave * share), min(all, (wave + 1) * share));
+  __syncthreads();
+  if (u != shared_unit) return;
+  float4 sum = part[0][lane];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (c + i < a.dim) to[i] = static_cast<O>(a.accumulate ? static_cast<float>(to[i]) + a.scale * x[i] : a.scale * x[i]);
+  for (int w = 1; w < kJoinWaves; ++w) {
+    const float4 x = part[w][lane];
+    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  }
+  store(key, sum);
 }
 
 int check(const char* who, const ppo_embedding_args* a, bool bwd) {
@@ -503,11 +593,13 @@ struct BwdLayout {
   size_t keys[2], idx[2], hist, partial, bytes;
 };
 
-// Positions of a unit: enough waves to fill the chip (8,192 hold 64 KiB of loads in flight each four SIMDs), but at least 8 rows,
-// since a run that crosses units costs a row of partial sums for each, and at most 64.
+// Positions of a unit: enough waves to fill the chip (16 KiB of loads in flight each), but no fewer than a run may reach past its
+// unit.
 uint32_t unit_for(int64_t count, int32_t dim) {
-  uint32_t unit = 8;
-  while (unit < 64 && count * ceil_div(dim, 512) > static_cast<int64_t>(unit) * 8192) unit *= 2;
+  const int64_t waves = count * ceil_div(dim, 512);  // of one position each (of 16-bit rows; the workspace goes by it too)
+  if (count <= 32) return 32;  // one unit, nothing to join
+  uint32_t unit = kReach;
+  while (unit < 32 && waves > static_cast<int64_t>(unit) * 8192) unit *= 2;
   return unit;
 }
 
@@ -527,20 +619,21 @@ BwdLayout bwd_layout(int64_t count, int64_t vocab, int32_t dim) {
     l.keys[k] = take(4 * static_cast<size_t>(count));
     l.idx[k] = take(4 * static_cast<size_t>(count));
   }
-  l.hist = take(l.sort.tiles > 1 ? 4 * static_cast<size_t>(l.sort.digits()) * l.sort.tiles : 0);
+  l.hist = take(l.sort.tiles > 0 ? 4 * static_cast<size_t>(l.sort.digits()) * l.sort.tiles : 0);
   l.partial = take(8 * static_cast<size_t>(l.units) * l.ld_partial);
   l.bytes = at;
   return l;
 }
 
 template <class T, class O>
-int launch_sums(const SumArgs& s, hipStream_t st) {
+int launch_sums(SumArgs s, hipStream_t st) {
   const int dim = s.e.dim;
-  const dim3 grid(s.units, static_cast<uint32_t>(ceil_div(dim, kWave * kVec<T>)));
-  hipLaunchKernelGGL((embedding_sum_kernel<T, O>), grid, dim3(kWave), 0, st, s);
+  s.columns = static_cast<uint32_t>(ceil_div(dim, kWave * kVec<T>));
+  PPO_REQUIRE(static_cast<int64_t>(s.units) * s.columns < INT32_MAX, "ppo_embedding_bwd: count=%lld dim=%d", (long long)s.e.count, dim);
+  hipLaunchKernelGGL((embedding_sum_kernel<T, O>), dim3(s.units * s.columns), dim3(kWave), 0, st, s);
   if (int rc = check_launch("embedding_sum_kernel")) return rc;
   if (s.units < 2) return PPO_OK;
-  const dim3 join(s.units - 1, static_cast<uint32_t>(ceil_div(dim, kJoinColumns)));
+  const dim3 join(static_cast<uint32_t>(ceil_div(s.units, kJoinWaves)), static_cast<uint32_t>(ceil_div(dim, kJoinColumns)));
   hipLaunchKernelGGL(embedding_join_kernel<O>, join, dim3(kJoinThreads), 0, st, s);
   return check_launch("embedding_join_kernel");
 }
@@ -586,18 +679,20 @@ extern "C" int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace
   char* ws = static_cast<char*>(workspace);
   auto at = [&](size_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
   const int64_t size = type_size(a.dst_type);
-  Fill fill{static_cast<char*>(a.dst), a.vocab, a.dim * size, a.ld_dst * size, 0};
+  Fill fill{static_cast<char*>(a.dst), a.vocab, a.dim * size, a.ld_dst * size, 0,
+            (a.vocab * size + a.count * type_size(a.src_type)) * a.dim > kCacheBytes};
   const int64_t blocks = a.accumulate ? 0 : fill_blocks(fill);
   PPO_REQUIRE(blocks < (int64_t{1} << 30), "ppo_embedding_bwd: the table is too large");
   int last = 0;  // the buffer that holds the sorted tokens
   if (l.sort.tiles == 0) {
-    hipLaunchKernelGGL(fill_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kSortThreads), 0, st, fill);
-    return check_launch("fill_kernel");
-  }
-  if (l.sort.tiles == 1) {
-    hipLaunchKernelGGL(sort_tile_kernel, dim3(1 + static_cast<uint32_t>(blocks)), dim3(kSortThreads), 0, st, a, l.sort.passes,
-                       l.sort.bits, at(l.keys[0]), at(l.idx[0]), fill);
-    if (int rc = check_launch("sort_tile_kernel")) return rc;
+    const int own = static_cast<int>(ceil_div(a.count, kRankOwn));
+    const dim3 grid(own + static_cast<uint32_t>(blocks));
+    if (a.token_type == PPO_TOKENS_I64)
+      hipLaunchKernelGGL(rank_kernel<int64_t>, grid, dim3(kRankThreads), 0, st, a, at(l.keys[0]), at(l.idx[0]), own, fill);
+    else
+      hipLaunchKernelGGL(rank_kernel<int32_t>, grid, dim3(kRankThreads), 0, st, a, at(l.keys[0]), at(l.idx[0]), own, fill);
+    if (int rc = check_launch("rank_kernel")) return rc;
+    if (a.count == 0) return PPO_OK;
   } else {
     // the launches' shares of the filling, about as their own work lasts: 1 for a count, 2 for a move
     const int64_t share = ceil_div(blocks, 3 * l.sort.passes);
@@ -619,7 +714,7 @@ extern "C" int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace
       last = to;
     }
   }
-  const SumArgs s{a, at(l.keys[last]), at(l.idx[last]), reinterpret_cast<float*>(ws + l.partial), l.ld_partial, l.unit, l.units};
+  const SumArgs s{a, at(l.keys[last]), at(l.idx[last]), reinterpret_cast<float*>(ws + l.partial), l.ld_partial, l.unit, l.units, 0};
   int rc = PPO_OK;
   with_type(a.src_type, [&](auto t) {
     using T = decltype(t);

@@ -28,6 +28,7 @@ struct LossKernelArgs {
   ppo_token_loss_args a;
   float* inv_n;   // 1 / N of token_count_kernel, where that ran
   float* terms;   // [rows][kTermStride]
+  bool stream;    // (kCacheBytes)
   int32_t count;  // 1: the block counts the rows, 2: inv_n holds 1 / N, 0: given_inv_n does
   float given_inv_n;
   float c, inv_temp, clip_lo, clip_hi, kl_coef, entropy_coef;
@@ -233,10 +234,11 @@ struct RowPieces {
   __device__ __forceinline__ bool some(int k) const { return first + (k * NT + wave) * V < vocab; }
   __device__ __forceinline__ uint32_t offset(int j) const { return static_cast<uint32_t>(j) * static_cast<uint32_t>(sizeof(T)); }
 
+  template <bool STREAM>
   __device__ __forceinline__ void load(const T* x) {
 #pragma unroll
     for (int k = 0; k < K; ++k)  // a uniform base and 32 bits of offset
-      raw[k] = load_raw(reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + offset(min(column(k), vocab - V))));
+      raw[k] = load_raw<STREAM>(reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + offset(min(column(k), vocab - V))));
   }
 
   // The wave's maximum and sums.
@@ -276,7 +278,7 @@ struct RowPieces {
     return mine;
   }
 
-  __device__ __forceinline__ void gradient(T* dx, int tok, const RowCoefs& o) {
+  __device__ __forceinline__ void gradient(T* dx, int tok, const RowCoefs& o, bool stream) {
     forget(tid);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -291,7 +293,9 @@ struct RowPieces {
           for (int e = 0; e < V; ++e)
             if (static_cast<uint32_t>(e) == hit) d[e] += o.at;
         if (whole(k)) {
-          store_piece(reinterpret_cast<T*>(reinterpret_cast<char*>(dx) + offset(at)), d);
+          T* to = reinterpret_cast<T*>(reinterpret_cast<char*>(dx) + offset(at));
+          if (stream) store_piece<true>(to, d);
+          else store_piece(to, d);
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e)
@@ -319,14 +323,15 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void token_row_kernel(const 
     return;
   }
   RowPieces<T, NT, K> row(vocab, 0);
-  row.load(x);
+  if (q.stream) row.template load<true>(x);
+  else row.template load<false>(x);
   float x_tok = static_cast<float>(x[tok]);
   const int32_t counted = LOSS && q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x, NT)) : 0;
   const RowSums mine = row.sums(q.c);
   arrived(x_tok);
   const RowCoefs o = finish_row<NT, LOSS>(q, r, mine, x_tok, counted, sh, threadIdx.x == 0);
   if (dx == nullptr) return;
-  if (o.live) row.gradient(dx, static_cast<int>(tok), o);
+  if (o.live) row.gradient(dx, static_cast<int>(tok), o, q.stream);
   else zero_gradient<T, NT>(dx, 0, vocab);
 }
 
@@ -371,11 +376,11 @@ __global__ __launch_bounds__(NT) void token_stats_kernel(const LossKernelArgs q)
 // A few wide rows, which one compute unit each would leave waiting for its arithmetic: a row is cut into parts of
 // kPartThreads kPartPieces pieces, a block each.  token_part_kernel leaves a part's sums; then token_joined_kernel's one wave
 // per row joins them, or each block of token_part_gradient_kernel does before it reads its part again, and one more block the
-// means of all rows.  Worth it (us a call, in one kernel -> in parts) for the loss of up to kSplitLossRows = a wave's lanes of rows
-// from 40,000 logits on (8 x 50,021 bf16 18.8 -> 15.0, 64 x 131,072 27.0 -> 19.7; 8 x 32,000 fp32 13.5 -> 14.3), for log-probabilities
-// of up to kSplitRows from 65,536 on (8 x 131,072 bf16 10.8 -> 9.3, 257 23.3 -> 16.2, 512 fp32 42.8 -> 43.0; 8 x 50,021 8.5 -> 9.4).
+// means of all rows.  Worth it (us, in one kernel -> in parts) for the loss of up to kSplitLossRows = a wave's lanes of rows
+// from 16,384 logits on (waited for: 16 x 16,384 bf16 24.5 -> 23.6, 16 x 32,000 27.3 -> 23.9, 8 x 131,072 39.8 -> 23.7), for
+// log-probabilities of up to kSplitRows from 65,536 on (8 x 131,072 bf16 10.8 -> 9.3, 257 23.3 -> 16.2, 512 fp32 42.8 -> 43.0; 8 x 50,021 8.5 -> 9.4).
 constexpr int kPartThreads = 256, kPartPieces = 4, kMaxParts = kWave;
-constexpr int64_t kSplitRows = 256, kSplitVocab = 65536, kSplitLossRows = kWave, kSplitLossVocab = 40000;
+constexpr int64_t kSplitRows = 256, kSplitVocab = 65536, kSplitLossRows = kWave, kSplitLossVocab = 16384;
 
 struct RowPart {
   RowSums sums;
@@ -391,7 +396,7 @@ __global__ __launch_bounds__(kPartThreads) void token_part_kernel(const LossKern
   if (!row_counts(a, r, tok)) return;
   const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
   RowPieces<T, kPartThreads, kPartPieces> row(static_cast<int>(a.vocab), blockIdx.x * (kPartThreads * kPartPieces * kVec<T>));
-  row.load(x);
+  row.template load<false>(x);
   const float x_tok = blockIdx.x == 0 ? static_cast<float>(x[tok]) : 0.0f;
   RowSums mine = row.sums(q.c);
   if (threadIdx.x % kWave == 0) sh[threadIdx.x / kWave] = mine;
@@ -465,12 +470,12 @@ __global__ __launch_bounds__(kPartThreads) void token_part_gradient_kernel(const
     return;
   }
   RowPieces<T, kPartThreads, kPartPieces> row(vocab, first);
-  if (dx != nullptr) row.load(x);
+  if (dx != nullptr) row.template load<false>(x);
   const int32_t counted = q.count == 1 ? wave_sum(rows_counted(q, threadIdx.x % kWave, kWave)) : 0;
   const RowCoefs o = finish_row<kWave, true>(q, r, join_parts(parts + r * n, n, q.c), parts[r * n].x_tok, counted, sh,
                                              first == 0 && threadIdx.x == 0);
   if (dx == nullptr) return;
-  if (o.live) row.gradient(dx, static_cast<int>(tok), o);
+  if (o.live) row.gradient(dx, static_cast<int>(tok), o, false);
   else zero_gradient<T, kPartThreads>(dx, first, min(first + kPart, vocab));
 }
 
@@ -622,6 +627,7 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
   hipStream_t st = static_cast<hipStream_t>(stream);
   LossKernelArgs q{};
   q.a = a;
+  q.stream = a.rows * a.vocab * type_size(a.type) * (loss && a.d_logits != nullptr ? 2 : 1) > kCacheBytes;
   q.inv_n = static_cast<float*>(workspace);
   q.terms = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.terms);
   RowPart* parts = reinterpret_cast<RowPart*>(static_cast<char*>(workspace) + l.parts);

@@ -1223,7 +1223,7 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step:
         if ts is None:
             columns.append([0] * n)
             continue
-        if name == "masters" and None in ts or sizes is None:  # lists that need not hold a tensor for each parameter
+        if sizes is None or name == "masters" and any(t is None for t in ts):  # lists that need not hold a tensor for each parameter
             columns.append([0 if t is None else t.data_ptr() for t in ts])
             sizes = sizes or [-(-c // L.ADAMW_BLOCK) for c in counts]
             ts, sizes = zip(*[(t, c) for t, c in zip(ts, sizes) if t is not None]) if any(t is not None for t in ts) else ((), ())
