@@ -816,7 +816,8 @@ int ppo_token_ppo_loss(const ppo_token_loss_args* args, void* workspace, size_t 
  *   total = ||all gradients||_2 (fp64);   c = min(1, max_norm / (total + 1e-6))   (max_norm <= 0: no clip, c = 1);
  *   g' = c g;   m = m + (1-b1) (g' - m);   v = v b2 + ((1-b2) g') g';
  *   p = p fl(1 - lr weight_decay) + ((-lr/bc1) m) / (sqrt(v)/bc2_sqrt + eps),
- * in ppo_adam_step's fp32 operation order; lr and weight_decay are each tensor's.  param is fp32 or bf16.  A bf16 param may
+ * in ppo_adam_step's fp32 operation order; lr, weight_decay and the bias corrections bc1 = 1 - b1^step, bc2_sqrt =
+ * sqrt(1 - b2^step) are each tensor's.  param is fp32 or bf16.  A bf16 param may
  * have an fp32 master: p is then the master, and param its rounding; without one p is param itself, rounded once a step.
  * States in 32 bits are fp32 [count]; in 8 bits, each 256 consecutive elements (the last block may be shorter) share one fp32
  * scale per state: m = sign(q) m_scale (|q| / 127)^2 with q int8, v = v_scale (q / 255)^4 with q uint8; the scale is the
@@ -834,6 +835,8 @@ typedef struct ppo_adamw_tensor {
   int64_t count;
   double lr;
   double weight_decay;
+  double bc1;
+  double bc2_sqrt;
   int32_t param_type; /* PPO_TYPE_F32 or PPO_TYPE_BF16 */
   int32_t grad_type;
   int32_t state_bits; /* 32 or 8 */
@@ -842,8 +845,7 @@ typedef struct ppo_adamw_tensor {
 #define PPO_ADAMW_BLOCK 256
 size_t ppo_adamw_workspace_bytes(const ppo_adamw_tensor* tensors, int32_t count);
 int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, double max_norm, double beta1, double beta2, double eps,
-                   double bc1, double bc2_sqrt, float* norm_out, void* workspace, size_t workspace_bytes,
-                   ppo_stream_t stream);
+                   float* norm_out, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
 
 #ifdef __cplusplus
 }

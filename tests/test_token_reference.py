@@ -140,23 +140,23 @@ def test_entry_points_refuse_bad_arguments():
         L.call("ppo_token_log_probs", loss(temperature=-1.0), 256, 1 << 20, None)
 
     def adamw(**more):
-        d = dict(param=64, grad=64, exp_avg=64, exp_avg_sq=64, count=8, lr=1e-3, weight_decay=0.0, state_bits=32)
+        d = dict(param=64, grad=64, exp_avg=64, exp_avg_sq=64, count=8, lr=1e-3, weight_decay=0.0, bc1=0.1, bc2_sqrt=0.03, state_bits=32)
         return ctypes.cast(ctypes.pointer(L.AdamwTensor(**{**d, **more})), ctypes.c_void_p)
 
-    step = lambda t, *more: L.call("ppo_adamw_step", t, 1, *(more or (1.0, 0.9, 0.999, 1e-8, 0.1, 0.03)), None, 256, 1 << 20, None)  # noqa: E731
+    step = lambda t, *more: L.call("ppo_adamw_step", t, 1, *(more or (1.0, 0.9, 0.999, 1e-8)), None, 256, 1 << 20, None)  # noqa: E731
     for more, what in [(dict(count=-1), "elements"), (dict(param_type=2), "param_type"), (dict(grad_type=1), "gradient"),
                        (dict(state_bits=16), "state_bits"), (dict(master=64), "master"), (dict(grad=None), "null"),
                        (dict(state_bits=8), "null"), (dict(param=66), "aligned")]:
         with pytest.raises(ValueError, match=what):
             step(adamw(**more))
     with pytest.raises(ValueError, match="beta1"):
-        step(adamw(), 1.0, 1.0, 0.999, 1e-8, 0.1, 0.03)
+        step(adamw(), 1.0, 1.0, 0.999, 1e-8)
     with pytest.raises(ValueError, match="corrections"):
-        step(adamw(), 1.0, 0.9, 0.999, 1e-8, 0.0, 0.03)
+        step(adamw(bc1=0.0))
     with pytest.raises(ValueError, match="workspace"):
-        L.call("ppo_adamw_step", adamw(), 1, 1.0, 0.9, 0.999, 1e-8, 0.1, 0.03, None, None, 0, None)
+        L.call("ppo_adamw_step", adamw(), 1, 1.0, 0.9, 0.999, 1e-8, None, None, 0, None)
     with pytest.raises(ValueError, match="tensors"):
-        L.call("ppo_adamw_step", None, 0, 1.0, 0.9, 0.999, 1e-8, 0.1, 0.03, None, None, 0, None)
+        L.call("ppo_adamw_step", None, 0, 1.0, 0.9, 0.999, 1e-8, None, None, 0, None)
 
 
 def test_tensors_on_the_cpu_are_refused():

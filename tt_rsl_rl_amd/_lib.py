@@ -219,14 +219,15 @@ class TokenLossArgs(C.Structure):
 
 class AdamwTensor(C.Structure):
     _fields_ = [("param", vp), ("grad", vp), ("master", vp), ("exp_avg", vp), ("exp_avg_sq", vp), ("m_scale", vp),
-                ("v_scale", vp), ("count", i64), ("lr", C.c_double), ("weight_decay", C.c_double), ("param_type", i32),
+                ("v_scale", vp), ("count", i64), ("lr", C.c_double), ("weight_decay", C.c_double), ("bc1", C.c_double),
+                ("bc2_sqrt", C.c_double), ("param_type", i32),
                 ("grad_type", i32), ("state_bits", i32), ("reserved", i32)]
 
 
 # the same packed by hand, a third of the time of their fields
 EMBEDDING_ARGS = struct.Struct("@PPqPqqqiiiifi")
 TOKEN_LOSS_ARGS = struct.Struct("@PqPPPPPPqPPPqqddddddii")
-ADAMW_TENSOR = struct.Struct("@PPPPPPPqddiiii")
+ADAMW_TENSOR = struct.Struct("@PPPPPPPqddddiiii")
 assert (EMBEDDING_ARGS.size, TOKEN_LOSS_ARGS.size, ADAMW_TENSOR.size) == tuple(
     map(C.sizeof, (EmbeddingArgs, TokenLossArgs, AdamwTensor)))
 
@@ -322,8 +323,7 @@ _SIGNATURES = [
     ("ppo_token_log_probs", C.c_int, [vp, vp, C.c_size_t, vp]),
     ("ppo_token_ppo_loss", C.c_int, [vp, vp, C.c_size_t, vp]),
     ("ppo_adamw_workspace_bytes", C.c_size_t, [vp, i32]),
-    ("ppo_adamw_step", C.c_int, [vp, i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp,
-                                 C.c_size_t, vp]),
+    ("ppo_adamw_step", C.c_int, [vp, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp, C.c_size_t, vp]),
 ]
 
 EXPORTED_SYMBOLS = [name for name, _, _ in _SIGNATURES]

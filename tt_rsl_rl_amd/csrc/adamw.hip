@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kAdamwThreads = 256, kPer = 4;
 constexpr int kChunk = kAdamwThreads * kPer;  // elements a block takes at a time
-constexpr int kMaxTensors = 48, kMaxGrads = 160;
+constexpr int kMaxTensors = 44, kMaxGrads = 160;
 constexpr int kNormChunk = 8 * kChunk, kNormBlocks = 2048;  // elements a block's loads have in flight, blocks of one norm launch
 static_assert(kChunk % PPO_ADAMW_BLOCK == 0 && PPO_ADAMW_BLOCK == kWave * kPer, "a wave owns a scale's block");
 
@@ -40,9 +40,8 @@ struct Tensor {
   void* v;
   float* m_scale;
   float* v_scale;
-  int32_t count4;  // unused low bits of the count are in tail
-  int32_t tail;
-  float neg_step, decay;
+  int64_t count;
+  float neg_step, decay, bc2_sqrt, inv_bc2_sqrt;
 };
 
 struct UpdateTable {
@@ -53,7 +52,7 @@ struct UpdateTable {
 static_assert(sizeof(UpdateTable) <= 3800, "kernel arguments");
 
 struct Scalars {
-  float w1, b2, c2, eps, bc2_sqrt, inv_bc2_sqrt;
+  float w1, b2, c2, eps;
 };
 
 // The tensor of a chunk: the last one whose first chunk is not behind it.
@@ -222,7 +221,7 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
                                                                      const float* __restrict__ coef) {
   const int k = tensor_of(t.first, t.tensors, blockIdx.x);
   const Tensor& q = t.t[k];
-  const int64_t count = static_cast<int64_t>(q.count4) * 4 + q.tail;
+  const int64_t count = q.count;
   const int64_t i = static_cast<int64_t>(static_cast<int>(blockIdx.x) - t.first[k]) * kChunk + threadIdx.x * kPer;
   const int n = static_cast<int>(max<int64_t>(0, min<int64_t>(kPer, count - i)));
   if (!BITS8 && n == 0) return;
@@ -256,9 +255,9 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
     v[e] = v[e] + (s.c2 * d) * d;
     p[e] = p[e] * q.decay;
     if (BITS8 && s.eps >= 1e-16f)  // beside the states' rounding the last bit of the step does not count
-      p[e] = p[e] + (q.neg_step * m[e]) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * s.inv_bc2_sqrt + s.eps);
+      p[e] = p[e] + (q.neg_step * m[e]) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * q.inv_bc2_sqrt + s.eps);
     else
-      p[e] = p[e] + (q.neg_step * m[e]) / (sqrtf(v[e]) / s.bc2_sqrt + s.eps);
+      p[e] = p[e] + (q.neg_step * m[e]) / (sqrtf(v[e]) / q.bc2_sqrt + s.eps);
   }
   if constexpr (BITS8) {
     // elements past the end hold zeros: g, m and v
@@ -324,18 +323,18 @@ extern "C" size_t ppo_adamw_workspace_bytes(const ppo_adamw_tensor* tensors, int
 }
 
 extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, double max_norm, double beta1, double beta2,
-                              double eps, double bc1, double bc2_sqrt, float* norm_out, void* workspace,
-                              size_t workspace_bytes, ppo_stream_t stream) {
+                              double eps, float* norm_out, void* workspace, size_t workspace_bytes,
+                              ppo_stream_t stream) {
   PPO_REQUIRE(tensors != nullptr && count >= 1, "ppo_adamw_step: %d tensors", count);
   PPO_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0, "ppo_adamw_step: beta1=%g beta2=%g eps=%g",
               beta1, beta2, eps);
-  PPO_REQUIRE(bc1 > 0.0 && bc2_sqrt > 0.0, "ppo_adamw_step: bias corrections must be positive");
   for (int i = 0; i < count; ++i) {
     const ppo_adamw_tensor& t = tensors[i];
     PPO_REQUIRE(t.count >= 0 && t.count < (int64_t{1} << 33), "ppo_adamw_step: tensor %d holds %lld elements", i, (long long)t.count);
     PPO_REQUIRE((t.param_type == PPO_TYPE_F32 || t.param_type == PPO_TYPE_BF16) &&
                     (t.grad_type == PPO_TYPE_F32 || t.grad_type == PPO_TYPE_BF16),
                 "ppo_adamw_step: tensor %d: param_type=%d grad_type=%d", i, t.param_type, t.grad_type);
+    PPO_REQUIRE(t.bc1 > 0.0 && t.bc2_sqrt > 0.0, "ppo_adamw_step: tensor %d: bias corrections must be positive", i);
     PPO_REQUIRE(t.state_bits == 32 || t.state_bits == 8, "ppo_adamw_step: tensor %d: state_bits=%d", i, t.state_bits);
     PPO_REQUIRE(t.master == nullptr || t.param_type == PPO_TYPE_BF16, "ppo_adamw_step: tensor %d: a master of an fp32 param", i);
     PPO_REQUIRE(t.param_type == PPO_TYPE_BF16 || t.grad_type == PPO_TYPE_F32, "ppo_adamw_step: tensor %d: a bf16 gradient of an fp32 param", i);
@@ -389,7 +388,7 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
     if (int rc = check_launch("adamw_clip_kernel")) return rc;
   }
   const Scalars s{static_cast<float>(1.0 - beta1), static_cast<float>(beta2), static_cast<float>(1.0 - beta2),
-                  static_cast<float>(eps), static_cast<float>(bc2_sqrt), static_cast<float>(1.0 / bc2_sqrt)};
+                  static_cast<float>(eps)};
   int64_t bytes = 0;
   for (int i = 0; i < count; ++i) {
     const ppo_adamw_tensor& t = tensors[i];
@@ -405,9 +404,9 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
         const ppo_adamw_tensor& a = tensors[i];
         if (kind_of(a) != kind || a.count == 0) continue;
         Tensor& b = t.t[t.tensors];
-        b = Tensor{a.param, a.grad, a.master, a.exp_avg, a.exp_avg_sq, a.m_scale, a.v_scale,
-                   static_cast<int32_t>(a.count / 4), static_cast<int32_t>(a.count % 4),
-                   static_cast<float>(-(a.lr / bc1)), static_cast<float>(1.0 - a.lr * a.weight_decay)};
+        b = Tensor{a.param, a.grad, a.master, a.exp_avg, a.exp_avg_sq, a.m_scale, a.v_scale, a.count,
+                   static_cast<float>(-(a.lr / a.bc1)), static_cast<float>(1.0 - a.lr * a.weight_decay),
+                   static_cast<float>(a.bc2_sqrt), static_cast<float>(1.0 / a.bc2_sqrt)};
         t.first[t.tensors++] = static_cast<int32_t>(chunks);
         chunks += chunks_of(a);
         PPO_REQUIRE(chunks < INT32_MAX, "ppo_adamw_step: too many parameters");

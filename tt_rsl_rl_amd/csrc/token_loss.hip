@@ -566,7 +566,7 @@ int launch_rows(const LossKernelArgs& q, RowPart* parts, hipStream_t st) {
   }
   // As few threads to a row as hold it, so that a compute unit has several rows in different phases.
 #define PPO_ROWS(NT, K) hipLaunchKernelGGL((token_row_kernel<T, NT, K, LOSS>), grid, dim3(NT), 0, st, q)
-  if (vocab < kVec<T> || pieces > 1024 * 16)
+  if (vocab < kVec<T> || pieces > 1024 * 25)
     hipLaunchKernelGGL((token_wide_kernel<T, LOSS>), grid, dim3(kWideThreads), 0, st, q);
   else if (pieces <= 64) PPO_ROWS(64, 1);
   else if (pieces <= 64 * 4) PPO_ROWS(64, 4);
@@ -575,7 +575,8 @@ int launch_rows(const LossKernelArgs& q, RowPart* parts, hipStream_t st) {
   else if (pieces <= 256 * 16) PPO_ROWS(256, 16);
   else if (pieces <= 512 * 16) PPO_ROWS(512, 16);
   else if (pieces <= 512 * 25) PPO_ROWS(512, 25);
-  else PPO_ROWS(1024, 16);
+  else if (pieces <= 1024 * 16) PPO_ROWS(1024, 16);
+  else PPO_ROWS(1024, 25);
 #undef PPO_ROWS
   if (int rc = check_launch("token_row_kernel")) return rc;
   if (!LOSS) return PPO_OK;

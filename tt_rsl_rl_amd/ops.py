@@ -1191,7 +1191,7 @@ def token_ppo_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.T
     L.call("ppo_token_ppo_loss", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
 
 
-def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step: int, lr, beta1: float = 0.9,
+def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step, lr, beta1: float = 0.9,
                beta2: float = 0.999, eps: float = 1e-8, weight_decay=1e-2, max_grad_norm: float | None = None,
                masters: list | None = None, scales: tuple[list, list] | None = None, norm_out: torch.Tensor | None = None,
                ws: Workspace | None = None) -> None:
@@ -1199,16 +1199,16 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step:
     (max_grad_norm; the gradients themselves are left as they are).  params: float32, or bfloat16 with (masters) or without
     a float32 master each, in which case the master is stepped and the parameter is its rounding; grads: float32, or
     bfloat16 for a bfloat16 parameter; exp_avg / exp_avg_sq: float32, or int8 / uint8 with scales = (lists of) float32
-    [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  lr, weight_decay: one value, or one per tensor.
-    step counts from 1.  norm_out: float32 [2] for the norm and the clip coefficient."""
+    [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  step (from 1), lr and weight_decay: one
+    value, or one per tensor.  norm_out: float32 [2] for the norm and the clip coefficient."""
     n = len(params)
-    each_lr, each_wd = isinstance(lr, (list, tuple)), isinstance(weight_decay, (list, tuple))
+    each_step, each_lr, each_wd = (isinstance(x, (list, tuple)) for x in (step, lr, weight_decay))
     for name, v in (("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("masters", masters),
                     ("scales", scales and scales[0]), ("scales", scales and scales[1]), ("lr", lr if each_lr else None),
-                    ("weight_decay", weight_decay if each_wd else None)):
+                    ("weight_decay", weight_decay if each_wd else None), ("step", step if each_step else None)):
         if v is not None and len(v) != n:
             raise ValueError(f"adamw_step: {len(v)} {name} for {n} params")
-    if step < 1:
+    if n and (min(step) if each_step else step) < 1 or not each_step and step < 1:
         raise ValueError(f"adamw_step: step={step} (the first is 1)")
     if max_grad_norm is not None and not max_grad_norm > 0:
         raise ValueError(f"adamw_step: max_grad_norm={max_grad_norm}")
@@ -1246,12 +1246,13 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step:
                     or scales[0][i].dtype != f32 or scales[1][i].dtype != f32):
                 raise ValueError(f"adamw_step: tensor {i}: states {mtype}, {vtype} (float32, or int8 and uint8 with float32 scales)")
         kinds.append((L.TYPE_F32 if ptype == f32 else L.TYPE_BF16, L.TYPE_F32 if gtype == f32 else L.TYPE_BF16, bits, 0))
+    corrections = {k: (1.0 - beta1**k, math.sqrt(1.0 - beta2**k)) for k in (set(step) if each_step else (step,))}
     packed = b"".join(map(L.ADAMW_TENSOR.pack, *columns, counts, lr if each_lr else [lr] * n,
-                          weight_decay if each_wd else [weight_decay] * n, *zip(*kinds)))
+                          weight_decay if each_wd else [weight_decay] * n,
+                          *zip(*([corrections[k] for k in step] if each_step else [corrections[step]] * n)), *zip(*kinds)))
     buf = None
     if max_grad_norm is not None or norm_out is not None:
         _vector(norm_out, "adamw_step: norm_out", 2)
         buf = _scratch(ws, params[0].device, L.load().ppo_adamw_workspace_bytes(packed, n))
     L.call("ppo_adamw_step", packed, n, float(max_grad_norm or 0.0), float(beta1), float(beta2), float(eps),
-           1.0 - beta1**step, math.sqrt(1.0 - beta2**step), _ptr(norm_out), _ptr(buf), 0 if buf is None else buf.numel(),
-           _raw_stream(dev))
+           _ptr(norm_out), _ptr(buf), 0 if buf is None else buf.numel(), _raw_stream(dev))
