@@ -93,6 +93,27 @@ def test_adamw_state_round_trip(cuda, bits, dtype, tmp_path):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_mixed_types(cuda, bits):
+    """fp32 and bf16 parameters in one optimiser, with and without masters: what each gets alone."""
+    from tt_rsl_rl_amd.tokens import AdamW
+
+    for masters in (True, False):
+        together = [_params(cuda, torch.float32)[0], _params(cuda, torch.bfloat16)[1], _params(cuda, torch.float32)[2]]
+        alone = [torch.nn.Parameter(p.detach().clone()) for p in together]
+        opt, each = AdamW(together, lr=1e-2, state_bits=bits, masters=masters), [AdamW([p], lr=1e-2, state_bits=bits, masters=masters) for p in alone]
+        g = torch.Generator().manual_seed(4)
+        for _ in range(3):
+            for p, q in zip(together, alone):
+                p.grad = torch.randn(*p.shape, generator=g).to(device=cuda, dtype=p.dtype)
+                q.grad = p.grad.clone()
+            opt.step()
+            for o in each:
+                o.step()
+        for p, q in zip(together, alone):
+            assert torch.equal(p, q)
+
+
 def test_example_learns(cuda):
     spec = importlib.util.spec_from_file_location("token_policy", ROOT / "examples" / "token_policy.py")
     example = importlib.util.module_from_spec(spec)

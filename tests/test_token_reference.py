@@ -5,12 +5,16 @@ from __future__ import annotations
 
 import ctypes
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
 
 from tests import token_reference as ref
 
+ROOT = Path(__file__).resolve().parent.parent
 INF = float("inf")
 
 
@@ -173,3 +177,54 @@ def test_tensors_on_the_cpu_are_refused():
     with pytest.raises(ValueError, match="step"):
         ops.adamw_step([x], [x], [x], [x], step=0, lr=1e-3)
     ops.adamw_step([], [], [], [], step=1, lr=1e-3)
+
+
+def test_adamw_table_refuses_what_is_no_list_of_tensors():
+    from tt_rsl_rl_amd import ops
+
+    x = torch.zeros(2, 4)
+    for call, what in ((lambda: ops.adamw_step([x], [None], [x], [x], step=1, lr=1e-3), r"grads\[0\]"),
+                       (lambda: ops.adamw_step([1.0], [x], [x], [x], step=1, lr=1e-3), r"params\[0\]"),
+                       (lambda: ops.adamw_step([x], [x], [x], [x], step=[1, 2], lr=1e-3), "step for"),
+                       (lambda: ops.adamw_step([x], [x], [x], [x], step=[0], lr=1e-3), "step of tensor 0"),
+                       (lambda: ops.adamw_step([x], [x], [x], [x], step=1, lr=[1e-3, 1e-3]), "lr for"),
+                       (lambda: ops.adamw_step([x], [x], [x], [x], step=1, lr=1e-3, masters=[]), "masters for"),
+                       (lambda: ops.adamw_step([x], [x], [x], [x], step=1, lr=1e-3, scales=([], [])), "scales for")):
+        with pytest.raises(ValueError, match=what):
+            call()
+    with pytest.raises(TypeError):
+        ops.adamw_step([x], [x], [x], [x], step="one", lr=1e-3)
+    with pytest.raises(TypeError):
+        ops.adamw_step([x], 3, [x], [x], step=1, lr=1e-3)
+
+
+STRUCTS = {
+    "ppo_embedding_args": ("EmbeddingArgs", ["tokens", "src", "ld_src", "dst", "ld_dst", "count", "vocab", "dim", "token_type", "src_type",
+                                             "dst_type", "scale", "accumulate"]),
+    "ppo_token_loss_args": ("TokenLossArgs", ["logits", "ld_logits", "tokens", "mask", "old_logp", "ref_logp", "advantages", "d_logits",
+                                              "ld_d_logits", "logp", "entropy", "stats", "rows", "vocab", "clip_low", "clip_high", "kl_coef",
+                                              "entropy_coef", "temperature", "denom", "type", "token_type"]),
+    "ppo_adamw_tensor": ("AdamwTensor", ["param", "grad", "master", "exp_avg", "exp_avg_sq", "m_scale", "v_scale", "count", "lr", "weight_decay",
+                                         "bc1", "bc2_sqrt", "param_type", "grad_type", "state_bits", "reserved"]),
+}
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+def test_struct_layouts_match_the_c_compiler(tmp_path):
+    from tt_rsl_rl_amd import _lib
+
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{ROOT / "include" / "ppo_hip.h"}"', "int main(void) {"]
+    for cname, (_, fields) in STRUCTS.items():
+        lines.append(f'printf("%zu\\n", sizeof({cname}));')
+        lines += [f'printf("%zu\\n", offsetof({cname}, {f}));' for f in fields]
+    for macro in ("PPO_ADAMW_BLOCK", "PPO_TYPE_F32", "PPO_TYPE_BF16", "PPO_TYPE_F16", "PPO_TOKENS_I64", "PPO_TOKENS_I32"):
+        lines.append(f'printf("%d\\n", (int){macro});')
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c11", str(src), "-o", str(exe)], check=True)
+    got = list(map(int, subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()))
+    want = []
+    for pyname, fields in STRUCTS.values():
+        cls = getattr(_lib, pyname)
+        want += [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f in fields]
+    assert got == want + [_lib.ADAMW_BLOCK, _lib.TYPE_F32, _lib.TYPE_BF16, _lib.TYPE_F16, _lib.TOKENS_I64, _lib.TOKENS_I32]

@@ -227,9 +227,7 @@ class AdamwTensor(C.Structure):
 # the same packed by hand, a third of the time of their fields
 EMBEDDING_ARGS = struct.Struct("@PPqPqqqiiiifi")
 TOKEN_LOSS_ARGS = struct.Struct("@PqPPPPPPqPPPqqddddddii")
-ADAMW_TENSOR = struct.Struct("@PPPPPPPqddddiiii")
-assert (EMBEDDING_ARGS.size, TOKEN_LOSS_ARGS.size, ADAMW_TENSOR.size) == tuple(
-    map(C.sizeof, (EmbeddingArgs, TokenLossArgs, AdamwTensor)))
+assert (EMBEDDING_ARGS.size, TOKEN_LOSS_ARGS.size) == (C.sizeof(EmbeddingArgs), C.sizeof(TokenLossArgs))
 
 # (name, restype, argtypes)
 _SIGNATURES = [
@@ -350,6 +348,16 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     if path is None:
         _lib = lib
     return lib
+
+
+def tensor_table():
+    """The module that makes ppo_adamw_step's table from lists of tensors (csrc/tensor_table.cpp), built beside the library."""
+    try:
+        from . import _tensor_table
+    except ImportError as e:
+        raise RuntimeError(f"{__package__}._tensor_table is missing or not of this torch: build the HIP library first "
+                           f"(python -m tt_rsl_rl_amd.build): {e}") from e
+    return _tensor_table
 
 
 def last_error() -> str:

@@ -1,7 +1,8 @@
 """Build libppo_hip.so (all HIP sources under csrc/) for gfx950 with hipcc, in-tree.
 
 Usage: ``python -m tt_rsl_rl_amd.build`` (or ``__graft_entry__.build()``).  Sources are compiled in parallel
-to objects under ``csrc/_build/`` and linked into ``tt_rsl_rl_amd/libppo_hip.so``.
+to objects under ``csrc/_build/`` and linked into ``tt_rsl_rl_amd/libppo_hip.so``.  Beside it the host compiler builds
+``tt_rsl_rl_amd/_tensor_table.so`` (csrc/tensor_table.cpp), the one part that reads torch's objects.
 """
 
 from __future__ import annotations
@@ -18,6 +19,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD_DIR = CSRC / "_build"
 LIB = PKG / "libppo_hip.so"
+TABLE = PKG / "_tensor_table.so"
 ARCH = os.environ.get("PPO_HIP_ARCH", "gfx950")
 
 # -packed-fp32-ops: hipcc must not form v_pk_{add,mul,fma}_f32 by itself on this target.
@@ -57,14 +59,35 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def _compile_table() -> None:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: it builds the module that reads torch's tensors")
+    tmp = TABLE.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in include_paths()), f"-I{sysconfig.get_paths()['include']}", str(CSRC / "tensor_table.cpp"), "-o", str(tmp),
+           *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on tensor_table.cpp:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, TABLE)
+
+
 def build(verbose: bool = True) -> Path:
-    """Compile every csrc/*.hip and link libppo_hip.so.  Always rebuilds."""
+    """Compile every csrc/*.hip and link libppo_hip.so, and build _tensor_table.so.  Always rebuilds."""
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     srcs = sources()
     if not srcs:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
+        table = pool.submit(_compile_table)
         objs = list(pool.map(_compile, srcs))
+        table.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)

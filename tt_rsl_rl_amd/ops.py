@@ -8,7 +8,6 @@ on a GPU are rejected.
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -1201,58 +1200,20 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step,
     bfloat16 for a bfloat16 parameter; exp_avg / exp_avg_sq: float32, or int8 / uint8 with scales = (lists of) float32
     [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  step (from 1), lr and weight_decay: one
     value, or one per tensor.  norm_out: float32 [2] for the norm and the clip coefficient."""
-    n = len(params)
-    each_step, each_lr, each_wd = (isinstance(x, (list, tuple)) for x in (step, lr, weight_decay))
-    for name, v in (("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("masters", masters),
-                    ("scales", scales and scales[0]), ("scales", scales and scales[1]), ("lr", lr if each_lr else None),
-                    ("weight_decay", weight_decay if each_wd else None), ("step", step if each_step else None)):
-        if v is not None and len(v) != n:
-            raise ValueError(f"adamw_step: {len(v)} {name} for {n} params")
-    if n and (min(step) if each_step else step) < 1 or not each_step and step < 1:
-        raise ValueError(f"adamw_step: step={step} (the first is 1)")
     if max_grad_norm is not None and not max_grad_norm > 0:
         raise ValueError(f"adamw_step: max_grad_norm={max_grad_norm}")
+    n = len(params)
+    dev = _get_device() if n and getattr(params[0], "is_cuda", False) else -1
+    m_scales, v_scales = scales if scales is not None else (None, None)
+    packed = L.tensor_table().adamw_table(params, grads, masters, exp_avg, exp_avg_sq, m_scales, v_scales, step, lr, weight_decay, beta1,
+                                          beta2, dev)
     if n == 0:
         return
-    dev = _current_gpu("adamw_step", params[0], norm_out)
-    T, f32, bf16 = torch.Tensor, torch.float32, torch.bfloat16
-    counts = [t.numel() for t in params]
-    columns = []  # each list's pointers, in AdamwTensor's order, checked (through map: a call of Python's own per tensor costs more than the check)
-    for name, ts, sizes in (("params", params, counts), ("grads", grads, counts), ("masters", masters, counts),
-                            ("exp_avg", exp_avg, counts), ("exp_avg_sq", exp_avg_sq, counts), ("scales", scales and scales[0], None), ("scales", scales and scales[1], None)):
-        if ts is None:
-            columns.append([0] * n)
-            continue
-        if sizes is None or name == "masters" and any(t is None for t in ts):  # lists that need not hold a tensor for each parameter
-            columns.append([0 if t is None else t.data_ptr() for t in ts])
-            sizes = sizes or [-(-c // L.ADAMW_BLOCK) for c in counts]
-            ts, sizes = zip(*[(t, c) for t, c in zip(ts, sizes) if t is not None]) if any(t is not None for t in ts) else ((), ())
-        else:
-            columns.append(list(map(T.data_ptr, ts)))
-        if not (all(map(T.is_contiguous, ts)) and set(map(T.get_device, ts)) <= {dev} and list(map(T.numel, ts)) == list(sizes)):
-            raise ValueError(f"adamw_step: {name} must be contiguous tensors of the parameters' sizes (scales: a value for each "
-                             f"{L.ADAMW_BLOCK} elements) on GPU {dev}, got {[(tuple(t.shape), t.stride(), str(t.device)) for t in ts]}")
-    kinds = []
-    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avg, exp_avg_sq)):
-        ptype, gtype, mtype, vtype = p.dtype, g.dtype, m.dtype, v.dtype
-        if (ptype != f32 and ptype != bf16) or (gtype != f32 and gtype != ptype):
-            raise ValueError(f"adamw_step: tensor {i}: parameter {ptype}, gradient {gtype}")
-        if columns[2][i] and (masters[i].dtype != f32 or ptype != bf16):
-            raise ValueError(f"adamw_step: masters[{i}] must be float32, of a bfloat16 parameter")
-        bits = 32
-        if mtype != f32 or vtype != f32:
-            bits = 8
-            if (mtype != torch.int8 or vtype != torch.uint8 or scales is None or scales[0][i] is None or scales[1][i] is None
-                    or scales[0][i].dtype != f32 or scales[1][i].dtype != f32):
-                raise ValueError(f"adamw_step: tensor {i}: states {mtype}, {vtype} (float32, or int8 and uint8 with float32 scales)")
-        kinds.append((L.TYPE_F32 if ptype == f32 else L.TYPE_BF16, L.TYPE_F32 if gtype == f32 else L.TYPE_BF16, bits, 0))
-    corrections = {k: (1.0 - beta1**k, math.sqrt(1.0 - beta2**k)) for k in (set(step) if each_step else (step,))}
-    packed = b"".join(map(L.ADAMW_TENSOR.pack, *columns, counts, lr if each_lr else [lr] * n,
-                          weight_decay if each_wd else [weight_decay] * n,
-                          *zip(*([corrections[k] for k in step] if each_step else [corrections[step]] * n)), *zip(*kinds)))
     buf = None
     if max_grad_norm is not None or norm_out is not None:
-        _vector(norm_out, "adamw_step: norm_out", 2)
+        if norm_out is not None:
+            _current_gpu("adamw_step", norm_out)
+            _vector(norm_out, "adamw_step: norm_out", 2)
         buf = _scratch(ws, params[0].device, L.load().ppo_adamw_workspace_bytes(packed, n))
     L.call("ppo_adamw_step", packed, n, float(max_grad_norm or 0.0), float(beta1), float(beta2), float(eps),
            _ptr(norm_out), _ptr(buf), 0 if buf is None else buf.numel(), _raw_stream(dev))

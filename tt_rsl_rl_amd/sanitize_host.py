@@ -4,7 +4,8 @@
 on the host code only (device code is compiled as usual, unsanitized), links ``tt_rsl_rl_amd/libppo_hip_asan.so``, and
 runs the tests that call the library's host paths without a GPU -- the C ABI's argument validation and status codes
 (tests/test_lib_abi.py: every entry point's checks, struct layouts, the MT19937 / randperm ranges of the native
-permutation) and the CPU-generator skipping (tests/test_host_rng.py) -- in a child process with the sanitizer runtime
+permutation), the CPU-generator skipping (tests/test_host_rng.py) and the token operators' argument checks
+(tests/test_token_reference.py) -- in a child process with the sanitizer runtime
 preloaded.  Any sanitizer report aborts the run (halt_on_error, no recovery from undefined behaviour).  Leak checks are
 off: the Python interpreter itself keeps allocations until exit.
 """
@@ -24,7 +25,7 @@ BUILD_DIR = B.CSRC / "_build_asan"
 # the sanitizers apply to the host compilation only: each host flag goes behind its own -Xarch_host
 HOST_SANITIZE = ["-Xarch_host", "-fsanitize=address,undefined", "-Xarch_host", "-fno-sanitize-recover=undefined",
                  "-Xarch_host", "-fno-omit-frame-pointer", "-Xarch_host", "-g"]
-TESTS = ["tests/test_lib_abi.py", "tests/test_host_rng.py"]
+TESTS = ["tests/test_lib_abi.py", "tests/test_host_rng.py", "tests/test_token_reference.py"]
 
 
 def _compile(src: Path) -> Path:
