@@ -769,7 +769,8 @@ int ppo_embedding_fwd(const ppo_embedding_args* args, ppo_stream_t stream);
 size_t ppo_embedding_bwd_workspace_bytes(int64_t count, int64_t vocab, int32_t dim);
 int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
 
-/* Log-probabilities and the clipped policy loss of tokens.  Row r with z = logits[r, :] / temperature and t = tokens[r]:
+/* Log-probabilities and the clipped policy loss of tokens.  Row r with z = logits[r, :] / temperature (1e-6 to 1e6) and
+ * t = tokens[r]:
  *   lp = z_t - log sum_j exp(z_j);   p_j = exp(z_j - log sum exp z);   H = -sum_j p_j log p_j   (0 where p_j is 0);
  *   ratio = exp(lp - old_logp);   s = max(-A ratio, -A min(max(ratio, 1 - clip_low), 1 + clip_high));
  *   d = ref_logp - lp;   k = exp(d) - d - 1   (the estimate of KL(policy || reference) that is never negative);

@@ -7,5 +7,6 @@ kernels of ``libppo_hip.so`` (C ABI: ``include/ppo_hip.h``), loaded through ctyp
 from .models import EmpiricalNormalization, GaussianDistribution, MLPModel
 from .ppo import PPO, HipPPO
 from .storage import RolloutStorage
+from .tokens import AdamW, TokenEmbedding
 
-__all__ = ["PPO", "HipPPO", "MLPModel", "GaussianDistribution", "EmpiricalNormalization", "RolloutStorage"]
+__all__ = ["PPO", "HipPPO", "MLPModel", "GaussianDistribution", "EmpiricalNormalization", "RolloutStorage", "TokenEmbedding", "AdamW"]

@@ -14,7 +14,7 @@ namespace {
 // ---- forward ----
 
 // A thread moves one 16-byte piece of each of kFwdRows rows; a block's threads lie side by side on a row as far as it reaches.
-// 16,384 rows of 2,048 bf16: 18.4 us, 5.0 TB/s of the 93 MB that have to move.
+// 16,384 rows of 2,048 bf16: 17.8 us, 5.2 TB/s of the 93 MB that have to move.
 constexpr int kFwdThreads = 256, kFwdRows = 4;  // rows in flight per thread
 
 template <class T>
@@ -358,6 +358,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_move_kernel(const ppo_embed
 
 // ---- the sums ----
 
+// 131,072 bf16 rows of 1,024 into 65,536 fp32 rows: 74 us, 274 MB read and 118 written, 5.3 TB/s; the joins 12, the sort with the
+// zeros 53.
 // The sorted positions are cut into units; a wave sums a unit's rows over 64 16-byte pieces of columns.  A run of one token
 // that crosses into the next unit by at most kReach rows is finished where it began, and the next unit starts behind it.  A run
 // that goes on further leaves its parts in `partial` ([units][2][dim]: of the run that came into the unit, of the one that goes
