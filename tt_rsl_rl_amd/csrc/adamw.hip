@@ -11,7 +11,7 @@
 // smallest sqrt(v) 1.5e-5 of it.  A wave owns a block of elements, four per lane, so the new scale is one wave reduction.
 //
 // Bound by memory: 28 bytes per fp32 parameter with fp32 states, and the gradient once more for the norm.
-// 60 M bf16 with masters: update 268 us, 6.3 TB/s, norm 39; 250 M with 8-bit states: update 703 us, 5.8 TB/s, norm 124.
+// 60 M bf16 with masters: update 268 us, 6.3 TB/s, norm 25; 250 M with 8-bit states: update 705 us, 5.8 TB/s, norm 115.
 #include "elem.hpp"
 
 #pragma clang fp contract(off)
@@ -122,23 +122,24 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_norm_kernel(const NormTab
     const int64_t from = static_cast<int64_t>(c - t.first[k]) * kNormChunk;
     const int left = static_cast<int>(min<int64_t>(kNormChunk, t.count[k] - from));
     g += from;
-    if (left == kNormChunk) {
-      RawPiece x[K];
+    // (the pieces of a tensor's last chunk are in flight together too: with its elements one after another a thread waited for up
+    // to 32 loads in a row, and 150 tensors of 60 M bf16 took 39 us, 25 now)
+    RawPiece x[K];
 #pragma unroll
-      for (int i = 0; i < K; ++i) x[i] = load_raw(g + (i * kAdamwThreads + static_cast<int>(threadIdx.x)) * V);
-#pragma unroll
-      for (int i = 0; i < K; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const double d = element<G>(x[i], e);
-          sum[e % 4] = fma(d, d, sum[e % 4]);
-        }
-    } else {
-      for (int i = threadIdx.x; i < left; i += kAdamwThreads) {
-        const double d = static_cast<float>(g[i]);
-        sum[0] = fma(d, d, sum[0]);
-      }
+    for (int i = 0; i < K; ++i) {
+      const int at = (i * kAdamwThreads + static_cast<int>(threadIdx.x)) * V;
+      x[i] = at + V <= left ? load_raw(g + at) : RawPiece{};
     }
+    const int rest = left / V * V + static_cast<int>(threadIdx.x);  // the elements behind the last whole piece
+    const double odd = rest < left ? static_cast<double>(static_cast<float>(g[rest])) : 0.0;
+    sum[0] = fma(odd, odd, sum[0]);
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const double d = element<G>(x[i], e);
+        sum[e % 4] = fma(d, d, sum[e % 4]);
+      }
   }
   const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), red);
   if (threadIdx.x == 0) partial[blockIdx.x] = all;
@@ -186,7 +187,7 @@ __device__ __forceinline__ float block_scale(const float (&x)[kPer]) {
 
 // The codes of a block's four values: round(127 sqrt(x / scale)) and round(255 sqrt(sqrt(x / scale))), with every operation
 // correctly rounded, so that they are what any implementation in this order gives.  Correctly rounded quotients and roots take
-// ten instructions each and bound the kernel (250 M parameters: 1,026 us so, 703 as below), so they are computed
+// ten instructions each and bound the kernel (250 M parameters: 1,026 us so, 705 as below), so they are computed
 // from the hardware's reciprocal and root first (one unit in the last place each).  Those differ by less than 127 * 4e-7 and
 // 255 * 5e-7 codes; only where a value lies that near the middle between two codes, twice as near for safety, the wave
 // computes it the long way.
