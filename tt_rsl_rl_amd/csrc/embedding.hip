@@ -139,6 +139,8 @@ __device__ __forceinline__ uint32_t key_at(const ppo_embedding_args& a, int64_t 
 // tokens, which lie in scalar registers: two instructions each.  The loop is kept short and rolled: as straight-line code of
 // ten KB, and with a scalar count of each comparison's bits, it took 14 us for 5,003 tokens, most of it fetching instructions.
 // The time goes with count^2, but a sort of as many tokens in one block's LDS leaves the other compute units idle (16 us).
+// Four waves: gradients of 5,003 tokens take 22.6 us so, 28.9 with one, 26.0 with two, 25.6 with eight, 32.5 with sixteen (12,000:
+// 38.9, 52.5, 45.0, 44.4, 52.5): fewer wait for more loads in a row, more repeat the set-up and the exchanges at the end.
 constexpr int kRankThreads = 256, kRankWaves = kRankThreads / kWave, kRankOwn = 16;
 static_assert(4 * kRankOwn == kWave, "the reduction's exchanges");
 static_assert(kWave % kRankOwn == 0, "a block's tokens lie in one group of 64");
