@@ -1,18 +1,21 @@
 // Token log-probabilities and the clipped policy loss with a KL term, forward and gradient (ppo_token_log_probs,
 // ppo_token_ppo_loss): the categorical counterpart of loss.hip's Gaussian head.
 //
-// With c = log2(e) / temperature, m = max_j x_j and t_j = c x_j - c m:
+// With c = log2(e) / temperature, m = max_j x_j and t_j = c (x_j - m):
 //   S = sum_j 2^t_j,  E = sum_j 2^t_j t_j,  lp = ln2 (t_token - log2 S),  H = ln2 (log2 S - E / S),
 //   d_logits_j = 2^t_j (A + B t_j) + [j = token] g k,
 //   k = 1 / (N temperature),  B = k entropy_coef ln2 / S,  A = k (entropy_coef H - g) / S - B log2 S
-// (p_j = 2^t_j / S and log p_j = ln2 (t_j - log2 S) put into the header's formula; t_j is one fused multiply-add, so the
-// rounding of c m is the same in every term and cancels).  A logit of -inf has 2^t = 0 exactly; where t itself is a factor it
-// is raised to kFloor, 2^kFloor being 0 too, so that 0 t stays 0.
+// (p_j = 2^t_j / S and log p_j = ln2 (t_j - log2 S) put into the header's formula).  The difference comes first: next to the
+// maximum it is exact, however far from zero the row lies.  As one fused multiply-add, c x_j - (c m), t_j would carry the rounding
+// of c m, half an ulp of it and another one for each part's m: rows at 1e4 were 3e-4 off, rows masked by -1e10 not finite.
+// A logit of -inf has 2^t = 0 exactly; where t itself is a factor it is raised to kFloor, 2^kFloor being 0 too, so that 0 t
+// stays 0.
 //
 // Bound by memory: the logits once in, their gradient once out.  So a row is read once and stays in registers between its
 // sums and its gradient (token_row_kernel); only rows too wide for that are read twice (token_wide_kernel).  Each wave
 // takes its own maximum and sums, and the waves' (m, S, E) are joined after the one barrier of a row.
-// 8,192 x 131,072 bf16, a quarter of the rows masked: 710 us a call, 5.3 TB/s; log-probabilities of 8,192 x 32,000: 69 us.
+// 8,192 x 131,072 bf16, a quarter of the rows masked: 710 us a call, 5.3 TB/s; log-probabilities of 8,192 x 32,000: 73 us
+// (70 with the fused multiply-add above).
 #include "elem.hpp"
 
 namespace ppo {
@@ -82,10 +85,6 @@ __global__ __launch_bounds__(kCountThreads) void token_count_kernel(const LossKe
   }
 }
 
-// c, or where c m would not be finite a power of two that keeps it so: floats as large as that lie so far apart that
-// 2^t is 1 for the maximum itself and 0 for anything below it with either.
-__device__ __forceinline__ float scale_for(float m, float c) { return fabsf(m * c) < 1e30f ? c : 0x1p-20f; }
-
 struct RowSums {
   float m, s, e;
 };
@@ -95,8 +94,7 @@ __device__ __forceinline__ RowSums join(const RowSums& u, const RowSums& v, floa
 #pragma clang fp contract(off)
   RowSums o;  // (no fused multiply-add: the same bits whichever part comes first)
   o.m = fmaxf(u.m, v.m);
-  const float ce = scale_for(o.m, c);
-  const float du = u.m == o.m ? 0.0f : fmaxf((u.m - o.m) * ce, kFloor), dv = v.m == o.m ? 0.0f : fmaxf((v.m - o.m) * ce, kFloor);
+  const float du = u.m == o.m ? 0.0f : fmaxf((u.m - o.m) * c, kFloor), dv = v.m == o.m ? 0.0f : fmaxf((v.m - o.m) * c, kFloor);
   const float fu = __builtin_amdgcn_exp2f(du), fv = __builtin_amdgcn_exp2f(dv);
   o.s = u.s * fu + v.s * fv;
   o.e = (u.e + u.s * du) * fu + (v.e + v.s * dv) * fv;
@@ -147,9 +145,9 @@ __device__ __forceinline__ RowTerms row_terms(const LossKernelArgs& q, int64_t r
   return o;
 }
 
-// What its gradient needs: t = fma(x, c, -mc), d = 2^t (a + b t), + at at the token.
+// What its gradient needs: t = (x - m) c, d = 2^t (a + b t), + at at the token.
 struct RowCoefs {
-  float c, mc, a, b, at;
+  float c, m, a, b, at;
   bool live;
 };
 
@@ -180,8 +178,7 @@ __device__ __forceinline__ RowCoefs finish_row(const LossKernelArgs& q, int64_t 
 #pragma unroll
       for (int i = 0; i < kTerms; ++i) q.terms[r * kTermStride + i] = u.term[i];
   }
-  RowCoefs o{scale_for(mine.m, q.c), 0.0f, 0.0f, 0.0f, 0.0f, u.live};
-  o.mc = mine.m * o.c;
+  RowCoefs o{q.c, mine.m, 0.0f, 0.0f, 0.0f, u.live};
   if (LOSS && u.live) {
     const float inv_n = q.count == 1 ? 1.0f / static_cast<float>(counted) : q.count == 2 ? *q.inv_n : q.given_inv_n;
     const float k = inv_n * q.inv_temp, inv_s = 1.0f / mine.s;
@@ -214,7 +211,7 @@ __device__ __forceinline__ void skip_row(const LossKernelArgs& q, int64_t r) {
 }
 
 __device__ __forceinline__ float gradient_of(float x, const RowCoefs& o) {
-  const float t = fmaxf(fmaf(x, o.c, -o.mc), kFloor);
+  const float t = fmaxf((x - o.m) * o.c, kFloor);
   return __builtin_amdgcn_exp2f(t) * fmaf(o.b, t, o.a);
 }
 
@@ -244,7 +241,7 @@ struct RowPieces {
   }
 
   // The wave's maximum and sums.
-  __device__ __forceinline__ RowSums sums(float scale) {
+  __device__ __forceinline__ RowSums sums(float c) {
     RowSums mine{-INFINITY, 0.0f, 0.0f};
     forget(tid);  // (columns are computed again where they are needed, not kept)
 #pragma unroll
@@ -261,13 +258,13 @@ struct RowPieces {
       __builtin_amdgcn_sched_barrier(0);  // one piece at a time: its converted values are gone before the next one's
     }
     mine.m = wave_max(mine.m);
-    const float c = scale_for(mine.m, scale), mc = mine.m > -INFINITY ? mine.m * c : 0.0f;
+    const float m = mine.m > -INFINITY ? mine.m : 0.0f;  // (nothing but -inf: sums of 0)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (some(k)) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float t = fmaf(element<T>(raw[k], e), c, -mc), p = __builtin_amdgcn_exp2f(t);
+          const float t = (element<T>(raw[k], e) - m) * c, p = __builtin_amdgcn_exp2f(t);
           mine.s += p;
           mine.e = fmaf(p, fmaxf(t, kFloor), mine.e);
         }
@@ -519,10 +516,10 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
     for (int e = 0; e < V; ++e) part.m = fmaxf(part.m, v[e]);
     const float m = fmaxf(part.m, mine.m);
     if (m > mine.m) mine = join(mine, RowSums{m, 0.0f, 0.0f}, q.c);
-    const float c = scale_for(m, q.c), mc = m > -INFINITY ? m * c : 0.0f;
+    const float from = m > -INFINITY ? m : 0.0f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float t = fmaf(v[e], c, -mc), p = __builtin_amdgcn_exp2f(t);
+      const float t = (v[e] - from) * q.c, p = __builtin_amdgcn_exp2f(t);
       mine.s += p;
       mine.e = fmaf(p, fmaxf(t, kFloor), mine.e);
     }
