@@ -126,3 +126,19 @@ def test_infinite_logits_beside_masks(cuda, vocab):
     want = torch.log_softmax(x.double(), 1)[:, vocab - 1]
     err = (lp.cpu().double() - want).abs()[~bad]
     assert float(err.max()) < _loss_error(x[:3], vocab, 1.0) * (1 + float(want[~bad].abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [50, 9000, 16384, 20011, 50021, 65536, 100003, 131072, 140001])
+def test_means_are_of_the_returned_values(cuda, dtype, vocab):
+    """One row that counts among others: its means are the logp and entropy that the call returns, to the bit, also where a row's
+    parts are joined by several blocks and its means by another."""
+    ops, g, rows = _ops(), _gen(vocab), 40
+    x = (torch.randn(rows, vocab, generator=g) * 3).to(dtype).to(cuda)
+    tok = torch.randint(0, vocab, (rows,), generator=g).to(cuda)
+    zero, lp, h, stats = torch.zeros(rows, device=cuda), torch.empty(rows, device=cuda), torch.empty(rows, device=cuda), torch.empty(8, device=cuda)
+    for r in range(0, rows, 3):
+        mask = torch.zeros(rows, dtype=torch.bool, device=cuda)
+        mask[r] = True
+        ops.token_ppo_loss(x, tok, zero, zero, torch.empty_like(x), stats, logp=lp, entropy=h, mask=mask)
+        assert (float(stats[5]), float(stats[3])) == (-float(lp[r]), float(h[r]))
