@@ -1,5 +1,5 @@
-"""Values of the token loss where fp32 loses them easily: logits far from zero.  The bars are those of
-tests/test_gpu_token_ops.py, which go by how far logits lie below their row's largest and by nothing else."""
+"""Values of the token loss where fp32 loses them easily: logits far from zero, and a policy close to its reference.  The bars
+are those of tests/test_gpu_token_ops.py, which go by how far logits lie below their row's largest and by nothing else."""
 
 from __future__ import annotations
 
@@ -142,3 +142,43 @@ def test_means_are_of_the_returned_values(cuda, dtype, vocab):
         mask[r] = True
         ops.token_ppo_loss(x, tok, zero, zero, torch.empty_like(x), stats, logp=lp, entropy=h, mask=mask)
         assert (float(stats[5]), float(stats[3])) == (-float(lp[r]), float(h[r]))
+
+
+def _near_reference(cuda, vocab, sizes):
+    """logp as the loss itself computes it, and a reference that lies d from it, exactly."""
+    ops, g, rows = _ops(), _gen(vocab), len(sizes)
+    x = (torch.randn(rows, vocab, generator=g)).to(cuda)
+    tok = torch.randint(0, vocab, (rows,), generator=g).to(cuda)
+    lp, stats, zero = torch.empty(rows, device=cuda), torch.empty(8, device=cuda), torch.zeros(rows, device=cuda)
+    ops.token_ppo_loss(x, tok, zero, zero, torch.empty_like(x), stats, logp=lp)
+    refs = (lp.double() + sizes.to(cuda).double()).float()
+    return x, tok, lp, refs, refs.double() - lp.double()  # (fp32's own difference is exact: they lie within a factor of 2)
+
+
+@pytest.mark.parametrize("vocab", [64, 700, 20011])
+@pytest.mark.parametrize("size", [1e-6, 1e-5, 1e-4, 1e-3, 1e-2, 0.2, 0.3, 0.9])
+def test_kl_near_the_reference(cuda, vocab, size):
+    """k = exp(d) - d - 1 to 16 U of itself and never negative (a polynomial: 8 operations; exp - 1 less d: U |exp(d) - 1| / k, 9 U
+    from d = 0.25 on), its derivative 1 - exp(d) to 8 U, the mean to two roundings more."""
+    ops, rows = _ops(), 48
+    sizes = size * (1 + torch.rand(rows, generator=_gen(5))) * torch.where(torch.arange(rows) % 2 == 0, 1.0, -1.0)
+    x, tok, lp, refs, d = _near_reference(cuda, vocab, sizes)
+    dx, stats, zero = torch.empty_like(x), torch.empty(8, device=cuda), torch.zeros(rows, device=cuda)
+    ops.token_ppo_loss(x, tok, lp, zero, dx, stats, ref_logp=refs, kl_coef=1.0)
+    # exp(d) - d - 1 in 64 bits, by its series where that is the closer one
+    k = torch.where(d.abs() < 1e-2, d * d * (0.5 + d * (1 / 6 + d * (1 / 24 + d * (1 / 120 + d / 720)))), torch.expm1(d) - d)
+    assert abs(float(stats[2]) - float(k.mean())) <= 18 * U * float(k.mean())
+    assert float(stats[0]) == float(stats[2])
+    p = torch.softmax(x.double(), 1)
+    at = torch.arange(rows, device=cuda)
+    g = -torch.expm1(d)[:, None]
+    want = -g * p
+    want[at, tok] += g[:, 0]
+    e = _loss_error(x.cpu(), vocab, 1.0)
+    _inside(dx, want / rows, (e * (p + torch.nn.functional.one_hot(tok, vocab)) * g.abs() + 16 * U * g.abs() * p.amax(1, keepdim=True)).cpu()
+            / rows * 2, "d_logits")
+    # every row by itself: none is negative
+    for r in range(0, rows, 7):
+        one = slice(r, r + 1)
+        ops.token_ppo_loss(x[one], tok[one], lp[one], zero[one], None, stats, ref_logp=refs[one], kl_coef=1.0)
+        assert float(stats[2]) > 0.0

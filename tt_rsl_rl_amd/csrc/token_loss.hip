@@ -118,6 +118,13 @@ struct RowTerms {
   bool live;  // (nothing but -inf: no distribution; a NaN goes on)
 };
 
+// k = exp(d) - d - 1, never negative, grown = exp(d) - 1.  Near the reference policy k is d^2 / 2, far below the ones that exp(d) - 1
+// is made of, and below the last bit of `grown` too: there its series, whose first term left out is 1.2e-8 of it at the end.
+__device__ __forceinline__ float kl_of(float d, float grown) {
+  if (!(fabsf(d) < 0.25f)) return grown - d;
+  return d * d * (0.5f + d * (1.0f / 6 + d * (1.0f / 24 + d * (1.0f / 120 + d * (1.0f / 720 + d * (1.0f / 5040))))));
+}
+
 template <bool LOSS>
 __device__ __forceinline__ RowTerms row_terms(const LossKernelArgs& q, int64_t r, const RowSums& sums, float x_tok) {
   RowTerms o{};
@@ -135,9 +142,9 @@ __device__ __forceinline__ RowTerms row_terms(const LossKernelArgs& q, int64_t r
   o.g = first >= second ? first : first < second ? 0.0f : first + second;  // (NaN goes on)
   o.term[0] = first != first || second != second ? first + second : fmaxf(first, second);
   if (q.a.ref_logp != nullptr) {
-    const float d = q.a.ref_logp[r] - o.lp, x = expf(d);
-    o.term[1] = x - d - 1.0f;
-    o.g += q.kl_coef * (1.0f - x);
+    const float d = q.a.ref_logp[r] - o.lp, grown = expm1f(d);
+    o.term[1] = kl_of(d, grown);
+    o.g -= q.kl_coef * grown;
   }
   o.term[2] = o.h;
   o.term[3] = ratio != clipped ? 1.0f : 0.0f;
