@@ -783,8 +783,8 @@ int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace, size_t wo
  * and gives 0 too, though it counts in N.  If no row counts, everything is 0.
  * ppo_token_log_probs writes logp and entropy (either may be NULL).  ppo_token_ppo_loss writes also stats[8] = loss,
  * mean s, mean k, mean H, the share of rows whose ratio the range clips, mean old_logp - lp, N, 0 (each mean over N) and
- * d_logits, of the logits' type (NULL: not wanted); d_logits may be logits itself.  ref_logp NULL: no KL term.  The sums
- * over rows are fp64 in a fixed order. */
+ * d_logits, of the logits' type (NULL: not wanted); d_logits may be logits itself.  ref_logp NULL: no KL term; with kl_coef = 0
+ * it is reported and nothing else (it may be infinite).  The sums over rows are fp64 in a fixed order. */
 typedef struct ppo_token_loss_args {
   const void* logits; /* [rows, vocab] */
   int64_t ld_logits;

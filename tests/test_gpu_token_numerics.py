@@ -3,6 +3,8 @@ are those of tests/test_gpu_token_ops.py, which go by how far logits lie below t
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -182,3 +184,21 @@ def test_kl_near_the_reference(cuda, vocab, size):
         one = slice(r, r + 1)
         ops.token_ppo_loss(x[one], tok[one], lp[one], zero[one], None, stats, ref_logp=refs[one], kl_coef=1.0)
         assert float(stats[2]) > 0.0
+
+
+@pytest.mark.parametrize("vocab", [64, 20011])
+def test_kl_that_is_only_reported(cuda, vocab):
+    """kl_coef = 0 with a reference so far off that k is infinite: the loss and its gradient are those without a reference."""
+    ops, g, rows = _ops(), _gen(vocab), 9
+    x = torch.randn(rows, vocab, generator=g).to(cuda)
+    tok, adv = torch.randint(0, vocab, (rows,), generator=g).to(cuda), torch.randn(rows, generator=g).to(cuda)
+    old, refs = torch.full((rows,), -math.log(vocab), device=cuda), torch.full((rows,), 100.0, device=cuda)
+    out = []
+    for reference in (None, refs):
+        dx, stats = torch.empty_like(x), torch.empty(8, device=cuda)
+        ops.token_ppo_loss(x, tok, old, adv, dx, stats, ref_logp=reference, entropy_coef=0.01)
+        out.append((dx, stats))
+    assert torch.equal(out[0][0], out[1][0]) and bool(torch.isfinite(out[1][0]).all())
+    assert float(out[1][1][2]) == INF and float(out[0][1][2]) == 0.0
+    keep = [0, 1, 3, 4, 5, 6, 7]
+    assert torch.equal(out[0][1][keep], out[1][1][keep])

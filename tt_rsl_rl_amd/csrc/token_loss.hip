@@ -144,7 +144,7 @@ __device__ __forceinline__ RowTerms row_terms(const LossKernelArgs& q, int64_t r
   if (q.a.ref_logp != nullptr) {
     const float d = q.a.ref_logp[r] - o.lp, grown = expm1f(d);
     o.term[1] = kl_of(d, grown);
-    o.g -= q.kl_coef * grown;
+    if (q.kl_coef != 0.0f) o.g -= q.kl_coef * grown;  // (0: k is only reported, and may be infinite)
   }
   o.term[2] = o.h;
   o.term[3] = ratio != clipped ? 1.0f : 0.0f;
@@ -346,7 +346,7 @@ __device__ __forceinline__ void write_stats(const LossKernelArgs& q, double sum)
   const double rows = __shfl(sum, 5, kWave), n = q.a.denom > 0.0 ? q.a.denom : rows, inv = rows > 0.0 ? 1.0 / n : 0.0;
   const double s = __shfl(sum, 0, kWave), k = __shfl(sum, 1, kWave), h = __shfl(sum, 2, kWave);
   if (threadIdx.x < 5) q.a.stats[1 + threadIdx.x] = static_cast<float>(sum * inv);
-  if (threadIdx.x == 5) q.a.stats[0] = static_cast<float>((s + q.a.kl_coef * k - q.a.entropy_coef * h) * inv);
+  if (threadIdx.x == 5) q.a.stats[0] = static_cast<float>((s + (q.a.kl_coef != 0.0 ? q.a.kl_coef * k : 0.0) - q.a.entropy_coef * h) * inv);
   if (threadIdx.x == 6) q.a.stats[6] = static_cast<float>(n);
   if (threadIdx.x == 7) q.a.stats[7] = 0.0f;
 }
