@@ -46,6 +46,14 @@ __device__ __forceinline__ bool row_counts(const ppo_token_loss_args& a, int64_t
   return tok >= 0;
 }
 
+// A block per row, kGridRows of them along x, more along y: a launch may not hold 2^32 threads along one axis, which 4,194,304
+// blocks of 1,024 would.
+constexpr int64_t kGridRows = 1 << 20;
+dim3 row_grid(int64_t rows) {
+  return dim3(static_cast<uint32_t>(std::min(rows, kGridRows)), static_cast<uint32_t>(ceil_div(rows, kGridRows)));
+}
+__device__ __forceinline__ int64_t block_row() { return blockIdx.x + static_cast<int64_t>(blockIdx.y) * kGridRows; }
+
 template <class R>
 __device__ __forceinline__ R wave_sum(R x) {
   for (int d = kWave / 2; d > 0; d >>= 1) x += __shfl_xor(x, d, kWave);
@@ -318,7 +326,8 @@ template <class T, int NT, int K, bool LOSS>
 __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void token_row_kernel(const LossKernelArgs q) {
   __shared__ RowShared<NT / kWave> sh;
   const ppo_token_loss_args& a = q.a;
-  const int64_t r = blockIdx.x;
+  const int64_t r = block_row();
+  if (r >= a.rows) return;
   const int vocab = static_cast<int>(a.vocab);
   const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
   T* dx = LOSS && a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
@@ -523,7 +532,8 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
   constexpr int V = kVec<T>, NT = kWideThreads;
   __shared__ RowShared<NT / kWave> sh;
   const ppo_token_loss_args& a = q.a;
-  const int64_t r = blockIdx.x;
+  const int64_t r = block_row();
+  if (r >= a.rows) return;
   const T* x = static_cast<const T*>(a.logits) + r * a.ld_logits;
   T* dx = LOSS && a.d_logits != nullptr ? static_cast<T*>(a.d_logits) + r * a.ld_d_logits : nullptr;
   int64_t tok;
@@ -588,7 +598,7 @@ __global__ __launch_bounds__(kWideThreads) void token_wide_kernel(const LossKern
 template <class T, bool LOSS>
 int launch_rows(const LossKernelArgs& q, RowPart* parts, hipStream_t st) {
   const int64_t rows = q.a.rows, vocab = q.a.vocab, pieces = ceil_div(vocab, kVec<T>), n = ceil_div(pieces, kPartThreads * kPartPieces);
-  const dim3 grid(static_cast<uint32_t>(rows));
+  const dim3 grid = row_grid(rows);
   if (rows <= (LOSS ? kSplitLossRows : kSplitRows) && vocab >= (LOSS ? kSplitLossVocab : kSplitVocab) && n <= kMaxParts) {
     const dim3 split(static_cast<uint32_t>(n), static_cast<uint32_t>(rows));
     hipLaunchKernelGGL(token_part_kernel<T>, split, dim3(kPartThreads), 0, st, q, parts);
