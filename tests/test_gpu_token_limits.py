@@ -42,3 +42,21 @@ def test_many_rows_of_a_small_vocabulary(cuda, rows, vocab, dtype):
     d = adv[:, None] * (p - torch.nn.functional.one_hot(tok, vocab))
     assert float((dx - d).abs().sub(e * (1 + adv.abs())[:, None] * 4 + (2.0**-8 if dtype == BF16 else U) * 1.01 * d.abs()).max()) <= 0
     assert abs(float(stats[3]) - float(entropy.sum())) <= 2 * e * rows
+
+
+def test_adamw_of_more_elements_than_a_launch_takes(cuda):
+    """2^34 and more elements in tensors that a launch would take together; their gradient is one and the same tensor."""
+    ops = _ops()
+    n, tensors = 1 << 32, 5
+    zeros = lambda k, dtype: [torch.zeros(k, dtype=dtype, device=cuda) for _ in range(tensors)]  # noqa: E731
+    p, m, v = zeros(n, BF16), zeros(n, torch.int8), zeros(n, torch.uint8)
+    sm, sv = zeros(n // 256, F32), zeros(n // 256, F32)
+    g = torch.ones(n, dtype=BF16, device=cuda)
+    print("AdamW of 2.1e10 elements", flush=True)
+    ops.adamw_step(p, [g] * tensors, m, v, step=1, lr=0.5, weight_decay=0.0, scales=(sm, sv))
+    for t in p:
+        assert float(t.min()) == -0.5 and float(t.max()) == -0.5
+    for t in m:
+        assert int(t.min()) == 127
+    del p, m, v, sm, sv, g
+    torch.cuda.empty_cache()

@@ -292,6 +292,12 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_update_kernel(const Updat
 
 int64_t chunks_of(const ppo_adamw_tensor& t) { return ceil_div(t.count, kChunk); }
 
+// What a launch may hold: fewer than 2^32 threads.  Tensors that would make it more go to the next one.
+constexpr int64_t kMaxCount = int64_t{1} << 33;  // of a tensor
+constexpr int64_t kMaxChunks = (int64_t{1} << 32) / kAdamwThreads - 1;
+static_assert(kMaxCount / kChunk <= kMaxChunks, "any tensor by itself fits a launch");
+static_assert(kMaxGrads * (kMaxCount / kNormChunk) < INT32_MAX, "so do a norm launch's chunks a 32-bit index");
+
 int64_t norm_partials(const ppo_adamw_tensor* tensors, int32_t count) {
   // a bound: each launch writes at most kNormBlocks, and there is one per kMaxGrads tensors of a type
   return static_cast<int64_t>(kNormBlocks) * (count / kMaxGrads + 2);
@@ -332,7 +338,7 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
               beta1, beta2, eps);
   for (int i = 0; i < count; ++i) {
     const ppo_adamw_tensor& t = tensors[i];
-    PPO_REQUIRE(t.count >= 0 && t.count < (int64_t{1} << 33), "ppo_adamw_step: tensor %d holds %lld elements", i, (long long)t.count);
+    PPO_REQUIRE(t.count >= 0 && t.count < kMaxCount, "ppo_adamw_step: tensor %d holds %lld elements", i, (long long)t.count);
     PPO_REQUIRE((t.param_type == PPO_TYPE_F32 || t.param_type == PPO_TYPE_BF16) &&
                     (t.grad_type == PPO_TYPE_F32 || t.grad_type == PPO_TYPE_BF16),
                 "ppo_adamw_step: tensor %d: param_type=%d grad_type=%d", i, t.param_type, t.grad_type);
@@ -373,7 +379,6 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
           t.count[t.tensors] = tensors[i].count;
           t.first[t.tensors++] = static_cast<int32_t>(chunks);
           chunks += ceil_div(tensors[i].count, kNormChunk);
-          PPO_REQUIRE(chunks < INT32_MAX, "ppo_adamw_step: too many parameters");
         }
         if (t.tensors == 0) break;
         t.first[t.tensors] = static_cast<int32_t>(chunks);
@@ -405,13 +410,13 @@ extern "C" int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, do
       for (; i < count && t.tensors < kMaxTensors; ++i) {
         const ppo_adamw_tensor& a = tensors[i];
         if (kind_of(a) != kind || a.count == 0) continue;
+        if (chunks + chunks_of(a) > kMaxChunks) break;
         Tensor& b = t.t[t.tensors];
         b = Tensor{a.param, a.grad, a.master, a.exp_avg, a.exp_avg_sq, a.m_scale, a.v_scale, a.count,
                    static_cast<float>(-(a.lr / a.bc1)), static_cast<float>(1.0 - a.lr * a.weight_decay),
                    static_cast<float>(a.bc2_sqrt), static_cast<float>(1.0 / a.bc2_sqrt)};
         t.first[t.tensors++] = static_cast<int32_t>(chunks);
         chunks += chunks_of(a);
-        PPO_REQUIRE(chunks < INT32_MAX, "ppo_adamw_step: too many parameters");
       }
       if (t.tensors == 0) break;
       t.first[t.tensors] = static_cast<int32_t>(chunks);
