@@ -60,3 +60,23 @@ def test_adamw_of_more_elements_than_a_launch_takes(cuda):
         assert int(t.min()) == 127
     del p, m, v, sm, sv, g
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("count,dim", [((1 << 22) + 3, 1025), ((1 << 26) + 5, 1025)])
+def test_lookup_of_many_rows(cuda, count, dim):
+    """On both sides of what a launch holds along one axis: 2^20 blocks of 4 rows, and 2^32 threads."""
+    ops, vocab = _ops(), 251
+    if torch.cuda.mem_get_info()[0] < 2.2 * count * dim + (8 << 30):
+        pytest.skip("not enough memory")
+    table = torch.arange(vocab, device=cuda, dtype=F32)[:, None].to(BF16).expand(vocab, dim).contiguous()
+    tok = (torch.arange(count, device=cuda) % 263 - 1).int()  # (some outside of the vocabulary)
+    out = torch.empty(count, dim, dtype=BF16, device=cuda)
+    print(f"lookup {count} x {dim}", flush=True)
+    ops.embedding_fwd(tok, table, out, scale=0.5)
+    for i in range(0, count, 1 << 24):
+        t = tok[i:i + (1 << 24)]
+        want = torch.where((t >= 0) & (t < vocab), t * 0.5, 0.0)
+        for c in (0, 500, dim - 1):
+            assert torch.equal(out[i:i + (1 << 24), c].float(), want)
+    del out, tok
+    torch.cuda.empty_cache()

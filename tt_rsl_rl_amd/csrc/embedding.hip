@@ -16,13 +16,15 @@ namespace {
 // A thread moves one 16-byte piece of each of kFwdRows rows; a block's threads lie side by side on a row as far as it reaches.
 // 16,384 rows of 2,048 bf16: 17.8 us, 5.2 TB/s of the 93 MB that have to move.
 constexpr int kFwdThreads = 256, kFwdRows = 4;  // rows in flight per thread
+constexpr int64_t kFwdGrid = 1 << 20;  // blocks along x; more go along z (2^32 threads along one axis are refused)
 
 template <class T>
 __global__ __launch_bounds__(kFwdThreads) void embedding_fwd_kernel(const ppo_embedding_args a, int log_tpr) {
   constexpr int V = kVec<T>;
   const int tpr = 1 << log_tpr;  // threads side by side on a row
   const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x >> log_tpr, groups = kFwdThreads >> log_tpr;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * groups * kFwdRows + group;
+  const int64_t r0 = (blockIdx.x + blockIdx.z * kFwdGrid) * groups * kFwdRows + group;
+  if (r0 >= a.count) return;
   const T* table = static_cast<const T*>(a.src);
   T* out = static_cast<T*>(a.dst);
   int64_t tok[kFwdRows];
@@ -659,7 +661,8 @@ extern "C" int ppo_embedding_fwd(const ppo_embedding_args* args, ppo_stream_t st
     int log_tpr = 0;
     while ((1 << log_tpr) < pieces && (1 << log_tpr) < kFwdThreads) ++log_tpr;
     const int64_t blocks = ceil_div(a.count, static_cast<int64_t>(kFwdThreads >> log_tpr) * kFwdRows);
-    const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(ceil_div(pieces, 1 << log_tpr)));
+    const dim3 grid(static_cast<uint32_t>(std::min(blocks, kFwdGrid)), static_cast<uint32_t>(ceil_div(pieces, 1 << log_tpr)),
+                    static_cast<uint32_t>(ceil_div(blocks, kFwdGrid)));
     hipLaunchKernelGGL(embedding_fwd_kernel<T>, grid, dim3(kFwdThreads), 0, st, a, log_tpr);
     rc = check_launch("embedding_fwd_kernel");
   });
