@@ -53,21 +53,59 @@ class AdamW(torch.optim.Optimizer):
     """AdamW on ``ops.adamw_step``: one call for all parameters, their gradients clipped by their common norm first
     (max_grad_norm; ``norm`` holds the last norm and clip coefficient on the GPU).  Parameters are float32 or bfloat16; the
     latter get a float32 master unless ``masters`` is False.  state_bits: 32, or 8 for both moments in 8 bits.  Groups may
-    have their own lr and weight_decay; parameters without a gradient are left alone."""
+    have their own lr and weight_decay; their betas and eps are one value for all of them (a scheduler may change it between
+    steps).  Parameters without a gradient are left alone."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, max_grad_norm: float | None = None, state_bits: int = 32, masters: bool = True) -> None:
-        if lr < 0.0 or not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0 or eps < 0.0 or weight_decay < 0.0:
-            raise ValueError(f"AdamW: lr={lr} betas={betas} eps={eps} weight_decay={weight_decay}")
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits={state_bits} (8 or 32)")
         if max_grad_norm is not None and not max_grad_norm > 0.0:
             raise ValueError(f"AdamW: max_grad_norm={max_grad_norm}")
-        self.betas, self.eps, self.max_grad_norm = (float(betas[0]), float(betas[1])), float(eps), max_grad_norm
-        self.state_bits, self.masters = state_bits, masters
+        self.max_grad_norm, self.state_bits, self.masters = max_grad_norm, state_bits, masters
         self.norm: torch.Tensor | None = None
         self._ws = ops.Workspace()
-        super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
+        defaults = dict(lr=lr, betas=(float(betas[0]), float(betas[1])), eps=float(eps), weight_decay=weight_decay)
+        self._check_group(defaults)
+        super().__init__(params, defaults)
+
+    def _check_group(self, group: dict) -> None:
+        lr, betas, eps, weight_decay = (group[k] for k in ("lr", "betas", "eps", "weight_decay"))
+        if lr < 0.0 or not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0 or eps < 0.0 or weight_decay < 0.0:
+            raise ValueError(f"AdamW: lr={lr} betas={betas} eps={eps} weight_decay={weight_decay}")
+        for key in ("max_grad_norm", "state_bits", "masters"):
+            if key in group and group[key] != getattr(self, key):
+                raise ValueError(f"AdamW: {key} is the optimiser's, not a group's")
+        for key in ("amsgrad", "maximize"):
+            if group.get(key):
+                raise ValueError(f"AdamW: no {key}")
+
+    def _common(self) -> tuple[tuple[float, float], float]:
+        """betas and eps, which all groups share."""
+        first = self.param_groups[0]
+        betas, eps = tuple(first["betas"]), first["eps"]
+        for group in self.param_groups[1:]:
+            if tuple(group["betas"]) != betas or group["eps"] != eps:
+                raise ValueError(f"AdamW: betas and eps must be the same in all groups, got {betas}, {eps} and {group['betas']}, {group['eps']}")
+        return betas, eps
+
+    betas = property(lambda self: self._common()[0])
+    eps = property(lambda self: self._common()[1])
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        try:
+            self._check_group(self.param_groups[-1])
+            self._common()
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:  # (of a state_dict() from before they were the groups')
+            for key in ("betas", "eps"):
+                group.setdefault(key, self.defaults[key])
 
     def _init_state(self, p: torch.Tensor, state: dict) -> None:
         state["step"] = 0
@@ -89,6 +127,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        (beta1, beta2), eps = self._common()
         params, states, lr, decay = [], [], [], []
         for group in self.param_groups:
             for p in group["params"]:
@@ -109,7 +148,7 @@ class AdamW(torch.optim.Optimizer):
         column = lambda key: [s.get(key) for s in states]  # noqa: E731
         masters = column("master")
         ops.adamw_step(params, grads, column("exp_avg"), column("exp_avg_sq"), step=[s["step"] + 1 for s in states], lr=lr,
-                       beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, weight_decay=decay, max_grad_norm=self.max_grad_norm,
+                       beta1=beta1, beta2=beta2, eps=eps, weight_decay=decay, max_grad_norm=self.max_grad_norm,
                        masters=masters if any(m is not None for m in masters) else None,
                        scales=(column("exp_avg_scale"), column("exp_avg_sq_scale")) if self.state_bits == 8 else None,
                        norm_out=self.norm if self.max_grad_norm is not None else None, ws=self._ws)
