@@ -3,6 +3,9 @@ replaced by a recorder."""
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -81,3 +84,19 @@ def test_schedulers_that_cycle_the_momentum(calls):
         schedule.step()
     assert len({c["beta1"] for c in calls}) > 2 and {c["beta2"] for c in calls} == {0.999}
     assert [c["lr"][0] for c in calls] == [c["lr"][1] for c in calls]
+
+
+@pytest.mark.parametrize("how", ["copy", "pickle"])
+def test_copies_step(calls, how):
+    (a,) = _params(3)
+    opt = tokens.AdamW([a], lr=0.1, betas=(0.5, 0.6), eps=1e-3, max_grad_norm=0.7, state_bits=8, masters=False)
+    opt.step()
+    other = copy.deepcopy(opt) if how == "copy" else pickle.loads(pickle.dumps(opt))
+    p = other.param_groups[0]["params"][0]
+    p.grad = torch.ones_like(p)
+    other.step()
+    for key in ("beta1", "beta2", "eps", "max_grad_norm", "lr"):
+        assert calls[0][key] == calls[1][key]
+    assert calls[1]["step"] == [2] and calls[1]["scales"] is not None and calls[1]["ws"] is not calls[0]["ws"]
+    assert other.masters is False and calls[1]["params"][0].data_ptr() == p.data_ptr() != a.data_ptr()
+    assert opt.state[a]["step"] == 1

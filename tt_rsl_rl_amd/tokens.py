@@ -101,8 +101,14 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
-    def __setstate__(self, state: dict) -> None:
+    def __getstate__(self) -> dict:
+        """Copies and pickles: torch's part and the options beside it; scratch memory and the last norm stay behind."""
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "state_bits": self.state_bits, "masters": self.masters}
+
+    def __setstate__(self, state: dict) -> None:  # (load_state_dict() comes here too, with a state of two entries)
         super().__setstate__(state)
+        if "_ws" not in self.__dict__:
+            self.norm, self._ws = None, ops.Workspace()
         for group in self.param_groups:  # (of a state_dict() from before they were the groups')
             for key in ("betas", "eps"):
                 group.setdefault(key, self.defaults[key])
