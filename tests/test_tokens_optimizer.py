@@ -100,3 +100,37 @@ def test_copies_step(calls, how):
     assert calls[1]["step"] == [2] and calls[1]["scales"] is not None and calls[1]["ws"] is not calls[0]["ws"]
     assert other.masters is False and calls[1]["params"][0].data_ptr() == p.data_ptr() != a.data_ptr()
     assert opt.state[a]["step"] == 1
+
+
+def test_a_checkpoint_of_other_masters(calls):
+    """Into masters=True a missing master is the parameter's; into masters=False none is stepped."""
+    (a,) = _params(3, dtype=torch.bfloat16)
+    with torch.no_grad():
+        a.copy_(torch.tensor([1.0, -2.0, 3.0]))
+    without, with_ = tokens.AdamW([a], masters=False), tokens.AdamW([a], masters=True)
+    without.step()
+    with_.step()
+    assert calls[0]["masters"] is None and calls[1]["masters"][0].dtype == torch.float32
+    with_.load_state_dict(without.state_dict())
+    with_.step()
+    assert torch.equal(calls[2]["masters"][0], a.detach().float()) and calls[2]["step"] == [2]
+    without.load_state_dict(with_.state_dict())
+    without.step()
+    assert calls[3]["masters"] is None and calls[3]["step"] == [3] and "master" not in without.state[a]
+
+
+def test_a_checkpoint_of_torch_s_own(calls):
+    (a,) = _params(3)
+    theirs = torch.optim.AdamW([a], lr=0.1, betas=(0.5, 0.6), amsgrad=False)
+    theirs.step()
+    opt = tokens.AdamW([a])
+    opt.load_state_dict(theirs.state_dict())
+    opt.step()
+    assert calls[0]["step"] == [2] and opt.state[a]["step"] == 2 and isinstance(opt.state[a]["step"], int)
+    assert torch.equal(calls[0]["exp_avg"][0], theirs.state[a]["exp_avg"]) and (opt.betas, calls[0]["lr"]) == ((0.5, 0.6), [0.1])
+    theirs = torch.optim.AdamW([a], amsgrad=True)
+    theirs.step()
+    before = opt.state_dict()["param_groups"]
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(theirs.state_dict())
+    assert opt.state_dict()["param_groups"] == before

@@ -164,14 +164,25 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Takes a state_dict() of an optimiser of the same state_bits; the states keep their types (torch's own would be
-        cast to the parameters')."""
+        cast to the parameters').  Masters go by this optimiser's ``masters``: one that the state_dict() lacks is the
+        parameter as it is now, one that is not wanted is left out."""
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         for i in saved:
             state = state_dict["state"].get(i)
             if state and (state["exp_avg"].dtype == torch.int8) != (self.state_bits == 8):
                 raise ValueError(f"AdamW: states of another width than state_bits={self.state_bits}")
+        for group in state_dict["param_groups"]:
+            self._check_group({**self.defaults, **group})
         super().load_state_dict(state_dict)
         for i, p in zip(saved, (p for group in self.param_groups for p in group["params"]), strict=True):
-            for key, value in state_dict["state"].get(i, {}).items():
+            if not state_dict["state"].get(i):
+                continue
+            state = self.state[p]
+            for key, value in state_dict["state"][i].items():
                 if isinstance(value, torch.Tensor):
-                    self.state[p][key] = value.to(p.device, copy=True)
+                    state[key] = value.to(p.device, copy=True)
+            state["step"] = int(state["step"])  # (torch.optim.AdamW's is a tensor)
+            if not self.masters or p.dtype != torch.bfloat16:
+                state.pop("master", None)
+            elif "master" not in state:
+                state["master"] = p.detach().to(torch.float32)
