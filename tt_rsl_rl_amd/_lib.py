@@ -9,6 +9,7 @@ failures -> RuntimeError.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import struct
 from pathlib import Path
@@ -350,8 +351,10 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     return lib
 
 
+@functools.cache
 def tensor_table():
-    """The module that makes ppo_adamw_step's table from lists of tensors (csrc/tensor_table.cpp), built beside the library."""
+    """The module that makes ppo_adamw_step's table from lists of tensors and marks tensors as written
+    (csrc/tensor_table.cpp), built beside the library."""
     try:
         from . import _tensor_table
     except ImportError as e:

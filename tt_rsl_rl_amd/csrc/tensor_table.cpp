@@ -1,6 +1,7 @@
-// Host code: the table of tensors that ppo_adamw_step takes, made from Python lists of tensors in one call.  Reading each
-// tensor's pointer, size, type and device through Python's attributes takes about 2 us a tensor: 300 us for a model of 170
-// tensors whose step takes the GPU 15.  A module of CPython's (tt_rsl_rl_amd._tensor_table), since it reads torch's objects.
+// Host code that reads torch's objects: the table of tensors that ppo_adamw_step takes, made from Python lists of tensors in one
+// call, and the mark that autograd expects on tensors written behind its back.  Reading each tensor's pointer, size, type and
+// device through Python's attributes takes about 2 us a tensor: 300 us for a model of 170 tensors whose step takes the GPU 15.
+// A module of CPython's (tt_rsl_rl_amd._tensor_table).
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/Tensor.h>
@@ -167,8 +168,43 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
   }
 }
 
+// A tensor, or None; false for anything else.
+bool mark(PyObject* x) {
+  if (x == Py_None) return true;
+  if (!THPVariable_Check(x)) return false;
+  const at::Tensor& t = THPVariable_Unpack(x);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // (an inference tensor has no counter, and autograd none of it)
+  return true;
+}
+
+bool mark_all(PyObject* x) {
+  if (mark(x)) return true;
+  Tensors list("");
+  if (!list.take(x, -1, false)) return false;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(list.fast); ++i)
+    if (!mark(PySequence_Fast_GET_ITEM(list.fast, i))) {
+      PyErr_SetString(PyExc_TypeError, "written: tensors or sequences of them");
+      return false;
+    }
+  return true;
+}
+
+// written(*tensors): their version counters go up, as by torch's own in-place operations, so that a backward pass which has kept
+// one of them for itself says so instead of using what was written since.
+PyObject* written(PyObject*, PyObject* const* args, Py_ssize_t num) {
+  try {
+    for (Py_ssize_t i = 0; i < num; ++i)
+      if (!mark_all(args[i])) return nullptr;
+  } catch (const std::exception& ex) {
+    return PyErr_Format(PyExc_RuntimeError, "written: %s", ex.what());
+  }
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {{"adamw_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_table)), METH_FASTCALL,
                           "The bytes of ppo_adamw_step's table (ops.adamw_step)."},
+                         {"written", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(written)), METH_FASTCALL,
+                          "Raises the version counters of tensors and of sequences of them; None is skipped."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_table", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
