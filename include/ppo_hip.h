@@ -823,7 +823,11 @@ int ppo_token_ppo_loss(const ppo_token_loss_args* args, void* workspace, size_t 
  * States in 32 bits are fp32 [count]; in 8 bits, each 256 consecutive elements (the last block may be shorter) share one fp32
  * scale per state: m = sign(q) m_scale (|q| / 127)^2 with q int8, v = v_scale (q / 255)^4 with q uint8; the scale is the
  * block's largest |m| (v), q is rounded to nearest, and q >= 1 where v > 0 (a second moment rounded to zero would leave its
- * parameter a step of m / eps).  All zeros are the zero state.  norm_out (NULL: not wanted): total, c.  Tensors of count 0
+ * parameter a step of m / eps).  All zeros are the zero state.  Rounded to nearest, a state that changes by less than half a
+ * code's distance a step does not change at all: v (0.1 % a step with b2 = 0.999; the codes lie 4 / q apart, 1.6 % at least)
+ * never falls below what it was unless its block's scale rises, and m keeps what lies below 0.5 % of its block's largest.  So
+ * dither: where it is not 0, q is one of the two neighbouring codes, by chance, with the value kept on average (but for
+ * q >= 1).  It has to be another value at each step, the number of the step for instance; the same value gives the same codes.  norm_out (NULL: not wanted): total, c.  Tensors of count 0
  * are allowed. */
 typedef struct ppo_adamw_tensor {
   void* param;
@@ -842,6 +846,7 @@ typedef struct ppo_adamw_tensor {
   int32_t grad_type;
   int32_t state_bits; /* 32 or 8 */
   int32_t reserved;
+  int64_t dither;     /* 8-bit states: 0 rounds their codes to nearest */
 } ppo_adamw_tensor;
 #define PPO_ADAMW_BLOCK 256
 size_t ppo_adamw_workspace_bytes(const ppo_adamw_tensor* tensors, int32_t count);

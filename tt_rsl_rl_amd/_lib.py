@@ -222,7 +222,7 @@ class AdamwTensor(C.Structure):
     _fields_ = [("param", vp), ("grad", vp), ("master", vp), ("exp_avg", vp), ("exp_avg_sq", vp), ("m_scale", vp),
                 ("v_scale", vp), ("count", i64), ("lr", C.c_double), ("weight_decay", C.c_double), ("bc1", C.c_double),
                 ("bc2_sqrt", C.c_double), ("param_type", i32),
-                ("grad_type", i32), ("state_bits", i32), ("reserved", i32)]
+                ("grad_type", i32), ("state_bits", i32), ("reserved", i32), ("dither", i64)]
 
 
 # the same packed by hand, a third of the time of their fields
@@ -326,7 +326,7 @@ _SIGNATURES = [
 ]
 
 EXPORTED_SYMBOLS = [name for name, _, _ in _SIGNATURES]
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _lib: C.CDLL | None = None
 

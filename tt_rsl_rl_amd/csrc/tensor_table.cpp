@@ -121,9 +121,10 @@ bool entry(const Tensors (&lists)[7], const Numbers& lr, const Numbers& weight_d
   return lr.at(i, e.lr) && weight_decay.at(i, e.weight_decay);
 }
 
-// adamw_table(params, grads, masters, exp_avg, exp_avg_sq, m_scales, v_scales, step, lr, weight_decay, beta1, beta2, device) -> bytes
+// adamw_table(params, grads, masters, exp_avg, exp_avg_sq, m_scales, v_scales, step, lr, weight_decay, beta1, beta2, dither, device)
+// -> bytes
 PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
-  if (num != 13) return PyErr_Format(PyExc_TypeError, "adamw_table: 13 arguments, got %zd", num);
+  if (num != 14) return PyErr_Format(PyExc_TypeError, "adamw_table: 14 arguments, got %zd", num);
   try {
     Tensors lists[7] = {Tensors("params"), Tensors("grads"), Tensors("masters"), Tensors("exp_avg"), Tensors("exp_avg_sq"),
                         Tensors("scales"), Tensors("scales")};
@@ -135,7 +136,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
     }
     if (!step.take(args[7], n) || !lr.take(args[8], n) || !weight_decay.take(args[9], n)) return nullptr;
     const double beta1 = PyFloat_AsDouble(args[10]), beta2 = PyFloat_AsDouble(args[11]);
-    const long device = PyLong_AsLong(args[12]);
+    const int dither = PyObject_IsTrue(args[12]);
+    const long device = PyLong_AsLong(args[13]);
     if (PyErr_Occurred()) return nullptr;
     PyObject* out = PyBytes_FromStringAndSize(nullptr, n * static_cast<Py_ssize_t>(sizeof(ppo_adamw_tensor)));
     if (out == nullptr) return nullptr;
@@ -158,6 +160,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
         bc1 = 1.0 - std::pow(beta1, s);
         bc2_sqrt = std::sqrt(1.0 - std::pow(beta2, s));
       }
+      x.dither = dither != 0 && x.state_bits == 8 ? static_cast<int64_t>(std::fmin(s, 0x1p62)) : 0;
       x.bc1 = bc1;
       x.bc2_sqrt = bc2_sqrt;
       std::memcpy(e + i, &x, sizeof(x));

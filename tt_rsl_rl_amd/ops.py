@@ -1205,20 +1205,22 @@ def token_ppo_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.T
 def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step, lr, beta1: float = 0.9,
                beta2: float = 0.999, eps: float = 1e-8, weight_decay=1e-2, max_grad_norm: float | None = None,
                masters: list | None = None, scales: tuple[list, list] | None = None, norm_out: torch.Tensor | None = None,
-               ws: Workspace | None = None) -> None:
+               ws: Workspace | None = None, dither: bool = False) -> None:
     """One AdamW step over a list of contiguous tensors, in place, their gradients clipped by their common norm first
     (max_grad_norm; the gradients themselves are left as they are).  params: float32, or bfloat16 with (masters) or without
     a float32 master each, in which case the master is stepped and the parameter is its rounding; grads: float32, or
     bfloat16 for a bfloat16 parameter; exp_avg / exp_avg_sq: float32, or int8 / uint8 with scales = (lists of) float32
     [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  step (from 1), lr and weight_decay: one
-    value, or one per tensor.  norm_out: float32 [2] for the norm and the clip coefficient."""
+    value, or one per tensor.  norm_out: float32 [2] for the norm and the clip coefficient.  dither: 8-bit states are rounded
+    up or down by chance (the same for the same step), so that over many steps they follow the moments; rounded to nearest they
+    do not (ppo_hip.h)."""
     if max_grad_norm is not None and not max_grad_norm > 0:
         raise ValueError(f"adamw_step: max_grad_norm={max_grad_norm}")
     n = len(params)
     dev = _get_device() if n and getattr(params[0], "is_cuda", False) else -1
     m_scales, v_scales = scales if scales is not None else (None, None)
     packed = L.tensor_table().adamw_table(params, grads, masters, exp_avg, exp_avg_sq, m_scales, v_scales, step, lr, weight_decay, beta1,
-                                          beta2, dev)
+                                          beta2, dither, dev)
     if n == 0:
         return
     buf = None

@@ -52,7 +52,8 @@ class TokenEmbedding(nn.Module):
 class AdamW(torch.optim.Optimizer):
     """AdamW on ``ops.adamw_step``: one call for all parameters, their gradients clipped by their common norm first
     (max_grad_norm; ``norm`` holds the last norm and clip coefficient on the GPU).  Parameters are float32 or bfloat16; the
-    latter get a float32 master unless ``masters`` is False.  state_bits: 32, or 8 for both moments in 8 bits.  Groups may
+    latter get a float32 master unless ``masters`` is False.  state_bits: 32, or 8 for both moments in 8 bits, rounded by
+    chance that the step's number decides, so that the same steps give the same bits.  Groups may
     have their own lr and weight_decay; their betas and eps are one value for all of them (a scheduler may change it between
     steps).  Parameters without a gradient are left alone."""
 
@@ -157,7 +158,7 @@ class AdamW(torch.optim.Optimizer):
                        beta1=beta1, beta2=beta2, eps=eps, weight_decay=decay, max_grad_norm=self.max_grad_norm,
                        masters=masters if any(m is not None for m in masters) else None,
                        scales=(column("exp_avg_scale"), column("exp_avg_sq_scale")) if self.state_bits == 8 else None,
-                       norm_out=self.norm if self.max_grad_norm is not None else None, ws=self._ws)
+                       norm_out=self.norm if self.max_grad_norm is not None else None, ws=self._ws, dither=self.state_bits == 8)
         for s in states:  # (after the call: a refused one leaves the counts as they are)
             s["step"] += 1
         return loss
