@@ -749,7 +749,7 @@ enum { PPO_TOKENS_I64 = 0, PPO_TOKENS_I32 = 1 };
  * the table's gradient [vocab, dim], fp32 or of src's type.  Each row is summed in fp32 in an order that depends on the
  * tokens alone (the tokens are sorted first, stably), so the same call gives the same bits.  accumulate = 0 writes every
  * row, zeros where no token names it; otherwise the sum is added to the row and rows without tokens are left alone.
- * count may be 0; count < 2^31, vocab < 2^31. */
+ * count may be 0; count < 2^31, vocab < 2^31.  dst may not lie on src or the tokens. */
 typedef struct ppo_embedding_args {
   const void* tokens;
   const void* src;
@@ -783,7 +783,8 @@ int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace, size_t wo
  * and gives 0 too, though it counts in N.  If no row counts, everything is 0.
  * ppo_token_log_probs writes logp and entropy (either may be NULL).  ppo_token_ppo_loss writes also stats[8] = loss,
  * mean s, mean k, mean H, the share of rows whose ratio the range clips, mean old_logp - lp, N, 0 (each mean over N) and
- * d_logits, of the logits' type (NULL: not wanted); d_logits may be logits itself.  ref_logp NULL: no KL term; with kl_coef = 0
+ * d_logits, of the logits' type (NULL: not wanted); d_logits may be logits itself; but for that no output may lie on an
+ * input or another output.  ref_logp NULL: no KL term; with kl_coef = 0
  * it is reported and nothing else (it may be infinite).  The sums over rows are fp64 in a fixed order. */
 typedef struct ppo_token_loss_args {
   const void* logits; /* [rows, vocab] */

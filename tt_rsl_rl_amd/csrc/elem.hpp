@@ -92,6 +92,22 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int type, int64_
   return t >= 0 && t < vocab ? t : -1;
 }
 
+// Memory that a call reads and memory that it writes: one block may write what another has yet to read, so an output may not lie
+// on an input unless the header says so.  Rows of a matrix, in bytes.
+struct Rows {
+  const void* at;
+  int64_t rows, bytes, ld;
+};
+inline bool overlap(const Rows& x, const Rows& y) {
+  if (x.at == nullptr || y.at == nullptr || x.rows <= 0 || y.rows <= 0) return false;
+  const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(x.at)), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(y.at));
+  if (a + (x.rows - 1) * x.ld + x.bytes <= b || b + (y.rows - 1) * y.ld + y.bytes <= a) return false;
+  if (x.ld != y.ld) return true;
+  const int64_t apart = ((b - a) % x.ld + x.ld) % x.ld;  // columns of one matrix may lie side by side
+  return apart < x.bytes || apart + y.bytes > x.ld;
+}
+inline Rows vector_of(const void* p, int64_t bytes) { return Rows{p, 1, bytes, bytes}; }
+
 // f(T()) for the element type of `type`.
 template <class F>
 void with_type(int type, F&& f) {

@@ -592,6 +592,14 @@ int check(const char* who, const ppo_embedding_args* a, bool bwd) {
   return PPO_OK;
 }
 
+int check_apart(const char* who, const ppo_embedding_args& a, bool bwd) {
+  const int64_t in = type_size(a.src_type), out = type_size(a.dst_type);
+  const Rows src{a.src, bwd ? a.count : a.vocab, a.dim * in, a.ld_src * in}, dst{a.dst, bwd ? a.vocab : a.count, a.dim * out, a.ld_dst * out};
+  const Rows tokens = vector_of(a.tokens, a.count * (a.token_type == PPO_TOKENS_I64 ? 8 : 4));
+  PPO_REQUIRE(a.count == 0 || !(overlap(dst, src) || overlap(dst, tokens)), "%s: dst overlaps an input", who);
+  return PPO_OK;
+}
+
 struct BwdLayout {
   SortPlan sort;
   uint32_t unit, units;
@@ -653,6 +661,7 @@ extern "C" int ppo_embedding_fwd(const ppo_embedding_args* args, ppo_stream_t st
   if (int rc = check("ppo_embedding_fwd", args, false)) return rc;
   const ppo_embedding_args& a = *args;
   if (a.count == 0) return PPO_OK;
+  if (int rc = check_apart("ppo_embedding_fwd", a, false)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc = PPO_OK;
   with_type(a.src_type, [&](auto t) {
@@ -682,6 +691,7 @@ extern "C" int ppo_embedding_bwd(const ppo_embedding_args* args, void* workspace
   PPO_REQUIRE(workspace_bytes >= l.bytes && (workspace != nullptr || l.bytes == 0),
               "ppo_embedding_bwd: workspace too small (%zu < %zu)", workspace_bytes, l.bytes);
   PPO_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "ppo_embedding_bwd: the workspace must be 16-byte aligned");
+  if (int rc = check_apart("ppo_embedding_bwd", a, true)) return rc;
   if (a.count == 0 && a.accumulate) return PPO_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);

@@ -643,6 +643,23 @@ Layout workspace_for(int64_t rows) {
   return l;
 }
 
+int check_apart(const char* who, const ppo_token_loss_args& a, bool loss) {
+  const int64_t rows = a.rows, size = type_size(a.type);
+  const Rows logits{a.logits, rows, a.vocab * size, a.ld_logits * size};
+  const Rows d_logits{loss ? a.d_logits : nullptr, rows, a.vocab * size, a.ld_d_logits * size};
+  const Rows in[] = {vector_of(a.tokens, rows * (a.token_type == PPO_TOKENS_I64 ? 8 : 4)), vector_of(a.mask, rows),
+                     vector_of(loss ? a.old_logp : nullptr, rows * 4), vector_of(loss ? a.ref_logp : nullptr, rows * 4),
+                     vector_of(loss ? a.advantages : nullptr, rows * 4)};
+  const Rows out[] = {vector_of(a.logp, rows * 4), vector_of(a.entropy, rows * 4), vector_of(loss ? a.stats : nullptr, 32), d_logits};
+  PPO_REQUIRE(rows == 0 || d_logits.at == a.logits || !overlap(d_logits, logits), "%s: d_logits overlaps logits and is not in place", who);
+  for (int i = 0; i < 4; ++i) {
+    PPO_REQUIRE(rows == 0 || i == 3 || !overlap(out[i], logits), "%s: an output overlaps logits", who);
+    for (const Rows& x : in) PPO_REQUIRE(rows == 0 || !overlap(out[i], x), "%s: an output overlaps an input", who);
+    for (int k = 0; k < i; ++k) PPO_REQUIRE(rows == 0 || !overlap(out[i], out[k]), "%s: outputs overlap", who);
+  }
+  return PPO_OK;
+}
+
 int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream,
         bool loss) {
   PPO_REQUIRE(args != nullptr, "%s: null arguments", who);
@@ -671,6 +688,7 @@ int run(const char* who, const ppo_token_loss_args* args, void* workspace, size_
   const Layout l = workspace_for(a.rows);
   PPO_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= l.bytes,
               "%s: workspace too small or not 16-byte aligned (%zu < %zu)", who, workspace_bytes, l.bytes);
+  if (int rc = check_apart(who, a, loss)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LossKernelArgs q{};
   q.a = a;
