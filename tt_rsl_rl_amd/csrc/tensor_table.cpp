@@ -7,6 +7,8 @@
 #include <ATen/core/Tensor.h>
 
 #include <cmath>
+#include <cstring>
+#include <vector>
 
 #include "../../include/ppo_hip.h"
 
@@ -121,6 +123,27 @@ bool entry(const Tensors (&lists)[7], const Numbers& lr, const Numbers& weight_d
   return lr.at(i, e.lr) && weight_decay.at(i, e.weight_decay);
 }
 
+// Whether a parameter comes a second time: two blocks would step it at once.  An open hash table of twice as many places or more.
+struct Seen {
+  std::vector<const void*> places;
+  explicit Seen(Py_ssize_t n) {
+    size_t size = 2;
+    while (size < 2 * static_cast<size_t>(n)) size *= 2;
+    places.resize(size);
+  }
+  bool again(const void* p) {
+    size_t at = (reinterpret_cast<uintptr_t>(p) >> 4) * 0x9e3779b97f4a7c15u >> 20;
+    for (;; ++at) {
+      const void*& place = places[at & (places.size() - 1)];
+      if (place == p) return true;
+      if (place == nullptr) {
+        place = p;
+        return false;
+      }
+    }
+  }
+};
+
 // adamw_table(params, grads, masters, exp_avg, exp_avg_sq, m_scales, v_scales, step, lr, weight_decay, beta1, beta2, dither, device)
 // -> bytes
 PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
@@ -139,6 +162,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
     const int dither = PyObject_IsTrue(args[12]);
     const long device = PyLong_AsLong(args[13]);
     if (PyErr_Occurred()) return nullptr;
+    Seen seen(n);
     PyObject* out = PyBytes_FromStringAndSize(nullptr, n * static_cast<Py_ssize_t>(sizeof(ppo_adamw_tensor)));
     if (out == nullptr) return nullptr;
     auto* e = reinterpret_cast<ppo_adamw_tensor*>(PyBytes_AS_STRING(out));
@@ -152,6 +176,11 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t num) {
       }
       ppo_adamw_tensor x;
       if (!ok || !entry(lists, lr, weight_decay, i, static_cast<int>(device), x)) {
+        Py_DECREF(out);
+        return nullptr;
+      }
+      if (x.count > 0 && seen.again(x.param)) {
+        PyErr_Format(PyExc_ValueError, "adamw_step: params[%zd] comes a second time", i);
         Py_DECREF(out);
         return nullptr;
       }

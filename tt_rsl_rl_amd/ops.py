@@ -1207,7 +1207,7 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step,
                masters: list | None = None, scales: tuple[list, list] | None = None, norm_out: torch.Tensor | None = None,
                ws: Workspace | None = None, dither: bool = False) -> None:
     """One AdamW step over a list of contiguous tensors, in place, their gradients clipped by their common norm first
-    (max_grad_norm; the gradients themselves are left as they are).  params: float32, or bfloat16 with (masters) or without
+    (max_grad_norm; the gradients themselves are left as they are).  params, each once: float32, or bfloat16 with (masters) or without
     a float32 master each, in which case the master is stepped and the parameter is its rounding; grads: float32, or
     bfloat16 for a bfloat16 parameter; exp_avg / exp_avg_sq: float32, or int8 / uint8 with scales = (lists of) float32
     [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  step (from 1), lr and weight_decay: one
