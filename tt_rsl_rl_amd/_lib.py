@@ -10,11 +10,14 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib.util
 import os
 import struct
 from pathlib import Path
 
-# PPO_HIP_LIB names another build of the same library (the host-sanitizer build of sanitize_host.py)
+# PPO_HIP_LIB names another build of the same library (the host-sanitizer build of sanitize_host.py), PPO_HIP_TABLE one of the
+# module beside it
+TABLE_PATH = os.environ.get("PPO_HIP_TABLE")
 LIB_PATH = Path(os.environ.get("PPO_HIP_LIB") or Path(__file__).resolve().parent / "libppo_hip.so")
 
 PPO_OK = 0
@@ -355,10 +358,16 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
 def tensor_table():
     """The module that makes ppo_adamw_step's table from lists of tensors and marks tensors as written
     (csrc/tensor_table.cpp), built beside the library."""
+    name = f"{__package__}._tensor_table"
     try:
+        if TABLE_PATH:
+            spec = importlib.util.spec_from_file_location(name, TABLE_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            return module
         from . import _tensor_table
     except ImportError as e:
-        raise RuntimeError(f"{__package__}._tensor_table is missing or not of this torch: build the HIP library first "
+        raise RuntimeError(f"{name} is missing or not of this torch: build the HIP library first "
                            f"(python -m tt_rsl_rl_amd.build): {e}") from e
     return _tensor_table
 

@@ -59,23 +59,27 @@ def _compile(src: Path) -> Path:
     return obj
 
 
-def _compile_table() -> None:
+def compile_table(cxx: str, out: Path, flags: list[str]) -> None:
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
-    cxx = shutil.which("g++") or shutil.which("c++")
-    if cxx is None:
-        raise RuntimeError("g++ not found: it builds the module that reads torch's tensors")
-    tmp = TABLE.with_suffix(".so.tmp")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+    tmp = out.with_suffix(".so.tmp")
+    cmd = [cxx, *flags, "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-I{p}" for p in include_paths()), f"-I{sysconfig.get_paths()['include']}", str(CSRC / "tensor_table.cpp"), "-o", str(tmp),
            *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed on tensor_table.cpp:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, TABLE)
+        raise RuntimeError(f"{cxx} failed on tensor_table.cpp:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, out)
+
+
+def _compile_table() -> None:
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: it builds the module that reads torch's tensors")
+    compile_table(cxx, TABLE, ["-O2"])
 
 
 def build(verbose: bool = True) -> Path:
