@@ -749,7 +749,8 @@ enum { PPO_TOKENS_I64 = 0, PPO_TOKENS_I32 = 1 };
  * the table's gradient [vocab, dim], fp32 or of src's type.  Each row is summed in fp32 in an order that depends on the
  * tokens alone (the tokens are sorted first, stably), so the same call gives the same bits.  accumulate = 0 writes every
  * row, zeros where no token names it; otherwise the sum is added to the row and rows without tokens are left alone.
- * count may be 0; count < 2^31, vocab < 2^31.  dst may not lie on src or the tokens. */
+ * count may be 0; count < 2^31, vocab < 2^31.  (The gradient is made for calls of up to some million tokens: past that its sort
+ * takes time with the square of their number.)  dst may not lie on src or the tokens. */
 typedef struct ppo_embedding_args {
   const void* tokens;
   const void* src;

@@ -10,12 +10,13 @@
 // The powers place codes densely near zero, as the magnitudes lie: the smallest m but zero is 6e-5 of the block's largest, the
 // smallest sqrt(v) 1.5e-5 of it.  A wave owns a block of elements, four per lane, so the new scale is one wave reduction.
 // A step of beta2 = 0.999 lowers v by 0.1 % at most, and neighbouring codes of v lie 1.6 % or more apart: rounded to nearest, a v
-// below its block's largest never falls (gradients of half a block a tenth of what they were: 5,000 steps later their v is 120
+// below its block's largest never falls (gradients of half a block a tenth of what they were: 5,000 steps later their v is 82
 // times too large).  With `dither` a code is rounded up or down by chance, so that what it stands for is the value on average and
-// the moments follow (1.02 times, by the same count).
+// the moments follow (1.005 times, by the same count).
 //
 // Bound by memory: 28 bytes per fp32 parameter with fp32 states, and the gradient once more for the norm.
-// 60 M bf16 with masters: update 268 us, 6.3 TB/s, norm 25; 250 M with 8-bit states: update 705 us, 5.8 TB/s, norm 115.
+// 60 M bf16 with masters: update 269 us, 6.2 TB/s, norm 25; 250 M with 8-bit states: update 705 us, 5.8 TB/s, norm 114; with
+// dither the update is bound by its arithmetic (a step without a norm 804 us, 715 to nearest).
 #include "elem.hpp"
 
 #pragma clang fp contract(off)

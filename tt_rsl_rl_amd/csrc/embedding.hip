@@ -64,7 +64,8 @@ __global__ __launch_bounds__(kFwdThreads) void embedding_fwd_kernel(const ppo_em
 
 // Up to kRankMax tokens find their places by comparing each with all (rank_kernel, one launch); more are sorted in tiles of
 // kTile, two launches for each 9 bits of the token.  A tile's items lie as wave, round, lane: each wave owns kRounds * 64
-// consecutive ones.
+// consecutive ones.  Every block of a move reads all tiles' counts, so the sort's work has a part that grows with the square of
+// the tokens: 2 MB a pass for 131,072 of them, 34 GB for 16 M.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kRounds = 4, kTile = kRounds * kSortThreads;
 constexpr int64_t kRankMax = 12288;  // (gradients of 12,000 tokens 34 us so, 39 by the other; of 16,384 45 and 39)

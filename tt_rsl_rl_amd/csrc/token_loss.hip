@@ -14,8 +14,8 @@
 // Bound by memory: the logits once in, their gradient once out.  So a row is read once and stays in registers between its
 // sums and its gradient (token_row_kernel); only rows too wide for that are read twice (token_wide_kernel).  Each wave
 // takes its own maximum and sums, and the waves' (m, S, E) are joined after the one barrier of a row.
-// 8,192 x 131,072 bf16, a quarter of the rows masked: 710 us a call, 5.3 TB/s; log-probabilities of 8,192 x 32,000: 73 us
-// (70 with the fused multiply-add above).
+// 8,192 x 131,072 bf16, a quarter of the rows masked: 720 us a call, 5.2 TB/s; log-probabilities of 8,192 x 32,000: 73 us
+// (715 and 70 with the fused multiply-add above).
 #include "elem.hpp"
 
 namespace ppo {
@@ -391,8 +391,9 @@ __global__ __launch_bounds__(NT) void token_stats_kernel(const LossKernelArgs q)
 // A few wide rows, which one compute unit each would leave waiting for its arithmetic: a row is cut into parts of
 // kPartThreads kPartPieces pieces, a block each.  token_part_kernel leaves a part's sums; then token_joined_kernel's one wave
 // per row joins them, or each block of token_part_gradient_kernel does before it reads its part again, and one more block the
-// means of all rows.  Worth it (us, in one kernel -> in parts) for the loss of up to kSplitLossRows = a wave's lanes of rows
-// from 16,384 logits on (waited for: 16 x 16,384 bf16 24.5 -> 23.6, 16 x 32,000 27.3 -> 23.9, 8 x 131,072 39.8 -> 23.7), for
+// means of all rows.  Worth it (us, in one kernel -> in parts) for the loss of rows from 16,384 logits on (in a graph: 16 x 16,384
+// bf16 9.2 -> 8.0, 64 x 16,384 fp32 10.4 -> 7.9, 16 x 32,000 bf16 12.3 -> 8.2, 8 x 131,072 23.2 -> 8.0, 64 x 131,072 26.0 ->
+// 14.9), up to kSplitLossRows, since the block of the means has a lane for each row (more rows are not measured), and for
 // log-probabilities of up to kSplitRows from 65,536 on (8 x 131,072 bf16 10.8 -> 9.3, 257 23.3 -> 16.2, 512 fp32 42.8 -> 43.0; 8 x 50,021 8.5 -> 9.4).
 constexpr int kPartThreads = 256, kPartPieces = 4, kMaxParts = kWave;
 constexpr int64_t kSplitRows = 256, kSplitVocab = 65536, kSplitLossRows = kWave, kSplitLossVocab = 16384;

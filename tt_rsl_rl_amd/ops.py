@@ -1177,8 +1177,9 @@ def token_ppo_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.T
     """The clipped policy loss of tokens and its gradient: the mean over the rows that count (mask, as token_log_probs) of
     max(-A ratio, -A clip(ratio)) + kl_coef KL(policy || reference) - entropy_coef H, with ratio = exp(logp - old_logp) held
     to [1 - clip, 1 + clip] (a pair: its low and high width) and the KL estimated as exp(d) - d - 1, d = ref_logp - logp.
-    stats[8] float32 = loss, surrogate, KL, entropy, the share of clipped rows, mean old_logp - logp, rows, 0.
-    d_logits: like logits (may be logits itself), or None.  denom: divides the sums instead of the number of rows that
+    stats[8] float32 = loss, surrogate, KL, entropy, the share of clipped rows, mean old_logp - logp, the rows that count (or
+    denom), 0.  ref_logp with kl_coef 0: its KL is reported and nothing else.
+    d_logits: like logits (may be logits itself; no other output may lie on an input), or None.  denom: divides the sums instead of the number of rows that
     count, for calls that share one mean."""
     name = "token_ppo_loss"
     dev = _current_gpu(name, logits, tokens, old_logp, advantages, ref_logp, d_logits, stats, logp, entropy, mask)
@@ -1213,7 +1214,7 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step,
     [ceil(numel / ADAMW_BLOCK)] for each (all zeros is the zero state).  step (from 1), lr and weight_decay: one
     value, or one per tensor.  norm_out: float32 [2] for the norm and the clip coefficient.  dither: 8-bit states are rounded
     up or down by chance (the same for the same step), so that over many steps they follow the moments; rounded to nearest they
-    do not (ppo_hip.h)."""
+    do not (ppo_hip.h).  step and lr travel with the launch: replays of a captured one repeat them."""
     if max_grad_norm is not None and not max_grad_norm > 0:
         raise ValueError(f"adamw_step: max_grad_norm={max_grad_norm}")
     n = len(params)
