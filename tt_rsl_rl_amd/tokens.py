@@ -53,9 +53,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW on ``ops.adamw_step``: one call for all parameters, their gradients clipped by their common norm first
     (max_grad_norm; ``norm`` holds the last norm and clip coefficient on the GPU).  Parameters are float32 or bfloat16; the
     latter get a float32 master unless ``masters`` is False.  state_bits: 32, or 8 for both moments in 8 bits, rounded by
-    chance that the step's number decides, so that the same steps give the same bits.  Groups may
-    have their own lr and weight_decay; their betas and eps are one value for all of them (a scheduler may change it between
-    steps).  Parameters without a gradient are left alone."""
+    chance that the step's number decides, so that the same steps give the same bits.  Groups may have their own lr and
+    weight_decay; their betas and eps are one value for all of them (a scheduler may change it between steps).  Parameters
+    without a gradient are left alone."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, max_grad_norm: float | None = None, state_bits: int = 32, masters: bool = True) -> None:
