@@ -855,6 +855,148 @@ size_t ppo_adamw_workspace_bytes(const ppo_adamw_tensor* tensors, int32_t count)
 int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, double max_norm, double beta1, double beta2, double eps,
                    float* norm_out, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Between a token policy's embedding and its logits.  Tokens of all sequences lie one after another; a ppo_head_view is a
+ * view [tokens, heads, elements] of unit element stride, the other strides in elements (columns of a projection's output, heads
+ * before tokens: any of them; an input's may be 0).  Views of one call share its element type.
+ * ------------------------------------------------------------------------------------------------------------------ */
+typedef struct ppo_head_view {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} ppo_head_view;
+
+/* Queries and keys of each head, normed and turned by their token's position.  For one head's row x of D = head_dim elements:
+ *   n = x / sqrt(mean(x^2) + eps);   y = weight n;   and of y's first R = rotary_dim elements pair i = 0 .. R/2 - 1 (a, b) becomes
+ *   (a cos t - b sin t, b cos t + a sin t),   t = positions[token] freqs[i],
+ * where pair i is elements (i, i + R/2), or (2i, 2i + 1) with interleaved.  The angle is taken in fp64, so positions may be far (its
+ * error is some 2^-52 of the angle).  The weight is [D] for all heads, or [heads, D] (weight_per_head).
+ * The backward pass takes the gradients of the results (q_out, k_out), turns them back (g) and gives
+ *   d_weight = sum g n (over tokens, and heads where they share it);   d_x = (weight g - n mean(weight g n)) / sqrt(mean(x^2) + eps).
+ * Sums over tokens are fp32 over up to some hundred rows and fp64 over those, in a fixed order: the same call gives the same bits.
+ * D and R are even, D <= PPO_QK_MAX_DIM, 2 <= R <= D.  q_out and k_out (d_q and d_k) may be the very views that the call reads in
+ * their place (q and k; going back also q_out and k_out); no other output may lie on an input or another output. */
+#define PPO_QK_MAX_DIM 512
+typedef struct ppo_qk_rotary_args {
+  ppo_head_view q, k;
+  ppo_head_view q_out, k_out; /* written; by the backward pass read: their gradients */
+  ppo_head_view d_q, d_k;     /* backward only */
+  const void* q_weight;
+  const void* k_weight;
+  void* d_q_weight; /* backward only, of the weights' type */
+  void* d_k_weight;
+  const void* positions; /* [tokens] */
+  const double* freqs;   /* [rotary_dim / 2] */
+  int64_t tokens;
+  double eps;
+  int32_t q_heads, kv_heads;
+  int32_t head_dim, rotary_dim;
+  int32_t type;          /* PPO_TYPE_* */
+  int32_t weight_type;   /* `type`, or PPO_TYPE_F32 */
+  int32_t position_type; /* PPO_TOKENS_* */
+  int32_t interleaved;
+  int32_t weight_per_head;
+  int32_t reserved;
+} ppo_qk_rotary_args;
+int ppo_qk_rotary_fwd(const ppo_qk_rotary_args* args, ppo_stream_t stream);
+size_t ppo_qk_rotary_bwd_workspace_bytes(const ppo_qk_rotary_args* args);
+int ppo_qk_rotary_bwd(const ppo_qk_rotary_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+
+/* Linear attention whose past fades by a factor for each head, f = exp(log_decay[h]).  Token t of a sequence, key-value head h and
+ * the q_heads / kv_heads queries that share it:
+ *   S_t = f S_{t-1} + k_t v_t^T   (S [key_dim, value_dim], fp32);   o_t = scale q_t^T S_t,
+ * in chunks: what a chunk's tokens say to each other goes by the matrix scale (q_i . k_j) f^(i-j), i >= j, what lies before by S.
+ * cu_seqlens: sequence b is tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1 (non-decreasing, from 0 up; what leaves [0, tokens] is
+ * cut; NULL: one sequence of all tokens).  Tokens before the first sequence and behind the last one are left as they are, in inputs
+ * and outputs.  S starts at initial_state[b] (NULL: zeros) and ends in final_state[b] (NULL: not wanted), both
+ * [sequences, kv_heads, key_dim, value_dim]; a sequence without tokens hands the one to the other.  A log_decay of -inf leaves each
+ * token alone with itself; above 0 the past grows.  log_decay is a constant: it gets no gradient.
+ * Backward, with R_t = f R_{t+1} + scale q_t d_out_t^T from d_final_state[b] (NULL: zeros) on:
+ *   d_q_t = scale S_t d_out_t;   d_k_t = R_t v_t;   d_v_t = R_t^T k_t   (summed over the queries that share a head);
+ *   d_initial_state[b] = f R_first (NULL: not wanted).
+ * States, sums and the powers of f are fp32 or more.  Of 16-bit inputs the matrix cores' operands that the call makes itself (S,
+ * R, the chunks' matrices) are held as sums of two 16-bit parts, those that make a state as three.  Everything is summed in a fixed
+ * order.  key_dim, value_dim <= PPO_DECAY_MAX_DIM.  No output may lie on an input or another output, but d_initial_state may be
+ * d_final_state and final_state may be initial_state. */
+#define PPO_DECAY_MAX_DIM 128
+typedef struct ppo_decay_attention_args {
+  ppo_head_view q, k, v;
+  ppo_head_view out; /* written; by the backward pass read: its gradient */
+  ppo_head_view d_q, d_k, d_v; /* backward only */
+  const float* log_decay; /* [kv_heads] */
+  const void* cu_seqlens; /* [sequences + 1], int64 or int32 */
+  const float* initial_state;
+  float* final_state;           /* forward only */
+  const float* d_final_state;   /* backward only */
+  float* d_initial_state;
+  int64_t tokens;
+  int64_t sequences;
+  double scale;
+  int32_t q_heads, kv_heads;
+  int32_t key_dim, value_dim;
+  int32_t type;        /* PPO_TYPE_* */
+  int32_t cu_type;     /* PPO_TOKENS_* */
+} ppo_decay_attention_args;
+size_t ppo_decay_attention_workspace_bytes(const ppo_decay_attention_args* args, int32_t backward);
+int ppo_decay_attention_fwd(const ppo_decay_attention_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+int ppo_decay_attention_bwd(const ppo_decay_attention_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+
+/* One token of each of `rows` sequences: S = f S + k v^T in place and o = scale q^T S, on states[slots[row]] (slots NULL:
+ * states[row]).  fresh[row] not 0: the sequence begins here, its S is taken as zeros and not read.  A slot outside [0, num_slots) is
+ * a row of padding: no state is touched, its output is 0.  Two rows may not name the same slot. */
+typedef struct ppo_decay_step_args {
+  ppo_head_view q, k, v, out; /* [rows, heads, elements] */
+  const float* log_decay;
+  float* states; /* [num_slots, kv_heads, key_dim, value_dim] */
+  const void* slots;
+  const uint8_t* fresh;
+  int64_t rows;
+  int64_t num_slots;
+  double scale;
+  int32_t q_heads, kv_heads;
+  int32_t key_dim, value_dim;
+  int32_t type;
+  int32_t slot_type; /* PPO_TOKENS_* */
+} ppo_decay_step_args;
+int ppo_decay_attention_step(const ppo_decay_step_args* args, ppo_stream_t stream);
+
+/* Cross entropy of tokens under a head as wide as the vocabulary, without its logits in memory.  Row r with z = hidden[r, :] weight^T
+ * / temperature (1e-6 to 1e6) and t = tokens[r]:
+ *   lp = z_t - log sum_j exp(z_j);   p_j = exp(z_j - log sum exp z);   H = -sum_j p_j log p_j;   loss = -sum_r lp / N;
+ *   d_z[r, j] = (p_j - [j = t]) / (N temperature);   d_hidden = d_z weight;   d_weight = d_z^T hidden.
+ * Rows count, and N is, as in ppo_token_ppo_loss; a row that does not count gives lp = H = 0 and d_hidden 0.  Rows whose hidden or
+ * products are not finite give what the formulas give.  If no row counts, everything is 0.
+ * ppo_linear_log_probs writes logp and entropy (either may be NULL).  ppo_linear_cross_entropy writes also stats[4] = loss, mean H,
+ * N, 0 and d_hidden and d_weight, of their operands' type (either may be NULL: not wanted); logp and entropy as before.
+ * Products are exact in fp32 sums (fp32 operands as three bf16 parts, six products); d_z is rounded to the operands' type for the
+ * second products (fp32: three parts again), once, before 1 / (N temperature) is applied.  Everything is summed in a fixed order.
+ * The workspace holds a piece of d_z, some tens of thousands of columns at a time.  No output may lie on an input or another output. */
+typedef struct ppo_linear_loss_args {
+  const void* hidden; /* [rows, dim] */
+  int64_t ld_hidden;
+  const void* weight; /* [vocab, dim] */
+  int64_t ld_weight;
+  const void* tokens;
+  const uint8_t* mask;
+  void* d_hidden;
+  int64_t ld_d_hidden;
+  void* d_weight;
+  int64_t ld_d_weight;
+  float* logp;
+  float* entropy;
+  float* stats;
+  int64_t rows;
+  int64_t vocab;
+  int64_t dim;
+  double temperature;
+  double denom;
+  int32_t type;       /* PPO_TYPE_* */
+  int32_t token_type; /* PPO_TOKENS_* */
+} ppo_linear_loss_args;
+size_t ppo_linear_loss_workspace_bytes(const ppo_linear_loss_args* args, int32_t gradient);
+int ppo_linear_log_probs(const ppo_linear_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+int ppo_linear_cross_entropy(const ppo_linear_loss_args* args, void* workspace, size_t workspace_bytes, ppo_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -228,10 +228,50 @@ class AdamwTensor(C.Structure):
                 ("grad_type", i32), ("state_bits", i32), ("reserved", i32), ("dither", i64)]
 
 
+QK_MAX_DIM = 512     # largest head of ppo_qk_rotary_*
+DECAY_MAX_DIM = 128  # largest key and value head of ppo_decay_attention_*
+
+
+class HeadView(C.Structure):
+    _fields_ = [("data", vp), ("token_stride", i64), ("head_stride", i64)]
+
+
+class QkRotaryArgs(C.Structure):
+    _fields_ = [(name, HeadView) for name in ("q", "k", "q_out", "k_out", "d_q", "d_k")] + [
+        ("q_weight", vp), ("k_weight", vp), ("d_q_weight", vp), ("d_k_weight", vp), ("positions", vp), ("freqs", vp), ("tokens", i64),
+        ("eps", C.c_double), ("q_heads", i32), ("kv_heads", i32), ("head_dim", i32), ("rotary_dim", i32), ("type", i32), ("weight_type", i32),
+        ("position_type", i32), ("interleaved", i32), ("weight_per_head", i32), ("reserved", i32)]
+
+
+class DecayAttentionArgs(C.Structure):
+    _fields_ = [(name, HeadView) for name in ("q", "k", "v", "out", "d_q", "d_k", "d_v")] + [
+        ("log_decay", vp), ("cu_seqlens", vp), ("initial_state", vp), ("final_state", vp), ("d_final_state", vp), ("d_initial_state", vp),
+        ("tokens", i64), ("sequences", i64), ("scale", C.c_double), ("q_heads", i32), ("kv_heads", i32), ("key_dim", i32), ("value_dim", i32),
+        ("type", i32), ("cu_type", i32)]
+
+
+class DecayStepArgs(C.Structure):
+    _fields_ = [(name, HeadView) for name in ("q", "k", "v", "out")] + [
+        ("log_decay", vp), ("states", vp), ("slots", vp), ("fresh", vp), ("rows", i64), ("num_slots", i64), ("scale", C.c_double), ("q_heads", i32),
+        ("kv_heads", i32), ("key_dim", i32), ("value_dim", i32), ("type", i32), ("slot_type", i32)]
+
+
+class LinearLossArgs(C.Structure):
+    _fields_ = [("hidden", vp), ("ld_hidden", i64), ("weight", vp), ("ld_weight", i64), ("tokens", vp), ("mask", vp), ("d_hidden", vp),
+                ("ld_d_hidden", i64), ("d_weight", vp), ("ld_d_weight", i64), ("logp", vp), ("entropy", vp), ("stats", vp), ("rows", i64),
+                ("vocab", i64), ("dim", i64), ("temperature", C.c_double), ("denom", C.c_double), ("type", i32), ("token_type", i32)]
+
+
 # the same packed by hand, a third of the time of their fields
 EMBEDDING_ARGS = struct.Struct("@PPqPqqqiiiifi")
 TOKEN_LOSS_ARGS = struct.Struct("@PqPPPPPPqPPPqqddddddii")
+QK_ROTARY_ARGS = struct.Struct("@" + 6 * "Pqq" + "PPPPPPqdiiiiiiiiii")
+DECAY_ATTENTION_ARGS = struct.Struct("@" + 7 * "Pqq" + "PPPPPPqqdiiiiii")
+DECAY_STEP_ARGS = struct.Struct("@" + 4 * "Pqq" + "PPPPqqdiiiiii")
+LINEAR_LOSS_ARGS = struct.Struct("@PqPqPPPqPqPPPqqqddii")
 assert (EMBEDDING_ARGS.size, TOKEN_LOSS_ARGS.size) == (C.sizeof(EmbeddingArgs), C.sizeof(TokenLossArgs))
+assert (QK_ROTARY_ARGS.size, DECAY_ATTENTION_ARGS.size) == (C.sizeof(QkRotaryArgs), C.sizeof(DecayAttentionArgs))
+assert (DECAY_STEP_ARGS.size, LINEAR_LOSS_ARGS.size) == (C.sizeof(DecayStepArgs), C.sizeof(LinearLossArgs))
 
 # (name, restype, argtypes)
 _SIGNATURES = [
@@ -326,10 +366,20 @@ _SIGNATURES = [
     ("ppo_token_ppo_loss", C.c_int, [vp, vp, C.c_size_t, vp]),
     ("ppo_adamw_workspace_bytes", C.c_size_t, [vp, i32]),
     ("ppo_adamw_step", C.c_int, [vp, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp, C.c_size_t, vp]),
+    ("ppo_qk_rotary_fwd", C.c_int, [vp, vp]),
+    ("ppo_qk_rotary_bwd_workspace_bytes", C.c_size_t, [vp]),
+    ("ppo_qk_rotary_bwd", C.c_int, [vp, vp, C.c_size_t, vp]),
+    ("ppo_decay_attention_workspace_bytes", C.c_size_t, [vp, i32]),
+    ("ppo_decay_attention_fwd", C.c_int, [vp, vp, C.c_size_t, vp]),
+    ("ppo_decay_attention_bwd", C.c_int, [vp, vp, C.c_size_t, vp]),
+    ("ppo_decay_attention_step", C.c_int, [vp, vp]),
+    ("ppo_linear_loss_workspace_bytes", C.c_size_t, [vp, i32]),
+    ("ppo_linear_log_probs", C.c_int, [vp, vp, C.c_size_t, vp]),
+    ("ppo_linear_cross_entropy", C.c_int, [vp, vp, C.c_size_t, vp]),
 ]
 
 EXPORTED_SYMBOLS = [name for name, _, _ in _SIGNATURES]
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 _lib: C.CDLL | None = None
 

@@ -1233,3 +1233,268 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step,
     L.call("ppo_adamw_step", packed, n, float(max_grad_norm or 0.0), float(beta1), float(beta2), float(eps),
            _ptr(norm_out), _ptr(buf), 0 if buf is None else buf.numel(), _raw_stream(dev))
     _written(params, masters, exp_avg, exp_avg_sq, m_scales, v_scales, norm_out)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# token policies, between embedding and logits: normed and turned queries and keys, decaying linear attention, cross entropy of a head
+# without its logits
+# ----------------------------------------------------------------------------------------------------------------------
+
+
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None, shape: tuple | None = None) -> tuple[int, int, int]:
+    """Address, token stride and head stride of a view [tokens, heads, elements] of unit element stride, of like's type."""
+    if like is not None and t.dtype != like.dtype:
+        raise ValueError(f"{name} must be {like.dtype}, got {t.dtype}")
+    if t.dim() != 3 or shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be [tokens, heads, elements]{'' if shape is None else f' {list(shape)}'}, got {list(t.shape)}")
+    token, head, unit = t.stride()
+    if unit != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name} must have unit element stride, got strides {t.stride()}")
+    return t.data_ptr(), token, head
+
+
+_NO_VIEW = (0, 0, 0)
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """The angles a position of 1 turns pairs by, base^(-2i / dim), float64 [dim / 2]: what qk_norm_rotary_fwd takes as ``freqs``."""
+    if dim < 2 or dim % 2 or not base > 0:
+        raise ValueError(f"rotary_frequencies: dim={dim} base={base}")
+    return base ** (torch.arange(0, dim, 2, dtype=torch.float64, device=device) / -dim)
+
+
+def _qk_of(name: str, q, k, q_weight, k_weight, positions, freqs, more: list) -> tuple:
+    """(device, packing of the arguments between the views and the sizes, of the sizes), checked."""
+    dev = _current_gpu(name, q, k, q_weight, k_weight, positions, freqs, *more)
+    elem = _element_type(q, f"{name}: q")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"{name}: q and k must be [tokens, heads, elements], got {list(q.shape)} and {list(k.shape)}")
+    tokens, q_heads, dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape[0] != tokens or k.shape[2] != dim:
+        raise ValueError(f"{name}: k must be [{tokens}, heads, {dim}], got {list(k.shape)}")
+    weight_type = _element_type(q_weight, f"{name}: q_weight")
+    if k_weight.dtype != q_weight.dtype or weight_type not in (elem, L.TYPE_F32):
+        raise ValueError(f"{name}: weights must both be {q.dtype} or float32, got {q_weight.dtype} and {k_weight.dtype}")
+    per_head = q_weight.dim() == 2
+    for w, heads, what in ((q_weight, q_heads, "q_weight"), (k_weight, kv_heads, "k_weight")):
+        if tuple(w.shape) != ((heads, dim) if per_head else (dim,)) or not w.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous [{dim}] or (both weights) [{heads}, {dim}], got {list(w.shape)}")
+    if positions.numel() != tokens:
+        raise ValueError(f"{name}: {positions.numel()} positions for {tokens} tokens")
+    position_type = TOKEN_TYPES.get(positions.dtype)
+    if position_type is None or not positions.is_contiguous():
+        raise ValueError(f"{name}: positions must be contiguous int64 or int32, got {positions.dtype}")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise ValueError(f"{name}: freqs must be contiguous float64 [rotary_dim / 2], got {freqs.dtype} {list(freqs.shape)}")
+    return dev, (positions.data_ptr(), freqs.data_ptr(), tokens), (q_heads, kv_heads, dim, 2 * freqs.numel(), elem, weight_type, position_type), per_head
+
+
+def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                       freqs: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor, eps: float = 1e-6, interleaved: bool = False) -> None:
+    """Each head's row of q [tokens, q_heads, dim] and k [tokens, kv_heads, dim] (views of any token and head strides: columns of a
+    projection's output) over its root mean square, times its weight ([dim], or [heads, dim]; of q's type or float32), its first
+    2 * freqs.numel() elements then turned by positions[token] * freqs (int64 or int32; float64, rotary_frequencies()): pair i is elements
+    (i, i + n) of n pairs, or (2i, 2i + 1) with interleaved.  q_out / k_out: like q / k; may be q / k themselves.  dim is even, up to
+    512."""
+    name = "qk_norm_rotary_fwd"
+    dev, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs, [q_out, k_out])
+    args = L.QK_ROTARY_ARGS.pack(*_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(q_out, f"{name}: q_out", q, tuple(q.shape)),
+                                 *_heads(k_out, f"{name}: k_out", q, tuple(k.shape)), *_NO_VIEW, *_NO_VIEW, q_weight.data_ptr(),
+                                 k_weight.data_ptr(), 0, 0, *middle, eps, *sizes, bool(interleaved), per_head, 0)
+    L.call("ppo_qk_rotary_fwd", args, _raw_stream(dev))
+    _written(q_out, k_out)
+
+
+def qk_norm_rotary_bwd(d_q_out: torch.Tensor, d_k_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                       k_weight: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, d_q: torch.Tensor, d_k: torch.Tensor,
+                       d_q_weight: torch.Tensor, d_k_weight: torch.Tensor, eps: float = 1e-6, interleaved: bool = False,
+                       ws: Workspace | None = None) -> None:
+    """The gradients of qk_norm_rotary_fwd's inputs from those of its outputs: d_q / d_k like q / k (may be d_q_out or q themselves, d_k_out
+    or k), d_q_weight / d_k_weight like the weights.  The weights' sums go in a fixed order: the same call gives the same bits."""
+    name = "qk_norm_rotary_bwd"
+    dev, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs,
+                                          [d_q_out, d_k_out, d_q, d_k, d_q_weight, d_k_weight])
+    for d, w, what in ((d_q_weight, q_weight, "d_q_weight"), (d_k_weight, k_weight, "d_k_weight")):
+        if d.dtype != w.dtype or d.shape != w.shape or not d.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous {w.dtype} {list(w.shape)}, got {d.dtype} {list(d.shape)}")
+    of_q, of_k = tuple(q.shape), tuple(k.shape)
+    args = L.QK_ROTARY_ARGS.pack(*_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(d_q_out, f"{name}: d_q_out", q, of_q),
+                                 *_heads(d_k_out, f"{name}: d_k_out", q, of_k), *_heads(d_q, f"{name}: d_q", q, of_q),
+                                 *_heads(d_k, f"{name}: d_k", q, of_k), q_weight.data_ptr(), k_weight.data_ptr(), d_q_weight.data_ptr(),
+                                 d_k_weight.data_ptr(), *middle, eps, *sizes, bool(interleaved), per_head, 0)
+    buf = _scratch(ws, q.device, L.load().ppo_qk_rotary_bwd_workspace_bytes(args))
+    L.call("ppo_qk_rotary_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    _written(d_q, d_k, d_q_weight, d_k_weight)
+
+
+def _decay_of(name: str, q, k, v, out, log_decay) -> tuple[int, int, int, int, int, int]:
+    """(tokens, q_heads, kv_heads, key_dim, value_dim, element type), checked."""
+    elem = _element_type(q, f"{name}: q")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"{name}: q, k and v must be [tokens, heads, elements], got {list(q.shape)}, {list(k.shape)} and {list(v.shape)}")
+    tokens, q_heads, key_dim = q.shape
+    kv_heads, value_dim = v.shape[1:]
+    if tuple(k.shape) != (tokens, kv_heads, key_dim) or v.shape[0] != tokens or kv_heads == 0 or q_heads % kv_heads:
+        raise ValueError(f"{name}: k and v must be [{tokens}, heads, {key_dim}] and [{tokens}, heads, elements] with heads that divide {q_heads}, "
+                         f"got {list(k.shape)} and {list(v.shape)}")
+    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (kv_heads,) or not log_decay.is_contiguous():
+        raise ValueError(f"{name}: log_decay must be contiguous float32 [{kv_heads}], got {log_decay.dtype} {list(log_decay.shape)}")
+    return tokens, q_heads, kv_heads, key_dim, value_dim, elem
+
+
+def _sequences_of(name: str, cu_seqlens: torch.Tensor | None) -> tuple[int, int, int]:
+    """(sequences, address, type) of cu_seqlens."""
+    if cu_seqlens is None:
+        return 1, 0, L.TOKENS_I32
+    code = TOKEN_TYPES.get(cu_seqlens.dtype)
+    if code is None or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous():
+        raise ValueError(f"{name}: cu_seqlens must be contiguous int64 or int32 [sequences + 1], got {cu_seqlens.dtype} {list(cu_seqlens.shape)}")
+    return cu_seqlens.numel() - 1, cu_seqlens.data_ptr(), code
+
+
+def _state(t: torch.Tensor | None, name: str, shape: tuple) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t.data_ptr()
+
+
+def decay_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, out: torch.Tensor, scale: float = 1.0,
+                        cu_seqlens: torch.Tensor | None = None, initial_state: torch.Tensor | None = None,
+                        final_state: torch.Tensor | None = None, ws: Workspace | None = None) -> None:
+    """Linear attention with a decay for each head over packed sequences: S_t = exp(log_decay[h]) S_(t-1) + k_t v_t^T, out_t = scale
+    q_t^T S_t.  q [tokens, q_heads, key_dim], k [tokens, kv_heads, key_dim], v [tokens, kv_heads, value_dim], out [tokens, q_heads, value_dim]
+    of one type, float32, bfloat16 or float16 (views of any token and head strides; query heads share key-value heads in groups of
+    neighbours); log_decay float32 [kv_heads].  Sequence b is tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1 (int64 or int32, on the GPU;
+    None: one sequence); tokens outside are left as they are.  States are float32 [sequences, kv_heads, key_dim, value_dim], what a sequence
+    starts from (None: zeros) and ends with; final_state may be initial_state.  Key and value heads of up to 128 elements.  A token whose key
+    or value is not finite makes NaN of its heads' results from there to its sequence's end, and of no others."""
+    name = "decay_attention_fwd"
+    dev = _current_gpu(name, q, k, v, log_decay, out, cu_seqlens, initial_state, final_state)
+    tokens, q_heads, kv_heads, key_dim, value_dim, elem = _decay_of(name, q, k, v, out, log_decay)
+    sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
+    shape = (sequences, kv_heads, key_dim, value_dim)
+    args = L.DECAY_ATTENTION_ARGS.pack(
+        *_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(v, f"{name}: v", q),
+        *_heads(out, f"{name}: out", q, (tokens, q_heads, value_dim)), *_NO_VIEW, *_NO_VIEW, *_NO_VIEW, log_decay.data_ptr(), cu,
+        _state(initial_state, f"{name}: initial_state", shape), _state(final_state, f"{name}: final_state", shape), 0, 0, tokens, sequences, scale,
+        q_heads, kv_heads, key_dim, value_dim, elem, cu_type)
+    buf = _scratch(ws, q.device, L.load().ppo_decay_attention_workspace_bytes(args, 0))
+    L.call("ppo_decay_attention_fwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    _written(out, final_state)
+
+
+def decay_attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, d_q: torch.Tensor,
+                        d_k: torch.Tensor, d_v: torch.Tensor, scale: float = 1.0, cu_seqlens: torch.Tensor | None = None,
+                        initial_state: torch.Tensor | None = None, d_final_state: torch.Tensor | None = None,
+                        d_initial_state: torch.Tensor | None = None, ws: Workspace | None = None) -> None:
+    """The gradients of decay_attention_fwd's q, k, v and initial_state from those of its out and final_state (None: zeros).  log_decay is a
+    constant.  d_initial_state may be d_final_state."""
+    name = "decay_attention_bwd"
+    dev = _current_gpu(name, q, k, v, log_decay, d_out, d_q, d_k, d_v, cu_seqlens, initial_state, d_final_state, d_initial_state)
+    tokens, q_heads, kv_heads, key_dim, value_dim, elem = _decay_of(name, q, k, v, d_out, log_decay)
+    sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
+    shape = (sequences, kv_heads, key_dim, value_dim)
+    args = L.DECAY_ATTENTION_ARGS.pack(
+        *_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(v, f"{name}: v", q),
+        *_heads(d_out, f"{name}: d_out", q, (tokens, q_heads, value_dim)), *_heads(d_q, f"{name}: d_q", q, tuple(q.shape)),
+        *_heads(d_k, f"{name}: d_k", q, tuple(k.shape)), *_heads(d_v, f"{name}: d_v", q, tuple(v.shape)), log_decay.data_ptr(), cu,
+        _state(initial_state, f"{name}: initial_state", shape), 0, _state(d_final_state, f"{name}: d_final_state", shape),
+        _state(d_initial_state, f"{name}: d_initial_state", shape), tokens, sequences, scale, q_heads, kv_heads, key_dim, value_dim, elem, cu_type)
+    buf = _scratch(ws, q.device, L.load().ppo_decay_attention_workspace_bytes(args, 1))
+    L.call("ppo_decay_attention_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    _written(d_q, d_k, d_v, d_initial_state)
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, out: torch.Tensor,
+                         scale: float = 1.0, slots: torch.Tensor | None = None, fresh: torch.Tensor | None = None) -> None:
+    """One token of each of several sequences through decay_attention_fwd's recurrence, the states updated in place.  q, k, v, out: as there,
+    with rows for tokens; state float32 [slots, kv_heads, key_dim, value_dim].  slots (int64 or int32; None: row r's state is state[r]):
+    each row's state, no two the same; one outside the states is a row of padding, whose output is 0.  fresh (bool or uint8): the
+    sequence begins with this token, whatever its state held."""
+    name = "decay_attention_step"
+    dev = _current_gpu(name, q, k, v, log_decay, state, out, slots, fresh)
+    rows, q_heads, kv_heads, key_dim, value_dim, elem = _decay_of(name, q, k, v, out, log_decay)
+    if state.dim() != 4:
+        raise ValueError(f"{name}: state must be [slots, {kv_heads}, {key_dim}, {value_dim}], got {list(state.shape)}")
+    at, slot_type = 0, L.TOKENS_I32
+    if slots is not None:
+        slot_type = TOKEN_TYPES.get(slots.dtype)
+        if slot_type is None or slots.numel() != rows or not slots.is_contiguous():
+            raise ValueError(f"{name}: slots must be contiguous int64 or int32 of {rows} elements, got {slots.dtype} {list(slots.shape)}")
+        at = slots.data_ptr()
+    begins = 0
+    if fresh is not None:
+        if fresh.dtype not in (torch.bool, torch.uint8) or fresh.numel() != rows or not fresh.is_contiguous():
+            raise ValueError(f"{name}: fresh must be contiguous bool or uint8 of {rows} elements, got {fresh.dtype} {list(fresh.shape)}")
+        begins = fresh.data_ptr()
+    args = L.DECAY_STEP_ARGS.pack(
+        *_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(v, f"{name}: v", q),
+        *_heads(out, f"{name}: out", q, (rows, q_heads, value_dim)), log_decay.data_ptr(),
+        _state(state, f"{name}: state", (state.shape[0], kv_heads, key_dim, value_dim)), at, begins, rows, state.shape[0], scale, q_heads, kv_heads,
+        key_dim, value_dim, elem, slot_type)
+    L.call("ppo_decay_attention_step", args, _raw_stream(dev))
+    _written(state, out)
+
+
+def _linear_of(name: str, hidden, weight, tokens, mask) -> tuple:
+    """(rows, vocab, dim, leading dimensions, element type, token type, mask pointer), checked."""
+    rows, dim, ld_hidden = _matrix(hidden, f"{name}: hidden")
+    vocab, cols, ld_weight = _matrix(weight, f"{name}: weight")
+    if cols != dim or weight.dtype != hidden.dtype:
+        raise ValueError(f"{name}: weight must be {hidden.dtype} [vocab, {dim}], got {weight.dtype} {list(weight.shape)}")
+    if tokens.numel() != rows:
+        raise ValueError(f"{name}: {tokens.numel()} tokens for {rows} rows")
+    kept = 0
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != rows or not mask.is_contiguous():
+            raise ValueError(f"{name}: mask must be contiguous bool or uint8 of {rows} elements, got {mask.dtype} {tuple(mask.shape)}")
+        kept = mask.data_ptr()
+    return rows, vocab, dim, ld_hidden, ld_weight, _element_type(hidden, f"{name}: hidden"), _tokens(tokens, name), kept
+
+
+def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor | None,
+                     entropy: torch.Tensor | None = None, mask: torch.Tensor | None = None, temperature: float = 1.0,
+                     ws: Workspace | None = None) -> None:
+    """token_log_probs of the logits hidden weight^T, without the logits: hidden [rows, dim], weight [vocab, dim] of one type, float32,
+    bfloat16 or float16; the products are summed in fp32.  Rows that do not count (as there) are not read and give 0."""
+    name = "linear_log_probs"
+    dev = _current_gpu(name, hidden, weight, tokens, logp, entropy, mask)
+    rows, vocab, dim, ld_hidden, ld_weight, elem, token_type, kept = _linear_of(name, hidden, weight, tokens, mask)
+    args = L.LINEAR_LOSS_ARGS.pack(hidden.data_ptr(), ld_hidden, weight.data_ptr(), ld_weight, tokens.data_ptr(), kept, 0, 0, 0, 0,
+                                   _vector(logp, f"{name}: logp", rows), _vector(entropy, f"{name}: entropy", rows), 0, rows, vocab, dim, temperature, 0.0,
+                                   elem, token_type)
+    buf = _scratch(ws, hidden.device, L.load().ppo_linear_loss_workspace_bytes(args, 0))
+    L.call("ppo_linear_log_probs", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    _written(logp, entropy)
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, d_hidden: torch.Tensor | None,
+                         d_weight: torch.Tensor | None, stats: torch.Tensor, logp: torch.Tensor | None = None,
+                         entropy: torch.Tensor | None = None, mask: torch.Tensor | None = None, temperature: float = 1.0,
+                         denom: float | None = None, ws: Workspace | None = None) -> None:
+    """The mean over the rows that count (as token_log_probs) of -log softmax(hidden weight^T / temperature)[token], and its gradients, in
+    pieces of the vocabulary: the logits are never all in memory.  hidden [rows, dim] and weight [vocab, dim] of one type; d_hidden and
+    d_weight like them (None: not wanted), d_hidden 0 where a row does not count.  stats[4] float32 = loss, mean entropy, the rows that
+    count (or denom), 0.  denom: divides the sums instead of the number of rows that count, for calls that share one mean."""
+    name = "linear_cross_entropy"
+    dev = _current_gpu(name, hidden, weight, tokens, d_hidden, d_weight, stats, logp, entropy, mask)
+    rows, vocab, dim, ld_hidden, ld_weight, elem, token_type, kept = _linear_of(name, hidden, weight, tokens, mask)
+    grads = []
+    for d, x, what in ((d_hidden, hidden, "d_hidden"), (d_weight, weight, "d_weight")):
+        if d is None:
+            grads += [0, 0]
+            continue
+        if d.dtype != x.dtype or d.shape != x.shape:
+            raise ValueError(f"{name}: {what} must be {x.dtype} {list(x.shape)}, got {d.dtype} {list(d.shape)}")
+        grads += [d.data_ptr(), _matrix(d, f"{name}: {what}")[2]]
+    if denom is not None and not denom > 0:
+        raise ValueError(f"{name}: denom must be positive, got {denom}")
+    args = L.LINEAR_LOSS_ARGS.pack(hidden.data_ptr(), ld_hidden, weight.data_ptr(), ld_weight, tokens.data_ptr(), kept, *grads,
+                                   _vector(logp, f"{name}: logp", rows), _vector(entropy, f"{name}: entropy", rows), _vector(stats, f"{name}: stats", 4),
+                                   rows, vocab, dim, temperature, 0.0 if denom is None else denom, elem, token_type)
+    buf = _scratch(ws, hidden.device, L.load().ppo_linear_loss_workspace_bytes(args, 1))
+    L.call("ppo_linear_cross_entropy", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
+    _written(d_hidden, d_weight, stats, logp, entropy)
