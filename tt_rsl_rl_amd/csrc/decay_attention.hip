@@ -35,13 +35,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kInfoThreads = 256;
 constexpr int kScanThreads = 256;
 
-// The matrix cores' operand types.  A step sums over K elements: QUADS groups of four for each of a wave's four lane groups g, group h
-// being elements 16 h + 4 g + 0..3 of the step.
+// The matrix cores' operand types.  A step sums over K elements, of which a wave's lane group g = lane / 16 holds K / 4 neighbours: one 16-byte
+// piece.  An accumulator tile's rows 4 g + 0..3 lie in group g; row_of() says which element a tile's row is, so that QUADS tiles together hold in each
+// group the neighbours that the next product's step wants there.
 template <class M>
 struct Math;
 template <>
@@ -52,6 +51,7 @@ struct Math<__bf16> {
   static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ int row_of(int tile, int row) { return 32 * (tile / 2) + 8 * (row / 4) + 4 * (tile % 2) + row % 4; }
 };
 template <>
 struct Math<float> {
@@ -63,31 +63,56 @@ struct Math<float> {
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
     return c;
   }
+  static __device__ __forceinline__ int row_of(int tile, int row) { return 16 * tile + row; }
 };
 
-// An operand from LDS: row[base + 16 h + 4 g ..], g the lane's group.
-template <class M>
-__device__ __forceinline__ typename Math<M>::Frag load_frag(const M* row, int base, int g) {
-  typedef typename Math<M>::Quad Quad;
-  if constexpr (Math<M>::QUADS == 1) {
-    return *reinterpret_cast<const Quad*>(row + base + 4 * g);
-  } else {
-    const Quad u = *reinterpret_cast<const Quad*>(row + base + 4 * g), v = *reinterpret_cast<const Quad*>(row + base + 16 + 4 * g);
-    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+// Arrays in LDS: rows of 16-byte pieces, whose places in their row are exchanged by the row's number, so that what a wave reads or writes
+// together meets all banks (a read: 16 rows of a tile, four neighbouring pieces; a write: one row, or one piece of rows 8, 4 or 1 apart).
+// turn() is made of exclusive ors, so a row that is a lane's part and a constant, without a bit in common, is turned by the one's turn xor the other's:
+// from() goes from the lane's place to that of a constant further on with one operation.
+template <class M, int ROW_, bool TURNED>
+struct Places {
+  static constexpr int ROW = ROW_, PIECE = 16 / static_cast<int>(sizeof(M)), PIECES = ROW / PIECE;
+  static constexpr __device__ __forceinline__ int turn(int row) {
+    return TURNED ? (row >> 1 ^ row >> 4) & 7 : PIECES == 8 ? (row >> 1 ^ (row >> 3 & 2)) & 7 : (row ^ row >> 2) & 15;
   }
+  static __device__ __forceinline__ int at(int row, int piece) { return row * ROW + (piece ^ turn(row)) * PIECE; }
+  static __device__ __forceinline__ int from(int base, int row, int piece) { return (base ^ (turn(row) ^ piece) * PIECE) + row * ROW; }
+};
+template <class M, int ROW>  // tokens' rows of ROW elements
+using Natural = Places<M, ROW, false>;
+template <class M>  // elements' rows of a chunk's tokens: 128 bytes
+using Turned = Places<M, Math<M>::CHUNK, true>;
+
+template <class M>
+__device__ __forceinline__ typename Math<M>::Frag load_frag(const M* at) {
+  return *reinterpret_cast<const typename Math<M>::Frag*>(at);
 }
 
-// Values of a step as NP operands whose sum they are, to 8 bits each (bf16), or as they are (fp32).
+// Values of a step as NP operands whose sum they are, to 8 bits each (bf16; converted in pairs), or as they are (fp32).
 template <class M, int NP>
 __device__ __forceinline__ void split(float (&x)[4 * Math<M>::QUADS], typename Math<M>::Frag (&out)[NP]) {
+  if constexpr (sizeof(M) == 4) {
 #pragma unroll
-  for (int p = 0; p < NP; ++p)
+    for (int i = 0; i < 4; ++i) out[0][i] = x[i];
+  } else {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < 4 * Math<M>::QUADS; ++i) {
-      const M part = static_cast<M>(x[i]);
-      out[p][i] = part;
-      if (p + 1 < NP) x[i] -= static_cast<float>(part);
+    for (int p = 0; p < NP; ++p) {
+      Words w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const Pair pair{static_cast<__bf16>(x[2 * i]), static_cast<__bf16>(x[2 * i + 1])};
+        w[i] = __builtin_bit_cast(uint32_t, pair);
+        if (p + 1 < NP) {
+          x[2 * i] -= __builtin_bit_cast(float, w[i] << 16);
+          x[2 * i + 1] -= __builtin_bit_cast(float, w[i] & 0xffff0000u);
+        }
+      }
+      out[p] = __builtin_bit_cast(typename Math<M>::Frag, w);
     }
+  }
 }
 
 struct Span {
@@ -106,6 +131,8 @@ struct MixArgs {
   int32_t heads, ga, gb;  // heads of b, c and S times gb; of a per head
   int32_t db, dc;
   int32_t reverse, w, cut;  // cut: chunks end with their sequence
+  int32_t lost;             // states come in, which need not be finite
+  int32_t whole;            // rows are whole 16-byte pieces, not far apart
   float x, y, z;
 };
 
@@ -176,355 +203,482 @@ __global__ __launch_bounds__(kScanThreads) void decay_scan_kernel(const MixArgs 
   }
 }
 
-// Four tokens' pieces of 16 bytes of one view, as they lie in memory; zeros past the view's rows and columns.
+// Whether any of the values is not finite: 0 x is 0 but for those.
 template <class T>
-struct Unit {
-  RawPiece r[4];
-};
-
-template <class T>
-__device__ __forceinline__ RawPiece load_columns(const T* row, int col, int dim) {
-  constexpr int V = kVec<T>;
-  if (col + V <= dim) return load_raw(row + col);
-  RawPiece r{};
-  for (int e = 0; e < V; ++e)
-    if (col + e < dim) {
-      if constexpr (sizeof(T) == 4) r.w[e] = __builtin_bit_cast(uint32_t, row[col + e]);
-      else r.w[e / 2] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, row[col + e])) << (e % 2 * 16);
-    }
-  return r;
-}
-
-// Whether any of the piece's values is not finite.
-template <class T>
-__device__ __forceinline__ uint32_t not_finite(const RawPiece& r) {
-  uint32_t any = 0;
+__device__ __forceinline__ float sum_of_nothing(const RawPiece& r, float sum) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) any |= ((r.w[i] & 0x7fffffffu) + 0x00800000u) & 0x80000000u;
-    else if constexpr (__is_same(T, __bf16)) any |= ((r.w[i] & 0x7fff7fffu) + 0x00800080u) & 0x80008000u;
-    else any |= ((r.w[i] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+    if constexpr (sizeof(T) == 4) {
+      sum = fmaf(__builtin_bit_cast(float, r.w[i]), 0.0f, sum);
+    } else if constexpr (__is_same(T, __bf16)) {
+      typedef __bf16 Two __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, r.w[i]), Two{}, sum, false);
+    } else {
+      typedef _Float16 Two __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(Two, r.w[i]), Two{}, sum, false);
+    }
   }
-  return any;
+  return sum;
+}
+template <class T>
+__device__ __forceinline__ bool not_finite(const RawPiece& r) { return !(sum_of_nothing<T>(r, 0.0f) == 0.0f); }
+template <class T>
+__device__ __forceinline__ bool not_finite(const RawPiece (&r)[4]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sum = sum_of_nothing<T>(r[k], sum);
+  return !(sum == 0.0f);
 }
 
-template <class M>
-constexpr int natural_stride(int dim) { return dim + (sizeof(M) == 2 ? 8 : 4); }
-template <class M>
-constexpr int turned_stride() { return Math<M>::CHUNK + 4; }
+// Four tokens' pieces of 16 bytes, columns d .., into rows of tokens and into rows of elements.
+template <class T, class M, int ROW>
+__device__ __forceinline__ void put_rows(const RawPiece (&r)[4], M* rows, int j4, int d, bool there) {
+  typedef Natural<M, ROW> N;
+  constexpr int V = kVec<T>;
+  const int base = N::at(j4, d / N::PIECE);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == sizeof(M)) {
+      RawPiece x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.w[i] = there ? r[k].w[i] : 0;
+      *reinterpret_cast<RawPiece*>(rows + N::from(base, k, 0)) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        f32x4 x;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) x[f] = there ? element<T>(r[k], e + f) : 0.0f;
+        *reinterpret_cast<f32x4*>(rows + N::from(base, k, e / 4)) = x;
+      }
+    }
+  }
+}
 
-// T: the views' type, M: the products', DBT: tiles of 16 of b's dims, NT: tiles of 16 of c's dims a wave owns, STATE_ONLY: the first pass over
-// segments, which makes their own states.
+template <class T, class M>
+__device__ __forceinline__ void put_turned(const RawPiece (&r)[4], M* turned, int j4, int d) {
+  typedef Turned<M> N;
+  constexpr int V = kVec<T>;
+  const int base = N::at(d, j4 / N::PIECE) + j4 % N::PIECE;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    typename Math<M>::Quad x;
+    if constexpr (sizeof(M) == 2) {
+      typedef uint32_t Two __attribute__((ext_vector_type(2)));
+      const uint32_t pick = e % 2 != 0 ? 0x07060302u : 0x05040100u;  // the high, the low halves
+      x = __builtin_bit_cast(typename Math<M>::Quad, Two{__builtin_amdgcn_perm(r[1].w[e / 2], r[0].w[e / 2], pick),
+                                                         __builtin_amdgcn_perm(r[3].w[e / 2], r[2].w[e / 2], pick)});
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = static_cast<M>(element<T>(r[k], e));
+    }
+    *reinterpret_cast<typename Math<M>::Quad*>(turned + N::from(base, e, 0)) = x;
+  }
+}
+
+// T: the views' type, M: the products', DBT: tiles of 16 of b's elements, NT: tiles of 16 of c's elements to each of four waves, STATE_ONLY:
+// the first pass over segments, which makes their own states.
+//
+// A block goes through items: a piece of up to CHUNK tokens (times the heads that share it).  An item's rows are loaded into registers while
+// the item before is computed.
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+
+// All waves' LDS accesses are done.  (__syncthreads() would also wait for the loads and stores on their way to and from memory, which no other wave
+// of the block looks at.)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 template <class T, class M, int DBT, int NT, bool STATE_ONLY>
-__global__ __launch_bounds__(kThreads, sizeof(M) == 2 ? 2 : 1) void decay_mix_kernel(const MixArgs q) {
+__global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q) {
   typedef Math<M> X;
   typedef typename X::Frag Frag;
   constexpr int C = X::CHUNK, K = X::K, Q = X::QUADS, DB = DBT * 16, DC = kWaves * NT * 16, IT = C / 16, V = kVec<T>;
-  constexpr int SN = natural_stride<M>(DB), ST = turned_stride<M>();
-  __shared__ __align__(16) M a_rows[STATE_ONLY ? 8 : C * SN];
-  __shared__ __align__(16) M b_rows[STATE_ONLY ? 8 : C * SN];
-  __shared__ __align__(16) M b_turned[DB * ST];
-  __shared__ __align__(16) M c_turned[DC * ST];
+  constexpr int PARTS = X::PARTS2;
+  typedef Natural<M, DB> Rows_;
+  typedef Turned<M> Cols_;
+  constexpr int B_ROWS = C * DB > PARTS * C * C ? C * DB : PARTS * C * C;
+  __shared__ __align__(16) M a_rows[STATE_ONLY ? 8 : C * DB];
+  __shared__ __align__(16) M b_rows[STATE_ONLY ? 8 : B_ROWS];  // then the chunk's matrix, [part][i][j]
+  __shared__ __align__(16) M b_turned[DB * C];
+  __shared__ __align__(16) M c_turned[DC * C];
+  __shared__ __align__(16) float weights[C], sights[C];  // of each token in the next state; of the state before in each output
   __shared__ float fades[C + 1];
-  __shared__ int first[C + 1], last[C + 1], seqs[C];
-  __shared__ uint32_t bad_any;
-  __shared__ uint32_t bad[(C + 31) / 32];
+  __shared__ int first[2][C], last[2][C], seqs[2][C];  // of the chunk's tokens and the next one's
+  __shared__ uint32_t bad_any, bad[(C + 31) / 32];
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = lane % 16, g = lane / 16;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int head = blockIdx.y, seg = blockIdx.x;
   const int dc0 = wave * NT * 16;
   const bool works = dc0 < q.dc;
   const int seg_begin = seg * q.segment, seg_end = min(seg_begin + q.segment, q.tokens);
-  const double ld = static_cast<double>(q.log_decay[head]);
-  if (threadIdx.x <= C) fades[threadIdx.x] = threadIdx.x == 0 ? 1.0f : static_cast<float>(exp(ld * threadIdx.x));
-  if (threadIdx.x == 0) bad_any = 0;
 
-  f32x4 S[DBT][NT];
+  f32x4 S[DBT][NT];  // rows row_of(mb, 4 g + 0..3), column column_of(nt)
+  // Where a lane owns outputs' elements: with two tiles 8 neighbours, so that they leave in 16 bytes.
+  auto column_of = [](int nt, int col) { return NT == 2 ? 8 * (col / 4) + 4 * nt + col % 4 : col; };
   auto each_state = [&](auto&& f) {
+    int group = 4 * (lane / 16), col = lane % 16;
+    forget(group), forget(col);  // (or else every element's address is kept from one chunk to the next, in 128 registers)
 #pragma unroll
     for (int mb = 0; mb < DBT; ++mb)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[mb][nt][r] = f(S[mb][nt][r], 16 * mb + 4 * g + r, dc0 + 16 * nt + col);
+        for (int r = 0; r < 4; ++r) S[mb][nt][r] = f(S[mb][nt][r], X::row_of(mb, group + r), dc0 + column_of(nt, col));
   };
-  each_state([](float, int, int) { return 0.0f; });
-  bool fresh = true;  // S is zeros
+  auto token_at_place = [&](int u) { return q.reverse ? q.tokens - 1 - u : u; };
+  auto put_span = [&](int buffer, int u, const Span& s) {  // positions in the order that is walked
+    const int i = threadIdx.x;
+    first[buffer][i] = q.reverse ? q.tokens - s.end : s.start;
+    last[buffer][i] = q.reverse ? q.tokens - s.start : s.end;
+    seqs[buffer][i] = s.seq;
+  };
 
-  for (int c0 = seg_begin; c0 < seg_end; c0 += C) {
-    const int cn = min(C, seg_end - c0);
-    __syncthreads();
-    if (threadIdx.x < static_cast<uint32_t>(cn)) {
-      const int u = c0 + threadIdx.x;
-      const Span s = span_of(q, q.reverse ? q.tokens - 1 - u : u);
-      first[threadIdx.x] = q.reverse ? q.tokens - s.end : s.start;
-      last[threadIdx.x] = q.reverse ? q.tokens - s.start : s.end;
-      seqs[threadIdx.x] = s.seq;
-    }
-    __syncthreads();
-    if (!STATE_ONLY && c0 == seg_begin && first[0] < c0) {  // goes on from the segment before
-      const float* from = q.carry + (static_cast<int64_t>(seg - 1) * q.heads + head) * q.db * q.dc;
-      each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[static_cast<int64_t>(i) * q.dc + j] : 0.0f; });
-      fresh = false;
-    }
-    for (int p = 0; p < cn;) {
-      const int begin = c0 + p, seq = __builtin_amdgcn_readfirstlane(seqs[p]), first0 = __builtin_amdgcn_readfirstlane(first[p]);
-      const int n = __builtin_amdgcn_readfirstlane(q.cut ? min(cn - p, last[p] - begin) : cn - p);
-      if (first0 == begin) {  // a sequence begins
-        fresh = q.s_in == nullptr || seq < 0;
-        const float* from = q.s_in + (static_cast<int64_t>(seq) * q.heads + head) * q.state_size;
-        each_state([&](float, int i, int j) { return !fresh && works && i < q.db && j < q.dc ? from[i * q.si + j * q.sj] : 0.0f; });
+  // An item's rows: units of four tokens by 16 bytes, first b's, then c's, then a's; a wave's 64 are of one view.  What is loaded past the
+  // last token is that token again: it has no weight anywhere.
+  constexpr int UB = DB / V * (C / 4), UC = DC / V * (C / 4), UA = STATE_ONLY ? 0 : UB, ROUNDS = (UB + UC + UA + kThreads - 1) / kThreads;
+  static_assert(UB % kWave == 0 && UC % kWave == 0);
+  RawPiece r[ROUNDS][4];
+  auto kind_of = [&](int round) {  // 0: b, 1: c, 2: a, 3: none
+    const int i = (round * kWaves + wave) * kWave;
+    return i < UB ? 0 : i < UB + UC ? 1 : i < UB + UC + UA ? 2 : 3;
+  };
+  auto place_of = [&](int thread, int round, int kind, int& j4, int& d) {
+    const int i = thread + round * kThreads - (kind == 0 ? 0 : kind == 1 ? UB : UB + UC);
+    const int pieces = (kind == 1 ? DC : DB) / V;
+    j4 = i / pieces % (C / 4) * 4;
+    d = i % pieces * V;
+  };
+  auto load_rows = [&](int begin, int n, int ab) {
+    const int ha = q.ga > 1 ? head * q.ga + ab : head, hb = q.gb > 1 ? head * q.gb + ab : head;
+    const int64_t lowest = q.reverse ? q.tokens - begin - n : begin;
+    int thread = threadIdx.x;
+    forget(thread);  // (addresses again)
+#pragma unroll
+    for (int round = 0; round < ROUNDS; ++round) {
+      const int kind = kind_of(round);
+      int j4, d;
+      place_of(thread, round, kind, j4, d);
+      const ppo_head_view& v = kind == 0 ? q.b : kind == 1 || STATE_ONLY ? q.c : q.a;
+      const char* from = reinterpret_cast<const char*>(static_cast<const T*>(v.data) + (kind >= 2 ? ha : hb) * v.head_stride + lowest * v.token_stride);
+      const uint32_t step = static_cast<uint32_t>(v.token_stride) * sizeof(T);
+      const uint32_t column = min(d, (kind == 1 || (STATE_ONLY && kind == 3) ? q.dc : q.db) - V) * static_cast<int>(sizeof(T));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = min(j4 + k, n - 1);
+        r[round][k] = load_raw(reinterpret_cast<const T*>(from + (__umul24(q.reverse ? n - 1 - j : j, step) + column)));
       }
-      const int first_last = __builtin_amdgcn_readfirstlane(first[p + n - 1]);  // where the sequence of the last token begins
-      f32x4 acc[IT][NT];
-      for (int ab = 0; ab < q.ga * q.gb; ++ab) {
-        const int ha = q.ga > 1 ? head * q.ga + ab : head, hb = q.gb > 1 ? head * q.gb + ab : head;
-        const bool new_b = q.gb > 1 || ab == 0, new_a = !STATE_ONLY && (q.ga > 1 || ab == 0);
-        __syncthreads();
-        // rows into LDS: units of four tokens by 16 bytes of a head
-        auto stage = [&](const ppo_head_view& v, int h, int dim, int padded, M* rows, M* turned, bool check) {
-          const int pieces = padded / V;
-          for (int i = threadIdx.x; i < pieces * (C / 4); i += kThreads) {
-            const int j4 = i / pieces * 4, d = i % pieces * V;
-            RawPiece r[4];
-            uint32_t any[4];
+    }
+  };
+
+  if (threadIdx.x <= C) fades[threadIdx.x] = threadIdx.x == 0 ? 1.0f : static_cast<float>(exp(static_cast<double>(q.log_decay[head]) * threadIdx.x));
+  if (threadIdx.x == 0) bad_any = 0;
+  if (threadIdx.x < (C + 31) / 32) bad[threadIdx.x] = 0;
+  if (seg_begin + static_cast<int>(threadIdx.x) < min(seg_begin + C, seg_end))
+    put_span(0, seg_begin + threadIdx.x, span_of(q, token_at_place(seg_begin + threadIdx.x)));
+  lds_barrier();
+  bool fresh = true;  // S is zeros
+  bool lost = q.lost != 0;  // S may be not finite
+  each_state([](float, int, int) { return 0.0f; });
+  if (!STATE_ONLY && first[0][0] < seg_begin) {  // goes on from the segment before
+    const float* from = q.carry + (static_cast<int64_t>(seg - 1) * q.heads + head) * q.db * q.dc;
+    each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[static_cast<int64_t>(i) * q.dc + j] : 0.0f; });
+    fresh = false;
+  }
+
+  int c0 = seg_begin, p = 0, ab = 0, buffer = 0;  // the item: chunk, place in it, head
+  auto length = [&](int b, int at, int chunk) {
+    const int cn = min(C, seg_end - chunk);
+    return __builtin_amdgcn_readfirstlane(q.cut ? min(cn - at, last[b][at] - (chunk + at)) : cn - at);
+  };
+  int n = length(0, 0, c0);
+  if (q.whole) load_rows(c0, n, 0);
+  f32x4 acc[IT][NT];
+  const int abs = q.ga * q.gb;
+  while (true) {
+    const int begin = c0 + p, seq = __builtin_amdgcn_readfirstlane(seqs[buffer][p]), first0 = __builtin_amdgcn_readfirstlane(first[buffer][p]);
+    const int first_last = __builtin_amdgcn_readfirstlane(first[buffer][p + n - 1]);  // where the sequence of the last token begins
+    const int* const from_first = first[buffer] + p;
+    const uint64_t valid = __ballot(lane < n && seqs[buffer][p + min(lane, n - 1)] >= 0);  // tokens of sequences
+    const bool new_b = q.gb > 1 || ab == 0, new_a = !STATE_ONLY && (q.ga > 1 || ab == 0);
+    const bool ahead = ab == 0 && p == 0 && c0 + C + static_cast<int>(threadIdx.x) < min(c0 + 2 * C, seg_end);
+    Span next_span{};
+    if (ahead) next_span = span_of(q, token_at_place(c0 + C + threadIdx.x));
+    if (ab == 0 && first0 == begin) {  // a sequence begins
+      fresh = q.s_in == nullptr || seq < 0;
+      const float* from = q.s_in + (static_cast<int64_t>(seq) * q.heads + head) * q.state_size;
+      if (fresh) each_state([](float, int, int) { return 0.0f; });
+      else each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[i * q.si + j * q.sj] : 0.0f; });
+    }
+    int thread = threadIdx.x;
+    forget(thread);
+    const int col = thread % 16, g = thread % kWave / 16;
+    const int a_at = Rows_::at(col, g), b_at = Rows_::at(X::row_of(0, col), g), m_at = Cols_::at(col, g), bt_at = Cols_::at(X::row_of(0, col), g);
+    const int ct_at = Cols_::at(dc0 + column_of(0, col), g);  // operands' places, to go on from
+    // ---- rows into LDS ----
+    lds_barrier();  // the last products have read what is there
+    if (q.whole) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int j = j4 + k;
-              r[k] = RawPiece{};
-              if (j < n && seqs[p + j] >= 0) {
-                const int u = begin + j, t = q.reverse ? q.tokens - 1 - u : u;
-                r[k] = load_columns(static_cast<const T*>(v.data) + t * v.token_stride + h * v.head_stride, d, dim);
-              }
-            }
-            if (check) {
+      for (int round = 0; round < ROUNDS; ++round) {
+        const int kind = kind_of(round);
+        int j4, d;
+        place_of(thread, round, kind, j4, d);
+        if (kind < 2 && not_finite<T>(r[round])) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) any[k] = not_finite<T>(r[k]);
-              if ((any[0] | any[1] | any[2] | any[3]) != 0) {
-                for (int k = 0; k < 4; ++k)
-                  if (any[k] != 0) atomicOr(&bad[(j4 + k) / 32], 1u << ((j4 + k) % 32));
-                bad_any = 1;
-              }
-            }
-            if (rows != nullptr)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                typedef M Row __attribute__((ext_vector_type(V)));
-                Row x;
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[e] = static_cast<M>(element<T>(r[k], e));
-                typedef M Part __attribute__((ext_vector_type(16 / sizeof(M))));
-                constexpr int PV = 16 / static_cast<int>(sizeof(M));
-#pragma unroll
-                for (int e = 0; e < V; e += PV) {
-                  Part y;
-#pragma unroll
-                  for (int f = 0; f < PV; ++f) y[f] = x[e + f];
-                  *reinterpret_cast<Part*>(rows + (j4 + k) * SN + d + e) = y;
-                }
-              }
-            if (turned != nullptr)
-#pragma unroll
-              for (int e = 0; e < V; ++e) {
-                typename X::Quad x;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = static_cast<M>(element<T>(r[k], e));
-                *reinterpret_cast<typename X::Quad*>(turned + (d + e) * ST + j4) = x;
-              }
+          for (int k = 0; k < 4; ++k)
+            if (not_finite<T>(r[round][k])) atomicOr(&bad[(j4 + k) / 32], 1u << ((j4 + k) % 32));
+          bad_any = 1;
+        }
+        if (!STATE_ONLY && kind == 0) put_rows<T, M, DB>(r[round], b_rows, j4, d, true);  // (b's rows have made room for the last matrix)
+        if (kind == 0 && new_b) put_turned<T, M>(r[round], b_turned, j4, d);
+        if (kind == 1 && new_b) put_turned<T, M>(r[round], c_turned, j4, d);
+        // (past b's elements a is zeros, and what b and S hold there is not seen)
+        if (!STATE_ONLY && kind == 2 && new_a) put_rows<T, M, DB>(r[round], a_rows, j4, d, d < q.db);
+      }
+    } else {  // heads of odd widths: element by element
+      auto elements = [&](const ppo_head_view& v, int h, int dim, int padded, M* rows, M* turned) {
+#pragma unroll 1
+        for (int i = thread; i < C * padded; i += kThreads) {
+          const int j = i / padded, d = i % padded;
+          T x = static_cast<T>(0.0f);
+          if (d < dim && (valid >> j & 1) != 0)
+            x = static_cast<const T*>(v.data)[h * v.head_stride + token_at_place(begin + j) * v.token_stride + d];
+          if (turned != nullptr && !(fabsf(static_cast<float>(x)) < INFINITY)) {
+            atomicOr(&bad[j / 32], 1u << (j % 32));
+            bad_any = 1;
           }
-        };
-        if (new_b && threadIdx.x < (C + 31) / 32) bad[threadIdx.x] = 0;
-        if (new_b) __syncthreads();
-        if (new_a) stage(q.a, ha, q.db, DB, a_rows, nullptr, false);
-        if (new_b) {
-          stage(q.b, hb, q.db, DB, STATE_ONLY ? nullptr : b_rows, b_turned, true);
-          stage(q.c, hb, q.dc, DC, nullptr, c_turned, true);
+          if (rows != nullptr) rows[Rows_::at(j, d / Rows_::PIECE) + d % Rows_::PIECE] = static_cast<M>(x);
+          if (turned != nullptr) turned[Cols_::at(d, j / Cols_::PIECE) + j % Cols_::PIECE] = static_cast<M>(x);
         }
-        __syncthreads();
-        const bool poisoned = __builtin_amdgcn_readfirstlane(bad_any) != 0;
-        if (poisoned) {  // zeros where a token is not finite; rare, so one token after another
-          for (int j = 0; j < n; ++j)
-            if (bad[j / 32] >> (j % 32) & 1) {
-              for (int d = threadIdx.x; d < DB; d += kThreads) {
-                if (!STATE_ONLY) b_rows[j * SN + d] = static_cast<M>(0.0f);
-                b_turned[d * ST + j] = static_cast<M>(0.0f);
-              }
-              for (int d = threadIdx.x; d < DC; d += kThreads) c_turned[d * ST + j] = static_cast<M>(0.0f);
-            }
-          __syncthreads();
+      };
+      const int ha = q.ga > 1 ? head * q.ga + ab : head, hb = q.gb > 1 ? head * q.gb + ab : head;
+      if (new_a) elements(q.a, ha, q.db, DB, a_rows, nullptr);
+      elements(q.b, hb, q.db, DB, STATE_ONLY ? nullptr : b_rows, b_turned);
+      if (new_b) elements(q.c, hb, q.dc, DC, nullptr, c_turned);
+    }
+    if (thread < C) {
+      const int i = min(thread, n - 1);
+      weights[thread] = thread < n && from_first[i] == first_last ? q.z * fades[n - q.w - i] : 0.0f;
+      sights[thread] = thread < n && from_first[i] == first0 ? q.y * fades[i + q.w] : 0.0f;
+    }
+    if (ahead) put_span(buffer ^ 1, c0 + C + threadIdx.x, next_span);
+    lds_barrier();
+    const bool poisoned = __builtin_amdgcn_readfirstlane(bad_any) != 0;
+    if (poisoned) {  // zeros where a token is not finite
+      for (int j = 0; j < n; ++j)
+        if (bad[j / 32] >> (j % 32) & 1) {
+          for (int d = thread; d < DB; d += kThreads) {
+            if (!STATE_ONLY) b_rows[Rows_::at(j, d / Rows_::PIECE) + d % Rows_::PIECE] = static_cast<M>(0.0f);
+            b_turned[Cols_::at(d, j / Cols_::PIECE) + j % Cols_::PIECE] = static_cast<M>(0.0f);
+          }
+          for (int d = thread; d < DC; d += kThreads) c_turned[Cols_::at(d, j / Cols_::PIECE) + j % Cols_::PIECE] = static_cast<M>(0.0f);
         }
-        // ---- what lies before the piece ----
-        if (!STATE_ONLY && (ab == 0 || q.ga > 1)) {
+      lds_barrier();
+    }
+    // ---- the next item, and its rows on their way ----
+    int next_ab = ab + 1, next_p = p, next_c0 = c0, next_buffer = buffer, next_n = n;
+    if (next_ab == abs) {
+      next_ab = 0, next_p = p + n;
+      if (next_p >= min(C, seg_end - c0)) next_p = 0, next_c0 = c0 + C, next_buffer = buffer ^ 1;
+      if (next_c0 < seg_end) next_n = length(next_buffer, next_p, next_c0);
+    }
+    const bool done = next_c0 >= seg_end;
+    if (q.whole) load_rows(done ? begin : next_c0 + next_p, next_n, done ? ab : next_ab);  // (once more at the end: loads without a branch stay in their registers)
+
+    if constexpr (!STATE_ONLY) {
+      // ---- the chunk's matrix, its steps of tiles with i >= j shared among the waves ----
+      {
+        constexpr int EACH = kWaves / IT, STEPS = (C / K + EACH - 1) / EACH;
+        const int it = wave / EACH, step0 = wave % EACH, i = 16 * it + col;
+        Frag matrix[STEPS][PARTS];
+        Frag a[DB / K];
 #pragma unroll
-          for (int it = 0; it < IT; ++it)
+        for (int ks = 0; ks < DB / K; ++ks) a[ks] = load_frag<M>(a_rows + Rows_::from(a_at, 16 * it, 4 * ks));
+        const int lowest = i < n ? from_first[min(i, n - 1)] - begin : C;  // the first of the piece's tokens that i sees
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[it][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          if (works && !fresh) {
+        for (int step = 0; step < STEPS; ++step) {
+          const int kj = step0 + step * EACH;
+          if (kj * Q > it) continue;
+          float v[4 * Q];
 #pragma unroll
-            for (int ks = 0; ks < DB / K; ++ks) {
-              Frag s[NT][X::PARTS2];
+          for (int h = 0; h < Q; ++h) {
+            const int jt = kj * Q + h;
+            f32x4 m{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float v[4 * Q];
+            for (int ks = 0; ks < DB / K; ++ks) m = X::mma(load_frag<M>(b_rows + Rows_::from(b_at, X::row_of(jt, 0), 4 * ks)), a[ks], m);
+            const int j0 = X::row_of(jt, 4 * g);
 #pragma unroll
-                for (int i = 0; i < 4 * Q; ++i) v[i] = S[ks * Q + i / 4][nt][i % 4];
-                split<M, X::PARTS2>(v, s[nt]);
-              }
-#pragma unroll
-              for (int it = 0; it < IT; ++it) {
-                const Frag a = load_frag<M>(a_rows + (16 * it + col) * SN, K * ks, g);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int k = 0; k < X::PARTS2; ++k) acc[it][nt] = X::mma(s[nt][k], a, acc[it][nt]);
-              }
-            }
-#pragma unroll
-            for (int it = 0; it < IT; ++it) {
-              const int i = 16 * it + col;
-              const bool sees = i < n && first[p + min(i, n - 1)] == first0;
-              const float f = q.y * fades[min(i + q.w, C)];
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[it][nt][r] = sees ? acc[it][nt][r] * f : 0.0f;
+            for (int r4 = 0; r4 < 4; ++r4) {  // (no branches: a wait for each fade would be one each)
+              const int j = j0 + r4;
+              const float f = q.x * fades[max(i - j, 0)];
+              v[4 * h + r4] = (j <= i) & (j >= lowest) ? m[r4] * f : 0.0f;
             }
           }
+          split<M, PARTS>(v, matrix[step]);
         }
-        // c's columns that the wave owns, as operands
-        Frag c[NT][C / K];
-        if (works)
+        lds_barrier();  // b's rows have been read
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int step = 0; step < STEPS; ++step) {
+          const int kj = step0 + step * EACH;
+          if (kj * Q > it) continue;
 #pragma unroll
-            for (int ks = 0; ks < C / K; ++ks) c[nt][ks] = load_frag<M>(c_turned + (dc0 + 16 * nt + col) * ST, K * ks, g);
-        // ---- the piece's tokens among each other ----
-        if (!STATE_ONLY && works) {
-          const bool one = first_last == first0 && seq >= 0;  // one sequence
+          for (int k = 0; k < PARTS; ++k) *reinterpret_cast<Frag*>(b_rows + k * C * C + Cols_::from(m_at, 16 * it, 4 * kj)) = matrix[step][k];
+        }
+      }
+      // ---- what lies before the piece ----
+      if (ab == 0 || q.ga > 1) {
 #pragma unroll
-          for (int it = 0; it < IT; ++it) {
-            if (16 * it >= n) break;
-            Frag a[DB / K];
+        for (int i = 0; i < IT; ++i)
 #pragma unroll
-            for (int ks = 0; ks < DB / K; ++ks) a[ks] = load_frag<M>(a_rows + (16 * it + col) * SN, K * ks, g);
-            const int i = 16 * it + col, first_i = first[p + min(i, n - 1)];
+          for (int nt = 0; nt < NT; ++nt) acc[i][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (works && !fresh) {
 #pragma unroll
-            for (int kj = 0; kj < C / K; ++kj) {
-              if (kj * Q > it) continue;
+          for (int ks = 0; ks < DB / K; ++ks) {
+            Frag s[NT][PARTS];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
               float v[4 * Q];
 #pragma unroll
-              for (int h = 0; h < Q; ++h) {
-                const int jt = kj * Q + h;
-                f32x4 m{0.0f, 0.0f, 0.0f, 0.0f};
-                if (jt <= it) {
-#pragma unroll
-                  for (int ks = 0; ks < DB / K; ++ks) m = X::mma(load_frag<M>(b_rows + (16 * jt + col) * SN, K * ks, g), a[ks], m);
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * jt + 4 * g + r;
-                    const bool sees = j <= i && i < n && (one || first[p + min(j, n - 1)] == first_i);
-                    m[r] = sees ? m[r] * (q.x * fades[max(i - j, 0)]) : 0.0f;
-                  }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[4 * h + r] = m[r];
-              }
-              Frag part[X::PARTS2];
-              split<M, X::PARTS2>(v, part);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < X::PARTS2; ++k) acc[it][nt] = X::mma(c[nt][kj], part[k], acc[it][nt]);
+              for (int i = 0; i < 4 * Q; ++i) v[i] = S[ks * Q + i / 4][nt][i % 4];
+              split<M, PARTS>(v, s[nt]);
             }
-            if (poisoned)
-              for (int j = 0; j <= min(i, n - 1); ++j)
-                if ((bad[j / 32] >> (j % 32) & 1) && first[p + j] == first_i)
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
+            for (int i = 0; i < IT; ++i) {
+              const Frag a = load_frag<M>(a_rows + Rows_::from(a_at, 16 * i, 4 * ks));
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[it][nt][r] = __builtin_nanf("");
-          }
-        }
-        // ---- the outputs ----
-        if (!STATE_ONLY && works && (q.ga > 1 || ab == q.gb - 1)) {
+              for (int k = 0; k < PARTS; ++k)
 #pragma unroll
-          for (int it = 0; it < IT; ++it) {
-            const int i = 16 * it + col;
-            if (i < n && seqs[p + min(i, n - 1)] >= 0) {
-              const int u = begin + i, t = q.reverse ? q.tokens - 1 - u : u;
-              T* row = static_cast<T*>(q.out.data) + t * q.out.token_stride + ha * q.out.head_stride;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const int d = dc0 + 16 * nt + 4 * g;
-                if (d + 4 <= q.dc) {
-                  typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-                  Four o;
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[it][nt][r]);
-                  *reinterpret_cast<Four*>(row + d) = o;
-                } else {
-#pragma unroll
-                  for (int r = 0; r < 4; ++r)
-                    if (d + r < q.dc) row[d + r] = static_cast<T>(acc[it][nt][r]);
-                }
-              }
+                for (int nt = 0; nt < NT; ++nt) acc[i][nt] = X::mma(s[nt][k], a, acc[i][nt]);
             }
           }
-        }
-        // ---- the state ----
-        if (ab >= q.ga - 1) {
-          const bool kept = first_last == first0;
-          if (ab == q.ga - 1) {
-            const float f = fades[n];
-            each_state([&](float s, int, int) { return kept ? s * f : 0.0f; });
-          }
-          if (works) {
 #pragma unroll
-            for (int kj = 0; kj < C / K; ++kj) {
-              float w[4 * Q];
+          for (int i = 0; i < IT; ++i) {
+            const float f = sights[16 * i + col];
 #pragma unroll
-              for (int i = 0; i < 4 * Q; ++i) {
-                const int j = K * kj + 16 * (i / 4) + 4 * g + i % 4;
-                w[i] = j < n && first[p + min(j, n - 1)] == first_last ? q.z * fades[max(n - q.w - j, 0)] : 0.0f;
-              }
-              Frag weighted[NT][X::PARTS3];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float v[4 * Q];
-#pragma unroll
-                for (int i = 0; i < 4 * Q; ++i) v[i] = w[i] * static_cast<float>(c[nt][kj][i]);
-                split<M, X::PARTS3>(v, weighted[nt]);
-              }
-#pragma unroll
-              for (int mb = 0; mb < DBT; ++mb) {
-                const Frag b = load_frag<M>(b_turned + (16 * mb + col) * ST, K * kj, g);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int k = 0; k < X::PARTS3; ++k) S[mb][nt] = X::mma(b, weighted[nt][k], S[mb][nt]);
-              }
-            }
-          }
-          if (poisoned) {
-            bool hit = false;
-            for (int j = 0; j < n; ++j) hit |= (bad[j / 32] >> (j % 32) & 1) && first[p + j] == first_last;
-            if (hit) each_state([](float, int, int) { return __builtin_nanf(""); });
-            __syncthreads();
-            if (threadIdx.x == 0) bad_any = 0;
-            __syncthreads();
+              for (int r4 = 0; r4 < 4; ++r4) acc[i][nt][r4] = f != 0.0f ? acc[i][nt][r4] * f : 0.0f;
           }
         }
       }
+      lds_barrier();  // the matrix is there
+    }
+    if (works) {
+      Frag c[NT][C / K];  // c's columns that the wave owns
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kj = 0; kj < C / K; ++kj) c[nt][kj] = load_frag<M>(c_turned + Cols_::from(ct_at, column_of(nt, 0), 4 * kj));
+      if constexpr (!STATE_ONLY) {
+        // ---- the piece's tokens among each other ----
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+          for (int kj = 0; kj < C / K; ++kj) {
+            if (kj * Q > i) continue;
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) {
+              const Frag m = load_frag<M>(b_rows + k * C * C + Cols_::from(m_at, 16 * i, 4 * kj));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) acc[i][nt] = X::mma(c[nt][kj], m, acc[i][nt]);
+            }
+          }
+        if (poisoned)
+#pragma unroll
+          for (int i = 0; i < IT; ++i) {
+            const int at = 16 * i + col, mine = from_first[min(at, n - 1)];
+            bool hit = false;
+            for (int j = 0; j <= min(at, n - 1); ++j) hit |= (bad[j / 32] >> (j % 32) & 1) && from_first[j] == mine;
+            if (hit)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) acc[i][nt] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+          }
+        // ---- the outputs ----
+        if (q.ga > 1 || ab == q.gb - 1) {
+          const int ha = q.ga > 1 ? head * q.ga + ab : head, d = dc0 + 4 * NT * g;
+          const int64_t lowest = q.reverse ? q.tokens - begin - n : begin;
+          T* const to = static_cast<T*>(q.out.data) + ha * q.out.head_stride + lowest * q.out.token_stride;
+#pragma unroll
+          for (int i = 0; i < IT; ++i) {
+            const int at = 16 * i + col;
+            if (valid >> at & 1) {
+              T* row = to + (static_cast<uint64_t>(static_cast<uint32_t>(q.reverse ? n - 1 - at : at)) * static_cast<uint32_t>(q.out.token_stride) + d);
+              typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+              typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+              if (NT == 2 && d + 8 <= q.dc) {
+                Eight o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(acc[i][e / 4 * (NT - 1)][e % 4]);
+                *reinterpret_cast<Eight*>(row) = o;
+              } else if (NT == 1 && d + 4 <= q.dc) {
+                Four o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[i][0][e]);
+                *reinterpret_cast<Four*>(row) = o;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4 * NT; ++e)
+                  if (d + e < q.dc) row[e] = static_cast<T>(acc[i][e / 4][e % 4]);
+              }
+            }
+          }
+        }
+      }
+      // ---- the state ----
+      if (ab >= q.ga - 1) {
+        if (ab == q.ga - 1) {
+          const float f = first_last == first0 ? fades[n] : 0.0f;
+#pragma unroll
+          for (int mb = 0; mb < DBT; ++mb)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int r4 = 0; r4 < 4; ++r4) S[mb][nt][r4] *= f;
+          if (first_last != first0 && lost) each_state([](float, int, int) { return 0.0f; }), lost = false;
+        }
+#pragma unroll
+        for (int kj = 0; kj < C / K; ++kj) {
+          f32x4 w[Q];
+#pragma unroll
+          for (int h = 0; h < Q; ++h) w[h] = *reinterpret_cast<const f32x4*>(weights + K * kj + K / 4 * g + 4 * h);
+          Frag weighted[NT][X::PARTS3];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float v[4 * Q];
+#pragma unroll
+            for (int i = 0; i < 4 * Q; ++i) v[i] = w[i / 4][i % 4] * static_cast<float>(c[nt][kj][i]);
+            split<M, X::PARTS3>(v, weighted[nt]);
+          }
+#pragma unroll
+          for (int mb = 0; mb < DBT; ++mb) {
+            const Frag b = load_frag<M>(b_turned + Cols_::from(bt_at, X::row_of(mb, 0), 4 * kj));
+#pragma unroll
+            for (int k = 0; k < X::PARTS3; ++k)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) S[mb][nt] = X::mma(b, weighted[nt][k], S[mb][nt]);
+          }
+        }
+      }
+    }
+    if (poisoned && ab >= q.ga - 1) {
+      bool hit = false;
+      for (int j = 0; j < n; ++j) hit |= (bad[j / 32] >> (j % 32) & 1) && from_first[j] == first_last;
+      if (hit) each_state([](float, int, int) { return __builtin_nanf(""); }), lost = true;
+      lds_barrier();
+      if (threadIdx.x == 0) bad_any = 0;
+      if (threadIdx.x < (C + 31) / 32) bad[threadIdx.x] = 0;
+    }
+    if (ab == abs - 1) {
       fresh = false;
-      if (!STATE_ONLY && q.s_out != nullptr && works && seq >= 0 && last[p + n - 1] == begin + n) {
-        float* to = q.s_out + (static_cast<int64_t>(seqs[p + n - 1]) * q.heads + head) * q.state_size;
+      if (!STATE_ONLY && q.s_out != nullptr && works && seq >= 0 && last[buffer][p + n - 1] == begin + n) {
+        float* to = q.s_out + (static_cast<int64_t>(seqs[buffer][p + n - 1]) * q.heads + head) * q.state_size;
         each_state([&](float s, int i, int j) {
           if (i < q.db && j < q.dc) to[i * q.si + j * q.sj] = s;
           return s;
         });
       }
-      p += n;
     }
+    if (done) break;
+    c0 = next_c0, p = next_p, ab = next_ab, buffer = next_buffer, n = next_n;
   }
   if (STATE_ONLY && works) {
     float* to = q.carry + (static_cast<int64_t>(seg) * q.heads + head) * q.db * q.dc;
@@ -624,6 +778,8 @@ int check(const char* who, const ppo_decay_attention_args* args, bool backward) 
   const int count = backward ? 7 : 4;
   for (int i = 0; i < count; ++i)
     if (int rc = check_view(who, views[i].name, *views[i].v, n, views[i].heads, views[i].dim, size, views[i].written)) return rc;
+  PPO_REQUIRE(n <= 1 || (!backward ? a.out.token_stride : std::max(std::max(a.d_q.token_stride, a.d_k.token_stride), a.d_v.token_stride)) < (int64_t{1} << 31),
+              "%s: outputs' tokens lie 2^31 elements apart or more", who);
   // every output apart from every input and the other outputs
   const int64_t states = a.sequences * hk * dk * dv * 4;
   struct Region {
@@ -680,7 +836,12 @@ int hand_on(const ppo_decay_attention_args& a, const float* from, float* to, hip
   return check_launch("decay_empty_kernel");
 }
 
-int mix(const ppo_decay_attention_args& a, const MixArgs& q, hipStream_t st) {
+int mix(const ppo_decay_attention_args& a, MixArgs q, hipStream_t st) {
+  const int piece = 16 / type_size(a.type);
+  q.lost = q.s_in != nullptr || q.segments > 1;
+  q.whole = a.key_dim % piece == 0 && a.value_dim % piece == 0;
+  for (const ppo_head_view* v : {&q.a, &q.b, &q.c})  // (rows' offsets within a chunk are products of 24 bits)
+    if (v->token_stride * type_size(a.type) >= 1 << 24) q.whole = 0;
   int rc = PPO_OK;
   with_type(a.type, [&](auto t) { rc = launch_type<decltype(t)>(q, st); });
   return rc;
