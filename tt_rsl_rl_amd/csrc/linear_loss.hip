@@ -11,10 +11,12 @@
 // Four products of 2 R V D operations each for three that any way needs: the first one a second time instead of logits kept.
 //
 // All products are one kernel: out[m, n] = sum_k X[m, k] Y[n, k], both operands with k innermost (what is turned is turned by a copy, a
-// few per cent of the products' time), 256 m by 256, 128 or 32 n, eight waves of 32 x 32 x 16 matrix instructions, tiles of 64 k brought
-// straight to LDS two deep.  In LDS a row's eight 16-byte pieces change places by the row's number, so that reading a column of pieces
+// few per cent of the products' time), 256 m by 256, 128 or 32 n, eight waves of 32 x 32 x 16 matrix instructions, tiles of 64 (32) k brought
+// straight to LDS, two to four deep.  In LDS a row's 16-byte pieces change places by the row's number, so that reading a column of pieces
 // meets all banks.  An accumulator lane holds one n and rows of m: with the vocabulary along m a row's sums stay in its lane but for one
-// shuffle and the waves' join.  fp32 operands are three bf16 parts, and k runs six times over pairs of parts (error 2^-24 and below).
+// shuffle and the waves' join.  fp32 operands are three bf16 parts, six products of which are taken (what is left out is 2^-24 and below).
+#include <numeric>
+
 #include "elem.hpp"
 
 namespace ppo {
@@ -26,12 +28,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kFloor = -1000.0f;
 constexpr int kGemmThreads = 512;
-constexpr int kTileM = 256, kTileK = 64;
-constexpr int kRowBytes = kTileK * 2;  // of a tile in LDS
-constexpr int kPairs = 6;              // products of fp32 operands' parts
+constexpr int kTileM = 256, kTileK = 64;  // (operands' k is padded to whole tiles of 64)
 constexpr int kMaxParts = 3;
-constexpr int64_t kPieceBytes = int64_t{1} << 28;  // of d in one layout, at most
-constexpr int64_t kMinPiece = 2048, kMaxPiece = 32768;
+// A piece's columns: d in both layouts and the weight's copies take up to so much (a piece more costs a reading and a writing of d_hidden's sums).
+constexpr int64_t kPieceBytes = int64_t{3} << 28;
+constexpr int64_t kMinPiece = 2048;
+constexpr int64_t kKeptBytes = int64_t{1} << 28;
 
 // The operands' 16-bit type: bf16 for fp32's parts.
 template <class T>
@@ -44,9 +46,17 @@ struct Half<float> {
 };
 template <class T>
 constexpr int kParts = sizeof(T) == 4 ? kMaxParts : 1;
+template <class T>
+constexpr int kStep = sizeof(T) == 4 ? 32 : 64;  // k of a stage (bf16: 32, four stages deep, took 6 to 9 % longer)
 // d lies in [-1, 1]; fp16's smallest step near zero would be 6e-8 of that, many tokens' whole probability.
 template <class T>
 constexpr float kLift = __is_same(T, _Float16) ? 16384.0f : 1.0f;
+
+// d_hidden may have few tiles: their k is then cut into slices, as many as make two rounds of blocks.  Only the device knows how many rows count.  (Four slices
+// of 192 tiles, three whole rounds instead of three quarters of one, gained nothing: the sums are read and written four times.)
+__device__ __forceinline__ int slices_of(int tiles, int cus, int steps) {
+  return 2 * tiles < cus ? static_cast<int>(min(ceil_div(2 * cus, max(tiles, 1)), static_cast<int64_t>(max(steps / 8, 1)))) : 1;
+}
 
 struct Operand {
   const void* at;     // [part][rows][ld], 16-bit
@@ -58,9 +68,9 @@ constexpr int kSums = 0, kDiffs = 1, kRowGrad = 2, kWeightGrad = 3;  // what a p
 
 struct GemmArgs {
   Operand x, y;          // m, n
-  int32_t m, n, steps;   // of 64 k
+  int32_t m, n, steps;   // of the kernel's STEP k
   const int32_t* count;  // rows that count
-  int32_t m_tiles, n_tiles;
+  int32_t m_tiles, n_tiles, xcds;
   // sums and differences
   int64_t vocab, column0;  // of the piece
   float c;
@@ -69,12 +79,13 @@ struct GemmArgs {
   int64_t sum_rows, tile0;
   float* x_token;
   const float *row_m, *row_inv_s;
+  float* kept;  // [row][ld_kept]: the products themselves, NULL: not kept
+  int64_t ld_kept;
   void *d, *d_turned;  // [part][rows][ld_d], [part][columns][ld_t]
   int64_t ld_d, d_part, ld_t, t_part;
   // gradients
   float* partial;  // [slice][rows][m]
-  int64_t slice_size;
-  int32_t slices, add;
+  int32_t cus, all_steps, add;  // all_steps: of a whole piece, which decides the slices
   void* out;  // [n][m]
   int64_t ld_out;
   float denom, inv_temp;
@@ -99,7 +110,9 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, uint32_
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, off, 0, 0, 0);
 }
 
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// All but the wave's last N loads have arrived.
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // WM x WN waves of TM x TN tiles of 32 x 32.
 template <class T, int WM, int WN, int TM, int TN, int JOB>
@@ -107,58 +120,62 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
   typedef typename Half<T>::type M;
   constexpr int BN = 32 * TN * WN, BM = 32 * TM * WM, PARTS = kParts<T>;
   static_assert(BM == kTileM && WM * WN * kWave == kGemmThreads);
-  constexpr int STAGE = (BM + BN) * kRowBytes;
-  constexpr int LOADS_X = BM / 64, LOADS_Y = BN >= 64 ? BN / 64 : 1;  // 1 KB each, per wave
-  __shared__ __align__(16) unsigned char lds[2 * STAGE];
+  // A stage of LDS: STEP k of all parts of both tiles.  fp32's three parts are there together, so that each meets the others from LDS (six products of
+  // what is loaded once; pairs of parts one after another load everything twice, and 257 rows' d_hidden came at the last-level cache's 6.5 TB/s).
+  constexpr int STEP = kStep<T>, ROW = STEP * 2, PIECES = ROW / 16, PART = (BM + BN) * ROW, STAGE = PARTS * PART;
+  // As many stages as fit, all but one of them on their way while that one is used.
+  constexpr int STAGES = 155648 / STAGE < 4 ? 155648 / STAGE : 4;
+  constexpr int LOAD_ROWS = 1024 / ROW;  // rows of a wave's load
+  constexpr int LOADS_X = BM / LOAD_ROWS / 8, Y_WAVES = BN / LOAD_ROWS < 8 ? BN / LOAD_ROWS : 8, LOADS_Y = BN / LOAD_ROWS / Y_WAVES;  // per wave and part
+  __shared__ __align__(16) unsigned char lds[STAGES * STAGE];
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WN, wn = wave % WN;
-  const int tile = blockIdx.x, mt = tile % q.m_tiles, nt = tile / q.m_tiles;
-  const int m0 = mt * BM, n0 = nt * BN;
+  // Tiles with rows that count, a run of them to each XCD (blocks go to XCDs in turn), four n by m after m: what an XCD's blocks read together lies in
+  // its L2 as often as can be.  (The last 64 rows' d is made past the count too, as zeros: the second products sum over whole steps.)
   const int32_t count = *q.count;
-  // (of the last 64 rows the ones past the count are made all the same, as zeros: the second products sum over whole steps)
-  if (JOB != kWeightGrad && n0 >= (JOB == kDiffs ? ceil_div(count, kTileK) * kTileK : count)) return;
+  const int n_there = JOB == kWeightGrad ? q.n_tiles : static_cast<int>(ceil_div(JOB == kDiffs ? ceil_div(count, kTileK) * kTileK : count, BN));
+  const int tiles = q.m_tiles * n_there, slices = JOB == kRowGrad ? slices_of(tiles, q.cus, q.all_steps) : 1, all = tiles * slices, each = static_cast<int>(ceil_div(all, q.xcds));
+  const int local = blockIdx.x / q.xcds, item = blockIdx.x % q.xcds * each + local;
+  if (local >= each || item >= all) return;
+  const int slice = JOB == kRowGrad ? item / tiles : 0, tile = item - slice * tiles;
+  const int first_n = tile / (4 * q.m_tiles) * 4, wide = min(4, n_there - first_n), inside = tile - first_n * q.m_tiles;
+  const int mt = inside / wide, nt = first_n + inside % wide;
+  const int m0 = mt * BM, n0 = nt * BN;
   int steps = q.steps;
-  if (JOB == kWeightGrad) steps = static_cast<int>(ceil_div(count, kTileK));
+  if (JOB == kWeightGrad) steps = static_cast<int>(ceil_div(count, kTileK)) * (kTileK / STEP);
   int from = 0, to = steps;
   if (JOB == kRowGrad) {  // a slice of k
-    const int each = static_cast<int>(ceil_div(steps, q.slices));
-    from = min(static_cast<int>(blockIdx.y) * each, steps);
-    to = min(from + each, steps);
+    const int span = static_cast<int>(ceil_div(steps, slices));
+    from = min(slice * span, steps);
+    to = min(from + span, steps);
   }
 
-  // Addresses: a wave's load covers 8 rows of 128 bytes; lane l brings the piece that belongs at its place.
+  // Addresses: a wave's load covers LOAD_ROWS rows; lane l brings the piece that belongs at its place.
   uint32_t off_x[LOADS_X], off_y[LOADS_Y];
-  const auto place = [&](int row) { return static_cast<uint32_t>(((lane % 8) ^ (row / 2 % 8)) * 16); };
+  const auto turn = [](int row) { return PIECES == 8 ? row / 2 % 8 : row / 4 % 4; };
+  const auto offset = [&](int row, int tile0, const Operand& o) {
+    return static_cast<uint32_t>(min(tile0 + row, o.rows - 1) - tile0) * static_cast<uint32_t>(o.ld * 2) + static_cast<uint32_t>((lane % PIECES ^ turn(row)) * 16);
+  };
 #pragma unroll
-  for (int i = 0; i < LOADS_X; ++i) {
-    const int row = (wave * LOADS_X + i) * 8 + lane / 8;
-    off_x[i] = static_cast<uint32_t>(min(m0 + row, q.x.rows - 1) - m0) * static_cast<uint32_t>(q.x.ld * 2) + place(row);
-  }
+  for (int i = 0; i < LOADS_X; ++i) off_x[i] = offset((wave * LOADS_X + i) * LOAD_ROWS + lane / PIECES, m0, q.x);
 #pragma unroll
-  for (int i = 0; i < LOADS_Y; ++i) {
-    const int row = (wave * LOADS_Y + i) * 8 + lane / 8;
-    off_y[i] = static_cast<uint32_t>(min(n0 + row, q.y.rows - 1) - n0) * static_cast<uint32_t>(q.y.ld * 2) + place(row);
-  }
+  for (int i = 0; i < LOADS_Y; ++i) off_y[i] = offset((wave * LOADS_Y + i) * LOAD_ROWS + lane / PIECES, n0, q.y);
   const char* const base_x = static_cast<const char*>(q.x.at) + static_cast<int64_t>(m0) * q.x.ld * 2;
   const char* const base_y = static_cast<const char*>(q.y.at) + static_cast<int64_t>(n0) * q.y.ld * 2;
-  const int per_pair = to - from, total = PARTS == 1 ? per_pair : per_pair * kPairs;
+  const int total = to - from;
   auto load_stage = [&](int s) {
-    int k = s, px = 0, py = 0;
-    if constexpr (PARTS > 1) {
-      const int pair = s / per_pair;
-      k = s - pair * per_pair;
-      px = pair == 2 || pair == 3 ? 1 : pair == 5 ? 2 : 0;
-      py = pair == 1 || pair == 3 ? 1 : pair == 4 ? 2 : 0;
+    const int64_t k_bytes = static_cast<int64_t>(from + s) * ROW;
+    unsigned char* to_lds = lds + s % STAGES * STAGE;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      const auto rx = buffer_at(base_x + part * q.x.part * 2 + k_bytes), ry = buffer_at(base_y + part * q.y.part * 2 + k_bytes);
+#pragma unroll
+      for (int i = 0; i < LOADS_X; ++i) load_to_lds(rx, off_x[i], to_lds + part * PART + (wave * LOADS_X + i) * 1024);
+      if (Y_WAVES == 8 || wave < Y_WAVES)
+#pragma unroll
+        for (int i = 0; i < LOADS_Y; ++i) load_to_lds(ry, off_y[i], to_lds + part * PART + BM * ROW + (wave * LOADS_Y + i) * 1024);
     }
-    const int64_t k_bytes = static_cast<int64_t>(from + k) * kRowBytes;
-    const auto rx = buffer_at(base_x + px * q.x.part * 2 + k_bytes), ry = buffer_at(base_y + py * q.y.part * 2 + k_bytes);
-    unsigned char* to_lds = lds + (s & 1) * STAGE;
-#pragma unroll
-    for (int i = 0; i < LOADS_X; ++i) load_to_lds(rx, off_x[i], to_lds + (wave * LOADS_X + i) * 1024);
-    if (BN >= 64 || wave < BN / 8)
-#pragma unroll
-      for (int i = 0; i < LOADS_Y; ++i) load_to_lds(ry, off_y[i], to_lds + BM * kRowBytes + (wave * LOADS_Y + i) * 1024);
   };
 
   f32x16 acc[TM][TN];
@@ -170,31 +187,43 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
   const int r32 = lane % 32, half = lane / 32;
-  if (total > 0) load_stage(0);
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < total) load_stage(s);
   for (int s = 0; s < total; ++s) {
-    wait_loads();
+    if (STAGES == 2 || s + STAGES - 2 >= total) wait_loads<0>();
+    else if (Y_WAVES == 8 || wave < Y_WAVES) wait_loads<(STAGES - 2) * PARTS * (LOADS_X + LOADS_Y)>();
+    else wait_loads<(STAGES - 2) * PARTS * LOADS_X>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < total) load_stage(s + 1);
-    const unsigned char* at = lds + (s & 1) * STAGE;
+    if (s + STAGES - 1 < total) load_stage(s + STAGES - 1);
+    const unsigned char* at = lds + s % STAGES * STAGE;
 #pragma unroll
-    for (int kk = 0; kk < kTileK / 16; ++kk) {
-      u32x4 x[TM], y[TN];
+    for (int kk = 0; kk < STEP / 16; ++kk) {
+      u32x4 x[PARTS][TM], y[PARTS][TN];
       const int piece = 2 * kk + half;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row = (wm * TM + i) * 32 + r32;
-        x[i] = *reinterpret_cast<const u32x4*>(at + row * kRowBytes + (piece ^ (row / 2 % 8)) * 16);
+      for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int row = (wm * TM + i) * 32 + r32;
+          x[part][i] = *reinterpret_cast<const u32x4*>(at + part * PART + row * ROW + (piece ^ turn(row)) * 16);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int row = (wn * TN + j) * 32 + r32;
+          y[part][j] = *reinterpret_cast<const u32x4*>(at + part * PART + BM * ROW + row * ROW + (piece ^ turn(row)) * 16);
+        }
       }
+      // (the smallest products first: x3 y1, x2 y2, x1 y3, x2 y1, x1 y2, x1 y1)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int row = (wn * TN + j) * 32 + r32;
-        y[j] = *reinterpret_cast<const u32x4*>(at + BM * kRowBytes + row * kRowBytes + (piece ^ (row / 2 % 8)) * 16);
-      }
+      for (int sum = PARTS - 1; sum >= 0; --sum)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int px = sum; px >= 0; --px)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mma<M>(x[i], y[j], acc[i][j]);
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = mma<M>(x[px][i], y[sum - px][j], acc[i][j]);
     }
   }
 
@@ -204,20 +233,41 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
     __syncthreads();
     float* join_at = reinterpret_cast<float*>(lds);  // [WM][3][BN]
     const int64_t left = q.vocab - q.column0 - m0;   // columns of the tile that are there
+    if (PARTS > 1 && q.kept != nullptr)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + 32 * (wn * TN + j) + r32;
+        if (n < count)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+              typedef float Four __attribute__((ext_vector_type(4)));
+              *reinterpret_cast<Four*>(q.kept + static_cast<int64_t>(n) * q.ld_kept + m0 + m_of(i, 4 * r4)) =
+                  Four{acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]};
+            }
+      }
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + 32 * (wn * TN + j) + r32;
       const int64_t tok = n < count ? q.token[n] - q.column0 - m0 : -1;
       float m = -INFINITY;
+      if (left < BM)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (m_of(i, r) >= left) acc[i][j][r] = -INFINITY;
+      if (__any(tok >= 0 && tok < BM))
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (m_of(i, r) == tok) q.x_token[n] = acc[i][j][r];
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int col = m_of(i, r);
-          if (col >= left) acc[i][j][r] = -INFINITY;
-          if (col == tok) q.x_token[n] = acc[i][j][r];
-          m = fmaxf(m, acc[i][j][r]);
-        }
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
       m = fmaxf(m, __shfl_xor(m, 32, kWave));
       const float zero = m > -INFINITY ? m : 0.0f;
       float s = 0.0f, e = 0.0f;
@@ -261,34 +311,69 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
       const int n = n0 + 32 * (wn * TN + j) + r32;
       const bool live = n < count;
       const int64_t tok = live ? q.token[n] - q.column0 - m0 : -1;
-      const float m = live ? q.row_m[n] : 0.0f, inv = live ? q.row_inv_s[n] : 0.0f;
+      const float m = live ? q.row_m[n] : 0.0f, inv = live ? q.row_inv_s[n] * kLift<T> : 0.0f;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          float v[4];
-          const int col = m_of(i, 4 * r4);
+        for (int r = 0; r < 16; ++r) {
+          const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - m) * q.c) * inv;
+          acc[i][j][r] = live && m_of(i, r) < left ? p : 0.0f;
+        }
+      if (__any(tok >= 0 && tok < BM))
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f((acc[i][j][4 * r4 + r] - m) * q.c) * inv;
-            v[r] = live && col + r < left ? (p - (col + r == tok ? 1.0f : 0.0f)) * kLift<T> : 0.0f;
-          }
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
+          for (int r = 0; r < 16; ++r)
+            if (m_of(i, r) == tok) acc[i][j][r] -= kLift<T>;
+    }
+    // Both layouts leave through LDS in 16-byte pieces: rows n of the tile's m, piece p at place p ^ n % 16 of its row.  (Rows of a tile past the gathered
+    // ones leave too, as zeros; columns up to the tile's end as well.)
+    static_assert(BN * BM * 2 <= STAGES * STAGE);
+    M* const rows = reinterpret_cast<M*>(lds);
+    const auto at = [](int n, int piece) { return n * BM + (piece ^ n % 16) * 8; };
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
             typedef M Four __attribute__((ext_vector_type(4)));
             Four f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              f[r] = static_cast<M>(v[r]);
-              v[r] -= static_cast<float>(f[r]);
+              f[r] = static_cast<M>(acc[i][j][4 * r4 + r]);
+              if (part + 1 < PARTS) acc[i][j][4 * r4 + r] -= static_cast<float>(f[r]);
             }
-            // (rows of a tile past the gathered ones are there too, as zeros, in both layouts; columns up to the tile's end as well)
-            if (q.d != nullptr && n < q.n) *reinterpret_cast<Four*>(static_cast<M*>(q.d) + part * q.d_part + static_cast<int64_t>(n) * q.ld_d + m0 + col) = f;
-            if (q.d_turned != nullptr && n < q.n)
+            *reinterpret_cast<Four*>(rows + at(32 * (wn * TN + j) + r32, 4 * (wm * TM + i) + r4) + 4 * half) = f;
+          }
+      __syncthreads();
+      if (q.d != nullptr) {
+        M* const to = static_cast<M*>(q.d) + part * q.d_part + m0;
+        for (int k = threadIdx.x; k < BN * (BM / 8); k += kGemmThreads) {
+          const int n = k / (BM / 8), piece = k % (BM / 8);
+          if (n0 + n < q.n) *reinterpret_cast<u32x4*>(to + static_cast<int64_t>(n0 + n) * q.ld_d + piece * 8) = *reinterpret_cast<const u32x4*>(rows + at(n, piece));
+        }
+      }
+      if (q.d_turned != nullptr) {
+        M* const to = static_cast<M*>(q.d_turned) + part * q.t_part + n0;
+        for (int k = threadIdx.x; k < (BN / 8) * (BM / 8); k += kGemmThreads) {
+          const int n = k % (BN / 8) * 8, piece = k / (BN / 8);
+          if (n0 + n >= q.n) continue;  // (q.n is a multiple of 64)
+          u32x4 x[8];
 #pragma unroll
-              for (int r = 0; r < 4; ++r) (static_cast<M*>(q.d_turned) + part * q.t_part)[static_cast<int64_t>(m0 + col + r) * q.ld_t + n] = f[r];
+          for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const u32x4*>(rows + at(n + e, piece));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            u32x4 y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) y[w] = __builtin_amdgcn_perm(x[2 * w + 1][e / 2], x[2 * w][e / 2], e % 2 != 0 ? 0x07060302u : 0x05040100u);
+            *reinterpret_cast<u32x4*>(to + static_cast<int64_t>(m0 + piece * 8 + e) * q.ld_t + n) = y;
           }
         }
+      }
     }
   } else {
     const float factor = 1.0f / kLift<T> * (JOB == kWeightGrad ? q.inv_temp / (q.denom > 0.0f ? q.denom : static_cast<float>(max(count, 1))) : 1.0f);
@@ -302,7 +387,7 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
         for (int r4 = 0; r4 < 4; ++r4) {
           const int m = m0 + m_of(i, 4 * r4);
           if constexpr (JOB == kRowGrad) {
-            float* at = q.partial + blockIdx.y * q.slice_size + static_cast<int64_t>(n) * q.m + m;
+            float* at = q.partial + (static_cast<int64_t>(slice) * n_there * BN + n) * q.m + m;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (m + r < q.m) at[r] = q.add != 0 ? at[r] + acc[i][j][4 * r4 + r] * factor : acc[i][j][4 * r4 + r] * factor;
@@ -339,8 +424,7 @@ struct RowArgs {
   float* x_token;
   float *row_m, *row_inv_s, *row_lp, *row_h;
   const float* partial;
-  int64_t slice_size;
-  int32_t slices;
+  int32_t cus, all_steps, n_tile;  // as d_hidden's products
   float c;
 };
 
@@ -363,6 +447,10 @@ __global__ __launch_bounds__(kRowThreads) void linear_rows_kernel(const RowArgs 
     }
     at += __popcll(in & ((uint64_t{1} << lane) - 1));
     if (r < q.a.rows) q.gathered[r] = tok >= 0 ? at : -1;
+    if (r < q.a.rows && tok < 0) {
+      if (q.a.logp != nullptr) q.a.logp[r] = 0.0f;
+      if (q.a.entropy != nullptr) q.a.entropy[r] = 0.0f;
+    }
     if (tok >= 0) q.source[at] = static_cast<int32_t>(r), q.token[at] = tok;
     before += all;
     __syncthreads();
@@ -379,6 +467,8 @@ struct PackArgs {
   const int32_t* count;
   void* dst;                 // [part][out_rows][ld_dst]
   int64_t ld_dst, part, out_rows;
+  void* turned;              // [part][dim][ld_turned]
+  int64_t ld_turned, turned_part;
 };
 
 template <class T, class M>
@@ -404,56 +494,144 @@ __global__ __launch_bounds__(kPackThreads) void linear_pack_kernel(const PackArg
     store_parts<T>(to + k, q.part, from != nullptr && k < q.dim ? static_cast<float>(from[k]) : 0.0f);
 }
 
-// dst[k][row]: 64 x 64 tiles through LDS.
+// turned[k][row], and dst[row][k] where it is wanted: 64 x 64 tiles through LDS.
 template <class T>
 __global__ __launch_bounds__(kPackThreads) void linear_turn_kernel(const PackArgs q) {
   typedef typename Half<T>::type M;
-  __shared__ float tile[64][65];
   const int64_t rows = q.count != nullptr ? static_cast<int64_t>(*q.count) : q.rows;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 64, k0 = static_cast<int64_t>(blockIdx.y) * 64;
+  if constexpr (sizeof(T) == 2) {
+    // 16 bytes a lane on either side; in LDS rows of 66 elements, whose columns lie on as many banks
+    __shared__ T half_tile[64][66];
+    const int piece = threadIdx.x % 8 * 8, first = threadIdx.x / 8;
+    const bool whole = k0 + 64 <= q.dim;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row = row0 + first + 32 * i;
+      RawPiece x{};
+      if (row < rows) {
+        const T* from = static_cast<const T*>(q.src) + (q.source != nullptr ? q.source[row] : row) * q.ld + k0 + piece;
+        if (whole) x = load_raw(from);
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (k0 + piece + e < q.dim) x.w[e / 2] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from[e])) << (e % 2 * 16);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&half_tile[first + 32 * i][piece + 2 * e]) = x.w[e];
+      if (q.dst != nullptr && row < q.out_rows) *reinterpret_cast<RawPiece*>(static_cast<T*>(q.dst) + row * q.ld_dst + k0 + piece) = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t k = k0 + first + 32 * i;
+      if (k >= q.dim) continue;
+      RawPiece x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x.w[e] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, half_tile[piece + 2 * e][first + 32 * i])) |
+                 static_cast<uint32_t>(__builtin_bit_cast(uint16_t, half_tile[piece + 2 * e + 1][first + 32 * i])) << 16;
+      *reinterpret_cast<RawPiece*>(static_cast<T*>(q.turned) + k * q.ld_turned + row0 + piece) = x;
+    }
+    return;
+  }
+  __shared__ float tile[64][65];
   const int lane = threadIdx.x % 64, part = threadIdx.x / 64;
-  for (int i = part; i < 64; i += 4) {
-    const int64_t row = row0 + i, k = k0 + lane;
-    float x = 0.0f;
-    if (row < rows && k < q.dim) x = static_cast<float>((static_cast<const T*>(q.src) + (q.source != nullptr ? q.source[row] : row) * q.ld)[k]);
-    tile[i][lane] = x;
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t row = row0 + part + 4 * i, k = k0 + lane;
+    x[i] = 0.0f;
+    if (row < rows && k < q.dim) x[i] = static_cast<float>((static_cast<const T*>(q.src) + (q.source != nullptr ? q.source[row] : row) * q.ld)[k]);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    tile[part + 4 * i][lane] = x[i];
+    if (q.dst != nullptr && row0 + part + 4 * i < q.out_rows) store_parts<T>(static_cast<M*>(q.dst) + (row0 + part + 4 * i) * q.ld_dst + k0 + lane, q.part, x[i]);
   }
   __syncthreads();
-  for (int i = part; i < 64; i += 4) {
-    const int64_t k = k0 + i;
-    if (k < q.dim) store_parts<T>(static_cast<M*>(q.dst) + k * q.ld_dst + row0 + lane, q.part, tile[lane][i]);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t k = k0 + part + 4 * i;
+    if (k < q.dim) store_parts<T>(static_cast<M*>(q.turned) + k * q.ld_turned + row0 + lane, q.turned_part, tile[lane][part + 4 * i]);
   }
+}
+
+// d from products that were kept: 64 x 64 tiles, in both layouts.
+template <class T>
+__global__ __launch_bounds__(kPackThreads) void linear_diffs_kernel(const GemmArgs q) {
+  typedef typename Half<T>::type M;
+  __shared__ float tile[64][65];
+  const int32_t count = *q.count;
+  const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
+  if (n0 >= count) return;
+  const int lane = threadIdx.x % 64, part = threadIdx.x / 64;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int n = n0 + part + 4 * i, m = m0 + lane;
+    float v = 0.0f;
+    if (n < count && m < q.vocab) {
+      const float p = __builtin_amdgcn_exp2f((q.kept[static_cast<int64_t>(n) * q.ld_kept + m] - q.row_m[n]) * q.c) * q.row_inv_s[n];
+      v = (p - (m == q.token[n] ? 1.0f : 0.0f)) * kLift<T>;
+    }
+    tile[part + 4 * i][lane] = v;
+    if (q.d != nullptr) store_parts<T>(static_cast<M*>(q.d) + static_cast<int64_t>(n) * q.ld_d + m, q.d_part, v);
+  }
+  if (q.d_turned == nullptr) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    store_parts<T>(static_cast<M*>(q.d_turned) + static_cast<int64_t>(m0 + part + 4 * i) * q.ld_t + n0 + lane, q.t_part, tile[lane][part + 4 * i]);
 }
 
 // ---- rows: the tiles' sums joined, log-probabilities, the loss ----
 
-constexpr int kJoinThreads = 256;
-__global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const RowArgs q) {
-  const int lane = threadIdx.x % kWave;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / kWave) + threadIdx.x / kWave;
-  if (n >= *q.count) return;
-  float m = -INFINITY;
-  for (int64_t t = lane; t < q.tiles; t += kWave) m = fmaxf(m, q.tile_m[t * q.sum_rows + n]);
-  for (int d = kWave / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
-  float s = 0.0f, e = 0.0f;
-  for (int64_t t = lane; t < q.tiles; t += kWave) {
-    const float mt = q.tile_m[t * q.sum_rows + n], st = q.tile_s[t * q.sum_rows + n], et = q.tile_e[t * q.sum_rows + n];
-    const float u = mt == m ? 0.0f : fmaxf((mt - m) * q.c, kFloor), f = __builtin_amdgcn_exp2f(u);
-    s = fmaf(st, f, s);
-    e = fmaf(et + st * u, f, e);
-  }
-  for (int d = kWave / 2; d > 0; d >>= 1) s += __shfl_xor(s, d, kWave), e += __shfl_xor(e, d, kWave);
-  if (lane != 0) return;
-  const float log2_s = log2f(s), lp = kLn2 * ((q.x_token[n] - m) * q.c - log2_s), h = kLn2 * (log2_s - e / s);
-  q.row_m[n] = m, q.row_inv_s[n] = 1.0f / s, q.row_lp[n] = lp, q.row_h[n] = h;
+// The sums st and et relative to mt, added to those relative to m >= mt.  (Without columns, st = 0, they are nothing.)
+__device__ __forceinline__ void add_sums(float& s, float& e, float m, float mt, float st, float et, float c) {
+  if (st == 0.0f) return;
+  const float d = mt == m ? 0.0f : fmaxf((mt - m) * c, kFloor), f = __builtin_amdgcn_exp2f(d);
+  s = fmaf(st, f, s);
+  e = fmaf(et + st * d, f, e);
 }
 
-__global__ __launch_bounds__(kJoinThreads) void linear_scatter_kernel(const RowArgs q) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * kJoinThreads + threadIdx.x;
-  if (r >= q.a.rows) return;
-  const int32_t n = q.gathered[r];
-  if (q.a.logp != nullptr) q.a.logp[r] = n >= 0 ? q.row_lp[n] : 0.0f;
-  if (q.a.entropy != nullptr) q.a.entropy[r] = n >= 0 ? q.row_h[n] : 0.0f;
+// A block: 16 rows (the tiles' sums of a row lie rows apart, so neighbouring lanes take neighbouring rows) by 16 groups of tiles.
+constexpr int kJoinThreads = 256, kJoinRows = 16, kJoinGroups = kJoinThreads / kJoinRows;
+__global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const RowArgs q) {
+  __shared__ float part_m[kJoinGroups][kJoinRows], part_s[kJoinGroups][kJoinRows], part_e[kJoinGroups][kJoinRows];
+  const int32_t count = *q.count;
+  const int row = threadIdx.x % kJoinRows, group = threadIdx.x / kJoinRows;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kJoinRows + row;
+  if (n - row >= count) return;
+  const int64_t from = min(n, static_cast<int64_t>(count) - 1);
+  constexpr int AHEAD = 8;  // tiles in flight
+  float m = -INFINITY, s = 0.0f, e = 0.0f;
+  for (int64_t t = group; t < q.tiles; t += kJoinGroups * AHEAD) {
+    float mt[AHEAD], st[AHEAD], et[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t at = min(t + u * kJoinGroups, q.tiles - 1) * q.sum_rows + from;
+      mt[u] = q.tile_m[at], st[u] = q.tile_s[at], et[u] = q.tile_e[at];
+    }
+    const float before = m;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) m = fmaxf(m, mt[u]);
+    const float d = before == m ? 0.0f : fmaxf((before - m) * q.c, kFloor), f = __builtin_amdgcn_exp2f(d);
+    e = (e + s * d) * f;
+    s *= f;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) add_sums(s, e, m, mt[u], t + u * kJoinGroups < q.tiles ? st[u] : 0.0f, et[u], q.c);
+  }
+  part_m[group][row] = m, part_s[group][row] = s, part_e[group][row] = e;
+  __syncthreads();
+  if (group != 0 || n >= count) return;
+  for (int g = 1; g < kJoinGroups; ++g) m = fmaxf(m, part_m[g][row]);
+  s = e = 0.0f;
+  for (int g = 0; g < kJoinGroups; ++g) add_sums(s, e, m, part_m[g][row], part_s[g][row], part_e[g][row], q.c);
+  const float log2_s = log2f(s), lp = kLn2 * ((q.x_token[n] - m) * q.c - log2_s), h = kLn2 * (log2_s - e / s);
+  q.row_m[n] = m, q.row_inv_s[n] = 1.0f / s, q.row_lp[n] = lp, q.row_h[n] = h;
+  const int32_t r = q.source[n];
+  if (q.a.logp != nullptr) q.a.logp[r] = lp;
+  if (q.a.entropy != nullptr) q.a.entropy[r] = h;
 }
 
 __global__ __launch_bounds__(kRowThreads) void linear_stats_kernel(const RowArgs q) {
@@ -481,10 +659,19 @@ __global__ __launch_bounds__(kPackThreads) void linear_row_grad_kernel(const Row
   const int32_t n = q.gathered[r];
   T* to = static_cast<T*>(q.a.d_hidden) + r * q.a.ld_d_hidden;
   const float factor = static_cast<float>(1.0 / (q.a.temperature * (q.a.denom > 0.0 ? q.a.denom : static_cast<double>(max(*q.count, 1)))));
+  const int64_t n_there = ceil_div(*q.count, q.n_tile), slice_size = n_there * q.n_tile * q.a.dim;
+  const int slices = slices_of(static_cast<int>(ceil_div(q.a.dim, kTileM) * n_there), q.cus, q.all_steps);
   for (int64_t k = threadIdx.x; k < q.a.dim; k += kPackThreads) {
     float x = 0.0f;
+    constexpr int AHEAD = 8;
     if (n >= 0)
-      for (int s = 0; s < q.slices; ++s) x += q.partial[s * q.slice_size + n * q.a.dim + k];
+      for (int s = 0; s < slices; s += AHEAD) {
+        float y[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) y[u] = q.partial[min(s + u, slices - 1) * slice_size + n * q.a.dim + k];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) x += s + u < slices ? y[u] : 0.0f;
+      }
     to[k] = static_cast<T>(x * factor);
   }
 }
@@ -493,9 +680,10 @@ __global__ __launch_bounds__(kPackThreads) void linear_row_grad_kernel(const Row
 
 struct Plan {
   int64_t rows, k, piece, pieces;  // rows and k padded to whole tiles of k
-  int parts, slices, n_tile;
+  int parts, cus, n_tile;
   bool direct;  // the weight is an operand as it lies
-  size_t count, source, gathered, token, sums, x_token, row, hidden, hidden_turned, weight, weight_turned, d, d_turned, partial, bytes;
+  bool keep;    // the products of the one piece are kept
+  size_t count, source, gathered, token, sums, x_token, row, hidden, hidden_turned, weight, weight_turned, d, d_turned, partial, kept, bytes;
 };
 
 int64_t up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
@@ -506,17 +694,24 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   p.rows = up(std::max<int64_t>(a.rows, 1), kTileK);
   p.k = up(a.dim, kTileK);
   p.direct = a.type != PPO_TYPE_F32 && a.dim % kTileK == 0 && a.ld_weight % 8 == 0 && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
-  // columns at a time: d of a piece up to kPieceBytes
-  int64_t piece = kPieceBytes / (p.rows * 2 * p.parts) / kTileM * kTileM;
-  piece = std::min(std::max(piece, kMinPiece), kMaxPiece);
+  const int64_t column = 2 * p.parts * ((gradient ? (a.d_hidden != nullptr) + (a.d_weight != nullptr) : 0) * p.rows + (p.direct ? 0 : p.k) +
+                                         (gradient && a.d_hidden != nullptr ? a.dim : 0));
+  int64_t piece = kPieceBytes / std::max<int64_t>(column, 1) / kTileM * kTileM;
+  piece = std::min(std::max(piece, kMinPiece), int64_t{1} << 22);
   if (!gradient && p.direct) piece = up(a.vocab, kTileM);
   p.piece = std::min(piece, up(a.vocab, kTileM));
-  p.pieces = ceil_div(a.vocab, p.piece);
-  p.n_tile = a.rows <= 32 ? 32 : a.rows <= 128 || (a.rows > 256 && a.rows <= 384) ? 128 : 256;
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
-  const int64_t tiles = ceil_div(a.dim, kTileM) * ceil_div(a.rows, p.n_tile), steps = p.piece / kTileK;
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min(cus / std::max<int64_t>(tiles, 1), steps / 8)));
+  p.pieces = ceil_div(a.vocab, p.piece);
+  if (p.pieces > 1) {
+    // columns whose d_weight takes whole rounds of the chip's blocks, or else pieces of one size (8,192 x 131,072 of 2,048: 16,384 columns 512 blocks and two rounds,
+    // 18,944 592 blocks and three)
+    const int64_t blocks = ceil_div(a.dim, kTileM), round = cus / std::gcd(cus, blocks) * kTileM;
+    p.piece = p.piece >= round ? p.piece / round * round : up(ceil_div(a.vocab, p.pieces), kTileM);
+    p.pieces = ceil_div(a.vocab, p.piece);
+  }
+  p.n_tile = a.rows <= 32 ? 32 : a.type == PPO_TYPE_F32 || a.rows <= 128 || (a.rows > 256 && a.rows <= 384) ? 128 : 256;
+  p.cus = static_cast<int>(cus);
   size_t at = 256;
   auto room = [&](size_t n) {
     const size_t from = at;
@@ -532,11 +727,16 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   p.row = room(4 * p.rows * 4);
   p.hidden = room(p.parts * p.rows * p.k * 2);
   p.weight = room(p.direct ? 0 : p.parts * p.piece * p.k * 2);
+  // fp32 products come six times as dear as 16-bit ones: where one piece holds the vocabulary and its products are small, they are kept for d instead of
+  // made again (257 rows of 515 over 50,021 columns: 183 us again, 62 from what was kept; bf16 products are made in the time that reading takes)
+  p.keep = gradient && a.type == PPO_TYPE_F32 && p.pieces == 1 && p.rows * p.piece * 4 <= kKeptBytes && (a.d_hidden != nullptr || a.d_weight != nullptr);
+  p.kept = room(p.keep ? p.rows * p.piece * 4 : 0);
   if (gradient) {
     if (a.d_hidden != nullptr) {
       p.weight_turned = room(p.parts * a.dim * p.piece * 2);
       p.d = room(p.parts * p.rows * p.piece * 2);
-      p.partial = room(static_cast<size_t>(p.slices) * p.rows * a.dim * 4);
+      // (as slices_of() cuts them: one of all rows, or blocks for two rounds and less than half a one)
+      p.partial = room(std::max<size_t>(up(p.rows, p.n_tile) * a.dim, ceil_div(5 * cus / 2, ceil_div(a.dim, kTileM)) * p.n_tile * a.dim) * 4);
     }
     if (a.d_weight != nullptr) {
       p.hidden_turned = room(p.parts * a.dim * p.rows * 2);
@@ -549,15 +749,19 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
 
 template <class T, int JOB>
 int launch_gemm(GemmArgs g, int n_tile, hipStream_t st) {
-  if (JOB == kWeightGrad) n_tile = 256;  // n is the vocabulary there
+  if (JOB == kWeightGrad) n_tile = sizeof(T) == 4 ? 128 : 256;  // n is the vocabulary there
   g.m_tiles = static_cast<int32_t>(ceil_div(g.m, kTileM));
   g.n_tiles = static_cast<int32_t>(ceil_div(g.n, n_tile));
-  const dim3 grid(static_cast<uint32_t>(g.m_tiles) * static_cast<uint32_t>(g.n_tiles), JOB == kRowGrad ? g.slices : 1);
-  if (n_tile == 256) hipLaunchKernelGGL((linear_gemm_kernel<T, 2, 4, 4, 2, JOB>), grid, dim3(kGemmThreads), 0, st, g);
-  else if constexpr (JOB != kWeightGrad) {
-    if (n_tile == 128) hipLaunchKernelGGL((linear_gemm_kernel<T, 4, 2, 2, 2, JOB>), grid, dim3(kGemmThreads), 0, st, g);
-    else hipLaunchKernelGGL((linear_gemm_kernel<T, 8, 1, 1, 1, JOB>), grid, dim3(kGemmThreads), 0, st, g);
-  }
+  g.xcds = std::max(1, device_info().xcds);
+  const dim3 grid(static_cast<uint32_t>(up(static_cast<int64_t>(g.m_tiles) * g.n_tiles + (JOB == kRowGrad ? 2 * g.cus : 0), g.xcds)));
+#define PPO_GEMM(...) hipLaunchKernelGGL((linear_gemm_kernel<T, __VA_ARGS__, JOB>), grid, dim3(kGemmThreads), 0, st, g)
+  if constexpr (sizeof(T) == 2)
+    if (n_tile == 256) PPO_GEMM(2, 4, 4, 2);
+  if constexpr (sizeof(T) == 4 || JOB != kWeightGrad)
+    if (n_tile == 128) PPO_GEMM(4, 2, 2, 2);
+  if constexpr (JOB != kWeightGrad)
+    if (n_tile == 32) PPO_GEMM(8, 1, 1, 1);
+#undef PPO_GEMM
   return check_launch("linear_gemm_kernel");
 }
 
@@ -582,25 +786,27 @@ int run_typed(const ppo_linear_loss_args& a, const Plan& p, char* ws, hipStream_
   r.row_h = r.row_lp + p.rows;
   r.c = static_cast<float>(1.4426950408889634 / a.temperature);
   r.partial = reinterpret_cast<const float*>(ws + p.partial);
-  r.slice_size = p.rows * a.dim;
-  r.slices = p.slices;
+  r.cus = p.cus, r.all_steps = static_cast<int32_t>(p.piece / kStep<T>), r.n_tile = p.n_tile;
   hipLaunchKernelGGL(linear_rows_kernel, dim3(1), dim3(kRowThreads), 0, st, r);
   if (int rc = check_launch("linear_rows_kernel")) return rc;
 
-  PackArgs h{a.hidden, a.ld_hidden, a.rows, a.dim, r.source, r.count, ws + p.hidden, p.k, p.rows * p.k, p.rows};
-  hipLaunchKernelGGL(linear_pack_kernel<T>, dim3(static_cast<uint32_t>(p.rows)), dim3(kPackThreads), 0, st, h);
-  if (int rc = check_launch("linear_pack_kernel")) return rc;
   const bool to_hidden = gradient && a.d_hidden != nullptr, to_weight = gradient && a.d_weight != nullptr;
-  if (to_weight) {
-    h.dst = ws + p.hidden_turned, h.ld_dst = p.rows, h.part = a.dim * p.rows;
-    hipLaunchKernelGGL(linear_turn_kernel<T>, dim3(static_cast<uint32_t>(p.rows / 64), static_cast<uint32_t>(ceil_div(a.dim, 64))), dim3(kPackThreads), 0, st, h);
-    if (int rc = check_launch("linear_turn_kernel")) return rc;
-  }
+  // Rows of `from` as an operand, turned, or both at once.
+  auto pack = [&](const void* from, int64_t ld, int64_t n, bool gathered, void* to, int64_t part, void* turned, int64_t ld_turned, int64_t turned_part) -> int {
+    const PackArgs w{from, ld, n, a.dim, gathered ? r.source : nullptr, gathered ? r.count : nullptr, to, p.k, part, n, turned, ld_turned, turned_part};
+    if (turned != nullptr) {  // (up to p.k: the operand's padding is this launch's too)
+      hipLaunchKernelGGL(linear_turn_kernel<T>, dim3(static_cast<uint32_t>(ceil_div(n, 64)), static_cast<uint32_t>(p.k / 64)), dim3(kPackThreads), 0, st, w);
+      return check_launch("linear_turn_kernel");
+    }
+    hipLaunchKernelGGL(linear_pack_kernel<T>, dim3(static_cast<uint32_t>(n)), dim3(kPackThreads), 0, st, w);
+    return check_launch("linear_pack_kernel");
+  };
+  if (int rc = pack(a.hidden, a.ld_hidden, p.rows, true, ws + p.hidden, p.rows * p.k, to_weight ? ws + p.hidden_turned : nullptr, p.rows, a.dim * p.rows)) return rc;
 
   GemmArgs g{};
   g.y = Operand{ws + p.hidden, p.k, p.rows * p.k, static_cast<int32_t>(p.rows)};
   g.n = static_cast<int32_t>(p.rows);
-  g.steps = static_cast<int32_t>(p.k / kTileK);
+  g.steps = static_cast<int32_t>(p.k / kStep<T>);
   g.count = r.count;
   g.vocab = a.vocab;
   g.c = r.c;
@@ -610,31 +816,28 @@ int run_typed(const ppo_linear_loss_args& a, const Plan& p, char* ws, hipStream_
   g.row_m = r.row_m, g.row_inv_s = r.row_inv_s;
   g.denom = static_cast<float>(a.denom);
   g.inv_temp = static_cast<float>(1.0 / a.temperature);
-  auto weight_piece = [&](int64_t v0, int64_t n) -> int {
+  g.kept = p.keep ? reinterpret_cast<float*>(ws + p.kept) : nullptr;
+  g.ld_kept = p.piece;
+  // A piece of the weight as an operand, and turned for d_hidden; `packed`: the operand is there.
+  auto weight_piece = [&](int64_t v0, int64_t n, bool turn, bool packed) -> int {
     const char* from = static_cast<const char*>(a.weight) + v0 * a.ld_weight * size;
     g.m = static_cast<int32_t>(n);
     g.column0 = v0;
-    if (p.direct) {
-      g.x = Operand{from, a.ld_weight, 0, static_cast<int32_t>(n)};
-      return PPO_OK;
-    }
-    const PackArgs w{from, a.ld_weight, n, a.dim, nullptr, nullptr, ws + p.weight, p.k, p.piece * p.k, n};
-    hipLaunchKernelGGL(linear_pack_kernel<T>, dim3(static_cast<uint32_t>(n)), dim3(kPackThreads), 0, st, w);
-    g.x = Operand{ws + p.weight, p.k, p.piece * p.k, static_cast<int32_t>(n)};
-    return check_launch("linear_pack_kernel");
+    if (p.direct) g.x = Operand{from, a.ld_weight, 0, static_cast<int32_t>(n)};
+    else g.x = Operand{ws + p.weight, p.k, p.piece * p.k, static_cast<int32_t>(n)};
+    void* to = p.direct || packed ? nullptr : ws + p.weight;
+    if (to == nullptr && !turn) return PPO_OK;
+    return pack(from, a.ld_weight, n, false, to, p.piece * p.k, turn ? ws + p.weight_turned : nullptr, p.piece, a.dim * p.piece);
   };
+  const bool once = p.pieces == 1;  // then the copies that the sums need serve the gradients too
   for (int64_t v0 = 0; v0 < a.vocab && a.rows > 0; v0 += p.piece) {
-    if (int rc = weight_piece(v0, std::min(p.piece, a.vocab - v0))) return rc;
+    if (int rc = weight_piece(v0, std::min(p.piece, a.vocab - v0), once && to_hidden, false)) return rc;
     g.tile0 = v0 / kTileM;
     if (int rc = launch_gemm<T, kSums>(g, p.n_tile, st)) return rc;
   }
   if (a.rows > 0) {
-    hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<uint32_t>(ceil_div(a.rows, kJoinThreads / kWave))), dim3(kJoinThreads), 0, st, r);
+    hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<uint32_t>(ceil_div(a.rows, kJoinRows))), dim3(kJoinThreads), 0, st, r);
     if (int rc = check_launch("linear_join_kernel")) return rc;
-    if (a.logp != nullptr || a.entropy != nullptr) {
-      hipLaunchKernelGGL(linear_scatter_kernel, dim3(static_cast<uint32_t>(ceil_div(a.rows, kJoinThreads))), dim3(kJoinThreads), 0, st, r);
-      if (int rc = check_launch("linear_scatter_kernel")) return rc;
-    }
   }
   if (!gradient) return PPO_OK;
   hipLaunchKernelGGL(linear_stats_kernel, dim3(1), dim3(kRowThreads), 0, st, r);
@@ -643,32 +846,27 @@ int run_typed(const ppo_linear_loss_args& a, const Plan& p, char* ws, hipStream_
 
   for (int64_t v0 = 0; v0 < a.vocab; v0 += p.piece) {
     const int64_t n = std::min(p.piece, a.vocab - v0);
-    if (p.pieces > 1 || v0 == 0) {
-      if (p.pieces > 1 || p.direct) {
-        if (int rc = weight_piece(v0, n)) return rc;
-      }
-    }
+    if (a.rows > 0 && !once)
+      if (int rc = weight_piece(v0, n, to_hidden, false)) return rc;
     const Operand hidden = g.y, weight = g.x;
     g.d = to_hidden ? ws + p.d : nullptr;
     g.d_turned = to_weight ? ws + p.d_turned : nullptr;
     g.ld_d = p.piece, g.d_part = p.rows * p.piece;
     g.ld_t = p.rows, g.t_part = p.piece * p.rows;
-    if (a.rows > 0)
+    if (a.rows > 0 && p.keep) {
+      hipLaunchKernelGGL(linear_diffs_kernel<T>, dim3(static_cast<uint32_t>(up(n, kTileK) / 64), static_cast<uint32_t>(p.rows / 64)), dim3(kPackThreads), 0, st, g);
+      if (int rc = check_launch("linear_diffs_kernel")) return rc;
+    } else if (a.rows > 0) {
       if (int rc = launch_gemm<T, kDiffs>(g, p.n_tile, st)) return rc;
+    }
     if (to_hidden && a.rows > 0) {
-      const PackArgs w{static_cast<const char*>(a.weight) + v0 * a.ld_weight * size, a.ld_weight, n, a.dim, nullptr, nullptr, ws + p.weight_turned, p.piece,
-                       a.dim * p.piece, 0};
-      hipLaunchKernelGGL(linear_turn_kernel<T>, dim3(static_cast<uint32_t>(ceil_div(n, 64)), static_cast<uint32_t>(ceil_div(a.dim, 64))), dim3(kPackThreads), 0, st,
-                         w);
-      if (int rc = check_launch("linear_turn_kernel")) return rc;
       GemmArgs b = g;
       b.x = Operand{ws + p.weight_turned, p.piece, a.dim * p.piece, static_cast<int32_t>(a.dim)};
       b.y = Operand{ws + p.d, p.piece, p.rows * p.piece, static_cast<int32_t>(p.rows)};
       b.m = static_cast<int32_t>(a.dim);
-      b.steps = static_cast<int32_t>(ceil_div(n, kTileK));
+      b.steps = static_cast<int32_t>(up(n, kTileK) / kStep<T>);
       b.partial = reinterpret_cast<float*>(ws + p.partial);
-      b.slice_size = r.slice_size;
-      b.slices = p.slices;
+      b.cus = p.cus, b.all_steps = r.all_steps;
       b.add = v0 > 0;
       if (int rc = launch_gemm<T, kRowGrad>(b, p.n_tile, st)) return rc;
     }

@@ -271,8 +271,15 @@ __global__ __launch_bounds__(kWave* kJoinWaves) void qk_rotary_join_kernel(const
   const int dim = q.a.head_dim, slots = per_head ? q.a.q_heads + q.a.kv_heads : 2, slot = blockIdx.y;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, i = blockIdx.x * kWave + lane;
   double sum = 0.0;
+  constexpr int AHEAD = 8;  // loads in flight
   if (i < dim)
-    for (int64_t r = wave; r < rows; r += kJoinWaves) sum += static_cast<double>(q.partial[(r * slots + slot) * dim + i]);
+    for (int64_t r = wave; r < rows; r += kJoinWaves * AHEAD) {
+      float x[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) x[u] = q.partial[(min(r + u * kJoinWaves, rows - 1) * slots + slot) * dim + i];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) sum += r + u * kJoinWaves < rows ? static_cast<double>(x[u]) : 0.0;
+    }
   part[wave][lane] = sum;
   __syncthreads();
   if (wave != 0 || i >= dim) return;
@@ -299,14 +306,16 @@ Plan plan_of(const ppo_qk_rotary_args& a, bool backward) {
   const int heads = a.q_heads + a.kv_heads, at_once = kThreads >> p.lanes_log2;
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
-  // tokens of a block: as many as share the sines, but blocks enough for the chip
+  // Tokens of a block: as many as share the sines, but blocks enough for the chip; going back, where a block takes a head's tokens at a time, as many
+  // as it has rows for at least (4,099 tokens of 8 heads of 80, a weight each: 4 tokens a block 40 us, 16 and a head a block 12).
   p.tile = std::min(kMaxTile, std::max(1, kTurns / std::max(1, half)));
   if (!backward) p.tile = std::min(p.tile, 16);
-  while (p.tile > 1 && ceil_div(a.tokens, p.tile) < 4 * cus) p.tile /= 2;
+  const int least = backward ? std::min(p.tile, at_once) : 1;
+  while (p.tile > least && ceil_div(a.tokens, p.tile) < 4 * cus) p.tile = std::max(least, p.tile / 2);
   p.tiles = ceil_div(a.tokens, p.tile);
   // heads of a block: all, unless that leaves the chip idle
   p.group = heads;
-  while (p.group > 1 && p.tiles * ceil_div(heads, p.group) < 2 * cus && (backward ? p.group > 1 : p.group * p.tile > at_once)) p.group = (p.group + 1) / 2;
+  while (p.group > 1 && p.tiles * ceil_div(heads, p.group) < 4 * cus && (backward || p.group * p.tile > at_once)) p.group = (p.group + 1) / 2;
   p.groups = ceil_div(heads, p.group);
   p.rows = a.weight_per_head != 0 ? p.tiles : p.tiles * p.groups;
   p.slots = a.weight_per_head != 0 ? heads : 2;
