@@ -7,6 +7,7 @@ kernels of ``libppo_hip.so`` (C ABI: ``include/ppo_hip.h``), loaded through ctyp
 from .models import EmpiricalNormalization, GaussianDistribution, MLPModel
 from .ppo import PPO, HipPPO
 from .storage import RolloutStorage
-from .tokens import AdamW, TokenEmbedding
+from .tokens import AdamW, DecayMixer, QkNormRotary, TokenEmbedding, decay_attention, linear_cross_entropy
 
-__all__ = ["PPO", "HipPPO", "MLPModel", "GaussianDistribution", "EmpiricalNormalization", "RolloutStorage", "TokenEmbedding", "AdamW"]
+__all__ = ["PPO", "HipPPO", "MLPModel", "GaussianDistribution", "EmpiricalNormalization", "RolloutStorage", "TokenEmbedding", "AdamW",
+           "QkNormRotary", "DecayMixer", "decay_attention", "linear_cross_entropy"]

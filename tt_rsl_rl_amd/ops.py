@@ -1241,15 +1241,14 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step,
 # ----------------------------------------------------------------------------------------------------------------------
 
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None, shape: tuple | None = None) -> tuple[int, int, int]:
-    """Address, token stride and head stride of a view [tokens, heads, elements] of unit element stride, of like's type."""
-    if like is not None and t.dtype != like.dtype:
-        raise ValueError(f"{name} must be {like.dtype}, got {t.dtype}")
-    if t.dim() != 3 or shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be [tokens, heads, elements]{'' if shape is None else f' {list(shape)}'}, got {list(t.shape)}")
+def _heads(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str, what: str) -> tuple[int, int, int]:
+    """Address, token stride and head stride of a view [tokens, heads, elements] of unit element stride.  (The message is made where it is
+    needed: a step of a few tokens takes less time than its checks.)"""
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name}: {what} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
     token, head, unit = t.stride()
-    if unit != 1 and t.shape[2] > 1:
-        raise ValueError(f"{name} must have unit element stride, got strides {t.stride()}")
+    if unit != 1 and shape[2] > 1:
+        raise ValueError(f"{name}: {what} must have unit element stride, got strides {t.stride()}")
     return t.data_ptr(), token, head
 
 
@@ -1263,31 +1262,30 @@ def rotary_frequencies(dim: int, base: float = 10000.0, device=None) -> torch.Te
     return base ** (torch.arange(0, dim, 2, dtype=torch.float64, device=device) / -dim)
 
 
-def _qk_of(name: str, q, k, q_weight, k_weight, positions, freqs, more: list) -> tuple:
-    """(device, packing of the arguments between the views and the sizes, of the sizes), checked."""
-    dev = _current_gpu(name, q, k, q_weight, k_weight, positions, freqs, *more)
-    elem = _element_type(q, f"{name}: q")
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError(f"{name}: q and k must be [tokens, heads, elements], got {list(q.shape)} and {list(k.shape)}")
-    tokens, q_heads, dim = q.shape
-    kv_heads = k.shape[1]
-    if k.shape[0] != tokens or k.shape[2] != dim:
-        raise ValueError(f"{name}: k must be [{tokens}, heads, {dim}], got {list(k.shape)}")
-    weight_type = _element_type(q_weight, f"{name}: q_weight")
-    if k_weight.dtype != q_weight.dtype or weight_type not in (elem, L.TYPE_F32):
+def _qk_of(name: str, q, k, q_weight, k_weight, positions, freqs) -> tuple:
+    """(shapes of q and k, packing of the arguments between the views and the sizes, of the sizes, whether weights are heads'), checked."""
+    of_q, of_k = q.shape, k.shape
+    if len(of_q) != 3 or len(of_k) != 3 or of_k[0] != of_q[0] or of_k[2] != of_q[2]:
+        raise ValueError(f"{name}: q and k must be [tokens, heads, elements] of the same tokens and elements, got {list(of_q)} and {list(of_k)}")
+    tokens, q_heads, dim = of_q
+    kv_heads = of_k[1]
+    elem, weight_type = ELEMENT_TYPES.get(q.dtype), ELEMENT_TYPES.get(q_weight.dtype)
+    if elem is None:
+        _element_type(q, f"{name}: q")
+    if k_weight.dtype is not q_weight.dtype or weight_type != elem and weight_type != L.TYPE_F32:
         raise ValueError(f"{name}: weights must both be {q.dtype} or float32, got {q_weight.dtype} and {k_weight.dtype}")
     per_head = q_weight.dim() == 2
-    for w, heads, what in ((q_weight, q_heads, "q_weight"), (k_weight, kv_heads, "k_weight")):
-        if tuple(w.shape) != ((heads, dim) if per_head else (dim,)) or not w.is_contiguous():
-            raise ValueError(f"{name}: {what} must be contiguous [{dim}] or (both weights) [{heads}, {dim}], got {list(w.shape)}")
-    if positions.numel() != tokens:
-        raise ValueError(f"{name}: {positions.numel()} positions for {tokens} tokens")
+    if (q_weight.shape != ((q_heads, dim) if per_head else (dim,)) or k_weight.shape != ((kv_heads, dim) if per_head else (dim,))
+            or not q_weight.is_contiguous() or not k_weight.is_contiguous()):
+        raise ValueError(f"{name}: q_weight and k_weight must be contiguous, both [{dim}], or [{q_heads}, {dim}] and [{kv_heads}, {dim}], got "
+                         f"{list(q_weight.shape)} and {list(k_weight.shape)}")
     position_type = TOKEN_TYPES.get(positions.dtype)
-    if position_type is None or not positions.is_contiguous():
-        raise ValueError(f"{name}: positions must be contiguous int64 or int32, got {positions.dtype}")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+    if position_type is None or positions.numel() != tokens or not positions.is_contiguous():
+        raise ValueError(f"{name}: positions must be contiguous int64 or int32 of {tokens} elements, got {positions.dtype} {list(positions.shape)}")
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise ValueError(f"{name}: freqs must be contiguous float64 [rotary_dim / 2], got {freqs.dtype} {list(freqs.shape)}")
-    return dev, (positions.data_ptr(), freqs.data_ptr(), tokens), (q_heads, kv_heads, dim, 2 * freqs.numel(), elem, weight_type, position_type), per_head
+    return (of_q, of_k, (positions.data_ptr(), freqs.data_ptr(), tokens),
+            (q_heads, kv_heads, dim, 2 * freqs.numel(), elem, weight_type, position_type), per_head)
 
 
 def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
@@ -1298,10 +1296,12 @@ def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     (i, i + n) of n pairs, or (2i, 2i + 1) with interleaved.  q_out / k_out: like q / k; may be q / k themselves.  dim is even, up to
     512."""
     name = "qk_norm_rotary_fwd"
-    dev, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs, [q_out, k_out])
-    args = L.QK_ROTARY_ARGS.pack(*_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(q_out, f"{name}: q_out", q, tuple(q.shape)),
-                                 *_heads(k_out, f"{name}: k_out", q, tuple(k.shape)), *_NO_VIEW, *_NO_VIEW, q_weight.data_ptr(),
-                                 k_weight.data_ptr(), 0, 0, *middle, eps, *sizes, bool(interleaved), per_head, 0)
+    dev = _current_gpu(name, q, k, q_weight, k_weight, positions, freqs, q_out, k_out)
+    of_q, of_k, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs)
+    t = q.dtype
+    args = L.QK_ROTARY_ARGS.pack(*_heads(q, t, of_q, name, "q"), *_heads(k, t, of_k, name, "k"), *_heads(q_out, t, of_q, name, "q_out"),
+                                 *_heads(k_out, t, of_k, name, "k_out"), 0, 0, 0, 0, 0, 0, q_weight.data_ptr(), k_weight.data_ptr(), 0, 0, *middle, eps,
+                                 *sizes, bool(interleaved), per_head, 0)
     L.call("ppo_qk_rotary_fwd", args, _raw_stream(dev))
     _written(q_out, k_out)
 
@@ -1313,34 +1313,35 @@ def qk_norm_rotary_bwd(d_q_out: torch.Tensor, d_k_out: torch.Tensor, q: torch.Te
     """The gradients of qk_norm_rotary_fwd's inputs from those of its outputs: d_q / d_k like q / k (may be d_q_out or q themselves, d_k_out
     or k), d_q_weight / d_k_weight like the weights.  The weights' sums go in a fixed order: the same call gives the same bits."""
     name = "qk_norm_rotary_bwd"
-    dev, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs,
-                                          [d_q_out, d_k_out, d_q, d_k, d_q_weight, d_k_weight])
+    dev = _current_gpu(name, q, k, q_weight, k_weight, positions, freqs, d_q_out, d_k_out, d_q, d_k, d_q_weight, d_k_weight)
+    of_q, of_k, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs)
     for d, w, what in ((d_q_weight, q_weight, "d_q_weight"), (d_k_weight, k_weight, "d_k_weight")):
         if d.dtype != w.dtype or d.shape != w.shape or not d.is_contiguous():
             raise ValueError(f"{name}: {what} must be contiguous {w.dtype} {list(w.shape)}, got {d.dtype} {list(d.shape)}")
-    of_q, of_k = tuple(q.shape), tuple(k.shape)
-    args = L.QK_ROTARY_ARGS.pack(*_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(d_q_out, f"{name}: d_q_out", q, of_q),
-                                 *_heads(d_k_out, f"{name}: d_k_out", q, of_k), *_heads(d_q, f"{name}: d_q", q, of_q),
-                                 *_heads(d_k, f"{name}: d_k", q, of_k), q_weight.data_ptr(), k_weight.data_ptr(), d_q_weight.data_ptr(),
-                                 d_k_weight.data_ptr(), *middle, eps, *sizes, bool(interleaved), per_head, 0)
+    t = q.dtype
+    args = L.QK_ROTARY_ARGS.pack(*_heads(q, t, of_q, name, "q"), *_heads(k, t, of_k, name, "k"), *_heads(d_q_out, t, of_q, name, "d_q_out"),
+                                 *_heads(d_k_out, t, of_k, name, "d_k_out"), *_heads(d_q, t, of_q, name, "d_q"), *_heads(d_k, t, of_k, name, "d_k"),
+                                 q_weight.data_ptr(), k_weight.data_ptr(), d_q_weight.data_ptr(), d_k_weight.data_ptr(), *middle, eps, *sizes,
+                                 bool(interleaved), per_head, 0)
     buf = _scratch(ws, q.device, L.load().ppo_qk_rotary_bwd_workspace_bytes(args))
     L.call("ppo_qk_rotary_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
     _written(d_q, d_k, d_q_weight, d_k_weight)
 
 
-def _decay_of(name: str, q, k, v, out, log_decay) -> tuple[int, int, int, int, int, int]:
-    """(tokens, q_heads, kv_heads, key_dim, value_dim, element type), checked."""
-    elem = _element_type(q, f"{name}: q")
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
-        raise ValueError(f"{name}: q, k and v must be [tokens, heads, elements], got {list(q.shape)}, {list(k.shape)} and {list(v.shape)}")
-    tokens, q_heads, key_dim = q.shape
-    kv_heads, value_dim = v.shape[1:]
-    if tuple(k.shape) != (tokens, kv_heads, key_dim) or v.shape[0] != tokens or kv_heads == 0 or q_heads % kv_heads:
-        raise ValueError(f"{name}: k and v must be [{tokens}, heads, {key_dim}] and [{tokens}, heads, elements] with heads that divide {q_heads}, "
-                         f"got {list(k.shape)} and {list(v.shape)}")
-    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (kv_heads,) or not log_decay.is_contiguous():
-        raise ValueError(f"{name}: log_decay must be contiguous float32 [{kv_heads}], got {log_decay.dtype} {list(log_decay.shape)}")
-    return tokens, q_heads, kv_heads, key_dim, value_dim, elem
+def _decay_of(name: str, q, k, v, out, what: str, log_decay) -> tuple:
+    """(q's, k's and v's shapes and element type, packing of the four views), checked."""
+    of_q, of_k, of_v, t = q.shape, k.shape, v.shape, q.dtype
+    if len(of_q) != 3 or len(of_v) != 3 or of_v[0] != of_q[0] or of_k != (of_q[0], of_v[1], of_q[2]) or of_v[1] == 0 or of_q[1] % of_v[1]:
+        raise ValueError(f"{name}: q, k and v must be [tokens, heads, elements], with k's elements q's and k's and v's heads, which divide q's, the same, got "
+                         f"{list(of_q)}, {list(of_k)} and {list(of_v)}")
+    elem = ELEMENT_TYPES.get(t)
+    if elem is None:
+        _element_type(q, f"{name}: q")
+    if log_decay.dtype is not torch.float32 or log_decay.shape != of_v[1:2] or not log_decay.is_contiguous():
+        raise ValueError(f"{name}: log_decay must be contiguous float32 [{of_v[1]}], got {log_decay.dtype} {list(log_decay.shape)}")
+    views = (*_heads(q, t, of_q, name, "q"), *_heads(k, t, of_k, name, "k"), *_heads(v, t, of_v, name, "v"),
+             *_heads(out, t, (of_q[0], of_q[1], of_v[2]), name, what))
+    return of_q, of_k, of_v, elem, views
 
 
 def _sequences_of(name: str, cu_seqlens: torch.Tensor | None) -> tuple[int, int, int]:
@@ -1373,14 +1374,12 @@ def decay_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
     or value is not finite makes NaN of its heads' results from there to its sequence's end, and of no others."""
     name = "decay_attention_fwd"
     dev = _current_gpu(name, q, k, v, log_decay, out, cu_seqlens, initial_state, final_state)
-    tokens, q_heads, kv_heads, key_dim, value_dim, elem = _decay_of(name, q, k, v, out, log_decay)
+    of_q, of_k, of_v, elem, views = _decay_of(name, q, k, v, out, "out", log_decay)
     sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
-    shape = (sequences, kv_heads, key_dim, value_dim)
+    shape = (sequences, of_v[1], of_q[2], of_v[2])
     args = L.DECAY_ATTENTION_ARGS.pack(
-        *_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(v, f"{name}: v", q),
-        *_heads(out, f"{name}: out", q, (tokens, q_heads, value_dim)), *_NO_VIEW, *_NO_VIEW, *_NO_VIEW, log_decay.data_ptr(), cu,
-        _state(initial_state, f"{name}: initial_state", shape), _state(final_state, f"{name}: final_state", shape), 0, 0, tokens, sequences, scale,
-        q_heads, kv_heads, key_dim, value_dim, elem, cu_type)
+        *views, *_NO_VIEW, *_NO_VIEW, *_NO_VIEW, log_decay.data_ptr(), cu, _state(initial_state, f"{name}: initial_state", shape),
+        _state(final_state, f"{name}: final_state", shape), 0, 0, of_q[0], sequences, scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
     buf = _scratch(ws, q.device, L.load().ppo_decay_attention_workspace_bytes(args, 0))
     L.call("ppo_decay_attention_fwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
     _written(out, final_state)
@@ -1394,15 +1393,13 @@ def decay_attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     constant.  d_initial_state may be d_final_state."""
     name = "decay_attention_bwd"
     dev = _current_gpu(name, q, k, v, log_decay, d_out, d_q, d_k, d_v, cu_seqlens, initial_state, d_final_state, d_initial_state)
-    tokens, q_heads, kv_heads, key_dim, value_dim, elem = _decay_of(name, q, k, v, d_out, log_decay)
+    of_q, of_k, of_v, elem, views = _decay_of(name, q, k, v, d_out, "d_out", log_decay)
     sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
-    shape = (sequences, kv_heads, key_dim, value_dim)
+    shape, t = (sequences, of_v[1], of_q[2], of_v[2]), q.dtype
     args = L.DECAY_ATTENTION_ARGS.pack(
-        *_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(v, f"{name}: v", q),
-        *_heads(d_out, f"{name}: d_out", q, (tokens, q_heads, value_dim)), *_heads(d_q, f"{name}: d_q", q, tuple(q.shape)),
-        *_heads(d_k, f"{name}: d_k", q, tuple(k.shape)), *_heads(d_v, f"{name}: d_v", q, tuple(v.shape)), log_decay.data_ptr(), cu,
+        *views, *_heads(d_q, t, of_q, name, "d_q"), *_heads(d_k, t, of_k, name, "d_k"), *_heads(d_v, t, of_v, name, "d_v"), log_decay.data_ptr(), cu,
         _state(initial_state, f"{name}: initial_state", shape), 0, _state(d_final_state, f"{name}: d_final_state", shape),
-        _state(d_initial_state, f"{name}: d_initial_state", shape), tokens, sequences, scale, q_heads, kv_heads, key_dim, value_dim, elem, cu_type)
+        _state(d_initial_state, f"{name}: d_initial_state", shape), of_q[0], sequences, scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
     buf = _scratch(ws, q.device, L.load().ppo_decay_attention_workspace_bytes(args, 1))
     L.call("ppo_decay_attention_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
     _written(d_q, d_k, d_v, d_initial_state)
@@ -1416,9 +1413,10 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     sequence begins with this token, whatever its state held."""
     name = "decay_attention_step"
     dev = _current_gpu(name, q, k, v, log_decay, state, out, slots, fresh)
-    rows, q_heads, kv_heads, key_dim, value_dim, elem = _decay_of(name, q, k, v, out, log_decay)
-    if state.dim() != 4:
-        raise ValueError(f"{name}: state must be [slots, {kv_heads}, {key_dim}, {value_dim}], got {list(state.shape)}")
+    of_q, _, of_v, elem, views = _decay_of(name, q, k, v, out, "out", log_decay)
+    rows, of_state = of_q[0], state.shape
+    if state.dtype is not torch.float32 or len(of_state) != 4 or of_state[1:] != (of_v[1], of_q[2], of_v[2]) or not state.is_contiguous():
+        raise ValueError(f"{name}: state must be contiguous float32 [slots, {of_v[1]}, {of_q[2]}, {of_v[2]}], got {state.dtype} {list(of_state)}")
     at, slot_type = 0, L.TOKENS_I32
     if slots is not None:
         slot_type = TOKEN_TYPES.get(slots.dtype)
@@ -1430,11 +1428,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
         if fresh.dtype not in (torch.bool, torch.uint8) or fresh.numel() != rows or not fresh.is_contiguous():
             raise ValueError(f"{name}: fresh must be contiguous bool or uint8 of {rows} elements, got {fresh.dtype} {list(fresh.shape)}")
         begins = fresh.data_ptr()
-    args = L.DECAY_STEP_ARGS.pack(
-        *_heads(q, f"{name}: q"), *_heads(k, f"{name}: k", q), *_heads(v, f"{name}: v", q),
-        *_heads(out, f"{name}: out", q, (rows, q_heads, value_dim)), log_decay.data_ptr(),
-        _state(state, f"{name}: state", (state.shape[0], kv_heads, key_dim, value_dim)), at, begins, rows, state.shape[0], scale, q_heads, kv_heads,
-        key_dim, value_dim, elem, slot_type)
+    args = L.DECAY_STEP_ARGS.pack(*views, log_decay.data_ptr(), state.data_ptr(), at, begins, rows, of_state[0], scale, of_q[1], of_v[1], of_q[2], of_v[2],
+                                  elem, slot_type)
     L.call("ppo_decay_attention_step", args, _raw_stream(dev))
     _written(state, out)
 

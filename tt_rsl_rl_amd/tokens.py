@@ -1,6 +1,8 @@
 """What a policy that acts in tokens is built from, beside torch's own layers: an embedding whose gradient is summed by sorted
-tokens, and AdamW over many tensors with fp32 masters and, if wanted, 8-bit states.  The loss is ``ops.token_ppo_loss``, which
-writes the logits' gradient itself: ``logits.backward(d_logits)`` goes on from there (examples/token_policy.py).
+tokens, a layer that mixes a sequence's tokens (normed and turned queries and keys, linear attention whose past fades), the cross
+entropy of a head without its logits, and AdamW over many tensors with fp32 masters and, if wanted, 8-bit states.  The policy's loss
+is ``ops.token_ppo_loss``, which writes the logits' gradient itself: ``logits.backward(d_logits)`` goes on from there
+(examples/token_policy.py; examples/sequence_policy.py is taught by demonstrations first).
 
 Everything runs in the HIP kernels of ``libppo_hip.so`` on the tensors' GPU; there is no CPU path.
 """
@@ -47,6 +49,162 @@ class TokenEmbedding(nn.Module):
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         return _Lookup.apply(tokens.contiguous(), self.weight, self.scale)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A gradient as the operators take it: of unit stride in its last dimension (one that is a broadcast scalar is not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, freqs, eps: float, interleaved: bool):
+        out = q.new_empty(q.shape), k.new_empty(k.shape)
+        ops.qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, freqs, *out, eps=eps, interleaved=interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, freqs)
+        ctx.options = eps, interleaved
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_q_out, d_k_out):
+        q, k, q_weight, k_weight, positions, freqs = ctx.saved_tensors
+        eps, interleaved = ctx.options
+        grads = q.new_empty(q.shape), k.new_empty(k.shape), torch.empty_like(q_weight), torch.empty_like(k_weight)
+        ops.qk_norm_rotary_bwd(_rows(d_q_out), _rows(d_k_out), q, k, q_weight, k_weight, positions, freqs, *grads, eps=eps, interleaved=interleaved)
+        return *grads, None, None, None, None
+
+
+class QkNormRotary(nn.Module):
+    """``ops.qk_norm_rotary_fwd`` with its gradient and weights: queries [tokens, heads, dim] and keys [tokens, kv_heads, dim] of each head
+    over their root mean square, times a weight of dim elements, turned by their token's position.  rotary: how many of a head's elements
+    are turned (all)."""
+
+    def __init__(self, dim: int, rotary: int | None = None, base: float = 10000.0, eps: float = 1e-6, interleaved: bool = False, device=None,
+                 dtype=None) -> None:
+        super().__init__()
+        self.rotary, self.base, self.eps, self.interleaved = dim if rotary is None else rotary, base, eps, interleaved
+        self.q_weight = nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+        self.k_weight = nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+        # not a buffer: angles stay float64 whatever the module is cast to
+        self._freqs = ops.rotary_frequencies(self.rotary, base, device=self.q_weight.device)
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        if self._freqs.device != q.device:
+            self._freqs = ops.rotary_frequencies(self.rotary, self.base, device=q.device)
+        return _QkNormRotary.apply(q, k, self.q_weight, self.k_weight, positions, self._freqs, self.eps, self.interleaved)
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale: float, cu_seqlens, initial_state, want_state: bool):
+        out = q.new_empty(*q.shape[:2], v.shape[2])
+        sequences = 1 if cu_seqlens is None else cu_seqlens.numel() - 1
+        final = q.new_empty(sequences, k.shape[1], k.shape[2], v.shape[2], dtype=torch.float32) if want_state else None
+        ops.decay_attention_fwd(q, k, v, log_decay, out, scale=scale, cu_seqlens=cu_seqlens, initial_state=initial_state, final_state=final)
+        ctx.save_for_backward(q, k, v, log_decay, cu_seqlens, initial_state)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_final):
+        q, k, v, log_decay, cu_seqlens, initial_state = ctx.saved_tensors
+        if d_out is None:
+            d_out = q.new_zeros(*q.shape[:2], v.shape[2])
+        grads = q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)  # (tokens of no sequence stay 0)
+        d_initial = torch.empty_like(initial_state) if initial_state is not None and ctx.needs_input_grad[6] else None
+        ops.decay_attention_bwd(_rows(d_out), q, k, v, log_decay, *grads, scale=ctx.scale, cu_seqlens=cu_seqlens, initial_state=initial_state,
+                                d_final_state=None if d_final is None else d_final.contiguous(), d_initial_state=d_initial)
+        return *grads, None, None, None, d_initial, None
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float = 1.0,
+                    cu_seqlens: torch.Tensor | None = None, initial_state: torch.Tensor | None = None,
+                    want_state: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``ops.decay_attention_fwd`` with its gradient: the output, and the state that each sequence ends with (None unless wanted).
+    log_decay is a constant; tokens of no sequence (cu_seqlens) get an output that means nothing and no gradient."""
+    if log_decay.requires_grad:
+        raise ValueError("decay_attention: log_decay is a constant, it gets no gradient")
+    return _DecayAttention.apply(q, k, v, log_decay, float(scale), cu_seqlens, initial_state, want_state)
+
+
+class DecayMixer(nn.Module):
+    """A layer that mixes the tokens of each sequence: queries, keys and values of one projection, queries and keys normed and turned, linear
+    attention whose past fades, head h's by 1 - 2^-reach[h] a token, and a projection back.  Sequences lie one after another
+    (cu_seqlens); ``forward`` takes them whole (prompts, training), ``step`` one token of each on the states that ``new_state`` makes
+    and ``forward`` returns."""
+
+    def __init__(self, dim: int, heads: int, kv_heads: int | None = None, head_dim: int = 64, rotary: int | None = None, base: float = 10000.0,
+                 reach: tuple[float, float] = (3.0, 9.0), device=None, dtype=None) -> None:
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"DecayMixer: heads={heads} kv_heads={kv_heads}")
+        self.heads, self.kv_heads, self.head_dim, self.scale = heads, kv_heads, head_dim, head_dim**-0.5
+        self.project = nn.Linear(dim, (heads + 2 * kv_heads) * head_dim, bias=False, device=device, dtype=dtype)
+        self.turn = QkNormRotary(head_dim, rotary, base, device=device, dtype=dtype)
+        self.back = nn.Linear(heads * head_dim, dim, bias=False, device=device, dtype=dtype)
+        # not a buffer: it stays float32 whatever the module is cast to
+        self._log_decay = torch.log1p(-torch.exp2(-torch.linspace(*reach, kv_heads, dtype=torch.float64))).float().to(self.back.weight.device)
+
+    @property
+    def log_decay(self) -> torch.Tensor:
+        if self._log_decay.device != self.back.weight.device:
+            self._log_decay = self._log_decay.to(self.back.weight.device)
+        return self._log_decay
+
+    def new_state(self, sequences: int) -> torch.Tensor:
+        return torch.zeros(sequences, self.kv_heads, self.head_dim, self.head_dim, device=self.back.weight.device)
+
+    def _heads(self, x: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        q, k, v = self.project(x).unflatten(-1, (-1, self.head_dim)).split((self.heads, self.kv_heads, self.kv_heads), dim=1)
+        return *self.turn(q, k, positions), v
+
+    def forward(self, x: torch.Tensor, positions: torch.Tensor, cu_seqlens: torch.Tensor | None = None, state: torch.Tensor | None = None,
+                want_state: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """x [tokens, dim] and its tokens' positions -> ([tokens, dim], states or None)."""
+        q, k, v = self._heads(x, positions)
+        out, state = decay_attention(q, k, v, self.log_decay, self.scale, cu_seqlens, state, want_state)
+        return self.back(out.flatten(1)), state
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, positions: torch.Tensor, state: torch.Tensor, slots: torch.Tensor | None = None,
+             fresh: torch.Tensor | None = None) -> torch.Tensor:
+        """One token of each sequence, x [rows, dim], on state[slots] in place (ops.decay_attention_step)."""
+        q, k, v = self._heads(x, positions)
+        out = q.new_empty(q.shape)
+        ops.decay_attention_step(q, k, v, self.log_decay, state, out, scale=self.scale, slots=slots, fresh=fresh)
+        return self.back(out.flatten(1))
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, tokens, mask, temperature: float, denom):
+        d_hidden = hidden.new_empty(hidden.shape) if ctx.needs_input_grad[0] else None
+        d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        stats = torch.empty(4, device=hidden.device)
+        ops.linear_cross_entropy(hidden, weight, tokens, d_hidden, d_weight, stats, mask=mask, temperature=temperature, denom=denom)
+        ctx.save_for_backward(d_hidden, d_weight)
+        return stats[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_loss):
+        d_hidden, d_weight = ctx.saved_tensors
+        # (in float32: the loss' factor need not be one of the operands' type)
+        scaled = [None if d is None else (d.float() * d_loss).to(d.dtype) for d in (d_hidden, d_weight)]
+        return *scaled, None, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
+                         temperature: float = 1.0, denom: float | None = None) -> torch.Tensor:
+    """The mean cross entropy of tokens under softmax(hidden weight^T / temperature), hidden [..., dim], without the logits: a float32 scalar
+    whose gradients are made with it (``ops.linear_cross_entropy``)."""
+    hidden = hidden.reshape(-1, hidden.shape[-1])
+    mask = None if mask is None else mask.reshape(-1).contiguous()
+    return _LinearCrossEntropy.apply(_rows(hidden), weight, tokens.reshape(-1).contiguous(), mask, float(temperature), denom)
 
 
 class AdamW(torch.optim.Optimizer):
