@@ -235,6 +235,25 @@ def test_views(cuda, dtype):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_states_in_place_over_many_segments(cuda, dtype):
+    """The block that ends a sequence is another one than that which began it, and may be done first."""
+    ops = _ops()
+    s = _case(12, [5000, 0, 3000, 2500], 2, 1, 32, 24, dtype)
+    d = _to(s, cuda)
+    want, want_last = _forward(ops, d, 0.1)
+    wants = _backward(ops, d, 0.1)
+    for _ in range(5):
+        out, state = torch.empty_like(want), d["s0"].clone()
+        ops.decay_attention_fwd(d["q"], d["k"], d["v"], d["ld"], out, scale=0.1, cu_seqlens=d["cu"], initial_state=state, final_state=state)
+        assert torch.equal(out, want) and torch.equal(state, want_last)
+        outs, state = [torch.empty_like(d[x]) for x in ("q", "k", "v")], d["g1"].clone()
+        ops.decay_attention_bwd(d["g"], d["q"], d["k"], d["v"], d["ld"], *outs, scale=0.1, cu_seqlens=d["cu"], initial_state=d["s0"], d_final_state=state,
+                                d_initial_state=state)
+        for x, y in zip((*outs, state), wants):
+            assert torch.equal(x, y)
+
+
 def test_no_tokens(cuda):
     ops = _ops()
     s = _case(9, [0, 0], 2, 1, 8, 8, F32)

@@ -125,13 +125,17 @@ struct MixArgs {
   const Span* spans;    // of each token; NULL: one sequence
   const float* s_in;    // [sequences][heads][elements], element (b's dim i, c's dim j) at i * si + j * sj
   float* s_out;
-  float* carry;         // [segments - 1][heads][db][dc]: the state that leaves a segment, then what enters the next
+  float* carry;         // [segments - 1][heads][elements]: the state that leaves a segment, then what enters the next; element (i, j) at i * ci + j * cj
   int64_t si, sj, state_size;
+  int32_t ci, cj;
+  int32_t carried;      // carry holds what enters the segments already
+  int32_t exact;        // states come out, in fp32: three parts of what makes them
   int32_t tokens, segment, segments;
   int32_t heads, ga, gb;  // heads of b, c and S times gb; of a per head
   int32_t db, dc;
   int32_t reverse, w, cut;  // cut: chunks end with their sequence
   int32_t lost;             // states come in, which need not be finite
+  int32_t near;             // the outputs' rows too, and aligned to four bytes
   int32_t whole;            // rows are whole 16-byte pieces, not far apart
   float x, y, z;
 };
@@ -161,21 +165,21 @@ __global__ __launch_bounds__(kInfoThreads) void decay_spans_kernel(const void* c
   spans[t] = s;
 }
 
-// A sequence without tokens hands its state on.
-__global__ __launch_bounds__(256) void decay_empty_kernel(const void* cu, int cu_type, int tokens, const float* from, float* to, int64_t size) {
+// The states of sequences without tokens, or all of them.
+__global__ __launch_bounds__(256) void decay_hand_on_kernel(const void* cu, int cu_type, int tokens, const float* from, float* to, int64_t size, bool all) {
   const int64_t b = blockIdx.x;
   auto at = [&](int64_t i) {
     const int64_t v = cu_type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(cu)[i] : static_cast<int64_t>(static_cast<const int32_t*>(cu)[i]);
     return min(max(v, static_cast<int64_t>(0)), static_cast<int64_t>(tokens));
   };
   const bool empty = cu == nullptr ? tokens == 0 : at(b + 1) <= at(b);
-  if (!empty) return;
+  if (!empty && !all) return;
   for (int64_t i = threadIdx.x; i < size; i += 256) to[b * size + i] = from == nullptr ? 0.0f : from[b * size + i];
 }
 
 // carry[s] holds what segment s makes of nothing; afterwards what enters segment s + 1.
 __global__ __launch_bounds__(kScanThreads) void decay_scan_kernel(const MixArgs q) {
-  const int64_t size = static_cast<int64_t>(q.db) * q.dc, i = static_cast<int64_t>(blockIdx.x) * kScanThreads + threadIdx.x;
+  const int64_t size = q.state_size, i = static_cast<int64_t>(blockIdx.x) * kScanThreads + threadIdx.x;
   const int h = blockIdx.y;
   if (i >= size) return;
   const float ld = q.log_decay[h], whole = static_cast<float>(exp(static_cast<double>(ld) * q.segment));
@@ -284,9 +288,21 @@ __device__ __forceinline__ void put_turned(const RawPiece (&r)[4], M* turned, in
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 
+// A raw buffer of 2 GiB at a wave-uniform address.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0, 0x7fffffff, 0x00020000);
+}
+
 // All waves' LDS accesses are done.  (__syncthreads() would also wait for the loads and stores on their way to and from memory, which no other wave
 // of the block looks at.)
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Everything on its way from and to memory has arrived.  At the end of a branch that is rarely taken: where paths meet, the compiler otherwise waits, at the first use of
+// what one of them loaded, for everything that was issued since on any, the next item's rows among it (65,536 tokens x 16 heads of 128: 440 us so, 300
+// with these waits and stores that are always issued).
+__device__ __forceinline__ void wait_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 template <class T, class M, int DBT, int NT, bool STATE_ONLY>
 __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q) {
@@ -381,7 +397,8 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
   each_state([](float, int, int) { return 0.0f; });
   if (!STATE_ONLY && first[0][0] < seg_begin) {  // goes on from the segment before
     const float* from = q.carry + (static_cast<int64_t>(seg - 1) * q.heads + head) * q.db * q.dc;
-    each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[static_cast<int64_t>(i) * q.dc + j] : 0.0f; });
+    each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[i * q.ci + j * q.cj] : 0.0f; });
+    wait_memory();
     fresh = false;
   }
 
@@ -408,6 +425,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
       const float* from = q.s_in + (static_cast<int64_t>(seq) * q.heads + head) * q.state_size;
       if (fresh) each_state([](float, int, int) { return 0.0f; });
       else each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[i * q.si + j * q.sj] : 0.0f; });
+      wait_memory();
     }
     int thread = threadIdx.x;
     forget(thread);
@@ -461,6 +479,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
       sights[thread] = thread < n && from_first[i] == first0 ? q.y * fades[i + q.w] : 0.0f;
     }
     if (ahead) put_span(buffer ^ 1, c0 + C + threadIdx.x, next_span);
+    wait_memory();  // (the spans, as the compiler sees it, on the path that did not load them)
     lds_barrier();
     const bool poisoned = __builtin_amdgcn_readfirstlane(bad_any) != 0;
     if (poisoned) {  // zeros where a token is not finite
@@ -506,12 +525,12 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
 #pragma unroll
             for (int ks = 0; ks < DB / K; ++ks) m = X::mma(load_frag<M>(b_rows + Rows_::from(b_at, X::row_of(jt, 0), 4 * ks)), a[ks], m);
             const int j0 = X::row_of(jt, 4 * g);
+            float f[4];
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {  // (no branches: a wait for each fade would be one each)
-              const int j = j0 + r4;
-              const float f = q.x * fades[max(i - j, 0)];
-              v[4 * h + r4] = (j <= i) & (j >= lowest) ? m[r4] * f : 0.0f;
-            }
+            for (int r4 = 0; r4 < 4; ++r4) f[r4] = fades[max(i - j0 - r4, 0)];
+            asm volatile("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));  // (or else each is read in a branch, with a wait)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) v[4 * h + r4] = (j0 + r4 <= i) & (j0 + r4 >= lowest) ? m[r4] * (q.x * f[r4]) : 0.0f;
           }
           split<M, PARTS>(v, matrix[step]);
         }
@@ -597,29 +616,46 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
           const int ha = q.ga > 1 ? head * q.ga + ab : head, d = dc0 + 4 * NT * g;
           const int64_t lowest = q.reverse ? q.tokens - begin - n : begin;
           T* const to = static_cast<T*>(q.out.data) + ha * q.out.head_stride + lowest * q.out.token_stride;
+          if (q.near) {
+            // stores that are always issued: a row that is none goes past the buffer's end, where nothing is written
+            const auto buffer = buffer_at(to);
+            const uint32_t step = static_cast<uint32_t>(q.out.token_stride) * sizeof(T);
 #pragma unroll
-          for (int i = 0; i < IT; ++i) {
-            const int at = 16 * i + col;
-            if (valid >> at & 1) {
-              T* row = to + (static_cast<uint64_t>(static_cast<uint32_t>(q.reverse ? n - 1 - at : at)) * static_cast<uint32_t>(q.out.token_stride) + d);
-              typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-              typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-              if (NT == 2 && d + 8 <= q.dc) {
-                Eight o;
+            for (int i = 0; i < IT; ++i) {
+              const int at = 16 * i + col;
+              const uint32_t off = (valid >> at & 1) != 0 && d < q.dc ? __umul24(q.reverse ? n - 1 - at : at, step) + d * static_cast<uint32_t>(sizeof(T)) : 0x80000000u;
+              typedef uint32_t Words __attribute__((ext_vector_type(4)));
+              typedef T Piece16 __attribute__((ext_vector_type(16 / sizeof(T))));
+              constexpr int PER = 16 / static_cast<int>(sizeof(T));
+              if constexpr (4 * NT * sizeof(T) >= 16) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(acc[i][e / 4 * (NT - 1)][e % 4]);
-                *reinterpret_cast<Eight*>(row) = o;
-              } else if (NT == 1 && d + 4 <= q.dc) {
+                for (int e = 0; e < 4 * NT; e += PER) {
+                  Piece16 o;
+#pragma unroll
+                  for (int f = 0; f < PER; ++f) o[f] = static_cast<T>(acc[i][(e + f) / 4][(e + f) % 4]);
+                  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, o), buffer, off, e * static_cast<int>(sizeof(T)), 0);
+                }
+              } else {
+                typedef uint32_t Pair __attribute__((ext_vector_type(2)));
+                typedef T Four __attribute__((ext_vector_type(4)));
                 Four o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[i][0][e]);
-                *reinterpret_cast<Four*>(row) = o;
-              } else {
+                for (int f = 0; f < 4; ++f) o[f] = static_cast<T>(acc[i][0][f]);
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(Pair, o), buffer, off, 0, 0);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+              const int at = 16 * i + col;
+              if (valid >> at & 1) {
+                T* row = to + (static_cast<uint64_t>(static_cast<uint32_t>(q.reverse ? n - 1 - at : at)) * static_cast<uint32_t>(q.out.token_stride) + d);
 #pragma unroll
                 for (int e = 0; e < 4 * NT; ++e)
                   if (d + e < q.dc) row[e] = static_cast<T>(acc[i][e / 4][e % 4]);
               }
             }
+            wait_memory();
           }
         }
       }
@@ -653,8 +689,9 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
             const Frag b = load_frag<M>(b_turned + Cols_::from(bt_at, X::row_of(mb, 0), 4 * kj));
 #pragma unroll
             for (int k = 0; k < X::PARTS3; ++k)
+              if (k < 2 || q.exact)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) S[mb][nt] = X::mma(b, weighted[nt][k], S[mb][nt]);
+                for (int nt = 0; nt < NT; ++nt) S[mb][nt] = X::mma(b, weighted[nt][k], S[mb][nt]);
           }
         }
       }
@@ -683,7 +720,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
   if (STATE_ONLY && works) {
     float* to = q.carry + (static_cast<int64_t>(seg) * q.heads + head) * q.db * q.dc;
     each_state([&](float s, int i, int j) {
-      if (i < q.db && j < q.dc) to[static_cast<int64_t>(i) * q.dc + j] = s;
+      if (i < q.db && j < q.dc) to[i * q.ci + j * q.cj] = s;
       return s;
     });
   }
@@ -693,13 +730,13 @@ struct Plan {
   int segment, segments;
 };
 
-// Segments: as many as give the chip two blocks a compute unit, none shorter than four chunks (a segment costs its share of the first
-// pass, and its state is written and read four times).
+// Segments: as many as give the chip two blocks a compute unit (a segment's state is written and read four times), down to a chunk each: a block alone
+// on its compute unit takes 5 to 7 us a chunk, waiting (577 tokens of 3 heads, fp32: segments of four chunks 120 us, of one 61).
 Plan plan_of(int64_t tokens, int heads, int chunk) {
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
   const int64_t want = std::max<int64_t>(1, ceil_div(2 * cus, heads)), chunks = ceil_div(tokens, chunk);
-  const int64_t n = std::max<int64_t>(1, std::min(want, chunks / 4));
+  const int64_t n = std::max<int64_t>(1, std::min(want, chunks));
   Plan p;
   p.segment = static_cast<int>(ceil_div(std::max<int64_t>(chunks, 1), n) * chunk);
   p.segments = static_cast<int>(std::max<int64_t>(1, ceil_div(tokens, p.segment)));
@@ -709,7 +746,7 @@ Plan plan_of(int64_t tokens, int heads, int chunk) {
 template <class T, class M, int DBT, int NT>
 int launch_mix(const MixArgs& q, hipStream_t st) {
   const uint32_t heads = static_cast<uint32_t>(q.heads);
-  if (q.segments > 1) {
+  if (q.segments > 1 && q.carried == 0) {
     MixArgs own = q;
     own.ga = 1;  // (no outputs, so no a)
     hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, true>), dim3(static_cast<uint32_t>(q.segments - 1), heads), dim3(kThreads), 0, st, own);
@@ -730,7 +767,7 @@ int launch_type(const MixArgs& q, hipStream_t st) {
 }
 
 struct Layout {
-  size_t spans, carry, bytes;
+  size_t spans, carry, copy, bytes;  // copy 0: none needed
 };
 Layout layout_of(const ppo_decay_attention_args& a) {
   const int chunk = a.type == PPO_TYPE_BF16 ? Math<__bf16>::CHUNK : Math<float>::CHUNK;
@@ -738,7 +775,14 @@ Layout layout_of(const ppo_decay_attention_args& a) {
   Layout l;
   l.spans = 256;
   l.carry = l.spans + (a.cu_seqlens != nullptr ? static_cast<size_t>(ceil_div(a.tokens * sizeof(Span), 256)) * 256 : 0);
-  l.bytes = l.carry + static_cast<size_t>(p.segments - 1) * a.kv_heads * a.key_dim * a.value_dim * sizeof(float);
+  const size_t states = static_cast<size_t>(a.kv_heads) * a.key_dim * a.value_dim * sizeof(float);
+  l.bytes = l.carry + (p.segments - 1) * states;
+  l.copy = 0;
+  const bool in_place = (a.initial_state != nullptr && a.initial_state == a.final_state) || (a.d_final_state != nullptr && a.d_final_state == a.d_initial_state);
+  if (in_place && p.segments > 1) {
+    l.copy = static_cast<size_t>(ceil_div(l.bytes, 256)) * 256;
+    l.bytes = l.copy + a.sequences * states;
+  }
   return l;
 }
 
@@ -829,19 +873,29 @@ int prepare(const char* who, const ppo_decay_attention_args& a, void* workspace,
   return PPO_OK;
 }
 
-int hand_on(const ppo_decay_attention_args& a, const float* from, float* to, hipStream_t st) {
-  if (to == nullptr || from == to) return PPO_OK;
-  hipLaunchKernelGGL(decay_empty_kernel, dim3(static_cast<uint32_t>(a.sequences)), dim3(256), 0, st, a.cu_seqlens, a.cu_type, static_cast<int>(a.tokens), from,
-                     to, static_cast<int64_t>(a.kv_heads) * a.key_dim * a.value_dim);
-  return check_launch("decay_empty_kernel");
+// What no chunk does for the states: sequences without tokens hand theirs on, and states that are replaced in place are read from a copy, since the block
+// that ends a sequence need not be the one that began it.
+int hand_on(const ppo_decay_attention_args& a, const float*& from, float* to, void* workspace, hipStream_t st) {
+  if (to == nullptr) return PPO_OK;
+  const bool in_place = from == to;
+  if (in_place && layout_of(a).copy == 0) return PPO_OK;
+  float* const target = in_place ? reinterpret_cast<float*>(static_cast<char*>(workspace) + layout_of(a).copy) : to;
+  hipLaunchKernelGGL(decay_hand_on_kernel, dim3(static_cast<uint32_t>(a.sequences)), dim3(256), 0, st, a.cu_seqlens, a.cu_type, static_cast<int>(a.tokens), from,
+                     target, static_cast<int64_t>(a.kv_heads) * a.key_dim * a.value_dim, in_place);
+  if (in_place) from = target;
+  return check_launch("decay_hand_on_kernel");
 }
 
 int mix(const ppo_decay_attention_args& a, MixArgs q, hipStream_t st) {
   const int piece = 16 / type_size(a.type);
   q.lost = q.s_in != nullptr || q.segments > 1;
+  if (q.carried == 0) q.ci = q.dc, q.cj = 1;
+  else q.ci = 1, q.cj = q.db;  // as the pass before left it, turned over
   q.whole = a.key_dim % piece == 0 && a.value_dim % piece == 0;
   for (const ppo_head_view* v : {&q.a, &q.b, &q.c})  // (rows' offsets within a chunk are products of 24 bits)
     if (v->token_stride * type_size(a.type) >= 1 << 24) q.whole = 0;
+  const int64_t row = q.out.token_stride * type_size(a.type), in_row = q.out.head_stride * type_size(a.type);
+  q.near = q.whole != 0 && row < 1 << 24 && row % 4 == 0 && in_row % 4 == 0 && reinterpret_cast<uintptr_t>(q.out.data) % 4 == 0;
   int rc = PPO_OK;
   with_type(a.type, [&](auto t) { rc = launch_type<decltype(t)>(q, st); });
   return rc;
@@ -863,10 +917,11 @@ extern "C" int ppo_decay_attention_fwd(const ppo_decay_attention_args* args, voi
   hipStream_t st = static_cast<hipStream_t>(stream);
   MixArgs q;
   if (int rc = prepare(who, a, workspace, workspace_bytes, st, q)) return rc;
-  if (int rc = hand_on(a, a.initial_state, a.final_state, st)) return rc;
+  const float* from = a.initial_state;
+  if (int rc = hand_on(a, from, a.final_state, workspace, st)) return rc;
   if (a.tokens == 0) return PPO_OK;
   q.a = a.q, q.b = a.k, q.c = a.v, q.out = a.out;
-  q.s_in = a.initial_state, q.s_out = a.final_state, q.cut = a.initial_state != nullptr || a.final_state != nullptr;
+  q.s_in = from, q.s_out = a.final_state, q.cut = a.initial_state != nullptr || a.final_state != nullptr, q.exact = a.final_state != nullptr;
   q.db = a.key_dim, q.dc = a.value_dim, q.si = a.value_dim, q.sj = 1;
   q.ga = a.q_heads / a.kv_heads, q.gb = 1, q.w = 1;
   q.x = q.y = static_cast<float>(a.scale), q.z = 1.0f;
@@ -880,7 +935,8 @@ extern "C" int ppo_decay_attention_bwd(const ppo_decay_attention_args* args, voi
   hipStream_t st = static_cast<hipStream_t>(stream);
   MixArgs q;
   if (int rc = prepare(who, a, workspace, workspace_bytes, st, q)) return rc;
-  if (int rc = hand_on(a, a.d_final_state, a.d_initial_state, st)) return rc;
+  const float* from = a.d_final_state;
+  if (int rc = hand_on(a, from, a.d_initial_state, workspace, st)) return rc;
   if (a.tokens == 0) return PPO_OK;
   const int group = a.q_heads / a.kv_heads;
   // d_q: in order, S turned over
@@ -890,14 +946,15 @@ extern "C" int ppo_decay_attention_bwd(const ppo_decay_attention_args* args, voi
   q.ga = group, q.gb = 1, q.w = 1;
   q.x = q.y = static_cast<float>(a.scale), q.z = 1.0f;
   if (int rc = mix(a, q, st)) return rc;
-  // d_k, then d_v, which also hands on the state's gradient: in reverse
+  // d_k, then d_v, whose states are d_k's turned over and which hands on the state's gradient (last: it may lie where d_k's came from): in reverse
   q.reverse = 1, q.w = 0, q.ga = 1, q.gb = group;
   q.x = q.z = static_cast<float>(a.scale), q.y = 1.0f;
-  q.s_in = a.d_final_state, q.cut = a.d_final_state != nullptr || a.d_initial_state != nullptr;
+  q.s_in = from, q.cut = a.d_final_state != nullptr || a.d_initial_state != nullptr;
+  q.exact = a.d_initial_state != nullptr;
   q.a = a.v, q.b = a.out, q.c = a.q, q.out = a.d_k;
   if (int rc = mix(a, q, st)) return rc;
   q.a = a.k, q.b = a.q, q.c = a.out, q.out = a.d_v;
   q.db = a.key_dim, q.dc = a.value_dim, q.si = a.value_dim, q.sj = 1;
-  q.s_out = a.d_initial_state;
+  q.s_out = a.d_initial_state, q.carried = 1;
   return mix(a, q, st);
 }
