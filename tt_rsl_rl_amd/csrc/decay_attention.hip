@@ -684,15 +684,19 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
             for (int i = 0; i < 4 * Q; ++i) v[i] = w[i / 4][i % 4] * static_cast<float>(c[nt][kj][i]);
             split<M, X::PARTS3>(v, weighted[nt]);
           }
+          auto add = [&](auto parts_from, auto parts_to) {
 #pragma unroll
-          for (int mb = 0; mb < DBT; ++mb) {
-            const Frag b = load_frag<M>(b_turned + Cols_::from(bt_at, X::row_of(mb, 0), 4 * kj));
+            for (int mb = 0; mb < DBT; ++mb) {
+              const Frag b = load_frag<M>(b_turned + Cols_::from(bt_at, X::row_of(mb, 0), 4 * kj));
 #pragma unroll
-            for (int k = 0; k < X::PARTS3; ++k)
-              if (k < 2 || q.exact)
+              for (int k = parts_from; k < parts_to; ++k)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) S[mb][nt] = X::mma(b, weighted[nt][k], S[mb][nt]);
-          }
+            }
+          };
+          constexpr int two = X::PARTS3 < 2 ? X::PARTS3 : 2;
+          add(std::integral_constant<int, 0>{}, std::integral_constant<int, two>{});
+          if (two < X::PARTS3 && q.exact) add(std::integral_constant<int, two>{}, std::integral_constant<int, X::PARTS3>{});
         }
       }
     }
