@@ -858,7 +858,7 @@ int ppo_adamw_step(const ppo_adamw_tensor* tensors, int32_t count, double max_no
 /* ------------------------------------------------------------------------------------------------------------------
  * Between a token policy's embedding and its logits.  Tokens of all sequences lie one after another; a ppo_head_view is a
  * view [tokens, heads, elements] of unit element stride, the other strides in elements (columns of a projection's output, heads
- * before tokens: any of them; an input's may be 0).  Views of one call share its element type.
+ * before tokens: any of them; an input's may be 0, none may be negative).  Views of one call share its element type.
  * ------------------------------------------------------------------------------------------------------------------ */
 typedef struct ppo_head_view {
   void* data;
@@ -874,7 +874,7 @@ typedef struct ppo_head_view {
  * The backward pass takes the gradients of the results (q_out, k_out), turns them back (g) and gives
  *   d_weight = sum g n (over tokens, and heads where they share it);   d_x = (weight g - n mean(weight g n)) / sqrt(mean(x^2) + eps).
  * Sums over tokens are fp32 over up to some hundred rows and fp64 over those, in a fixed order: the same call gives the same bits.
- * D and R are even, D <= PPO_QK_MAX_DIM, 2 <= R <= D.  q_out and k_out (d_q and d_k) may be the very views that the call reads in
+ * D and R are even, D <= PPO_QK_MAX_DIM, 2 <= R <= D; tokens < 2^28.  q_out and k_out (d_q and d_k) may be the very views that the call reads in
  * their place (q and k; going back also q_out and k_out); no other output may lie on an input or another output. */
 #define PPO_QK_MAX_DIM 512
 typedef struct ppo_qk_rotary_args {
@@ -914,10 +914,12 @@ int ppo_qk_rotary_bwd(const ppo_qk_rotary_args* args, void* workspace, size_t wo
  * Backward, with R_t = f R_{t+1} + scale q_t d_out_t^T from d_final_state[b] (NULL: zeros) on:
  *   d_q_t = scale S_t d_out_t;   d_k_t = R_t v_t;   d_v_t = R_t^T k_t   (summed over the queries that share a head);
  *   d_initial_state[b] = f R_first (NULL: not wanted).
- * States, sums and the powers of f are fp32 or more.  Of 16-bit inputs the matrix cores' operands that the call makes itself (S,
- * R, the chunks' matrices) are held as sums of two 16-bit parts, those that make a state as three.  Everything is summed in a fixed
- * order.  key_dim, value_dim <= PPO_DECAY_MAX_DIM.  No output may lie on an input or another output, but d_initial_state may be
- * d_final_state and final_state may be initial_state. */
+ * States, sums and the powers of f are fp32 or more.  Of bf16 inputs the matrix cores' operands that the call makes itself (S, R,
+ * the chunks' matrices, weighted rows) are held as sums of two bf16 parts, where a state comes out its own as three; fp16 and fp32
+ * inputs go through fp32 products.  Everything is summed in a fixed order.  What sees a token with an infinity or NaN
+ * becomes infinite or NaN, nothing else does: other sequences, what lies before it (behind it, going back) and rows of no sequence.
+ * key_dim, value_dim <= PPO_DECAY_MAX_DIM; q_heads <= 65535; the outputs' token_stride < 2^31.  No output may lie on an input or
+ * another output, but d_initial_state may be d_final_state and final_state may be initial_state. */
 #define PPO_DECAY_MAX_DIM 128
 typedef struct ppo_decay_attention_args {
   ppo_head_view q, k, v;
@@ -965,12 +967,14 @@ int ppo_decay_attention_step(const ppo_decay_step_args* args, ppo_stream_t strea
  *   lp = z_t - log sum_j exp(z_j);   p_j = exp(z_j - log sum exp z);   H = -sum_j p_j log p_j;   loss = -sum_r lp / N;
  *   d_z[r, j] = (p_j - [j = t]) / (N temperature);   d_hidden = d_z weight;   d_weight = d_z^T hidden.
  * Rows count, and N is, as in ppo_token_ppo_loss; a row that does not count gives lp = H = 0 and d_hidden 0.  Rows whose hidden or
- * products are not finite give what the formulas give.  If no row counts, everything is 0.
+ * products are not finite give what the formulas give.  If no row counts, every result is 0 (but stats[2], which is N).
  * ppo_linear_log_probs writes logp and entropy (either may be NULL).  ppo_linear_cross_entropy writes also stats[4] = loss, mean H,
  * N, 0 and d_hidden and d_weight, of their operands' type (either may be NULL: not wanted); logp and entropy as before.
  * Products are exact in fp32 sums (fp32 operands as three bf16 parts, six products); d_z is rounded to the operands' type for the
- * second products (fp32: three parts again), once, before 1 / (N temperature) is applied.  Everything is summed in a fixed order.
- * The workspace holds a piece of d_z, some tens of thousands of columns at a time.  No output may lie on an input or another output. */
+ * second products (fp32: three parts again), once, before 1 / (N temperature) is applied (and times 2^14 in fp16).  Everything is
+ * summed in a fixed order.  The workspace holds d_z and copies of the weight for a piece of the columns, up to some 768 MB (or 2,048
+ * columns), d_hidden's fp32 sums and some 12 bytes for each row and 256 columns; fp32 products of up to 256 MB are kept too.
+ * rows < 2^22, dim <= 2^20, vocab < 2^30, ld_weight <= 2^21.  No output may lie on an input or another output. */
 typedef struct ppo_linear_loss_args {
   const void* hidden; /* [rows, dim] */
   int64_t ld_hidden;

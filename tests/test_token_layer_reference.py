@@ -310,3 +310,16 @@ def test_shapes_and_types_are_checked(monkeypatch):
         with pytest.raises(ValueError, match="linear_cross_entropy"):
             loss(**more)
     assert called == ["ppo_qk_rotary_fwd", "ppo_decay_attention_fwd", "ppo_decay_attention_step", "ppo_linear_cross_entropy"]
+
+
+def test_launches_hold_fewer_than_2_to_the_32_threads():
+    """Sizes whose launches would hold more are refused, or cut: a linear loss's pieces, which the workspace shows, shrink as its rows grow."""
+    from tt_rsl_rl_amd import _lib as L
+
+    for entry in ("ppo_qk_rotary_fwd", "ppo_qk_rotary_bwd"):
+        with pytest.raises(ValueError, match="tokens"):
+            _qk(entry, tokens=1 << 28)
+    rows, vocab, dim = (1 << 22) - 1, 1 << 29, 63  # 2^14 tiles of rows, so that 2^8 tiles of columns are 2^22 blocks
+    args = ctypes.byref(L.LinearLossArgs(hidden=M, ld_hidden=dim, weight=2 * M, ld_weight=dim, rows=rows, vocab=vocab, dim=dim, temperature=1.0, type=1))
+    sums, hidden = 3 * (vocab >> 8) * (rows + 1) * 4, (rows + 1) * 64 * 2
+    assert L.load().ppo_linear_loss_workspace_bytes(args, 0) <= sums + hidden + 40 * (rows + 1) + (1 << 16) * 64 * 2 + 8192

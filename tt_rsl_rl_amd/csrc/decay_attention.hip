@@ -11,12 +11,12 @@
 //
 // A block walks the chunks of a segment of tokens for one head of b and c (GA heads of a read them) or of a (GB heads of b and c are
 // summed).  S stays in its waves' accumulators, each wave owning columns of c; the accumulator layout (column lane % 16, rows
-// 4 (lane / 16) + 0..3) is that of an operand whose sum runs over those rows, in fours, so neither S nor the chunk's matrix passes
-// through LDS on its way into the next product.  Each wave makes the chunk's whole matrix for itself: that costs less than the
-// barrier and the LDS traffic of sharing it.  Operands that are sums themselves (S, the matrix, weighted c) go into bf16 products as 2, 2
-// and 3 parts of 8 bits each: S and the matrix then add 2^-17 to outputs that are rounded to 2^-9 anyway, and a state, which is
-// fp32, keeps 2^-24.  fp16 goes through the fp32 products: a state may leave fp16's range, and two bf16 parts of it would need
-// two of q as well.
+// 4 (lane / 16) + 0..3) is that of an operand whose sum runs over those rows, in fours, so S goes into the next product as it lies.  The
+// chunk's matrix is made once, its tiles shared out over the waves, and handed round through LDS, where b's rows were: made by each
+// wave for itself it took 632 us where this takes 468 (65,536 tokens, 16 heads of 128).  Operands that are sums themselves (S, the matrix,
+// weighted c) go into bf16 products as two parts of 8 bits each, which adds 2^-17 to outputs that are rounded to 2^-9 anyway; where a state
+// comes out, which is fp32, weighted c has a third part, for 2^-24.  fp16 goes through the fp32 products: a state may leave fp16's
+// range, and two bf16 parts of it would need two of q as well.
 // With few heads the sequence is cut into segments: a first pass makes each segment's own state, a scan carries them on, and the second pass
 // starts every segment from the state before it.
 //
@@ -24,6 +24,10 @@
 // sequences differ; where states come in or go out, chunks are cut at the sequences' ends too.
 // A token whose b or c is not finite would reach, as 0 * inf, tokens that do not see it: its row is taken as zeros, and NaN put into
 // what does see it.
+//
+// Bound by what a wave has to issue, at two waves a SIMD: a chunk's matrix products (two and three parts) take a third of the time, the rest goes to splitting
+// parts, to LDS and to its barriers.  65,536 tokens of 16 heads of 128 in bf16, states in and out (1.07 GB in and out, 0.2 ms at the copy's rate): 391 us for the
+// outputs, 175 for the segments' states, 15 for the scan.
 #include <type_traits>
 
 #include "views.hpp"
@@ -166,15 +170,16 @@ __global__ __launch_bounds__(kInfoThreads) void decay_spans_kernel(const void* c
 }
 
 // The states of sequences without tokens, or all of them.
-__global__ __launch_bounds__(256) void decay_hand_on_kernel(const void* cu, int cu_type, int tokens, const float* from, float* to, int64_t size, bool all) {
-  const int64_t b = blockIdx.x;
+__global__ __launch_bounds__(256) void decay_hand_on_kernel(const void* cu, int cu_type, int tokens, const float* from, float* to, int64_t size, int64_t sequences, bool all) {
   auto at = [&](int64_t i) {
     const int64_t v = cu_type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(cu)[i] : static_cast<int64_t>(static_cast<const int32_t*>(cu)[i]);
     return min(max(v, static_cast<int64_t>(0)), static_cast<int64_t>(tokens));
   };
-  const bool empty = cu == nullptr ? tokens == 0 : at(b + 1) <= at(b);
-  if (!empty && !all) return;
-  for (int64_t i = threadIdx.x; i < size; i += 256) to[b * size + i] = from == nullptr ? 0.0f : from[b * size + i];
+  for (int64_t b = blockIdx.x; b < sequences; b += gridDim.x) {
+    const bool empty = cu == nullptr ? tokens == 0 : at(b + 1) <= at(b);
+    if (!empty && !all) continue;
+    for (int64_t i = threadIdx.x; i < size; i += 256) to[b * size + i] = from == nullptr ? 0.0f : from[b * size + i];
+  }
 }
 
 // carry[s] holds what segment s makes of nothing; afterwards what enters segment s + 1.
@@ -300,7 +305,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Everything on its way from and to memory has arrived.  At the end of a branch that is rarely taken: where paths meet, the compiler otherwise waits, at the first use of
-// what one of them loaded, for everything that was issued since on any, the next item's rows among it (65,536 tokens x 16 heads of 128: 440 us so, 300
+// what one of them loaded, for everything that was issued since on any, the next item's rows among it (65,536 tokens of 16 heads of 128: 427 us so, 391
 // with these waits and stores that are always issued).
 __device__ __forceinline__ void wait_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
@@ -735,7 +740,7 @@ struct Plan {
 };
 
 // Segments: as many as give the chip two blocks a compute unit (a segment's state is written and read four times), down to a chunk each: a block alone
-// on its compute unit takes 5 to 7 us a chunk, waiting (577 tokens of 3 heads, fp32: segments of four chunks 120 us, of one 61).
+// on its compute unit takes 5 to 7 us a chunk, waiting (577 tokens of 3 heads, fp32, the whole call: segments of four chunks 120 us, of one 47).
 Plan plan_of(int64_t tokens, int heads, int chunk) {
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
@@ -884,8 +889,8 @@ int hand_on(const ppo_decay_attention_args& a, const float*& from, float* to, vo
   const bool in_place = from == to;
   if (in_place && layout_of(a).copy == 0) return PPO_OK;
   float* const target = in_place ? reinterpret_cast<float*>(static_cast<char*>(workspace) + layout_of(a).copy) : to;
-  hipLaunchKernelGGL(decay_hand_on_kernel, dim3(static_cast<uint32_t>(a.sequences)), dim3(256), 0, st, a.cu_seqlens, a.cu_type, static_cast<int>(a.tokens), from,
-                     target, static_cast<int64_t>(a.kv_heads) * a.key_dim * a.value_dim, in_place);
+  hipLaunchKernelGGL(decay_hand_on_kernel, dim3(static_cast<uint32_t>(std::min<int64_t>(a.sequences, 1 << 20))), dim3(256), 0, st, a.cu_seqlens, a.cu_type,
+                     static_cast<int>(a.tokens), from, target, static_cast<int64_t>(a.kv_heads) * a.key_dim * a.value_dim, a.sequences, in_place);
   if (in_place) from = target;
   return check_launch("decay_hand_on_kernel");
 }

@@ -15,6 +15,10 @@
 // straight to LDS, two to four deep.  In LDS a row's 16-byte pieces change places by the row's number, so that reading a column of pieces
 // meets all banks.  An accumulator lane holds one n and rows of m: with the vocabulary along m a row's sums stay in its lane but for one
 // shuffle and the waves' join.  fp32 operands are three bf16 parts, six products of which are taken (what is left out is 2^-24 and below).
+//
+// Bound by the matrix cores.  8,192 rows, of which 6,144 count, of 2,048 over 131,072 columns, bf16, for each 16,384 columns (412 GFLOP a product): sums 384 us,
+// differences 435, d_hidden 482, d_weight 335 (1,230 TFLOP/s, what a large library product reaches too), turning the weight 27.  The d_hidden's 192 tiles leave a
+// quarter of 256 compute units idle.
 #include <numeric>
 
 #include "elem.hpp"
@@ -33,6 +37,7 @@ constexpr int kMaxParts = 3;
 // A piece's columns: d in both layouts and the weight's copies take up to so much (a piece more costs a reading and a writing of d_hidden's sums).
 constexpr int64_t kPieceBytes = int64_t{3} << 28;
 constexpr int64_t kMinPiece = 2048;
+constexpr int64_t kMostTiles = int64_t{1} << 22;  // of a product: a launch holds fewer than 2^32 threads
 constexpr int64_t kKeptBytes = int64_t{1} << 28;
 
 // The operands' 16-bit type: bf16 for fp32's parts.
@@ -696,9 +701,12 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   p.direct = a.type != PPO_TYPE_F32 && a.dim % kTileK == 0 && a.ld_weight % 8 == 0 && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
   const int64_t column = 2 * p.parts * ((gradient ? (a.d_hidden != nullptr) + (a.d_weight != nullptr) : 0) * p.rows + (p.direct ? 0 : p.k) +
                                          (gradient && a.d_hidden != nullptr ? a.dim : 0));
+  p.n_tile = a.rows <= 32 ? 32 : a.type == PPO_TYPE_F32 || a.rows <= 128 || (a.rows > 256 && a.rows <= 384) ? 128 : 256;
   int64_t piece = kPieceBytes / std::max<int64_t>(column, 1) / kTileM * kTileM;
-  piece = std::min(std::max(piece, kMinPiece), int64_t{1} << 22);
+  piece = std::min(std::max(piece, kMinPiece), int64_t{1} << 21);  // (a tile of d's offsets stay in 31 bits)
   if (!gradient && p.direct) piece = up(a.vocab, kTileM);
+  piece = std::min(piece, kMostTiles / ceil_div(p.rows, p.n_tile) * kTileM);
+  if (gradient) piece = std::min(piece, kMostTiles / ceil_div(a.dim, kTileM) * 128);
   p.piece = std::min(piece, up(a.vocab, kTileM));
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
@@ -710,7 +718,6 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
     p.piece = p.piece >= round ? p.piece / round * round : up(ceil_div(a.vocab, p.pieces), kTileM);
     p.pieces = ceil_div(a.vocab, p.piece);
   }
-  p.n_tile = a.rows <= 32 ? 32 : a.type == PPO_TYPE_F32 || a.rows <= 128 || (a.rows > 256 && a.rows <= 384) ? 128 : 256;
   p.cus = static_cast<int>(cus);
   size_t at = 256;
   auto room = [&](size_t n) {
@@ -728,7 +735,7 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   p.hidden = room(p.parts * p.rows * p.k * 2);
   p.weight = room(p.direct ? 0 : p.parts * p.piece * p.k * 2);
   // fp32 products come six times as dear as 16-bit ones: where one piece holds the vocabulary and its products are small, they are kept for d instead of
-  // made again (257 rows of 515 over 50,021 columns: 183 us again, 62 from what was kept; bf16 products are made in the time that reading takes)
+  // made again (257 rows of 515 over 50,021 columns: 121 us again, 34 from what was kept; bf16 products are made in the time that reading takes)
   p.keep = gradient && a.type == PPO_TYPE_F32 && p.pieces == 1 && p.rows * p.piece * 4 <= kKeptBytes && (a.d_hidden != nullptr || a.d_weight != nullptr);
   p.kept = room(p.keep ? p.rows * p.piece * 4 : 0);
   if (gradient) {
