@@ -265,13 +265,16 @@ class LinearLossArgs(C.Structure):
 # the same packed by hand, a third of the time of their fields
 EMBEDDING_ARGS = struct.Struct("@PPqPqqqiiiifi")
 TOKEN_LOSS_ARGS = struct.Struct("@PqPPPPPPqPPPqqddddddii")
-QK_ROTARY_ARGS = struct.Struct("@" + 6 * "Pqq" + "PPPPPPqdiiiiiiiiii")
-DECAY_ATTENTION_ARGS = struct.Struct("@" + 7 * "Pqq" + "PPPPPPqqdiiiiii")
-DECAY_STEP_ARGS = struct.Struct("@" + 4 * "Pqq" + "PPPPqqdiiiiii")
+# (what follows their views, which are packed by tensor_table().head_views)
+HEAD_VIEW = struct.Struct("@Pqq")
+QK_ROTARY_REST = struct.Struct("@PPPPPPqdiiiiiiiiii")
+DECAY_ATTENTION_REST = struct.Struct("@PPPPPPqqdiiiiii")
+DECAY_STEP_REST = struct.Struct("@PPPPqqdiiiiii")
 LINEAR_LOSS_ARGS = struct.Struct("@PqPqPPPqPqPPPqqqddii")
 assert (EMBEDDING_ARGS.size, TOKEN_LOSS_ARGS.size) == (C.sizeof(EmbeddingArgs), C.sizeof(TokenLossArgs))
-assert (QK_ROTARY_ARGS.size, DECAY_ATTENTION_ARGS.size) == (C.sizeof(QkRotaryArgs), C.sizeof(DecayAttentionArgs))
-assert (DECAY_STEP_ARGS.size, LINEAR_LOSS_ARGS.size) == (C.sizeof(DecayStepArgs), C.sizeof(LinearLossArgs))
+assert HEAD_VIEW.size == C.sizeof(HeadView) and 6 * HEAD_VIEW.size + QK_ROTARY_REST.size == C.sizeof(QkRotaryArgs)
+assert 7 * HEAD_VIEW.size + DECAY_ATTENTION_REST.size == C.sizeof(DecayAttentionArgs)
+assert 4 * HEAD_VIEW.size + DECAY_STEP_REST.size == C.sizeof(DecayStepArgs) and LINEAR_LOSS_ARGS.size == C.sizeof(LinearLossArgs)
 
 # (name, restype, argtypes)
 _SIGNATURES = [

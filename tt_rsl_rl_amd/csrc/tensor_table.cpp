@@ -233,8 +233,76 @@ PyObject* written(PyObject*, PyObject* const* args, Py_ssize_t num) {
   Py_RETURN_NONE;
 }
 
+// Whether x is a tensor of the GPU `device`, laid out by strides.
+const at::Tensor* on_gpu(PyObject* x, int64_t device) {
+  if (!THPVariable_Check(x)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(x);
+  return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device ? &t : nullptr;
+}
+
+// head_views(device, tensor, tokens, heads, elements, ...): the bytes of their ppo_head_views, or None unless all are of those shapes, of the first one's
+// type, of unit stride in their elements and on the device: then the caller's own checks say what is wrong.
+PyObject* head_views(PyObject*, PyObject* const* args, Py_ssize_t num) {
+  try {
+    constexpr Py_ssize_t most = 8;
+    ppo_head_view views[most];
+    const Py_ssize_t n = (num - 1) / 4;
+    if (n < 1 || n > most || num != 1 + 4 * n) return PyErr_Format(PyExc_TypeError, "head_views: a device and up to 8 tensors with their sizes");
+    const int64_t device = PyLong_AsLongLong(args[0]);
+    at::ScalarType type{};
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor* t = on_gpu(args[1 + 4 * i], device);
+      if (t == nullptr || t->dim() != 3 || (i > 0 && t->scalar_type() != type)) Py_RETURN_NONE;
+      type = t->scalar_type();
+      for (int k = 0; k < 3; ++k)
+        if (t->size(k) != PyLong_AsLongLong(args[2 + 4 * i + k])) Py_RETURN_NONE;
+      if (t->stride(2) != 1 && t->size(2) > 1) Py_RETURN_NONE;
+      views[i] = ppo_head_view{t->data_ptr(), t->stride(0), t->stride(1)};
+    }
+    if (PyErr_Occurred()) return nullptr;
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(views), n * static_cast<Py_ssize_t>(sizeof(ppo_head_view)));
+  } catch (const std::exception& ex) {
+    return PyErr_Format(PyExc_RuntimeError, "head_views: %s", ex.what());
+  }
+}
+
+// addresses(device, tensor, elements, ...): their addresses (0 for None), or None unless all are contiguous, of so many elements and on the device.
+PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t num) {
+  try {
+    constexpr Py_ssize_t most = 8;
+    const Py_ssize_t n = (num - 1) / 2;
+    if (n < 1 || n > most || num != 1 + 2 * n) return PyErr_Format(PyExc_TypeError, "addresses: a device and up to 8 tensors with their sizes");
+    const int64_t device = PyLong_AsLongLong(args[0]);
+    void* at[most];
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      at[i] = nullptr;
+      if (args[1 + 2 * i] == Py_None) continue;
+      const at::Tensor* t = on_gpu(args[1 + 2 * i], device);
+      if (t == nullptr || !t->is_contiguous() || t->numel() != PyLong_AsLongLong(args[2 + 2 * i])) Py_RETURN_NONE;
+      at[i] = t->data_ptr();
+    }
+    if (PyErr_Occurred()) return nullptr;
+    PyObject* out = PyTuple_New(n);
+    for (Py_ssize_t i = 0; out != nullptr && i < n; ++i) {
+      PyObject* x = PyLong_FromVoidPtr(at[i]);
+      if (x == nullptr) {
+        Py_DECREF(out);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(out, i, x);
+    }
+    return out;
+  } catch (const std::exception& ex) {
+    return PyErr_Format(PyExc_RuntimeError, "addresses: %s", ex.what());
+  }
+}
+
 PyMethodDef methods[] = {{"adamw_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_table)), METH_FASTCALL,
                           "The bytes of ppo_adamw_step's table (ops.adamw_step)."},
+                         {"head_views", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(head_views)), METH_FASTCALL,
+                          "The bytes of tensors' ppo_head_views, or None where one is not as it should be."},
+                         {"addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(addresses)), METH_FASTCALL,
+                          "Contiguous tensors' addresses, or None where one is not as it should be."},
                          {"written", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(written)), METH_FASTCALL,
                           "Raises the version counters of tensors and of sequences of them; None is skipped."},
                          {nullptr, nullptr, 0, nullptr}};

@@ -1241,18 +1241,40 @@ def adamw_step(params: list, grads: list, exp_avg: list, exp_avg_sq: list, step,
 # ----------------------------------------------------------------------------------------------------------------------
 
 
-def _heads(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str, what: str) -> tuple[int, int, int]:
-    """Address, token stride and head stride of a view [tokens, heads, elements] of unit element stride.  (The message is made where it is
-    needed: a step of a few tokens takes less time than its checks.)"""
+def _heads(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str, what: str) -> bytes:
+    """The ppo_head_view of a view [tokens, heads, elements] of unit element stride."""
     if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name}: {what} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
     token, head, unit = t.stride()
     if unit != 1 and shape[2] > 1:
         raise ValueError(f"{name}: {what} must have unit element stride, got strides {t.stride()}")
-    return t.data_ptr(), token, head
+    return L.HEAD_VIEW.pack(t.data_ptr(), token, head)
 
 
-_NO_VIEW = (0, 0, 0)
+def _views(name: str, dev: int, dtype: torch.dtype, *of) -> bytes:
+    """The ppo_head_views of (tensor, shape, name) each.  (A native call reads them in a tenth of the time of their attributes, which is more than a
+    step of a few tokens takes the GPU; what it does not take is checked here, which says what is wrong.)"""
+    sizes = [x for t, shape, _ in of for x in (t, *shape)]
+    packed = L.tensor_table().head_views(dev, *sizes)
+    if packed is not None and of[0][0].dtype is dtype:
+        return packed
+    _current_gpu(name, *(t for t, _, _ in of))
+    return b"".join(_heads(t, dtype, shape, name, what) for t, shape, what in of)
+
+
+def _addresses(name: str, dev: int, *of) -> tuple:
+    """Addresses of (contiguous tensor or None, elements, name) each."""
+    packed = L.tensor_table().addresses(dev, *(x for t, n, _ in of for x in (t, n)))
+    if packed is not None:
+        return packed
+    _current_gpu(name, *(t for t, _, _ in of if t is not None))
+    for t, n, what in of:
+        if t is not None and (t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{name}: {what} must be contiguous, of {n} elements, got {list(t.shape)}")
+    return tuple(0 if t is None else t.data_ptr() for t, _, _ in of)
+
+
+_NO_VIEWS = bytes(L.HEAD_VIEW.size)
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -1262,30 +1284,37 @@ def rotary_frequencies(dim: int, base: float = 10000.0, device=None) -> torch.Te
     return base ** (torch.arange(0, dim, 2, dtype=torch.float64, device=device) / -dim)
 
 
-def _qk_of(name: str, q, k, q_weight, k_weight, positions, freqs) -> tuple:
-    """(shapes of q and k, packing of the arguments between the views and the sizes, of the sizes, whether weights are heads'), checked."""
+def _qk_of(name: str, dev: int, q, k, q_weight, k_weight, positions, freqs, *more) -> tuple:
+    """(shapes of q and k, addresses of weights, positions, frequencies and more, sizes' packing), checked."""
     of_q, of_k = q.shape, k.shape
     if len(of_q) != 3 or len(of_k) != 3 or of_k[0] != of_q[0] or of_k[2] != of_q[2]:
         raise ValueError(f"{name}: q and k must be [tokens, heads, elements] of the same tokens and elements, got {list(of_q)} and {list(of_k)}")
     tokens, q_heads, dim = of_q
     kv_heads = of_k[1]
-    elem, weight_type = ELEMENT_TYPES.get(q.dtype), ELEMENT_TYPES.get(q_weight.dtype)
+    elem, of_weight = ELEMENT_TYPES.get(q.dtype), q_weight.dtype
+    weight_type = ELEMENT_TYPES.get(of_weight)
     if elem is None:
         _element_type(q, f"{name}: q")
-    if k_weight.dtype is not q_weight.dtype or weight_type != elem and weight_type != L.TYPE_F32:
-        raise ValueError(f"{name}: weights must both be {q.dtype} or float32, got {q_weight.dtype} and {k_weight.dtype}")
+    if k_weight.dtype is not of_weight or weight_type != elem and weight_type != L.TYPE_F32:
+        raise ValueError(f"{name}: weights must both be {q.dtype} or float32, got {of_weight} and {k_weight.dtype}")
     per_head = q_weight.dim() == 2
-    if (q_weight.shape != ((q_heads, dim) if per_head else (dim,)) or k_weight.shape != ((kv_heads, dim) if per_head else (dim,))
-            or not q_weight.is_contiguous() or not k_weight.is_contiguous()):
-        raise ValueError(f"{name}: q_weight and k_weight must be contiguous, both [{dim}], or [{q_heads}, {dim}] and [{kv_heads}, {dim}], got "
-                         f"{list(q_weight.shape)} and {list(k_weight.shape)}")
+    of_qw, of_kw = ((q_heads, dim), (kv_heads, dim)) if per_head else ((dim,), (dim,))
+    if q_weight.shape != of_qw or k_weight.shape != of_kw:
+        raise ValueError(f"{name}: q_weight and k_weight must both be [{dim}], or [{q_heads}, {dim}] and [{kv_heads}, {dim}], got {list(q_weight.shape)} and "
+                         f"{list(k_weight.shape)}")
+    for d, shape in zip(more, (of_qw, of_kw)):
+        if d.dtype is not of_weight or d.shape != shape:
+            raise ValueError(f"{name}: d_q_weight and d_k_weight must be like the weights, {of_weight} {list(shape)}, got {d.dtype} {list(d.shape)}")
     position_type = TOKEN_TYPES.get(positions.dtype)
-    if position_type is None or positions.numel() != tokens or not positions.is_contiguous():
-        raise ValueError(f"{name}: positions must be contiguous int64 or int32 of {tokens} elements, got {positions.dtype} {list(positions.shape)}")
-    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
-        raise ValueError(f"{name}: freqs must be contiguous float64 [rotary_dim / 2], got {freqs.dtype} {list(freqs.shape)}")
-    return (of_q, of_k, (positions.data_ptr(), freqs.data_ptr(), tokens),
-            (q_heads, kv_heads, dim, 2 * freqs.numel(), elem, weight_type, position_type), per_head)
+    if position_type is None:
+        raise ValueError(f"{name}: positions must be int64 or int32, got {positions.dtype}")
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1:
+        raise ValueError(f"{name}: freqs must be float64 [rotary_dim / 2], got {freqs.dtype} {list(freqs.shape)}")
+    pairs = freqs.numel()
+    n_q, n_k = (q_heads * dim, kv_heads * dim) if per_head else (dim, dim)
+    at = _addresses(name, dev, (q_weight, n_q, "q_weight"), (k_weight, n_k, "k_weight"), (positions, tokens, "positions"), (freqs, pairs, "freqs"),
+                    *zip(more, (n_q, n_k), ("d_q_weight", "d_k_weight")))
+    return of_q, of_k, at, (q_heads, kv_heads, dim, 2 * pairs, elem, weight_type, position_type), per_head
 
 
 def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
@@ -1296,12 +1325,10 @@ def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     (i, i + n) of n pairs, or (2i, 2i + 1) with interleaved.  q_out / k_out: like q / k; may be q / k themselves.  dim is even, up to
     512."""
     name = "qk_norm_rotary_fwd"
-    dev = _current_gpu(name, q, k, q_weight, k_weight, positions, freqs, q_out, k_out)
-    of_q, of_k, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs)
-    t = q.dtype
-    args = L.QK_ROTARY_ARGS.pack(*_heads(q, t, of_q, name, "q"), *_heads(k, t, of_k, name, "k"), *_heads(q_out, t, of_q, name, "q_out"),
-                                 *_heads(k_out, t, of_k, name, "k_out"), 0, 0, 0, 0, 0, 0, q_weight.data_ptr(), k_weight.data_ptr(), 0, 0, *middle, eps,
-                                 *sizes, bool(interleaved), per_head, 0)
+    dev = _current_gpu(name, q)
+    of_q, of_k, at, sizes, per_head = _qk_of(name, dev, q, k, q_weight, k_weight, positions, freqs)
+    views = _views(name, dev, q.dtype, (q, of_q, "q"), (k, of_k, "k"), (q_out, of_q, "q_out"), (k_out, of_k, "k_out"))
+    args = views + 2 * _NO_VIEWS + L.QK_ROTARY_REST.pack(at[0], at[1], 0, 0, at[2], at[3], of_q[0], eps, *sizes, bool(interleaved), per_head, 0)
     L.call("ppo_qk_rotary_fwd", args, _raw_stream(dev))
     _written(q_out, k_out)
 
@@ -1313,23 +1340,18 @@ def qk_norm_rotary_bwd(d_q_out: torch.Tensor, d_k_out: torch.Tensor, q: torch.Te
     """The gradients of qk_norm_rotary_fwd's inputs from those of its outputs: d_q / d_k like q / k (may be d_q_out or q themselves, d_k_out
     or k), d_q_weight / d_k_weight like the weights.  The weights' sums go in a fixed order: the same call gives the same bits."""
     name = "qk_norm_rotary_bwd"
-    dev = _current_gpu(name, q, k, q_weight, k_weight, positions, freqs, d_q_out, d_k_out, d_q, d_k, d_q_weight, d_k_weight)
-    of_q, of_k, middle, sizes, per_head = _qk_of(name, q, k, q_weight, k_weight, positions, freqs)
-    for d, w, what in ((d_q_weight, q_weight, "d_q_weight"), (d_k_weight, k_weight, "d_k_weight")):
-        if d.dtype != w.dtype or d.shape != w.shape or not d.is_contiguous():
-            raise ValueError(f"{name}: {what} must be contiguous {w.dtype} {list(w.shape)}, got {d.dtype} {list(d.shape)}")
-    t = q.dtype
-    args = L.QK_ROTARY_ARGS.pack(*_heads(q, t, of_q, name, "q"), *_heads(k, t, of_k, name, "k"), *_heads(d_q_out, t, of_q, name, "d_q_out"),
-                                 *_heads(d_k_out, t, of_k, name, "d_k_out"), *_heads(d_q, t, of_q, name, "d_q"), *_heads(d_k, t, of_k, name, "d_k"),
-                                 q_weight.data_ptr(), k_weight.data_ptr(), d_q_weight.data_ptr(), d_k_weight.data_ptr(), *middle, eps, *sizes,
-                                 bool(interleaved), per_head, 0)
+    dev = _current_gpu(name, q)
+    of_q, of_k, at, sizes, per_head = _qk_of(name, dev, q, k, q_weight, k_weight, positions, freqs, d_q_weight, d_k_weight)
+    views = _views(name, dev, q.dtype, (q, of_q, "q"), (k, of_k, "k"), (d_q_out, of_q, "d_q_out"), (d_k_out, of_k, "d_k_out"), (d_q, of_q, "d_q"),
+                   (d_k, of_k, "d_k"))
+    args = views + L.QK_ROTARY_REST.pack(at[0], at[1], at[4], at[5], at[2], at[3], of_q[0], eps, *sizes, bool(interleaved), per_head, 0)
     buf = _scratch(ws, q.device, L.load().ppo_qk_rotary_bwd_workspace_bytes(args))
     L.call("ppo_qk_rotary_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
     _written(d_q, d_k, d_q_weight, d_k_weight)
 
 
-def _decay_of(name: str, q, k, v, out, what: str, log_decay) -> tuple:
-    """(q's, k's and v's shapes and element type, packing of the four views), checked."""
+def _decay_of(name: str, dev: int, q, k, v, out, what: str, log_decay, *more) -> tuple:
+    """(q's, k's and v's shapes and element type, packing of the views: these four and more, (tensor, index of its shape, name) each), checked."""
     of_q, of_k, of_v, t = q.shape, k.shape, v.shape, q.dtype
     if len(of_q) != 3 or len(of_v) != 3 or of_v[0] != of_q[0] or of_k != (of_q[0], of_v[1], of_q[2]) or of_v[1] == 0 or of_q[1] % of_v[1]:
         raise ValueError(f"{name}: q, k and v must be [tokens, heads, elements], with k's elements q's and k's and v's heads, which divide q's, the same, got "
@@ -1337,10 +1359,11 @@ def _decay_of(name: str, q, k, v, out, what: str, log_decay) -> tuple:
     elem = ELEMENT_TYPES.get(t)
     if elem is None:
         _element_type(q, f"{name}: q")
-    if log_decay.dtype is not torch.float32 or log_decay.shape != of_v[1:2] or not log_decay.is_contiguous():
-        raise ValueError(f"{name}: log_decay must be contiguous float32 [{of_v[1]}], got {log_decay.dtype} {list(log_decay.shape)}")
-    views = (*_heads(q, t, of_q, name, "q"), *_heads(k, t, of_k, name, "k"), *_heads(v, t, of_v, name, "v"),
-             *_heads(out, t, (of_q[0], of_q[1], of_v[2]), name, what))
+    if log_decay.dtype is not torch.float32 or log_decay.dim() != 1:
+        raise ValueError(f"{name}: log_decay must be float32 [{of_v[1]}], got {log_decay.dtype} {list(log_decay.shape)}")
+    shapes = of_q, of_k, of_v
+    views = _views(name, dev, t, (q, of_q, "q"), (k, of_k, "k"), (v, of_v, "v"), (out, (of_q[0], of_q[1], of_v[2]), what),
+                   *((x, shapes[i], y) for x, i, y in more))
     return of_q, of_k, of_v, elem, views
 
 
@@ -1373,13 +1396,14 @@ def decay_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
     starts from (None: zeros) and ends with; final_state may be initial_state.  Key and value heads of up to 128 elements.  A token whose key
     or value is not finite makes NaN of its heads' results from there to its sequence's end, and of no others."""
     name = "decay_attention_fwd"
-    dev = _current_gpu(name, q, k, v, log_decay, out, cu_seqlens, initial_state, final_state)
-    of_q, of_k, of_v, elem, views = _decay_of(name, q, k, v, out, "out", log_decay)
+    dev = _current_gpu(name, q, cu_seqlens, initial_state, final_state)
+    of_q, of_k, of_v, elem, views = _decay_of(name, dev, q, k, v, out, "out", log_decay)
     sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
     shape = (sequences, of_v[1], of_q[2], of_v[2])
-    args = L.DECAY_ATTENTION_ARGS.pack(
-        *views, *_NO_VIEW, *_NO_VIEW, *_NO_VIEW, log_decay.data_ptr(), cu, _state(initial_state, f"{name}: initial_state", shape),
-        _state(final_state, f"{name}: final_state", shape), 0, 0, of_q[0], sequences, scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
+    (decay,) = _addresses(name, dev, (log_decay, of_v[1], "log_decay"))
+    args = views + 3 * _NO_VIEWS + L.DECAY_ATTENTION_REST.pack(
+        decay, cu, _state(initial_state, f"{name}: initial_state", shape), _state(final_state, f"{name}: final_state", shape), 0, 0, of_q[0], sequences, scale,
+        of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
     buf = _scratch(ws, q.device, L.load().ppo_decay_attention_workspace_bytes(args, 0))
     L.call("ppo_decay_attention_fwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
     _written(out, final_state)
@@ -1392,13 +1416,13 @@ def decay_attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     """The gradients of decay_attention_fwd's q, k, v and initial_state from those of its out and final_state (None: zeros).  log_decay is a
     constant.  d_initial_state may be d_final_state."""
     name = "decay_attention_bwd"
-    dev = _current_gpu(name, q, k, v, log_decay, d_out, d_q, d_k, d_v, cu_seqlens, initial_state, d_final_state, d_initial_state)
-    of_q, of_k, of_v, elem, views = _decay_of(name, q, k, v, d_out, "d_out", log_decay)
+    dev = _current_gpu(name, q, cu_seqlens, initial_state, d_final_state, d_initial_state)
+    of_q, of_k, of_v, elem, views = _decay_of(name, dev, q, k, v, d_out, "d_out", log_decay, (d_q, 0, "d_q"), (d_k, 1, "d_k"), (d_v, 2, "d_v"))
     sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
-    shape, t = (sequences, of_v[1], of_q[2], of_v[2]), q.dtype
-    args = L.DECAY_ATTENTION_ARGS.pack(
-        *views, *_heads(d_q, t, of_q, name, "d_q"), *_heads(d_k, t, of_k, name, "d_k"), *_heads(d_v, t, of_v, name, "d_v"), log_decay.data_ptr(), cu,
-        _state(initial_state, f"{name}: initial_state", shape), 0, _state(d_final_state, f"{name}: d_final_state", shape),
+    shape = (sequences, of_v[1], of_q[2], of_v[2])
+    (decay,) = _addresses(name, dev, (log_decay, of_v[1], "log_decay"))
+    args = views + L.DECAY_ATTENTION_REST.pack(
+        decay, cu, _state(initial_state, f"{name}: initial_state", shape), 0, _state(d_final_state, f"{name}: d_final_state", shape),
         _state(d_initial_state, f"{name}: d_initial_state", shape), of_q[0], sequences, scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
     buf = _scratch(ws, q.device, L.load().ppo_decay_attention_workspace_bytes(args, 1))
     L.call("ppo_decay_attention_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
@@ -1412,24 +1436,20 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     each row's state, no two the same; one outside the states is a row of padding, whose output is 0.  fresh (bool or uint8): the
     sequence begins with this token, whatever its state held."""
     name = "decay_attention_step"
-    dev = _current_gpu(name, q, k, v, log_decay, state, out, slots, fresh)
-    of_q, _, of_v, elem, views = _decay_of(name, q, k, v, out, "out", log_decay)
+    dev = _current_gpu(name, q)
+    of_q, _, of_v, elem, views = _decay_of(name, dev, q, k, v, out, "out", log_decay)
     rows, of_state = of_q[0], state.shape
-    if state.dtype is not torch.float32 or len(of_state) != 4 or of_state[1:] != (of_v[1], of_q[2], of_v[2]) or not state.is_contiguous():
-        raise ValueError(f"{name}: state must be contiguous float32 [slots, {of_v[1]}, {of_q[2]}, {of_v[2]}], got {state.dtype} {list(of_state)}")
-    at, slot_type = 0, L.TOKENS_I32
+    if state.dtype is not torch.float32 or len(of_state) != 4 or of_state[1:] != (of_v[1], of_q[2], of_v[2]):
+        raise ValueError(f"{name}: state must be float32 [slots, {of_v[1]}, {of_q[2]}, {of_v[2]}], got {state.dtype} {list(of_state)}")
+    slot_type = L.TOKENS_I32
     if slots is not None:
         slot_type = TOKEN_TYPES.get(slots.dtype)
-        if slot_type is None or slots.numel() != rows or not slots.is_contiguous():
-            raise ValueError(f"{name}: slots must be contiguous int64 or int32 of {rows} elements, got {slots.dtype} {list(slots.shape)}")
-        at = slots.data_ptr()
-    begins = 0
-    if fresh is not None:
-        if fresh.dtype not in (torch.bool, torch.uint8) or fresh.numel() != rows or not fresh.is_contiguous():
-            raise ValueError(f"{name}: fresh must be contiguous bool or uint8 of {rows} elements, got {fresh.dtype} {list(fresh.shape)}")
-        begins = fresh.data_ptr()
-    args = L.DECAY_STEP_ARGS.pack(*views, log_decay.data_ptr(), state.data_ptr(), at, begins, rows, of_state[0], scale, of_q[1], of_v[1], of_q[2], of_v[2],
-                                  elem, slot_type)
+        if slot_type is None:
+            raise ValueError(f"{name}: slots must be int64 or int32, got {slots.dtype}")
+    if fresh is not None and fresh.dtype is not torch.bool and fresh.dtype is not torch.uint8:
+        raise ValueError(f"{name}: fresh must be bool or uint8, got {fresh.dtype}")
+    at = _addresses(name, dev, (log_decay, of_v[1], "log_decay"), (state, state.numel(), "state"), (slots, rows, "slots"), (fresh, rows, "fresh"))
+    args = views + L.DECAY_STEP_REST.pack(*at, rows, of_state[0], scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, slot_type)
     L.call("ppo_decay_attention_step", args, _raw_stream(dev))
     _written(state, out)
 
