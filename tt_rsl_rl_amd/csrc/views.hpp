@@ -36,4 +36,8 @@ inline int check_view(const char* who, const char* name, const ppo_head_view& v,
   return PPO_OK;
 }
 
+// All waves' LDS accesses are done.  (__syncthreads() would also wait for the loads and stores on their way to and from memory, which no other wave
+// of the block looks at.)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 }  // namespace ppo
