@@ -148,38 +148,46 @@ __device__ __forceinline__ Span span_of(const MixArgs& q, int token) {
   return q.spans == nullptr ? Span{0, q.tokens, 0} : q.spans[token];
 }
 
-// One thread a token: the sequence that it lies in.
-__global__ __launch_bounds__(kInfoThreads) void decay_spans_kernel(const void* cu, int cu_type, int sequences, int tokens, Span* spans) {
+struct SequenceArgs {
+  const void* cu;
+  int32_t cu_type, tokens;
+  int64_t sequences;
+  Span* spans;  // of each token, by the first token_blocks blocks
+  int64_t token_blocks;
+  const float* from;  // the states of sequences without tokens, or of all, by the others
+  float* to;
+  int64_t size;
+  int32_t all;
+};
+
+// What chunks do not do: one thread a token, the sequence that it lies in; one block a sequence, its state handed on.
+__global__ __launch_bounds__(kInfoThreads) void decay_sequences_kernel(const SequenceArgs q) {
+  auto at = [&](int64_t i) {
+    return q.cu_type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(q.cu)[i] : static_cast<int64_t>(static_cast<const int32_t*>(q.cu)[i]);
+  };
+  const int64_t tokens = q.tokens;
+  if (blockIdx.x >= q.token_blocks) {
+    for (int64_t b = blockIdx.x - q.token_blocks; b < q.sequences; b += gridDim.x - q.token_blocks) {
+      const bool empty = q.cu == nullptr ? tokens == 0 : min(at(b + 1), tokens) <= max(at(b), static_cast<int64_t>(0));
+      if (!empty && q.all == 0) continue;
+      for (int64_t i = threadIdx.x; i < q.size; i += kInfoThreads) q.to[b * q.size + i] = q.from == nullptr ? 0.0f : q.from[b * q.size + i];
+    }
+    return;
+  }
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kInfoThreads + threadIdx.x;
   if (t >= tokens) return;
-  auto at = [&](int i) {
-    return cu_type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(cu)[i] : static_cast<int64_t>(static_cast<const int32_t*>(cu)[i]);
-  };
-  int lo = 0, hi = sequences + 1;  // the first entry above t
+  int64_t lo = 0, hi = q.sequences + 1;  // the first entry above t
   while (lo < hi) {
-    const int mid = (lo + hi) / 2;
+    const int64_t mid = (lo + hi) / 2;
     if (at(mid) > t) hi = mid;
     else lo = mid + 1;
   }
   Span s{static_cast<int32_t>(t), static_cast<int32_t>(t) + 1, -1};
-  if (lo >= 1 && lo <= sequences) {
-    const int64_t from = max(at(lo - 1), static_cast<int64_t>(0)), to = min(at(lo), static_cast<int64_t>(tokens));
-    if (from <= t && to > t) s = Span{static_cast<int32_t>(from), static_cast<int32_t>(to), lo - 1};
+  if (lo >= 1 && lo <= q.sequences) {
+    const int64_t from = max(at(lo - 1), static_cast<int64_t>(0)), to = min(at(lo), tokens);
+    if (from <= t && to > t) s = Span{static_cast<int32_t>(from), static_cast<int32_t>(to), static_cast<int32_t>(lo - 1)};
   }
-  spans[t] = s;
-}
-
-// The states of sequences without tokens, or all of them.
-__global__ __launch_bounds__(256) void decay_hand_on_kernel(const void* cu, int cu_type, int tokens, const float* from, float* to, int64_t size, int64_t sequences, bool all) {
-  auto at = [&](int64_t i) {
-    const int64_t v = cu_type == PPO_TOKENS_I64 ? static_cast<const int64_t*>(cu)[i] : static_cast<int64_t>(static_cast<const int32_t*>(cu)[i]);
-    return min(max(v, static_cast<int64_t>(0)), static_cast<int64_t>(tokens));
-  };
-  for (int64_t b = blockIdx.x; b < sequences; b += gridDim.x) {
-    const bool empty = cu == nullptr ? tokens == 0 : at(b + 1) <= at(b);
-    if (!empty && !all) continue;
-    for (int64_t i = threadIdx.x; i < size; i += 256) to[b * size + i] = from == nullptr ? 0.0f : from[b * size + i];
-  }
+  q.spans[t] = s;
 }
 
 // carry[s] holds what segment s makes of nothing; afterwards what enters segment s + 1.
@@ -325,7 +333,8 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int head = blockIdx.y, seg = blockIdx.x;
-  const int dc0 = wave * NT * 16;
+  const int col0 = NT == 1 ? blockIdx.z * DC : 0;  // a block has DC of c's columns
+  const int own0 = wave * NT * 16, dc0 = col0 + own0;
   const bool works = dc0 < q.dc;
   const int seg_begin = seg * q.segment, seg_end = min(seg_begin + q.segment, q.tokens);
 
@@ -378,7 +387,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
       const ppo_head_view& v = kind == 0 ? q.b : kind == 1 || STATE_ONLY ? q.c : q.a;
       const char* from = reinterpret_cast<const char*>(static_cast<const T*>(v.data) + (kind >= 2 ? ha : hb) * v.head_stride + lowest * v.token_stride);
       const uint32_t step = static_cast<uint32_t>(v.token_stride) * sizeof(T);
-      const uint32_t column = min(d, (kind == 1 || (STATE_ONLY && kind == 3) ? q.dc : q.db) - V) * static_cast<int>(sizeof(T));
+      const uint32_t column = min(d + (kind == 1 || (STATE_ONLY && kind == 3) ? col0 : 0), (kind == 1 || (STATE_ONLY && kind == 3) ? q.dc : q.db) - V) * static_cast<int>(sizeof(T));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int j = min(j4 + k, n - 1);
@@ -397,7 +406,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
   bool lost = q.lost != 0;  // S may be not finite
   each_state([](float, int, int) { return 0.0f; });
   if (!STATE_ONLY && first[0][0] < seg_begin) {  // goes on from the segment before
-    const float* from = q.carry + (static_cast<int64_t>(seg - 1) * q.heads + head) * q.db * q.dc;
+    const float* from = q.carry + (static_cast<int64_t>(seg - 1) * q.heads + head) * q.state_size;
     each_state([&](float, int i, int j) { return works && i < q.db && j < q.dc ? from[i * q.ci + j * q.cj] : 0.0f; });
     wait_memory();
     fresh = false;
@@ -432,7 +441,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     forget(thread);
     const int col = thread % 16, g = thread % kWave / 16;
     const int a_at = Rows_::at(col, g), b_at = Rows_::at(X::row_of(0, col), g), m_at = Cols_::at(col, g), bt_at = Cols_::at(X::row_of(0, col), g);
-    const int ct_at = Cols_::at(dc0 + column_of(0, col), g);  // operands' places, to go on from
+    const int ct_at = Cols_::at(own0 + column_of(0, col), g);  // operands' places, to go on from
     // ---- rows into LDS ----
     lds_barrier();  // the last products have read what is there
     if (q.whole) {
@@ -454,13 +463,13 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
         if (!STATE_ONLY && kind == 2 && new_a) put_rows<T, M, DB>(r[round], a_rows, j4, d, d < q.db);
       }
     } else {  // heads of odd widths: element by element
-      auto elements = [&](const ppo_head_view& v, int h, int dim, int padded, M* rows, M* turned) {
+      auto elements = [&](const ppo_head_view& v, int h, int dim, int from, int padded, M* rows, M* turned) {
 #pragma unroll 1
         for (int i = thread; i < C * padded; i += kThreads) {
           const int j = i / padded, d = i % padded;
           T x = static_cast<T>(0.0f);
-          if (d < dim && (valid >> j & 1) != 0)
-            x = static_cast<const T*>(v.data)[h * v.head_stride + token_at_place(begin + j) * v.token_stride + d];
+          if (from + d < dim && (valid >> j & 1) != 0)
+            x = static_cast<const T*>(v.data)[h * v.head_stride + token_at_place(begin + j) * v.token_stride + from + d];
           if (turned != nullptr && !(fabsf(static_cast<float>(x)) < INFINITY)) {
             atomicOr(&bad[j / 32], 1u << (j % 32));
             bad_any = 1;
@@ -470,9 +479,9 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
         }
       };
       const int ha = q.ga > 1 ? head * q.ga + ab : head, hb = q.gb > 1 ? head * q.gb + ab : head;
-      if (new_a) elements(q.a, ha, q.db, DB, a_rows, nullptr);
-      elements(q.b, hb, q.db, DB, STATE_ONLY ? nullptr : b_rows, b_turned);
-      if (new_b) elements(q.c, hb, q.dc, DC, nullptr, c_turned);
+      if (new_a) elements(q.a, ha, q.db, 0, DB, a_rows, nullptr);
+      elements(q.b, hb, q.db, 0, DB, STATE_ONLY ? nullptr : b_rows, b_turned);
+      if (new_b) elements(q.c, hb, q.dc, col0, DC, nullptr, c_turned);
     }
     if (thread < C) {
       const int i = min(thread, n - 1);
@@ -723,7 +732,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     c0 = next_c0, p = next_p, ab = next_ab, buffer = next_buffer, n = next_n;
   }
   if (STATE_ONLY && works) {
-    float* to = q.carry + (static_cast<int64_t>(seg) * q.heads + head) * q.db * q.dc;
+    float* to = q.carry + (static_cast<int64_t>(seg) * q.heads + head) * q.state_size;
     each_state([&](float s, int i, int j) {
       if (i < q.db && j < q.dc) to[i * q.ci + j * q.cj] = s;
       return s;
@@ -750,25 +759,27 @@ Plan plan_of(int64_t tokens, int heads, int chunk) {
 
 template <class T, class M, int DBT, int NT>
 int launch_mix(const MixArgs& q, hipStream_t st) {
-  const uint32_t heads = static_cast<uint32_t>(q.heads);
+  const uint32_t heads = static_cast<uint32_t>(q.heads), columns = static_cast<uint32_t>(ceil_div(q.dc, kWaves * NT * 16));
   if (q.segments > 1 && q.carried == 0) {
     MixArgs own = q;
     own.ga = 1;  // (no outputs, so no a)
-    hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, true>), dim3(static_cast<uint32_t>(q.segments - 1), heads), dim3(kThreads), 0, st, own);
+    hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, true>), dim3(static_cast<uint32_t>(q.segments - 1), heads, columns), dim3(kThreads), 0, st, own);
     if (int rc = check_launch("decay_mix_kernel")) return rc;
     const int64_t size = static_cast<int64_t>(q.db) * q.dc;
     hipLaunchKernelGGL(decay_scan_kernel, dim3(static_cast<uint32_t>(ceil_div(size, kScanThreads)), heads), dim3(kScanThreads), 0, st, q);
     if (int rc = check_launch("decay_scan_kernel")) return rc;
   }
-  hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, false>), dim3(static_cast<uint32_t>(q.segments), heads), dim3(kThreads), 0, st, q);
+  hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, false>), dim3(static_cast<uint32_t>(q.segments), heads, columns), dim3(kThreads), 0, st, q);
   return check_launch("decay_mix_kernel");
 }
 
 template <class T>
 int launch_type(const MixArgs& q, hipStream_t st) {
   using M = std::conditional_t<__is_same(T, __bf16), __bf16, float>;  // fp16 goes through fp32 products
-  if (q.db <= 64) return q.dc <= 64 ? launch_mix<T, M, 4, 1>(q, st) : launch_mix<T, M, 4, 2>(q, st);
-  return q.dc <= 64 ? launch_mix<T, M, 8, 1>(q, st) : launch_mix<T, M, 8, 2>(q, st);
+  // 64 of c's columns a block where 128 would leave half of the chip without one
+  const bool few = q.dc <= 64 || static_cast<int64_t>(q.segments) * q.heads * 2 <= device_info().cus;
+  if (q.db <= 64) return few ? launch_mix<T, M, 4, 1>(q, st) : launch_mix<T, M, 4, 2>(q, st);
+  return few ? launch_mix<T, M, 8, 1>(q, st) : launch_mix<T, M, 8, 2>(q, st);
 }
 
 struct Layout {
@@ -854,7 +865,10 @@ int check(const char* who, const ppo_decay_attention_args* args, bool backward) 
   return PPO_OK;
 }
 
-int prepare(const char* who, const ppo_decay_attention_args& a, void* workspace, size_t workspace_bytes, hipStream_t st, MixArgs& q) {
+// `from`, `to`: the states (or their gradients) that sequences begin and end with.  What no chunk does for them: sequences without tokens hand theirs on, and
+// those that are replaced in place are read from a copy (then `from`), since the block that ends a sequence need not be the one that began it.
+int prepare(const char* who, const ppo_decay_attention_args& a, const float*& from, float* to, void* workspace, size_t workspace_bytes, hipStream_t st,
+            MixArgs& q) {
   const Layout l = layout_of(a);
   PPO_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= l.bytes,
               "%s: workspace too small or not 16-byte aligned (%zu < %zu)", who, workspace_bytes, l.bytes);
@@ -870,25 +884,17 @@ int prepare(const char* who, const ppo_decay_attention_args& a, void* workspace,
   q.segment = p.segment;
   q.segments = p.segments;
   q.heads = a.kv_heads;
-  if (spans != nullptr && a.tokens > 0) {
-    hipLaunchKernelGGL(decay_spans_kernel, dim3(static_cast<uint32_t>(ceil_div(a.tokens, kInfoThreads))), dim3(kInfoThreads), 0, st, a.cu_seqlens, a.cu_type,
-                       static_cast<int>(a.sequences), q.tokens, spans);
-    return check_launch("decay_spans_kernel");
+  const bool in_place = to != nullptr && from == to, handed = to != nullptr && (in_place ? l.copy != 0 : a.cu_seqlens != nullptr || a.tokens == 0);
+  SequenceArgs n{a.cu_seqlens, a.cu_type, q.tokens, a.sequences, spans, spans != nullptr ? ceil_div(a.tokens, kInfoThreads) : 0, from, nullptr, 0, in_place};
+  if (handed) {
+    n.to = in_place ? reinterpret_cast<float*>(base + l.copy) : to;
+    n.size = a.kv_heads * q.state_size;
+    if (in_place) from = n.to;
   }
-  return PPO_OK;
-}
-
-// What no chunk does for the states: sequences without tokens hand theirs on, and states that are replaced in place are read from a copy, since the block
-// that ends a sequence need not be the one that began it.
-int hand_on(const ppo_decay_attention_args& a, const float*& from, float* to, void* workspace, hipStream_t st) {
-  if (to == nullptr) return PPO_OK;
-  const bool in_place = from == to;
-  if (in_place && layout_of(a).copy == 0) return PPO_OK;
-  float* const target = in_place ? reinterpret_cast<float*>(static_cast<char*>(workspace) + layout_of(a).copy) : to;
-  hipLaunchKernelGGL(decay_hand_on_kernel, dim3(static_cast<uint32_t>(std::min<int64_t>(a.sequences, 1 << 20))), dim3(256), 0, st, a.cu_seqlens, a.cu_type,
-                     static_cast<int>(a.tokens), from, target, static_cast<int64_t>(a.kv_heads) * a.key_dim * a.value_dim, a.sequences, in_place);
-  if (in_place) from = target;
-  return check_launch("decay_hand_on_kernel");
+  const int64_t blocks = n.token_blocks + (handed ? std::min<int64_t>(a.sequences, 1 << 20) : 0);
+  if (blocks == 0) return PPO_OK;
+  hipLaunchKernelGGL(decay_sequences_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kInfoThreads), 0, st, n);
+  return check_launch("decay_sequences_kernel");
 }
 
 int mix(const ppo_decay_attention_args& a, MixArgs q, hipStream_t st) {
@@ -921,9 +927,8 @@ extern "C" int ppo_decay_attention_fwd(const ppo_decay_attention_args* args, voi
   const ppo_decay_attention_args& a = *args;
   hipStream_t st = static_cast<hipStream_t>(stream);
   MixArgs q;
-  if (int rc = prepare(who, a, workspace, workspace_bytes, st, q)) return rc;
   const float* from = a.initial_state;
-  if (int rc = hand_on(a, from, a.final_state, workspace, st)) return rc;
+  if (int rc = prepare(who, a, from, a.final_state, workspace, workspace_bytes, st, q)) return rc;
   if (a.tokens == 0) return PPO_OK;
   q.a = a.q, q.b = a.k, q.c = a.v, q.out = a.out;
   q.s_in = from, q.s_out = a.final_state, q.cut = a.initial_state != nullptr || a.final_state != nullptr, q.exact = a.final_state != nullptr;
@@ -939,9 +944,8 @@ extern "C" int ppo_decay_attention_bwd(const ppo_decay_attention_args* args, voi
   const ppo_decay_attention_args& a = *args;
   hipStream_t st = static_cast<hipStream_t>(stream);
   MixArgs q;
-  if (int rc = prepare(who, a, workspace, workspace_bytes, st, q)) return rc;
   const float* from = a.d_final_state;
-  if (int rc = hand_on(a, from, a.d_initial_state, workspace, st)) return rc;
+  if (int rc = prepare(who, a, from, a.d_initial_state, workspace, workspace_bytes, st, q)) return rc;
   if (a.tokens == 0) return PPO_OK;
   const int group = a.q_heads / a.kv_heads;
   // d_q: in order, S turned over
