@@ -57,10 +57,23 @@ constexpr int kStep = sizeof(T) == 4 ? 32 : 64;  // k of a stage (bf16: 32, four
 template <class T>
 constexpr float kLift = __is_same(T, _Float16) ? 16384.0f : 1.0f;
 
-// d_hidden may have few tiles: their k is then cut into slices, as many as make two rounds of blocks.  Only the device knows how many rows count.  (Four slices
-// of 192 tiles, three whole rounds instead of three quarters of one, gained nothing: the sums are read and written four times.)
-__device__ __forceinline__ int slices_of(int tiles, int cus, int steps) {
-  return 2 * tiles < cus ? static_cast<int>(min(ceil_div(2 * cus, max(tiles, 1)), static_cast<int64_t>(max(steps / 8, 1)))) : 1;
+// How d_hidden's tiles are shared out to the compute units; only the device knows how many rows count.  Tiles that make whole rounds take one block each.  Of the
+// rest, few are cut into slices of k, as many as fill one round; many leave a part of their k, 1 / (per + 1), to the units that would idle, `per` tiles to each
+// of these.  Every share of a tile has its own sums, the first ones tile after tile, the others behind them.
+struct Shares {
+  int whole, rest, slots, per;  // per 0: slices
+};
+__device__ __forceinline__ Shares shares_of(int tiles, int cus, int steps) {
+  Shares s{tiles / cus * cus, 0, 1, 0};
+  s.rest = tiles - s.whole;
+  if (s.rest == 0) return s;
+  if (2 * s.rest <= cus) {
+    s.slots = min(cus / s.rest, max(steps / 8, 1));
+  } else {
+    const int per = static_cast<int>(ceil_div(s.rest, cus - s.rest));
+    if (per <= 8) s.slots = 2, s.per = per;
+  }
+  return s;
 }
 
 struct Operand {
@@ -140,263 +153,296 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
   // its L2 as often as can be.  (The last 64 rows' d is made past the count too, as zeros: the second products sum over whole steps.)
   const int32_t count = *q.count;
   const int n_there = JOB == kWeightGrad ? q.n_tiles : static_cast<int>(ceil_div(JOB == kDiffs ? ceil_div(count, kTileK) * kTileK : count, BN));
-  const int tiles = q.m_tiles * n_there, slices = JOB == kRowGrad ? slices_of(tiles, q.cus, q.all_steps) : 1, all = tiles * slices, each = static_cast<int>(ceil_div(all, q.xcds));
-  const int local = blockIdx.x / q.xcds, item = blockIdx.x % q.xcds * each + local;
-  if (local >= each || item >= all) return;
-  const int slice = JOB == kRowGrad ? item / tiles : 0, tile = item - slice * tiles;
-  const int first_n = tile / (4 * q.m_tiles) * 4, wide = min(4, n_there - first_n), inside = tile - first_n * q.m_tiles;
-  const int mt = inside / wide, nt = first_n + inside % wide;
-  const int m0 = mt * BM, n0 = nt * BN;
+  const int tiles = q.m_tiles * n_there, xcd = blockIdx.x % q.xcds, local = blockIdx.x / q.xcds;
   int steps = q.steps;
   if (JOB == kWeightGrad) steps = static_cast<int>(ceil_div(count, kTileK)) * (kTileK / STEP);
-  int from = 0, to = steps;
-  if (JOB == kRowGrad) {  // a slice of k
-    const int span = static_cast<int>(ceil_div(steps, slices));
-    from = min(slice * span, steps);
-    to = min(from + span, steps);
-  }
-
-  // Addresses: a wave's load covers LOAD_ROWS rows; lane l brings the piece that belongs at its place.
-  uint32_t off_x[LOADS_X], off_y[LOADS_Y];
-  const auto turn = [](int row) { return PIECES == 8 ? row / 2 % 8 : row / 4 % 4; };
-  const auto offset = [&](int row, int tile0, const Operand& o) {
-    return static_cast<uint32_t>(min(tile0 + row, o.rows - 1) - tile0) * static_cast<uint32_t>(o.ld * 2) + static_cast<uint32_t>((lane % PIECES ^ turn(row)) * 16);
-  };
-#pragma unroll
-  for (int i = 0; i < LOADS_X; ++i) off_x[i] = offset((wave * LOADS_X + i) * LOAD_ROWS + lane / PIECES, m0, q.x);
-#pragma unroll
-  for (int i = 0; i < LOADS_Y; ++i) off_y[i] = offset((wave * LOADS_Y + i) * LOAD_ROWS + lane / PIECES, n0, q.y);
-  const char* const base_x = static_cast<const char*>(q.x.at) + static_cast<int64_t>(m0) * q.x.ld * 2;
-  const char* const base_y = static_cast<const char*>(q.y.at) + static_cast<int64_t>(n0) * q.y.ld * 2;
-  const int total = to - from;
-  auto load_stage = [&](int s) {
-    const int64_t k_bytes = static_cast<int64_t>(from + s) * ROW;
-    unsigned char* to_lds = lds + s % STAGES * STAGE;
-#pragma unroll
-    for (int part = 0; part < PARTS; ++part) {
-      const auto rx = buffer_at(base_x + part * q.x.part * 2 + k_bytes), ry = buffer_at(base_y + part * q.y.part * 2 + k_bytes);
-#pragma unroll
-      for (int i = 0; i < LOADS_X; ++i) load_to_lds(rx, off_x[i], to_lds + part * PART + (wave * LOADS_X + i) * 1024);
-      if (Y_WAVES == 8 || wave < Y_WAVES)
-#pragma unroll
-        for (int i = 0; i < LOADS_Y; ++i) load_to_lds(ry, off_y[i], to_lds + part * PART + BM * ROW + (wave * LOADS_Y + i) * 1024);
+  int tile, last_tile, slot = 0, from = 0, to = steps;  // a block that helps goes through more tiles than one
+  Shares shares{tiles, 0, 1, 0};
+  if constexpr (JOB == kRowGrad) shares = shares_of(tiles, q.cus, q.all_steps);
+  const int each = static_cast<int>(ceil_div(shares.whole, q.xcds));
+  if (local < each) {
+    tile = xcd * each + local;
+    if (tile >= shares.whole) return;
+    last_tile = tile;
+  } else {
+    const int rest = shares.rest, items = shares.per == 0 ? rest * shares.slots : rest + static_cast<int>(ceil_div(rest, shares.per));
+    const int each_rest = static_cast<int>(ceil_div(items, q.xcds)), item = xcd * each_rest + local - each;
+    if (JOB != kRowGrad || local - each >= each_rest || item >= items) return;
+    if (shares.per == 0) {
+      slot = item / rest, tile = last_tile = shares.whole + item - slot * rest;
+      const int span = static_cast<int>(ceil_div(steps, shares.slots));
+      from = min(slot * span, steps), to = min(from + span, steps);
+    } else {
+      const int split = steps * shares.per / (shares.per + 1);
+      if (item < rest) tile = last_tile = shares.whole + item, to = split;
+      else slot = 1, tile = shares.whole + (item - rest) * shares.per, last_tile = min(tile + shares.per, tiles) - 1, from = split;
     }
-  };
+  }
+#pragma unroll 1
+  for (;; ++tile) {
+    const int first_n = tile / (4 * q.m_tiles) * 4, wide = min(4, n_there - first_n), inside = tile - first_n * q.m_tiles;
+    const int mt = inside / wide, nt = first_n + inside % wide;
+    const int m0 = mt * BM, n0 = nt * BN;
 
-  f32x16 acc[TM][TN];
+    // Addresses: a wave's load covers LOAD_ROWS rows; lane l brings the piece that belongs at its place.
+    uint32_t off_x[LOADS_X], off_y[LOADS_Y];
+    const auto turn = [](int row) { return PIECES == 8 ? row / 2 % 8 : row / 4 % 4; };
+    const auto offset = [&](int row, int tile0, const Operand& o) {
+      return static_cast<uint32_t>(min(tile0 + row, o.rows - 1) - tile0) * static_cast<uint32_t>(o.ld * 2) + static_cast<uint32_t>((lane % PIECES ^ turn(row)) * 16);
+    };
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < LOADS_X; ++i) off_x[i] = offset((wave * LOADS_X + i) * LOAD_ROWS + lane / PIECES, m0, q.x);
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-
-  const int r32 = lane % 32, half = lane / 32;
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < total) load_stage(s);
-  for (int s = 0; s < total; ++s) {
-    if (STAGES == 2 || s + STAGES - 2 >= total) wait_loads<0>();
-    else if (Y_WAVES == 8 || wave < Y_WAVES) wait_loads<(STAGES - 2) * PARTS * (LOADS_X + LOADS_Y)>();
-    else wait_loads<(STAGES - 2) * PARTS * LOADS_X>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (s + STAGES - 1 < total) load_stage(s + STAGES - 1);
-    const unsigned char* at = lds + s % STAGES * STAGE;
-#pragma unroll
-    for (int kk = 0; kk < STEP / 16; ++kk) {
-      u32x4 x[PARTS][TM], y[PARTS][TN];
-      const int piece = 2 * kk + half;
+    for (int i = 0; i < LOADS_Y; ++i) off_y[i] = offset((wave * LOADS_Y + i) * LOAD_ROWS + lane / PIECES, n0, q.y);
+    const char* const base_x = static_cast<const char*>(q.x.at) + static_cast<int64_t>(m0) * q.x.ld * 2;
+    const char* const base_y = static_cast<const char*>(q.y.at) + static_cast<int64_t>(n0) * q.y.ld * 2;
+    const int total = to - from;
+    auto load_stage = [&](int s) {
+      const int64_t k_bytes = static_cast<int64_t>(from + s) * ROW;
+      unsigned char* to_lds = lds + s % STAGES * STAGE;
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
+        const auto rx = buffer_at(base_x + part * q.x.part * 2 + k_bytes), ry = buffer_at(base_y + part * q.y.part * 2 + k_bytes);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const int row = (wm * TM + i) * 32 + r32;
-          x[part][i] = *reinterpret_cast<const u32x4*>(at + part * PART + row * ROW + (piece ^ turn(row)) * 16);
+        for (int i = 0; i < LOADS_X; ++i) load_to_lds(rx, off_x[i], to_lds + part * PART + (wave * LOADS_X + i) * 1024);
+        if (Y_WAVES == 8 || wave < Y_WAVES)
+#pragma unroll
+          for (int i = 0; i < LOADS_Y; ++i) load_to_lds(ry, off_y[i], to_lds + part * PART + BM * ROW + (wave * LOADS_Y + i) * 1024);
+      }
+    };
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+    const int r32 = lane % 32, half = lane / 32;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < total) load_stage(s);
+    for (int s = 0; s < total; ++s) {
+      if (STAGES == 2 || s + STAGES - 2 >= total) wait_loads<0>();
+      else if (Y_WAVES == 8 || wave < Y_WAVES) wait_loads<(STAGES - 2) * PARTS * (LOADS_X + LOADS_Y)>();
+      else wait_loads<(STAGES - 2) * PARTS * LOADS_X>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + STAGES - 1 < total) load_stage(s + STAGES - 1);
+      const unsigned char* at = lds + s % STAGES * STAGE;
+#pragma unroll
+      for (int kk = 0; kk < STEP / 16; ++kk) {
+        u32x4 x[PARTS][TM], y[PARTS][TN];
+        const int piece = 2 * kk + half;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const int row = (wm * TM + i) * 32 + r32;
+            x[part][i] = *reinterpret_cast<const u32x4*>(at + part * PART + row * ROW + (piece ^ turn(row)) * 16);
+          }
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int row = (wn * TN + j) * 32 + r32;
+            y[part][j] = *reinterpret_cast<const u32x4*>(at + part * PART + BM * ROW + row * ROW + (piece ^ turn(row)) * 16);
+          }
         }
+        // (the smallest products first: x3 y1, x2 y2, x1 y3, x2 y1, x1 y2, x1 y1)
+#pragma unroll
+        for (int sum = PARTS - 1; sum >= 0; --sum)
+#pragma unroll
+          for (int px = sum; px >= 0; --px)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int j = 0; j < TN; ++j) acc[i][j] = mma<M>(x[px][i], y[sum - px][j], acc[i][j]);
+      }
+    }
+
+    // Element r of acc[i][j]: m = m0 + 32 (wm TM + i) + 8 (r / 4) + 4 half + r % 4,  n = n0 + 32 (wn TN + j) + r32.
+    auto m_of = [&](int i, int r) { return 32 * (wm * TM + i) + 8 * (r / 4) + 4 * half + r % 4; };
+    if constexpr (JOB == kSums) {
+      __syncthreads();
+      float* join_at = reinterpret_cast<float*>(lds);  // [WM][3][BN]
+      const int64_t left = q.vocab - q.column0 - m0;   // columns of the tile that are there
+      if (PARTS > 1 && q.kept != nullptr)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          const int row = (wn * TN + j) * 32 + r32;
-          y[part][j] = *reinterpret_cast<const u32x4*>(at + part * PART + BM * ROW + row * ROW + (piece ^ turn(row)) * 16);
+          const int n = n0 + 32 * (wn * TN + j) + r32;
+          if (n < count)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r4 = 0; r4 < 4; ++r4) {
+                typedef float Four __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<Four*>(q.kept + static_cast<int64_t>(n) * q.ld_kept + m0 + m_of(i, 4 * r4)) =
+                    Four{acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]};
+              }
         }
-      }
-      // (the smallest products first: x3 y1, x2 y2, x1 y3, x2 y1, x1 y2, x1 y1)
-#pragma unroll
-      for (int sum = PARTS - 1; sum >= 0; --sum)
-#pragma unroll
-        for (int px = sum; px >= 0; --px)
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = mma<M>(x[px][i], y[sum - px][j], acc[i][j]);
-    }
-  }
-
-  // Element r of acc[i][j]: m = m0 + 32 (wm TM + i) + 8 (r / 4) + 4 half + r % 4,  n = n0 + 32 (wn TN + j) + r32.
-  auto m_of = [&](int i, int r) { return 32 * (wm * TM + i) + 8 * (r / 4) + 4 * half + r % 4; };
-  if constexpr (JOB == kSums) {
-    __syncthreads();
-    float* join_at = reinterpret_cast<float*>(lds);  // [WM][3][BN]
-    const int64_t left = q.vocab - q.column0 - m0;   // columns of the tile that are there
-    if (PARTS > 1 && q.kept != nullptr)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int n = n0 + 32 * (wn * TN + j) + r32;
-        if (n < count)
+        const int64_t tok = n < count ? q.token[n] - q.column0 - m0 : -1;
+        float m = -INFINITY;
+        if (left < BM)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (m_of(i, r) >= left) acc[i][j][r] = -INFINITY;
+        if (__any(tok >= 0 && tok < BM))
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (m_of(i, r) == tok) q.x_token[n] = acc[i][j][r];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+        m = fmaxf(m, __shfl_xor(m, 32, kWave));
+        const float zero = m > -INFINITY ? m : 0.0f;
+        float s = 0.0f, e = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float t = (acc[i][j][r] - zero) * q.c, p = __builtin_amdgcn_exp2f(t);
+            s += p;
+            e = fmaf(p, fmaxf(t, kFloor), e);
+          }
+        s += __shfl_xor(s, 32, kWave);
+        e += __shfl_xor(e, 32, kWave);
+        if (half == 0) {
+          const int b = 32 * (wn * TN + j) + r32;
+          join_at[(wm * 3 + 0) * BN + b] = m;
+          join_at[(wm * 3 + 1) * BN + b] = s;
+          join_at[(wm * 3 + 2) * BN + b] = e;
+        }
+      }
+      __syncthreads();
+      for (int b = threadIdx.x; b < BN; b += kGemmThreads) {
+        if (n0 + b >= count) continue;
+        float m = -INFINITY, s = 0.0f, e = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WM; ++w) m = fmaxf(m, join_at[(w * 3) * BN + b]);
+#pragma unroll
+        for (int w = 0; w < WM; ++w) {
+          const float mw = join_at[(w * 3) * BN + b], sw = join_at[(w * 3 + 1) * BN + b], ew = join_at[(w * 3 + 2) * BN + b];
+          const float t = mw == m ? 0.0f : fmaxf((mw - m) * q.c, kFloor), f = __builtin_amdgcn_exp2f(t);
+          s = fmaf(sw, f, s);
+          e = fmaf(ew + sw * t, f, e);
+        }
+        const int64_t at = (q.tile0 + mt) * q.sum_rows + n0 + b;
+        q.tile_m[at] = m, q.tile_s[at] = s, q.tile_e[at] = e;
+      }
+    } else if constexpr (JOB == kDiffs) {
+      const int64_t left = q.vocab - q.column0 - m0;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + 32 * (wn * TN + j) + r32;
+        const bool live = n < count;
+        const int64_t tok = live ? q.token[n] - q.column0 - m0 : -1;
+        const float m = live ? q.row_m[n] : 0.0f, inv = live ? q.row_inv_s[n] * kLift<T> : 0.0f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - m) * q.c) * inv;
+            acc[i][j][r] = live && m_of(i, r) < left ? p : 0.0f;
+          }
+        if (__any(tok >= 0 && tok < BM))
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (m_of(i, r) == tok) acc[i][j][r] -= kLift<T>;
+      }
+      // Both layouts leave through LDS in 16-byte pieces: rows n of the tile's m, piece p at place p ^ n % 16 of its row.  (Rows of a tile past the gathered
+      // ones leave too, as zeros; columns up to the tile's end as well.)
+      static_assert(BN * BM * 2 <= STAGES * STAGE);
+      M* const rows = reinterpret_cast<M*>(lds);
+      const auto at = [](int n, int piece) { return n * BM + (piece ^ n % 16) * 8; };
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
-              typedef float Four __attribute__((ext_vector_type(4)));
-              *reinterpret_cast<Four*>(q.kept + static_cast<int64_t>(n) * q.ld_kept + m0 + m_of(i, 4 * r4)) =
-                  Four{acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]};
+              typedef M Four __attribute__((ext_vector_type(4)));
+              Four f;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                f[r] = static_cast<M>(acc[i][j][4 * r4 + r]);
+                if (part + 1 < PARTS) acc[i][j][4 * r4 + r] -= static_cast<float>(f[r]);
+              }
+              *reinterpret_cast<Four*>(rows + at(32 * (wn * TN + j) + r32, 4 * (wm * TM + i) + r4) + 4 * half) = f;
             }
-      }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + 32 * (wn * TN + j) + r32;
-      const int64_t tok = n < count ? q.token[n] - q.column0 - m0 : -1;
-      float m = -INFINITY;
-      if (left < BM)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (m_of(i, r) >= left) acc[i][j][r] = -INFINITY;
-      if (__any(tok >= 0 && tok < BM))
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (m_of(i, r) == tok) q.x_token[n] = acc[i][j][r];
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-      m = fmaxf(m, __shfl_xor(m, 32, kWave));
-      const float zero = m > -INFINITY ? m : 0.0f;
-      float s = 0.0f, e = 0.0f;
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float t = (acc[i][j][r] - zero) * q.c, p = __builtin_amdgcn_exp2f(t);
-          s += p;
-          e = fmaf(p, fmaxf(t, kFloor), e);
+        __syncthreads();
+        if (q.d != nullptr) {
+          M* const to = static_cast<M*>(q.d) + part * q.d_part + m0;
+          for (int k = threadIdx.x; k < BN * (BM / 8); k += kGemmThreads) {
+            const int n = k / (BM / 8), piece = k % (BM / 8);
+            if (n0 + n < q.n) *reinterpret_cast<u32x4*>(to + static_cast<int64_t>(n0 + n) * q.ld_d + piece * 8) = *reinterpret_cast<const u32x4*>(rows + at(n, piece));
+          }
         }
-      s += __shfl_xor(s, 32, kWave);
-      e += __shfl_xor(e, 32, kWave);
-      if (half == 0) {
-        const int b = 32 * (wn * TN + j) + r32;
-        join_at[(wm * 3 + 0) * BN + b] = m;
-        join_at[(wm * 3 + 1) * BN + b] = s;
-        join_at[(wm * 3 + 2) * BN + b] = e;
+        if (q.d_turned != nullptr) {
+          M* const to = static_cast<M*>(q.d_turned) + part * q.t_part + n0;
+          for (int k = threadIdx.x; k < (BN / 8) * (BM / 8); k += kGemmThreads) {
+            const int n = k % (BN / 8) * 8, piece = k / (BN / 8);
+            if (n0 + n >= q.n) continue;  // (q.n is a multiple of 64)
+            u32x4 x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const u32x4*>(rows + at(n + e, piece));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              u32x4 y;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) y[w] = __builtin_amdgcn_perm(x[2 * w + 1][e / 2], x[2 * w][e / 2], e % 2 != 0 ? 0x07060302u : 0x05040100u);
+              *reinterpret_cast<u32x4*>(to + static_cast<int64_t>(m0 + piece * 8 + e) * q.ld_t + n) = y;
+            }
+          }
+        }
       }
-    }
-    __syncthreads();
-    for (int b = threadIdx.x; b < BN; b += kGemmThreads) {
-      if (n0 + b >= count) continue;
-      float m = -INFINITY, s = 0.0f, e = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WM; ++w) m = fmaxf(m, join_at[(w * 3) * BN + b]);
-#pragma unroll
-      for (int w = 0; w < WM; ++w) {
-        const float mw = join_at[(w * 3) * BN + b], sw = join_at[(w * 3 + 1) * BN + b], ew = join_at[(w * 3 + 2) * BN + b];
-        const float t = mw == m ? 0.0f : fmaxf((mw - m) * q.c, kFloor), f = __builtin_amdgcn_exp2f(t);
-        s = fmaf(sw, f, s);
-        e = fmaf(ew + sw * t, f, e);
-      }
-      const int64_t at = (q.tile0 + mt) * q.sum_rows + n0 + b;
-      q.tile_m[at] = m, q.tile_s[at] = s, q.tile_e[at] = e;
-    }
-  } else if constexpr (JOB == kDiffs) {
-    const int64_t left = q.vocab - q.column0 - m0;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + 32 * (wn * TN + j) + r32;
-      const bool live = n < count;
-      const int64_t tok = live ? q.token[n] - q.column0 - m0 : -1;
-      const float m = live ? q.row_m[n] : 0.0f, inv = live ? q.row_inv_s[n] * kLift<T> : 0.0f;
+    } else if constexpr (JOB == kRowGrad) {
+      static_assert(TM == WN && TN == (BN == 32 ? 1 : 2));  // as sum_at()
+      // The sums lie as the lanes hold them, so that they are read and written whole (in rows, 16 bytes a row each time, a piece of 605 us for 16,384 columns
+      // of 6,144 rows of 2,048 took 140 of them for that): see sum_at().
+      typedef float Four __attribute__((ext_vector_type(4)));
+      const int area = slot == 0 ? tile : tiles + (tile - shares.whole) * (shares.slots - 1) + slot - 1;
+      Four* at = reinterpret_cast<Four*>(q.partial + static_cast<int64_t>(area) * (BN * BM)) + threadIdx.x;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - m) * q.c) * inv;
-          acc[i][j][r] = live && m_of(i, r) < left ? p : 0.0f;
+        for (int j = 0; j < TN; ++j) {
+          Four before[4];
+          if (q.add != 0)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) before[r4] = at[r4 * kGemmThreads];
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            Four sum;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[r] = acc[i][j][4 * r4 + r] * (1.0f / kLift<T>);
+            at[r4 * kGemmThreads] = q.add != 0 ? before[r4] + sum : sum;
+          }
+          at += 4 * kGemmThreads;
         }
-      if (__any(tok >= 0 && tok < BM))
+    } else {
+      const float factor = 1.0f / kLift<T> * (q.inv_temp / (q.denom > 0.0f ? q.denom : static_cast<float>(max(count, 1))));
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (m_of(i, r) == tok) acc[i][j][r] -= kLift<T>;
-    }
-    // Both layouts leave through LDS in 16-byte pieces: rows n of the tile's m, piece p at place p ^ n % 16 of its row.  (Rows of a tile past the gathered
-    // ones leave too, as zeros; columns up to the tile's end as well.)
-    static_assert(BN * BM * 2 <= STAGES * STAGE);
-    M* const rows = reinterpret_cast<M*>(lds);
-    const auto at = [](int n, int piece) { return n * BM + (piece ^ n % 16) * 8; };
-#pragma unroll
-    for (int part = 0; part < PARTS; ++part) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + 32 * (wn * TN + j) + r32;
+        if (n >= q.n) continue;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
-            typedef M Four __attribute__((ext_vector_type(4)));
-            Four f;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              f[r] = static_cast<M>(acc[i][j][4 * r4 + r]);
-              if (part + 1 < PARTS) acc[i][j][4 * r4 + r] -= static_cast<float>(f[r]);
-            }
-            *reinterpret_cast<Four*>(rows + at(32 * (wn * TN + j) + r32, 4 * (wm * TM + i) + r4) + 4 * half) = f;
-          }
-      __syncthreads();
-      if (q.d != nullptr) {
-        M* const to = static_cast<M*>(q.d) + part * q.d_part + m0;
-        for (int k = threadIdx.x; k < BN * (BM / 8); k += kGemmThreads) {
-          const int n = k / (BM / 8), piece = k % (BM / 8);
-          if (n0 + n < q.n) *reinterpret_cast<u32x4*>(to + static_cast<int64_t>(n0 + n) * q.ld_d + piece * 8) = *reinterpret_cast<const u32x4*>(rows + at(n, piece));
-        }
-      }
-      if (q.d_turned != nullptr) {
-        M* const to = static_cast<M*>(q.d_turned) + part * q.t_part + n0;
-        for (int k = threadIdx.x; k < (BN / 8) * (BM / 8); k += kGemmThreads) {
-          const int n = k % (BN / 8) * 8, piece = k / (BN / 8);
-          if (n0 + n >= q.n) continue;  // (q.n is a multiple of 64)
-          u32x4 x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const u32x4*>(rows + at(n + e, piece));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            u32x4 y;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) y[w] = __builtin_amdgcn_perm(x[2 * w + 1][e / 2], x[2 * w][e / 2], e % 2 != 0 ? 0x07060302u : 0x05040100u);
-            *reinterpret_cast<u32x4*>(to + static_cast<int64_t>(m0 + piece * 8 + e) * q.ld_t + n) = y;
-          }
-        }
-      }
-    }
-  } else {
-    const float factor = 1.0f / kLift<T> * (JOB == kWeightGrad ? q.inv_temp / (q.denom > 0.0f ? q.denom : static_cast<float>(max(count, 1))) : 1.0f);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + 32 * (wn * TN + j) + r32;
-      if (n >= q.n) continue;
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int m = m0 + m_of(i, 4 * r4);
-          if constexpr (JOB == kRowGrad) {
-            float* at = q.partial + (static_cast<int64_t>(slice) * n_there * BN + n) * q.m + m;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (m + r < q.m) at[r] = q.add != 0 ? at[r] + acc[i][j][4 * r4 + r] * factor : acc[i][j][4 * r4 + r] * factor;
-          } else {
+            const int m = m0 + m_of(i, 4 * r4);
             T* at = static_cast<T*>(q.out) + static_cast<int64_t>(n) * q.ld_out + m;
             if (m + 4 <= q.m) {
               typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -410,8 +456,10 @@ __global__ __launch_bounds__(kGemmThreads, 1) void linear_gemm_kernel(const Gemm
                 if (m + r < q.m) at[r] = static_cast<T>(acc[i][j][4 * r4 + r] * factor);
             }
           }
-        }
+      }
     }
+    if (JOB != kRowGrad || tile == last_tile) break;
+    __syncthreads();  // the next tile's stages come where this one's are read
   }
 }
 
@@ -657,27 +705,57 @@ __global__ __launch_bounds__(kRowThreads) void linear_stats_kernel(const RowArgs
   q.a.stats[3] = 0.0f;
 }
 
-// d_hidden: the slices' sums of each row, zeros where a row does not count.
+// Where linear_gemm_kernel's lanes leave a tile's sums of n and of m .. m + 3, m a multiple of 4.
+__device__ __forceinline__ int sum_at(int n, int m, int n_tile) {
+  const int tn = n_tile == 32 ? 1 : 2, wn = n_tile / (32 * tn), tm = wn;  // (256 m by 8 / wn waves of tm tiles of 32)
+  const int thread = (m / (32 * tm) * wn + n / (32 * tn)) * kWave + m / 4 % 2 * 32 + n % 32;
+  return (((m / 32 % tm * tn + n / 32 % tn) * 4 + m / 8 % 4) * kGemmThreads + thread) * 4;
+}
+
+// d_hidden: the shares' sums of each row, zeros where a row does not count.  A block takes 8 rows, whose sums lie side by side if they all count (a row a block
+// reads eighths of lines: 107 us for 6,144 rows of 2,048).
+constexpr int kGradRows = 8, kGradColumns = kPackThreads / kGradRows * 4;
 template <class T>
 __global__ __launch_bounds__(kPackThreads) void linear_row_grad_kernel(const RowArgs q) {
-  const int64_t r = blockIdx.x;
+  typedef float Four __attribute__((ext_vector_type(4)));
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * kGradRows + threadIdx.x % kGradRows;
+  if (r >= q.a.rows) return;
   const int32_t n = q.gathered[r];
   T* to = static_cast<T*>(q.a.d_hidden) + r * q.a.ld_d_hidden;
   const float factor = static_cast<float>(1.0 / (q.a.temperature * (q.a.denom > 0.0 ? q.a.denom : static_cast<double>(max(*q.count, 1)))));
-  const int64_t n_there = ceil_div(*q.count, q.n_tile), slice_size = n_there * q.n_tile * q.a.dim;
-  const int slices = slices_of(static_cast<int>(ceil_div(q.a.dim, kTileM) * n_there), q.cus, q.all_steps);
-  for (int64_t k = threadIdx.x; k < q.a.dim; k += kPackThreads) {
-    float x = 0.0f;
-    constexpr int AHEAD = 8;
-    if (n >= 0)
-      for (int s = 0; s < slices; s += AHEAD) {
-        float y[AHEAD];
+  const int n_there = static_cast<int>(ceil_div(*q.count, q.n_tile)), m_tiles = static_cast<int>(ceil_div(q.a.dim, kTileM)), tiles = m_tiles * n_there;
+  const Shares shares = shares_of(tiles, q.cus, q.all_steps);
+  const int nt = n / q.n_tile, first_n = nt / 4 * 4, wide = min(4, n_there - first_n);
+  const int64_t area = static_cast<int64_t>(q.n_tile) * kTileM;
+#pragma unroll 4
+  for (int k = blockIdx.y * kGradColumns + threadIdx.x / kGradRows * 4; k < q.a.dim; k += gridDim.y * kGradColumns) {
+    Four x{};
+    if (n >= 0) {
+      const int tile = first_n * m_tiles + k / kTileM * wide + nt - first_n, slots = tile < shares.whole ? 0 : shares.slots - 1;
+      const float* at = q.partial + tile * area + sum_at(n % q.n_tile, k % kTileM, q.n_tile);
+      x = *reinterpret_cast<const Four*>(at);
+      at += (tiles - tile + static_cast<int64_t>(tile - shares.whole) * slots) * area;
+      constexpr int AHEAD = 8;
+      for (int s = 0; s < slots; s += AHEAD) {
+        Four y[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) y[u] = q.partial[min(s + u, slices - 1) * slice_size + n * q.a.dim + k];
+        for (int u = 0; u < AHEAD; ++u) y[u] = *reinterpret_cast<const Four*>(at + min(s + u, slots - 1) * area);
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) x += s + u < slices ? y[u] : 0.0f;
+        for (int u = 0; u < AHEAD; ++u)
+          if (s + u < slots) x += y[u];
       }
-    to[k] = static_cast<T>(x * factor);
+    }
+    if (k + 4 <= q.a.dim) {
+      typedef T Out __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+      Out o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(x[e] * factor);
+      *reinterpret_cast<Out*>(to + k) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k + e < q.a.dim) to[k + e] = static_cast<T>(x[e] * factor);
+    }
   }
 }
 
@@ -742,8 +820,7 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
     if (a.d_hidden != nullptr) {
       p.weight_turned = room(p.parts * a.dim * p.piece * 2);
       p.d = room(p.parts * p.rows * p.piece * 2);
-      // (as slices_of() cuts them: one of all rows, or blocks for two rounds and less than half a one)
-      p.partial = room(std::max<size_t>(up(p.rows, p.n_tile) * a.dim, ceil_div(5 * cus / 2, ceil_div(a.dim, kTileM)) * p.n_tile * a.dim) * 4);
+      p.partial = room((ceil_div(p.rows, p.n_tile) * ceil_div(a.dim, kTileM) + cus) * p.n_tile * kTileM * 4);  // (shares_of(): more than one less than cus times)
     }
     if (a.d_weight != nullptr) {
       p.hidden_turned = room(p.parts * a.dim * p.rows * 2);
@@ -760,7 +837,7 @@ int launch_gemm(GemmArgs g, int n_tile, hipStream_t st) {
   g.m_tiles = static_cast<int32_t>(ceil_div(g.m, kTileM));
   g.n_tiles = static_cast<int32_t>(ceil_div(g.n, n_tile));
   g.xcds = std::max(1, device_info().xcds);
-  const dim3 grid(static_cast<uint32_t>(up(static_cast<int64_t>(g.m_tiles) * g.n_tiles + (JOB == kRowGrad ? 2 * g.cus : 0), g.xcds)));
+  const dim3 grid(static_cast<uint32_t>(up(static_cast<int64_t>(g.m_tiles) * g.n_tiles, g.xcds) + (JOB == kRowGrad ? up(g.cus, g.xcds) : 0)));
 #define PPO_GEMM(...) hipLaunchKernelGGL((linear_gemm_kernel<T, __VA_ARGS__, JOB>), grid, dim3(kGemmThreads), 0, st, g)
   if constexpr (sizeof(T) == 2)
     if (n_tile == 256) PPO_GEMM(2, 4, 4, 2);
@@ -890,7 +967,8 @@ int run_typed(const ppo_linear_loss_args& a, const Plan& p, char* ws, hipStream_
     g.x = weight, g.y = hidden;
   }
   if (to_hidden && a.rows > 0) {
-    hipLaunchKernelGGL(linear_row_grad_kernel<T>, dim3(static_cast<uint32_t>(a.rows)), dim3(kPackThreads), 0, st, r);
+    const int64_t blocks = ceil_div(a.rows, kGradRows), columns = std::min(ceil_div(a.dim, kGradColumns), ceil_div(4 * p.cus, blocks));
+    hipLaunchKernelGGL(linear_row_grad_kernel<T>, dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(columns)), dim3(kPackThreads), 0, st, r);
     return check_launch("linear_row_grad_kernel");
   }
   return PPO_OK;
