@@ -47,6 +47,10 @@ def _run(ops, d, temperature=1.0, denom=None, mask=True, grads=(True, True)):
     return dict(d_hidden=dh, d_weight=dw, stats=stats, logp=lp, entropy=ent)
 
 
+def _within(got, want, bound, what):
+    _inside(got, want, bound.cpu(), what)
+
+
 def _check(s, got, temperature=1.0, denom=None, mask=True):
     dtype, (rows, dim), vocab = s["h"].dtype, s["h"].shape, s["w"].shape[0]
     want = ref.linear_cross_entropy(s["h"], s["w"], s["tok"], s["mask"] if mask else None, temperature, denom)
@@ -58,11 +62,11 @@ def _check(s, got, temperature=1.0, denom=None, mask=True):
     zmax = (z - z.amax(1, keepdim=True)).abs().clamp(max=110).amax(1)
     counts = want["logp"] != 0
     at = torch.where(counts | (want["entropy"] != 0), 2 * dz + E, torch.zeros_like(E))
-    _inside(got["logp"], want["logp"], at + U * want["logp"].abs(), "logp")
-    _inside(got["entropy"], want["entropy"], at * (2 + zmax), "entropy")
+    _within(got["logp"], want["logp"], at + U * want["logp"].abs(), "logp")
+    _within(got["entropy"], want["entropy"], at * (2 + zmax), "entropy")
     n = float(want["stats"][2]) if denom is None else denom
-    _inside(got["stats"][:1], want["stats"][:1], (at + U * want["logp"].abs()).sum()[None] / max(n, 1e-30) + 2 * U * want["stats"][:1].abs(), "loss")
-    _inside(got["stats"][1:2], want["stats"][1:2], (at * (2 + zmax)).sum()[None] / max(n, 1e-30) + 2 * U * want["stats"][1:2].abs(), "mean entropy")
+    _within(got["stats"][:1], want["stats"][:1], (at + U * want["logp"].abs()).sum()[None] / max(n, 1e-30) + 2 * U * want["stats"][:1].abs(), "loss")
+    _within(got["stats"][1:2], want["stats"][1:2], (at * (2 + zmax)).sum()[None] / max(n, 1e-30) + 2 * U * want["stats"][1:2].abs(), "mean entropy")
     assert float(got["stats"][2]) == float(want["stats"][2]) and float(got["stats"][3]) == 0.0
     k = 1.0 / (max(n, 1.0) if denom is None else n) / temperature
     p = torch.exp(z - torch.logsumexp(z, 1, keepdim=True))
@@ -71,10 +75,10 @@ def _check(s, got, temperature=1.0, denom=None, mask=True):
     safe = torch.where((want["d"] != 0).any(1)[:, None], h, torch.zeros_like(h))
     if got["d_hidden"] is not None:
         bound = k * (off @ w.abs() + (vocab + 64) * U * (want["d"].abs() @ w.abs()))
-        _inside(got["d_hidden"], want["d_hidden"], bound + (1.01 * HALF[dtype] + 4 * U) * want["d_hidden"].abs() + TINY[dtype], "d_hidden")
+        _within(got["d_hidden"], want["d_hidden"], bound + (1.01 * HALF[dtype] + 4 * U) * want["d_hidden"].abs() + TINY[dtype], "d_hidden")
     if got["d_weight"] is not None:
         bound = k * (off.t() @ safe.abs() + (rows + 64) * U * (want["d"].abs().t() @ safe.abs()))
-        _inside(got["d_weight"], want["d_weight"], bound + (1.01 * HALF[dtype] + 4 * U) * want["d_weight"].abs() + TINY[dtype], "d_weight")
+        _within(got["d_weight"], want["d_weight"], bound + (1.01 * HALF[dtype] + 4 * U) * want["d_weight"].abs() + TINY[dtype], "d_weight")
 
 
 SIZES = [(1, 1, 1), (1, 7, 3), (2, 255, 64), (8, 1000, 128), (33, 256, 65), (32, 257, 8), (100, 513, 200), (129, 2049, 64), (300, 1000, 40), (700, 515, 77),
@@ -161,3 +165,16 @@ def test_peaked_and_far_logits(cuda, dtype):
     s["h"][:20] = (40 * s["h"][:20].float()).to(dtype)
     d = {k: v.to(cuda) for k, v in s.items()}
     _check(s, _run(ops, d))
+
+
+# On 256 compute units and tiles of 256 x 256 (fp32: 128 rows): fewer than half a round of d_hidden's tiles, cut along the columns; more, some of whose columns go
+# to the units left over, one and two of them and in two pieces of the vocabulary; a whole round and some more.
+@pytest.mark.parametrize("dtype,rows,vocab,dim", [(BF16, 2500, 1500, 2304), (BF16, 4200, 1500, 2304), (F16, 4200, 1300, 2300), (F32, 2100, 1500, 2304),
+                                                  (BF16, 5900, 40000, 2304), (BF16, 9000, 1500, 2304), (F32, 4500, 1025, 2100)])
+def test_many_tiles(cuda, dtype, rows, vocab, dim):
+    ops = _ops()
+    d = {k: v.to(cuda) for k, v in _case(rows, rows, vocab, dim, dtype, masked=0.02).items()}
+    got = _run(ops, d)
+    _check(d, got)
+    again = _run(ops, d)
+    assert all(torch.equal(got[k], again[k]) for k in got)

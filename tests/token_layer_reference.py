@@ -147,21 +147,22 @@ def linear_cross_entropy(hidden, weight, tokens, mask=None, temperature=1.0, den
         counts &= mask != 0
     n = float(denom) if denom is not None else max(1.0, float(counts.sum()))
     h, w = hidden.double(), weight.double()
-    out = {"logp": torch.zeros(rows, dtype=torch.float64), "entropy": torch.zeros(rows, dtype=torch.float64), "d": torch.zeros(rows, vocab, dtype=torch.float64)}
+    zeros = lambda *sizes: torch.zeros(*sizes, dtype=torch.float64, device=hidden.device)  # noqa: E731
+    out = {"logp": zeros(rows), "entropy": zeros(rows), "d": zeros(rows, vocab)}
     at = counts.nonzero()[:, 0]
     z = (h[at] @ w.t()) / temperature
     z = z - z.amax(1, keepdim=True)
     p = torch.exp(z) / torch.exp(z).sum(1, keepdim=True)
     logs = z - torch.log(torch.exp(z).sum(1, keepdim=True))
     t = tokens[at].long()
-    out["logp"][at] = logs[torch.arange(len(at)), t]
+    out["logp"][at] = logs[torch.arange(len(at), device=t.device), t]
     out["entropy"][at] = -(p * logs).sum(1)
     d = p.clone()
-    d[torch.arange(len(at)), t] -= 1.0
+    d[torch.arange(len(at), device=t.device), t] -= 1.0
     out["d"][at] = d
     safe = torch.where(counts[:, None], h, torch.zeros_like(h))
     out["d_hidden"] = out["d"] @ w / (n * temperature)
     out["d_weight"] = out["d"].t() @ safe / (n * temperature)
     out["stats"] = torch.tensor([-float(out["logp"].sum()) / n, float(out["entropy"].sum()) / n, float(denom) if denom is not None else float(counts.sum()), 0.0],
-                                dtype=torch.float64)
+                                dtype=torch.float64, device=hidden.device)
     return out
