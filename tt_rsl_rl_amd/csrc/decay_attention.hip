@@ -135,7 +135,8 @@ struct MixArgs {
   int32_t carried;      // carry holds what enters the segments already
   int32_t exact;        // states come out, in fp32: three parts of what makes them
   int32_t tokens, segment, segments;
-  int32_t heads, ga, gb;  // heads of b, c and S times gb; of a per head
+  int32_t heads, ga, gb;  // heads of b, c and S times gb; of a per head and block
+  int32_t spread;         // blocks that share a's heads of a head
   int32_t db, dc;
   int32_t reverse, w, cut;  // cut: chunks end with their sequence
   int32_t lost;             // states come in, which need not be finite
@@ -317,6 +318,7 @@ template <class T, class M, int DBT, int NT, bool STATE_ONLY>
 __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q) {
   typedef Math<M> X;
   typedef typename X::Frag Frag;
+  static_assert(2 * kWaves * 16 >= PPO_DECAY_MAX_DIM);
   constexpr int C = X::CHUNK, K = X::K, Q = X::QUADS, DB = DBT * 16, DC = kWaves * NT * 16, IT = C / 16, V = kVec<T>;
   constexpr int PARTS = X::PARTS2;
   typedef Natural<M, DB> Rows_;
@@ -333,7 +335,8 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int head = blockIdx.y, seg = blockIdx.x;
-  const int col0 = NT == 1 ? blockIdx.z * DC : 0;  // a block has DC of c's columns
+  const int columns = NT == 1 && q.dc > DC ? 2 : 1, share = blockIdx.z / columns, col0 = blockIdx.z % columns * DC;  // a block has DC of c's columns
+  const int a_head = (head * q.spread + share) * q.ga;
   const int own0 = wave * NT * 16, dc0 = col0 + own0;
   const bool works = dc0 < q.dc;
   const int seg_begin = seg * q.segment, seg_end = min(seg_begin + q.segment, q.tokens);
@@ -375,7 +378,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     d = i % pieces * V;
   };
   auto load_rows = [&](int begin, int n, int ab) {
-    const int ha = q.ga > 1 ? head * q.ga + ab : head, hb = q.gb > 1 ? head * q.gb + ab : head;
+    const int ha = q.ga > 1 ? a_head + ab : a_head, hb = q.gb > 1 ? head * q.gb + ab : head;
     const int64_t lowest = q.reverse ? q.tokens - begin - n : begin;
     int thread = threadIdx.x;
     forget(thread);  // (addresses again)
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
           if (turned != nullptr) turned[Cols_::at(d, j / Cols_::PIECE) + j % Cols_::PIECE] = static_cast<M>(x);
         }
       };
-      const int ha = q.ga > 1 ? head * q.ga + ab : head, hb = q.gb > 1 ? head * q.gb + ab : head;
+      const int ha = q.ga > 1 ? a_head + ab : a_head, hb = q.gb > 1 ? head * q.gb + ab : head;
       if (new_a) elements(q.a, ha, q.db, 0, DB, a_rows, nullptr);
       elements(q.b, hb, q.db, 0, DB, STATE_ONLY ? nullptr : b_rows, b_turned);
       if (new_b) elements(q.c, hb, q.dc, col0, DC, nullptr, c_turned);
@@ -623,7 +626,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
           }
         // ---- the outputs ----
         if (q.ga > 1 || ab == q.gb - 1) {
-          const int ha = q.ga > 1 ? head * q.ga + ab : head, d = dc0 + 4 * NT * g;
+          const int ha = q.ga > 1 ? a_head + ab : a_head, d = dc0 + 4 * NT * g;
           const int64_t lowest = q.reverse ? q.tokens - begin - n : begin;
           T* const to = static_cast<T*>(q.out.data) + ha * q.out.head_stride + lowest * q.out.token_stride;
           if (q.near) {
@@ -720,7 +723,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     }
     if (ab == abs - 1) {
       fresh = false;
-      if (!STATE_ONLY && q.s_out != nullptr && works && seq >= 0 && last[buffer][p + n - 1] == begin + n) {
+      if (!STATE_ONLY && q.s_out != nullptr && share == 0 && works && seq >= 0 && last[buffer][p + n - 1] == begin + n) {
         float* to = q.s_out + (static_cast<int64_t>(seqs[buffer][p + n - 1]) * q.heads + head) * q.state_size;
         each_state([&](float s, int i, int j) {
           if (i < q.db && j < q.dc) to[i * q.si + j * q.sj] = s;
@@ -746,14 +749,18 @@ struct Plan {
 
 // Segments: as many as give the chip two blocks a compute unit (a segment's state is written and read four times), down to a chunk each: a block alone
 // on its compute unit takes 5 to 7 us a chunk, waiting (577 tokens of 3 heads, fp32, the whole call: segments of four chunks 120 us, of one 47).
-Plan plan_of(int64_t tokens, int heads, int chunk) {
+// Where states make a piece of each sequence, segments go down to the sequences' mean length.
+Plan plan_of(const ppo_decay_attention_args& a) {
+  const int chunk = a.type == PPO_TYPE_BF16 ? Math<__bf16>::CHUNK : Math<float>::CHUNK;
+  const bool states = a.initial_state != nullptr || a.final_state != nullptr || a.d_final_state != nullptr || a.d_initial_state != nullptr;
+  const int64_t least = states ? std::min<int64_t>(std::max<int64_t>(a.tokens / a.sequences, 1), chunk) : chunk;
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
-  const int64_t want = std::max<int64_t>(1, ceil_div(2 * cus, heads)), chunks = ceil_div(tokens, chunk);
-  const int64_t n = std::max<int64_t>(1, std::min(want, chunks));
+  const int64_t want = std::max<int64_t>(1, ceil_div(2 * cus, a.kv_heads)), pieces = ceil_div(a.tokens, least);
+  const int64_t n = std::max<int64_t>(1, std::min(want, pieces));
   Plan p;
-  p.segment = static_cast<int>(ceil_div(std::max<int64_t>(chunks, 1), n) * chunk);
-  p.segments = static_cast<int>(std::max<int64_t>(1, ceil_div(tokens, p.segment)));
+  p.segment = static_cast<int>(ceil_div(std::max<int64_t>(pieces, 1), n) * least);
+  p.segments = static_cast<int>(std::max<int64_t>(1, ceil_div(a.tokens, p.segment)));
   return p;
 }
 
@@ -762,14 +769,19 @@ int launch_mix(const MixArgs& q, hipStream_t st) {
   const uint32_t heads = static_cast<uint32_t>(q.heads), columns = static_cast<uint32_t>(ceil_div(q.dc, kWaves * NT * 16));
   if (q.segments > 1 && q.carried == 0) {
     MixArgs own = q;
-    own.ga = 1;  // (no outputs, so no a)
+    own.ga = own.spread = 1;  // (no outputs, so no a)
     hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, true>), dim3(static_cast<uint32_t>(q.segments - 1), heads, columns), dim3(kThreads), 0, st, own);
     if (int rc = check_launch("decay_mix_kernel")) return rc;
     const int64_t size = static_cast<int64_t>(q.db) * q.dc;
     hipLaunchKernelGGL(decay_scan_kernel, dim3(static_cast<uint32_t>(ceil_div(size, kScanThreads)), heads), dim3(kScanThreads), 0, st, q);
     if (int rc = check_launch("decay_scan_kernel")) return rc;
   }
-  hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, false>), dim3(static_cast<uint32_t>(q.segments), heads, columns), dim3(kThreads), 0, st, q);
+  // a's heads one to a block, or a few, where that many blocks still find a compute unit each
+  MixArgs whole = q;
+  whole.spread = q.ga;
+  while (whole.spread > 1 && (q.ga % whole.spread != 0 || static_cast<int64_t>(q.segments) * heads * columns * whole.spread > device_info().cus)) --whole.spread;
+  whole.ga = q.ga / whole.spread;
+  hipLaunchKernelGGL((decay_mix_kernel<T, M, DBT, NT, false>), dim3(static_cast<uint32_t>(q.segments), heads, columns * whole.spread), dim3(kThreads), 0, st, whole);
   return check_launch("decay_mix_kernel");
 }
 
@@ -786,8 +798,7 @@ struct Layout {
   size_t spans, carry, copy, bytes;  // copy 0: none needed
 };
 Layout layout_of(const ppo_decay_attention_args& a) {
-  const int chunk = a.type == PPO_TYPE_BF16 ? Math<__bf16>::CHUNK : Math<float>::CHUNK;
-  const Plan p = plan_of(a.tokens, a.kv_heads, chunk);
+  const Plan p = plan_of(a);
   Layout l;
   l.spans = 256;
   l.carry = l.spans + (a.cu_seqlens != nullptr ? static_cast<size_t>(ceil_div(a.tokens * sizeof(Span), 256)) * 256 : 0);
@@ -872,7 +883,7 @@ int prepare(const char* who, const ppo_decay_attention_args& a, const float*& fr
   const Layout l = layout_of(a);
   PPO_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= l.bytes,
               "%s: workspace too small or not 16-byte aligned (%zu < %zu)", who, workspace_bytes, l.bytes);
-  const Plan p = plan_of(a.tokens, a.kv_heads, a.type == PPO_TYPE_BF16 ? Math<__bf16>::CHUNK : Math<float>::CHUNK);
+  const Plan p = plan_of(a);
   char* base = static_cast<char*>(workspace);
   Span* spans = a.cu_seqlens != nullptr ? reinterpret_cast<Span*>(base + l.spans) : nullptr;
   q = MixArgs{};
