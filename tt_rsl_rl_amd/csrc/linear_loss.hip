@@ -535,16 +535,22 @@ __device__ __forceinline__ void store_parts(M* at, int64_t part, float x) {
 }
 
 constexpr int kPackThreads = 256;
+// A block: some thousand elements of whole rows (80,542 rows of 64, a row a block: 22 us for 21 MB, so 10).
+int64_t pack_rows(int64_t ld_dst) { return std::max<int64_t>(1, 4 * kPackThreads / ld_dst); }
 template <class T>
-__global__ __launch_bounds__(kPackThreads) void linear_pack_kernel(const PackArgs q) {
+__global__ __launch_bounds__(kPackThreads) void linear_pack_kernel(const PackArgs q, int rows_each) {
   typedef typename Half<T>::type M;
-  const int64_t row = blockIdx.x;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_each;
   const int64_t rows = q.count != nullptr ? static_cast<int64_t>(*q.count) : q.rows;
-  const T* from = nullptr;
-  if (row < rows) from = static_cast<const T*>(q.src) + (q.source != nullptr ? q.source[row] : row) * q.ld;
-  M* to = static_cast<M*>(q.dst) + row * q.ld_dst;
-  for (int64_t k = threadIdx.x; k < q.ld_dst; k += kPackThreads)
-    store_parts<T>(to + k, q.part, from != nullptr && k < q.dim ? static_cast<float>(from[k]) : 0.0f);
+  const uint32_t width = static_cast<uint32_t>(q.ld_dst), all = static_cast<uint32_t>(min(static_cast<int64_t>(rows_each), q.out_rows - row0)) * width;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < all; i += kPackThreads) {
+    const int64_t row = row0 + i / width;
+    const uint32_t k = i % width;
+    float x = 0.0f;
+    if (row < rows && k < q.dim) x = static_cast<float>(static_cast<const T*>(q.src)[(q.source != nullptr ? q.source[row] : row) * q.ld + k]);
+    store_parts<T>(static_cast<M*>(q.dst) + row * q.ld_dst + k, q.part, x);
+  }
 }
 
 // turned[k][row], and dst[row][k] where it is wanted: 64 x 64 tiles through LDS.
@@ -647,8 +653,8 @@ __device__ __forceinline__ void add_sums(float& s, float& e, float m, float mt, 
   e = fmaf(et + st * d, f, e);
 }
 
-// A block: 16 rows (the tiles' sums of a row lie rows apart, so neighbouring lanes take neighbouring rows) by 16 groups of tiles.
-constexpr int kJoinThreads = 256, kJoinRows = 16, kJoinGroups = kJoinThreads / kJoinRows;
+// A block: 16 rows (the tiles' sums of a row lie rows apart, so neighbouring lanes take neighbouring rows) by 64 groups of tiles, so that 512 tiles (131,072 columns) are one round of loads (16 groups, four rounds: 8 rows 11.6 us, so 8).
+constexpr int kJoinThreads = 1024, kJoinRows = 16, kJoinGroups = kJoinThreads / kJoinRows;
 __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const RowArgs q) {
   __shared__ float part_m[kJoinGroups][kJoinRows], part_s[kJoinGroups][kJoinRows], part_e[kJoinGroups][kJoinRows];
   const int32_t count = *q.count;
@@ -675,11 +681,18 @@ __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const RowArgs
     for (int u = 0; u < AHEAD; ++u) add_sums(s, e, m, mt[u], t + u * kJoinGroups < q.tiles ? st[u] : 0.0f, et[u], q.c);
   }
   part_m[group][row] = m, part_s[group][row] = s, part_e[group][row] = e;
-  __syncthreads();
+  for (int half = kJoinGroups / 2; half > 0; half /= 2) {  // (in pairs: the same order every time)
+    __syncthreads();
+    if (group >= half) continue;
+    const float mo = part_m[group + half][row], before = m;
+    m = fmaxf(m, mo);
+    float s2 = 0.0f, e2 = 0.0f;
+    add_sums(s2, e2, m, before, s, e, q.c);
+    add_sums(s2, e2, m, mo, part_s[group + half][row], part_e[group + half][row], q.c);
+    s = s2, e = e2;
+    part_m[group][row] = m, part_s[group][row] = s, part_e[group][row] = e;
+  }
   if (group != 0 || n >= count) return;
-  for (int g = 1; g < kJoinGroups; ++g) m = fmaxf(m, part_m[g][row]);
-  s = e = 0.0f;
-  for (int g = 0; g < kJoinGroups; ++g) add_sums(s, e, m, part_m[g][row], part_s[g][row], part_e[g][row], q.c);
   const float log2_s = log2f(s), lp = kLn2 * ((q.x_token[n] - m) * q.c - log2_s), h = kLn2 * (log2_s - e / s);
   q.row_m[n] = m, q.row_inv_s[n] = 1.0f / s, q.row_lp[n] = lp, q.row_h[n] = h;
   const int32_t r = q.source[n];
@@ -771,8 +784,18 @@ struct Plan {
 
 int64_t up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
 
+// Narrower tiles of n where their blocks, too, find a compute unit each (4,524 rows, 6,290 columns of 33: the weight's gradient in 25 blocks of 256 columns
+// 95 us, in 197 of 32 36).
+int narrow(int n_tile, int64_t m_tiles, int64_t n, int64_t cus) {
+  if (n_tile == 256 && 2 * m_tiles * ceil_div(n, 256) <= cus) n_tile = 128;
+  if (n_tile == 128 && 4 * m_tiles * ceil_div(n, 128) <= cus) n_tile = 32;
+  return n_tile;
+}
+
 Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   Plan p{};
+  int64_t cus = device_info().cus;
+  if (cus <= 0) cus = 256;
   p.parts = a.type == PPO_TYPE_F32 ? kMaxParts : 1;
   p.rows = up(std::max<int64_t>(a.rows, 1), kTileK);
   p.k = up(a.dim, kTileK);
@@ -780,14 +803,13 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   const int64_t column = 2 * p.parts * ((gradient ? (a.d_hidden != nullptr) + (a.d_weight != nullptr) : 0) * p.rows + (p.direct ? 0 : p.k) +
                                          (gradient && a.d_hidden != nullptr ? a.dim : 0));
   p.n_tile = a.rows <= 32 ? 32 : a.type == PPO_TYPE_F32 || a.rows <= 128 || (a.rows > 256 && a.rows <= 384) ? 128 : 256;
+  p.n_tile = narrow(p.n_tile, ceil_div(a.vocab, kTileM), a.rows, cus);
   int64_t piece = kPieceBytes / std::max<int64_t>(column, 1) / kTileM * kTileM;
   piece = std::min(std::max(piece, kMinPiece), int64_t{1} << 21);  // (a tile of d's offsets stay in 31 bits)
   if (!gradient && p.direct) piece = up(a.vocab, kTileM);
   piece = std::min(piece, kMostTiles / ceil_div(p.rows, p.n_tile) * kTileM);
   if (gradient) piece = std::min(piece, kMostTiles / ceil_div(a.dim, kTileM) * 128);
   p.piece = std::min(piece, up(a.vocab, kTileM));
-  int64_t cus = device_info().cus;
-  if (cus <= 0) cus = 256;
   p.pieces = ceil_div(a.vocab, p.piece);
   if (p.pieces > 1) {
     // columns whose d_weight takes whole rounds of the chip's blocks, or else pieces of one size (8,192 x 131,072 of 2,048: 16,384 columns 512 blocks and two rounds,
@@ -833,18 +855,16 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
 
 template <class T, int JOB>
 int launch_gemm(GemmArgs g, int n_tile, hipStream_t st) {
-  if (JOB == kWeightGrad) n_tile = sizeof(T) == 4 ? 128 : 256;  // n is the vocabulary there
   g.m_tiles = static_cast<int32_t>(ceil_div(g.m, kTileM));
+  if (JOB == kWeightGrad) n_tile = narrow(sizeof(T) == 4 ? 128 : 256, g.m_tiles, g.n, g.cus);  // n is the vocabulary there
   g.n_tiles = static_cast<int32_t>(ceil_div(g.n, n_tile));
   g.xcds = std::max(1, device_info().xcds);
   const dim3 grid(static_cast<uint32_t>(up(static_cast<int64_t>(g.m_tiles) * g.n_tiles, g.xcds) + (JOB == kRowGrad ? up(g.cus, g.xcds) : 0)));
 #define PPO_GEMM(...) hipLaunchKernelGGL((linear_gemm_kernel<T, __VA_ARGS__, JOB>), grid, dim3(kGemmThreads), 0, st, g)
   if constexpr (sizeof(T) == 2)
     if (n_tile == 256) PPO_GEMM(2, 4, 4, 2);
-  if constexpr (sizeof(T) == 4 || JOB != kWeightGrad)
-    if (n_tile == 128) PPO_GEMM(4, 2, 2, 2);
-  if constexpr (JOB != kWeightGrad)
-    if (n_tile == 32) PPO_GEMM(8, 1, 1, 1);
+  if (n_tile == 128) PPO_GEMM(4, 2, 2, 2);
+  if (n_tile == 32) PPO_GEMM(8, 1, 1, 1);
 #undef PPO_GEMM
   return check_launch("linear_gemm_kernel");
 }
@@ -882,7 +902,7 @@ int run_typed(const ppo_linear_loss_args& a, const Plan& p, char* ws, hipStream_
       hipLaunchKernelGGL(linear_turn_kernel<T>, dim3(static_cast<uint32_t>(ceil_div(n, 64)), static_cast<uint32_t>(p.k / 64)), dim3(kPackThreads), 0, st, w);
       return check_launch("linear_turn_kernel");
     }
-    hipLaunchKernelGGL(linear_pack_kernel<T>, dim3(static_cast<uint32_t>(n)), dim3(kPackThreads), 0, st, w);
+    hipLaunchKernelGGL(linear_pack_kernel<T>, dim3(static_cast<uint32_t>(ceil_div(n, pack_rows(p.k)))), dim3(kPackThreads), 0, st, w, static_cast<int>(pack_rows(p.k)));
     return check_launch("linear_pack_kernel");
   };
   if (int rc = pack(a.hidden, a.ld_hidden, p.rows, true, ws + p.hidden, p.rows * p.k, to_weight ? ws + p.hidden_turned : nullptr, p.rows, a.dim * p.rows)) return rc;
@@ -962,6 +982,7 @@ int run_typed(const ppo_linear_loss_args& a, const Plan& p, char* ws, hipStream_
       b.n = static_cast<int32_t>(n);
       b.out = static_cast<char*>(a.d_weight) + v0 * a.ld_d_weight * size;
       b.ld_out = a.ld_d_weight;
+      b.cus = p.cus;
       if (int rc = launch_gemm<T, kWeightGrad>(b, p.n_tile, st)) return rc;
     }
     g.x = weight, g.y = hidden;
