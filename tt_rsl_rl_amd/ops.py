@@ -1393,8 +1393,8 @@ def decay_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
     of one type, float32, bfloat16 or float16 (views of any token and head strides; query heads share key-value heads in groups of
     neighbours); log_decay float32 [kv_heads].  Sequence b is tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1 (int64 or int32, on the GPU;
     None: one sequence); tokens outside are left as they are.  States are float32 [sequences, kv_heads, key_dim, value_dim], what a sequence
-    starts from (None: zeros) and ends with; final_state may be initial_state.  Key and value heads of up to 128 elements.  A token whose key
-    or value is not finite makes NaN of its heads' results from there to its sequence's end, and of no others."""
+    starts from (None: zeros) and ends with; final_state may be initial_state.  Key and value heads of up to 128 elements.  A key or value
+    that is not finite reaches its heads' results from its token to its sequence's end, and no others."""
     name = "decay_attention_fwd"
     dev = _current_gpu(name, q, cu_seqlens, initial_state, final_state)
     of_q, of_k, of_v, elem, views = _decay_of(name, dev, q, k, v, out, "out", log_decay)
