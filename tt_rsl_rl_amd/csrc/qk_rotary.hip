@@ -10,8 +10,9 @@
 //
 // Bound by memory: x once in, y once out (dx: x and dy in).  Weight gradients stay in registers over a block's tokens (and, where heads
 // share the weight, over its heads), then go to the workspace, and a last launch adds the blocks' in a fixed order in fp64.
-// 16,384 tokens of 24 heads of 128 (201 MB in and out): 37 us, the copy's rate; going back 32,768 tokens of 24 heads of 128 (604 MB): 146 us, 4.1 TB/s, and 12
-// for the join: a row's sums have to be there before it is written, and few of a wave's rows are on their way meanwhile.
+// 16,384 tokens of 24 heads of 128 (201 MB in and out): 37 us, the copy's rate; going back 32,768 tokens of 24 heads of 128 (604 MB): 132 us, 4.6 TB/s (144 with a
+// head's tokens one after another, whose rows lie apart, where the heads share a weight), and 5 for the join: a row's sums have to be there before it is
+// written, and few of a wave's rows are on their way meanwhile.
 #include "views.hpp"
 
 namespace ppo {
@@ -184,10 +185,13 @@ __global__ __launch_bounds__(kThreads) void qk_rotary_bwd_kernel(const QkArgs q)
   fill_turns(q, first, count, turns);
   const int lane = threadIdx.x & (lanes - 1);
   float da[UNITS][V] = {}, db[UNITS][V] = {};
-  for (int h = head0; h < head0 + heads; ++h) {
+  for (int h = head0, next; h < head0 + heads; h = next) {
+    // one head, or all that share a weight: then rows in the order in which they lie
     const bool key = h >= q.a.q_heads;
-    const int head = key ? h - q.a.q_heads : h;
-    for (int t = threadIdx.x >> q.lanes_log2; t < count; t += kThreads >> q.lanes_log2) {
+    next = per_head ? h + 1 : key ? head0 + heads : min(head0 + heads, q.a.q_heads);
+    const int together = next - h;
+    for (int i = threadIdx.x >> q.lanes_log2; i < count * together; i += kThreads >> q.lanes_log2) {
+      const int t = together == 1 ? i : i / together, head = (key ? h - q.a.q_heads : h) + i - t * together;
       const T* x = row_at<const T>(key ? q.a.k : q.a.q, first + t, head);
       const T* dy = row_at<const T>(key ? q.a.k_out : q.a.q_out, first + t, head);
       float xa[UNITS][V], xb[UNITS][V], ga[UNITS][V], gb[UNITS][V], sum = 0.0f, dot = 0.0f;
@@ -232,7 +236,6 @@ __global__ __launch_bounds__(kThreads) void qk_rotary_bwd_kernel(const QkArgs q)
         }
       }
     }
-    if (!per_head && h != head0 + heads - 1 && h != q.a.q_heads - 1) continue;
     // lanes of the same pairs, then waves, in order
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -264,28 +267,31 @@ __global__ __launch_bounds__(kThreads) void qk_rotary_bwd_kernel(const QkArgs q)
   }
 }
 
-// The blocks' sums of one weight gradient's 64 elements: each of 16 waves adds every 16th block's, then the waves' are added.
-constexpr int kJoinWaves = 16;
+// The blocks' sums of 16 elements of one weight gradient: each of 64 rows of lanes adds every 64th block's, then these are added.  (Blocks of 64 elements, 16 rows
+// of lanes: 12 us for 1,024 tiles' 2 x 128 elements, four blocks, so 5.)
+constexpr int kJoinThreads = 1024, kJoinWidth = 16, kJoinRows = kJoinThreads / kJoinWidth;
 template <class W>
-__global__ __launch_bounds__(kWave* kJoinWaves) void qk_rotary_join_kernel(const QkArgs q, int64_t rows) {
-  __shared__ double part[kJoinWaves][kWave];
+__global__ __launch_bounds__(kJoinThreads) void qk_rotary_join_kernel(const QkArgs q, int64_t rows) {
+  __shared__ double part[kJoinRows][kJoinWidth];
   const bool per_head = q.a.weight_per_head != 0;
   const int dim = q.a.head_dim, slots = per_head ? q.a.q_heads + q.a.kv_heads : 2, slot = blockIdx.y;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, i = blockIdx.x * kWave + lane;
+  const int column = threadIdx.x % kJoinWidth, mine = threadIdx.x / kJoinWidth, i = blockIdx.x * kJoinWidth + column;
   double sum = 0.0;
   constexpr int AHEAD = 8;  // loads in flight
   if (i < dim)
-    for (int64_t r = wave; r < rows; r += kJoinWaves * AHEAD) {
+    for (int64_t r = mine; r < rows; r += kJoinRows * AHEAD) {
       float x[AHEAD];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) x[u] = q.partial[(min(r + u * kJoinWaves, rows - 1) * slots + slot) * dim + i];
+      for (int u = 0; u < AHEAD; ++u) x[u] = q.partial[(min(r + u * kJoinRows, rows - 1) * slots + slot) * dim + i];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) sum += r + u * kJoinWaves < rows ? static_cast<double>(x[u]) : 0.0;
+      for (int u = 0; u < AHEAD; ++u) sum += r + u * kJoinRows < rows ? static_cast<double>(x[u]) : 0.0;
     }
-  part[wave][lane] = sum;
-  __syncthreads();
-  if (wave != 0 || i >= dim) return;
-  for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
+  part[mine][column] = sum;
+  for (int n = kJoinRows / 2; n > 0; n /= 2) {  // (in pairs: the same order every time)
+    __syncthreads();
+    if (mine < n) part[mine][column] = sum += part[mine + n][column];
+  }
+  if (mine != 0 || i >= dim) return;
   const bool key = per_head ? slot >= q.a.q_heads : slot == 1;
   W* out = static_cast<W*>(key ? q.a.d_k_weight : q.a.d_q_weight);
   const int head = per_head ? (key ? slot - q.a.q_heads : slot) : 0;
@@ -439,10 +445,10 @@ extern "C" int ppo_qk_rotary_bwd(const ppo_qk_rotary_args* args, void* workspace
   int rc = PPO_OK;
   if (args->tokens > 0) with_type(args->type, [&](auto t) { rc = launch<decltype(t), true>(q, p, st); });
   if (rc != PPO_OK) return rc;
-  const dim3 grid(static_cast<uint32_t>(ceil_div(args->head_dim, kWave)), static_cast<uint32_t>(p.slots));
+  const dim3 grid(static_cast<uint32_t>(ceil_div(args->head_dim, kJoinWidth)), static_cast<uint32_t>(p.slots));
   const int64_t rows = args->tokens > 0 ? p.rows : 0;  // (no tokens: zeros)
   with_type(args->weight_type, [&](auto t) {
-    hipLaunchKernelGGL(qk_rotary_join_kernel<decltype(t)>, grid, dim3(kWave * kJoinWaves), 0, st, q, rows);
+    hipLaunchKernelGGL(qk_rotary_join_kernel<decltype(t)>, grid, dim3(kJoinThreads), 0, st, q, rows);
   });
   return check_launch("qk_rotary_join_kernel");
 }
