@@ -303,3 +303,37 @@ def test_step_is_the_prompts_recurrence(cuda):
     for t in range(40):
         ops.decay_attention_step(by["q"][:, t], by["k"][:, t], by["v"][:, t], d["ld"], state, out[:, t], scale=0.5)
     _check_forward(s, out.flatten(0, 1), state, 0.5, "steps: ")
+
+
+# Blocks enough for 128 columns each on 256 compute units, query heads together; and fewer, with 64 columns and a query head or a few each.
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("q_heads,kv_heads,dk,dv,lengths", [(8, 4, 128, 128, [1900, 3, 1300, 64, 700]), (4, 4, 40, 128, [2600]), (4, 4, 99, 77, [1000, 1500]),
+                                                            (8, 1, 128, 104, [700, 90]), (12, 2, 30, 128, [400]), (6, 1, 77, 101, [65, 65])])
+def test_shares_of_blocks(cuda, q_heads, kv_heads, dk, dv, lengths, dtype):
+    ops = _ops()
+    for states in (True, False):
+        s = _case(dk, lengths, q_heads, kv_heads, dk, dv, dtype, states)
+        d = _to(s, cuda)
+        _check_forward(s, *_forward(ops, d, 0.2), 0.2)
+        _check_backward(s, _backward(ops, d, 0.2), 0.2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_that_are_not_finite_in_wide_heads(cuda, dtype):
+    """A block may have half of a head's columns: an infinite key reaches all of them, an infinite value its own at least; no other token, head or sequence."""
+    ops = _ops()
+    s = _case(9, [50, 40, 90], 2, 2, 128, 128, dtype)
+    clean = _to(s, cuda)
+    want, want_last = _forward(ops, clean, 0.5)
+    for which in ("k", "v"):
+        d = {k: v.clone() for k, v in clean.items()}
+        d[which][60, 1, 100] = math.inf
+        out, last = _forward(ops, d, 0.5)
+        columns = slice(None) if which == "k" else slice(100, 101)
+        assert not bool(out[60:90, 1, columns].isfinite().any()) and not bool(last[1, 1, 100 if which == "k" else slice(None), columns].isfinite().any())
+        touched = torch.zeros(180, 2, dtype=torch.bool, device=cuda)
+        touched[60:90, 1] = True
+        assert torch.equal(out[~touched], want[~touched])
+        keep = torch.ones(3, 2, dtype=torch.bool, device=cuda)
+        keep[1, 1] = False
+        assert torch.equal(last[keep], want_last[keep])

@@ -26,8 +26,8 @@
 // what does see it.
 //
 // Bound by what a wave has to issue, at two waves a SIMD: a chunk's matrix products (two and three parts) take a third of the time, the rest goes to splitting
-// parts, to LDS and to its barriers.  65,536 tokens of 16 heads of 128 in bf16, states in and out (1.07 GB in and out, 0.2 ms at the copy's rate): 391 us for the
-// outputs, 175 for the segments' states, 15 for the scan.
+// parts, to LDS and to its barriers.  65,536 tokens of 16 heads of 128 in bf16, states in and out (1.07 GB in and out, 0.2 ms at the copy's rate): 400 us for the
+// outputs, 180 for the segments' states, 16 for the scan.
 #include <type_traits>
 
 #include "views.hpp"
@@ -758,7 +758,7 @@ struct Plan {
 
 // Segments: as many as give the chip two blocks a compute unit (a segment's state is written and read four times), down to a chunk each: a block alone
 // on its compute unit takes 5 to 7 us a chunk, waiting (577 tokens of 3 heads, fp32, the whole call: segments of four chunks 120 us, of one 47).
-// Where states make a piece of each sequence, segments go down to the sequences' mean length.
+// Where states make a piece of each sequence, segments go down to the sequences' mean length (14 sequences of a token, 12 heads: 79 us as one segment, 47 so).
 Plan plan_of(const ppo_decay_attention_args& a) {
   const int chunk = a.type == PPO_TYPE_BF16 ? Math<__bf16>::CHUNK : Math<float>::CHUNK;
   const bool states = a.initial_state != nullptr || a.final_state != nullptr || a.d_final_state != nullptr || a.d_initial_state != nullptr;
@@ -785,7 +785,7 @@ int launch_mix(const MixArgs& q, hipStream_t st) {
     hipLaunchKernelGGL(decay_scan_kernel, dim3(static_cast<uint32_t>(ceil_div(size, kScanThreads)), heads), dim3(kScanThreads), 0, st, q);
     if (int rc = check_launch("decay_scan_kernel")) return rc;
   }
-  // a's heads one to a block, or a few, where that many blocks still find a compute unit each
+  // a's heads one to a block, or a few, where that many blocks still find a compute unit each (the same tokens, 6 query heads: 22 us together, 15 so)
   MixArgs whole = q;
   whole.spread = q.ga;
   while (whole.spread > 1 && (q.ga % whole.spread != 0 || static_cast<int64_t>(q.segments) * heads * columns * whole.spread > device_info().cus)) --whole.spread;
@@ -797,7 +797,7 @@ int launch_mix(const MixArgs& q, hipStream_t st) {
 template <class T>
 int launch_type(const MixArgs& q, hipStream_t st) {
   using M = std::conditional_t<__is_same(T, __bf16), __bf16, float>;  // fp16 goes through fp32 products
-  // 64 of c's columns a block where 128 would leave half of the chip without one
+  // 64 of c's columns a block where 128 would leave half of the chip without one (577 tokens of 3 heads of 40 x 72, fp32: the outputs 28 us with 128, 22 so)
   const bool few = q.dc <= 64 || static_cast<int64_t>(q.segments) * q.heads * 2 <= device_info().cus;
   if (q.db <= 64) return few ? launch_mix<T, M, 4, 1>(q, st) : launch_mix<T, M, 4, 2>(q, st);
   return few ? launch_mix<T, M, 8, 1>(q, st) : launch_mix<T, M, 8, 2>(q, st);

@@ -4,7 +4,7 @@
 // Bound by memory: S is read once and written once, 64 KB each way for 128 x 128.  A block takes a slice of S's columns of one row and
 // head, so that few rows still fill the chip; a thread holds V neighbouring columns of up to ROWS of S's rows, all their loads in flight
 // together, adds to them, stores them and sums its part of every query's product; lanes of the same columns are joined by shuffles,
-// waves through LDS, in a fixed order.  1,024 rows of 8 heads of 128 x 128 (1.07 GB in and out): 205 us, the copy's rate.
+// waves through LDS, in a fixed order.  1,024 rows of 8 heads of 128 x 128 (1.07 GB in and out): 209 us, the copy's rate.
 #include <type_traits>
 
 #include "views.hpp"

@@ -16,9 +16,8 @@
 // meets all banks.  An accumulator lane holds one n and rows of m: with the vocabulary along m a row's sums stay in its lane but for one
 // shuffle and the waves' join.  fp32 operands are three bf16 parts, six products of which are taken (what is left out is 2^-24 and below).
 //
-// Bound by the matrix cores.  8,192 rows, of which 6,144 count, of 2,048 over 131,072 columns, bf16, for each 16,384 columns (412 GFLOP a product): sums 384 us,
-// differences 435, d_hidden 482, d_weight 335 (1,230 TFLOP/s, what a large library product reaches too), turning the weight 27.  The d_hidden's 192 tiles leave a
-// quarter of 256 compute units idle.
+// Bound by the matrix cores.  8,192 rows, of which 6,144 count, of 2,048 over 131,072 columns, bf16, for each 16,384 columns (412 GFLOP a product): sums 379 us,
+// differences 431, d_hidden 394, d_weight 329 (1,250 TFLOP/s), turning the weight 28 (134 MB in and out, 4.8 TB/s).
 #include <numeric>
 
 #include "elem.hpp"
@@ -59,7 +58,8 @@ constexpr float kLift = __is_same(T, _Float16) ? 16384.0f : 1.0f;
 
 // How d_hidden's tiles are shared out to the compute units; only the device knows how many rows count.  Tiles that make whole rounds take one block each.  Of the
 // rest, few are cut into slices of k, as many as fill one round; many leave a part of their k, 1 / (per + 1), to the units that would idle, `per` tiles to each
-// of these.  Every share of a tile has its own sums, the first ones tile after tile, the others behind them.
+// of these.  Every share of a tile has its own sums, the first ones tile after tile, the others behind them.  (192 tiles on 256 units, 16,384 columns: 482 us a tile
+// each, so 400; 6 tiles of 193 rows by 515, fp32, 50,021 columns: 155 us in two rounds of slices, 123 in one.)
 struct Shares {
   int whole, rest, slots, per;  // per 0: slices
 };
