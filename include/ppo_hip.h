@@ -974,7 +974,8 @@ int ppo_decay_attention_step(const ppo_decay_step_args* args, ppo_stream_t strea
  * Products are exact in fp32 sums (fp32 operands as three bf16 parts, six products); d_z is rounded to the operands' type for the
  * second products (fp32: three parts again), once, before 1 / (N temperature) is applied (and times 2^14 in fp16).  Everything is
  * summed in a fixed order.  The workspace holds d_z and copies of the weight for a piece of the columns, up to some 768 MB (or 2,048
- * columns), d_hidden's fp32 sums and some 12 bytes for each row and 256 columns; fp32 products of up to 256 MB are kept too.
+ * columns), d_hidden's fp32 sums (in tiles of 256 elements, and up to 64 MB of shares of tiles) and some 12 bytes for each row and
+ * 256 columns; fp32 products of up to 256 MB are kept too.
  * rows < 2^22, dim <= 2^20, vocab < 2^30, ld_weight <= 2^21.  No output may lie on an input or another output. */
 typedef struct ppo_linear_loss_args {
   const void* hidden; /* [rows, dim] */

@@ -337,3 +337,22 @@ def test_values_that_are_not_finite_in_wide_heads(cuda, dtype):
         keep = torch.ones(3, 2, dtype=torch.bool, device=cuda)
         keep[1, 1] = False
         assert torch.equal(last[keep], want_last[keep])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lengths", [[1], [40], [20, 11], [64, 0, 3, 60]])
+def test_states_in_place_with_query_heads_apart(cuda, dtype, lengths):
+    """Query heads of a head may be blocks of their own, which all read the state that one of them replaces."""
+    ops = _ops()
+    s = _case(13, lengths, 16, 2, 128, 128, dtype)
+    d = _to(s, cuda)
+    want, want_last = _forward(ops, d, 0.1)
+    wants = _backward(ops, d, 0.1)
+    for _ in range(5):
+        state, grad, out = d["s0"].clone(), d["g1"].clone(), torch.empty_like(want)
+        ops.decay_attention_fwd(d["q"], d["k"], d["v"], d["ld"], out, scale=0.1, cu_seqlens=d["cu"], initial_state=state, final_state=state)
+        assert torch.equal(out, want) and torch.equal(state, want_last)
+        grads = [torch.empty_like(d[x]) for x in ("q", "k", "v")]
+        ops.decay_attention_bwd(d["g"], d["q"], d["k"], d["v"], d["ld"], *grads, scale=0.1, cu_seqlens=d["cu"], initial_state=d["s0"],
+                                d_final_state=grad, d_initial_state=grad)
+        assert all(torch.equal(a, b) for a, b in zip((*grads, grad), wants))

@@ -814,8 +814,9 @@ Layout layout_of(const ppo_decay_attention_args& a) {
   const size_t states = static_cast<size_t>(a.kv_heads) * a.key_dim * a.value_dim * sizeof(float);
   l.bytes = l.carry + (p.segments - 1) * states;
   l.copy = 0;
-  const bool in_place = (a.initial_state != nullptr && a.initial_state == a.final_state) || (a.d_final_state != nullptr && a.d_final_state == a.d_initial_state);
-  if (in_place && p.segments > 1) {
+  // (query heads of a head may be blocks apart, which read the state that one of them writes)
+  const bool forward = a.initial_state != nullptr && a.initial_state == a.final_state, backward = a.d_final_state != nullptr && a.d_final_state == a.d_initial_state;
+  if ((forward && (p.segments > 1 || a.q_heads > a.kv_heads)) || (backward && p.segments > 1)) {
     l.copy = static_cast<size_t>(ceil_div(l.bytes, 256)) * 256;
     l.bytes = l.copy + a.sequences * states;
   }
@@ -886,7 +887,7 @@ int check(const char* who, const ppo_decay_attention_args* args, bool backward) 
 }
 
 // `from`, `to`: the states (or their gradients) that sequences begin and end with.  What no chunk does for them: sequences without tokens hand theirs on, and
-// those that are replaced in place are read from a copy (then `from`), since the block that ends a sequence need not be the one that began it.
+// those that are replaced in place are read from a copy (then `from`), since the block that ends a sequence need not be the only one that begins it.
 int prepare(const char* who, const ppo_decay_attention_args& a, const float*& from, float* to, void* workspace, size_t workspace_bytes, hipStream_t st,
             MixArgs& q) {
   const Layout l = layout_of(a);
