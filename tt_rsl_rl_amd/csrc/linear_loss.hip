@@ -808,7 +808,7 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   piece = std::min(std::max(piece, kMinPiece), int64_t{1} << 21);  // (a tile of d's offsets stay in 31 bits)
   if (!gradient && p.direct) piece = up(a.vocab, kTileM);
   piece = std::min(piece, kMostTiles / ceil_div(p.rows, p.n_tile) * kTileM);
-  if (gradient) piece = std::min(piece, kMostTiles / ceil_div(a.dim, kTileM) * 128);
+  if (gradient) piece = std::min(piece, kMostTiles / (2 * ceil_div(a.dim, kTileM)) * kTileM);
   p.piece = std::min(piece, up(a.vocab, kTileM));
   p.pieces = ceil_div(a.vocab, p.piece);
   if (p.pieces > 1) {

@@ -1251,27 +1251,26 @@ def _heads(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str, what: s
     return L.HEAD_VIEW.pack(t.data_ptr(), token, head)
 
 
-def _views(name: str, dev: int, dtype: torch.dtype, *of) -> bytes:
-    """The ppo_head_views of (tensor, shape, name) each.  (A native call reads them in a tenth of the time of their attributes, which is more than a
-    step of a few tokens takes the GPU; what it does not take is checked here, which says what is wrong.)"""
-    sizes = [x for t, shape, _ in of for x in (t, *shape)]
-    packed = L.tensor_table().head_views(dev, *sizes)
-    if packed is not None and of[0][0].dtype is dtype:
-        return packed
-    _current_gpu(name, *(t for t, _, _ in of))
-    return b"".join(_heads(t, dtype, shape, name, what) for t, shape, what in of)
-
-
-def _addresses(name: str, dev: int, *of) -> tuple:
-    """Addresses of (contiguous tensor or None, elements, name) each."""
-    packed = L.tensor_table().addresses(dev, *(x for t, n, _ in of for x in (t, n)))
+def _views(name: str, dev: int, dtype: torch.dtype, names: tuple, *flat) -> bytes:
+    """The ppo_head_views of (tensor, tokens, heads, elements) one after another.  (A native call reads them in a tenth of the time of their
+    attributes, which is more than a step of a few tokens takes the GPU; what it does not take is checked here, which says what is wrong.)"""
+    packed = L.tensor_table().head_views(dev, *flat)
     if packed is not None:
         return packed
-    _current_gpu(name, *(t for t, _, _ in of if t is not None))
-    for t, n, what in of:
+    _current_gpu(name, *flat[::4])
+    return b"".join(_heads(flat[4 * i], dtype, flat[4 * i + 1 : 4 * i + 4], name, what) for i, what in enumerate(names))
+
+
+def _addresses(name: str, dev: int, names: tuple, *flat) -> tuple:
+    """Addresses of (contiguous tensor or None, elements) one after another."""
+    packed = L.tensor_table().addresses(dev, *flat)
+    if packed is not None:
+        return packed
+    _current_gpu(name, *(t for t in flat[::2] if t is not None))
+    for t, n, what in zip(flat[::2], flat[1::2], names):
         if t is not None and (t.numel() != n or not t.is_contiguous()):
             raise ValueError(f"{name}: {what} must be contiguous, of {n} elements, got {list(t.shape)}")
-    return tuple(0 if t is None else t.data_ptr() for t, _, _ in of)
+    return tuple(0 if t is None else t.data_ptr() for t in flat[::2])
 
 
 _NO_VIEWS = bytes(L.HEAD_VIEW.size)
@@ -1312,8 +1311,9 @@ def _qk_of(name: str, dev: int, q, k, q_weight, k_weight, positions, freqs, *mor
         raise ValueError(f"{name}: freqs must be float64 [rotary_dim / 2], got {freqs.dtype} {list(freqs.shape)}")
     pairs = freqs.numel()
     n_q, n_k = (q_heads * dim, kv_heads * dim) if per_head else (dim, dim)
-    at = _addresses(name, dev, (q_weight, n_q, "q_weight"), (k_weight, n_k, "k_weight"), (positions, tokens, "positions"), (freqs, pairs, "freqs"),
-                    *zip(more, (n_q, n_k), ("d_q_weight", "d_k_weight")))
+    grads = (more[0], n_q, more[1], n_k) if more else ()
+    at = _addresses(name, dev, ("q_weight", "k_weight", "positions", "freqs", "d_q_weight", "d_k_weight"), q_weight, n_q, k_weight, n_k, positions, tokens,
+                    freqs, pairs, *grads)
     return of_q, of_k, at, (q_heads, kv_heads, dim, 2 * pairs, elem, weight_type, position_type), per_head
 
 
@@ -1327,7 +1327,7 @@ def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     name = "qk_norm_rotary_fwd"
     dev = _current_gpu(name, q)
     of_q, of_k, at, sizes, per_head = _qk_of(name, dev, q, k, q_weight, k_weight, positions, freqs)
-    views = _views(name, dev, q.dtype, (q, of_q, "q"), (k, of_k, "k"), (q_out, of_q, "q_out"), (k_out, of_k, "k_out"))
+    views = _views(name, dev, q.dtype, ("q", "k", "q_out", "k_out"), q, *of_q, k, *of_k, q_out, *of_q, k_out, *of_k)
     args = views + 2 * _NO_VIEWS + L.QK_ROTARY_REST.pack(at[0], at[1], 0, 0, at[2], at[3], of_q[0], eps, *sizes, bool(interleaved), per_head, 0)
     L.call("ppo_qk_rotary_fwd", args, _raw_stream(dev))
     _written(q_out, k_out)
@@ -1342,8 +1342,8 @@ def qk_norm_rotary_bwd(d_q_out: torch.Tensor, d_k_out: torch.Tensor, q: torch.Te
     name = "qk_norm_rotary_bwd"
     dev = _current_gpu(name, q)
     of_q, of_k, at, sizes, per_head = _qk_of(name, dev, q, k, q_weight, k_weight, positions, freqs, d_q_weight, d_k_weight)
-    views = _views(name, dev, q.dtype, (q, of_q, "q"), (k, of_k, "k"), (d_q_out, of_q, "d_q_out"), (d_k_out, of_k, "d_k_out"), (d_q, of_q, "d_q"),
-                   (d_k, of_k, "d_k"))
+    views = _views(name, dev, q.dtype, ("q", "k", "d_q_out", "d_k_out", "d_q", "d_k"), q, *of_q, k, *of_k, d_q_out, *of_q, d_k_out, *of_k, d_q, *of_q,
+                   d_k, *of_k)
     args = views + L.QK_ROTARY_REST.pack(at[0], at[1], at[4], at[5], at[2], at[3], of_q[0], eps, *sizes, bool(interleaved), per_head, 0)
     buf = _scratch(ws, q.device, L.load().ppo_qk_rotary_bwd_workspace_bytes(args))
     L.call("ppo_qk_rotary_bwd", args, buf.data_ptr(), buf.numel(), _raw_stream(dev))
@@ -1351,7 +1351,7 @@ def qk_norm_rotary_bwd(d_q_out: torch.Tensor, d_k_out: torch.Tensor, q: torch.Te
 
 
 def _decay_of(name: str, dev: int, q, k, v, out, what: str, log_decay, *more) -> tuple:
-    """(q's, k's and v's shapes and element type, packing of the views: these four and more, (tensor, index of its shape, name) each), checked."""
+    """(q's, k's and v's shapes and element type, packing of the views: these four and, going back, d_q, d_k and d_v), checked."""
     of_q, of_k, of_v, t = q.shape, k.shape, v.shape, q.dtype
     if len(of_q) != 3 or len(of_v) != 3 or of_v[0] != of_q[0] or of_k != (of_q[0], of_v[1], of_q[2]) or of_v[1] == 0 or of_q[1] % of_v[1]:
         raise ValueError(f"{name}: q, k and v must be [tokens, heads, elements], with k's elements q's and k's and v's heads, which divide q's, the same, got "
@@ -1361,9 +1361,8 @@ def _decay_of(name: str, dev: int, q, k, v, out, what: str, log_decay, *more) ->
         _element_type(q, f"{name}: q")
     if log_decay.dtype is not torch.float32 or log_decay.dim() != 1:
         raise ValueError(f"{name}: log_decay must be float32 [{of_v[1]}], got {log_decay.dtype} {list(log_decay.shape)}")
-    shapes = of_q, of_k, of_v
-    views = _views(name, dev, t, (q, of_q, "q"), (k, of_k, "k"), (v, of_v, "v"), (out, (of_q[0], of_q[1], of_v[2]), what),
-                   *((x, shapes[i], y) for x, i, y in more))
+    grads = (more[0], *of_q, more[1], *of_k, more[2], *of_v) if more else ()
+    views = _views(name, dev, t, ("q", "k", "v", what, "d_q", "d_k", "d_v")[: 4 + len(more)], q, *of_q, k, *of_k, v, *of_v, out, of_q[0], of_q[1], of_v[2], *grads)
     return of_q, of_k, of_v, elem, views
 
 
@@ -1400,7 +1399,7 @@ def decay_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
     of_q, of_k, of_v, elem, views = _decay_of(name, dev, q, k, v, out, "out", log_decay)
     sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
     shape = (sequences, of_v[1], of_q[2], of_v[2])
-    (decay,) = _addresses(name, dev, (log_decay, of_v[1], "log_decay"))
+    (decay,) = _addresses(name, dev, ("log_decay",), log_decay, of_v[1])
     args = views + 3 * _NO_VIEWS + L.DECAY_ATTENTION_REST.pack(
         decay, cu, _state(initial_state, f"{name}: initial_state", shape), _state(final_state, f"{name}: final_state", shape), 0, 0, of_q[0], sequences, scale,
         of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
@@ -1417,10 +1416,10 @@ def decay_attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     constant.  d_initial_state may be d_final_state."""
     name = "decay_attention_bwd"
     dev = _current_gpu(name, q, cu_seqlens, initial_state, d_final_state, d_initial_state)
-    of_q, of_k, of_v, elem, views = _decay_of(name, dev, q, k, v, d_out, "d_out", log_decay, (d_q, 0, "d_q"), (d_k, 1, "d_k"), (d_v, 2, "d_v"))
+    of_q, of_k, of_v, elem, views = _decay_of(name, dev, q, k, v, d_out, "d_out", log_decay, d_q, d_k, d_v)
     sequences, cu, cu_type = _sequences_of(name, cu_seqlens)
     shape = (sequences, of_v[1], of_q[2], of_v[2])
-    (decay,) = _addresses(name, dev, (log_decay, of_v[1], "log_decay"))
+    (decay,) = _addresses(name, dev, ("log_decay",), log_decay, of_v[1])
     args = views + L.DECAY_ATTENTION_REST.pack(
         decay, cu, _state(initial_state, f"{name}: initial_state", shape), 0, _state(d_final_state, f"{name}: d_final_state", shape),
         _state(d_initial_state, f"{name}: d_initial_state", shape), of_q[0], sequences, scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, cu_type)
@@ -1448,7 +1447,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
             raise ValueError(f"{name}: slots must be int64 or int32, got {slots.dtype}")
     if fresh is not None and fresh.dtype is not torch.bool and fresh.dtype is not torch.uint8:
         raise ValueError(f"{name}: fresh must be bool or uint8, got {fresh.dtype}")
-    at = _addresses(name, dev, (log_decay, of_v[1], "log_decay"), (state, state.numel(), "state"), (slots, rows, "slots"), (fresh, rows, "fresh"))
+    at = _addresses(name, dev, ("log_decay", "state", "slots", "fresh"), log_decay, of_v[1], state, state.numel(), slots, rows, fresh, rows)
     args = views + L.DECAY_STEP_REST.pack(*at, rows, of_state[0], scale, of_q[1], of_v[1], of_q[2], of_v[2], elem, slot_type)
     L.call("ppo_decay_attention_step", args, _raw_stream(dev))
     _written(state, out)
