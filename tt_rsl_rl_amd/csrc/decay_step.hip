@@ -210,7 +210,8 @@ extern "C" int ppo_decay_attention_step(const ppo_decay_step_args* args, ppo_str
   const bool fours = a.value_dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.states) % 16 == 0;
   int64_t cus = device_info().cus;
   if (cus <= 0) cus = 256;
-  // as many columns as a block takes, unless that leaves the chip idle
+  // as many columns as a block takes, unless that leaves the chip idle (8 rows of 4 heads: 6.5 us with 128 columns a block, 4.5 with 32; 256 rows of 8 heads:
+  // 42.8 and 44.5)
   const int v = fours ? 4 : 1;
   q.lanes_log2 = 0;
   while ((1 << q.lanes_log2) * v < a.value_dim && q.lanes_log2 < (fours ? 5 : 6)) ++q.lanes_log2;

@@ -653,7 +653,8 @@ __device__ __forceinline__ void add_sums(float& s, float& e, float m, float mt, 
   e = fmaf(et + st * d, f, e);
 }
 
-// A block: 16 rows (the tiles' sums of a row lie rows apart, so neighbouring lanes take neighbouring rows) by 64 groups of tiles, so that 512 tiles (131,072 columns) are one round of loads (16 groups, four rounds: 8 rows 11.6 us, so 8).
+// A block: 16 rows (the tiles' sums of a row lie rows apart, so neighbouring lanes take neighbouring rows) by 64 groups of tiles, so that 512 tiles (131,072
+// columns) are one round of loads (16 groups, four rounds: 8 rows 11.6 us, so 8).
 constexpr int kJoinThreads = 1024, kJoinRows = 16, kJoinGroups = kJoinThreads / kJoinRows;
 __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const RowArgs q) {
   __shared__ float part_m[kJoinGroups][kJoinRows], part_s[kJoinGroups][kJoinRows], part_e[kJoinGroups][kJoinRows];
@@ -802,6 +803,8 @@ Plan plan_of(const ppo_linear_loss_args& a, bool gradient) {
   p.direct = a.type != PPO_TYPE_F32 && a.dim % kTileK == 0 && a.ld_weight % 8 == 0 && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
   const int64_t column = 2 * p.parts * ((gradient ? (a.d_hidden != nullptr) + (a.d_weight != nullptr) : 0) * p.rows + (p.direct ? 0 : p.k) +
                                          (gradient && a.d_hidden != nullptr ? a.dim : 0));
+  // rows of a tile: few rows' tiles hold nothing else, three fp32 parts of 256 do not fit into LDS (131,072 columns of 1,024, bf16: 32 rows 56 us in tiles of 32, 60
+  // of 128; 128 rows 63 of 128, 82 of 256; 200 rows 92 and 84; 384 rows 130 and 143; 512 rows 167 and 145)
   p.n_tile = a.rows <= 32 ? 32 : a.type == PPO_TYPE_F32 || a.rows <= 128 || (a.rows > 256 && a.rows <= 384) ? 128 : 256;
   p.n_tile = narrow(p.n_tile, ceil_div(a.vocab, kTileM), a.rows, cus);
   int64_t piece = kPieceBytes / std::max<int64_t>(column, 1) / kTileM * kTileM;

@@ -323,7 +323,8 @@ Plan plan_of(const ppo_qk_rotary_args& a, bool backward) {
   const int least = backward ? std::min(p.tile, at_once) : 1;
   while (p.tile > least && ceil_div(a.tokens, p.tile) < 4 * cus) p.tile = std::max(least, p.tile / 2);
   p.tiles = ceil_div(a.tokens, p.tile);
-  // heads of a block: all, unless that leaves the chip idle
+  // heads of a block: all, which share the sines (512 tokens of 20 heads of 128: 3.9 us, 5 a block 5.8), unless that leaves the chip idle: more than a block has
+  // rows for, or going back
   p.group = heads;
   while (p.group > 1 && p.tiles * ceil_div(heads, p.group) < 4 * cus && (backward || p.group * p.tile > at_once)) p.group = (p.group + 1) / 2;
   p.groups = ceil_div(heads, p.group);
