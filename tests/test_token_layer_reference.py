@@ -318,7 +318,7 @@ def test_launches_hold_fewer_than_2_to_the_32_threads():
 
     for entry in ("ppo_qk_rotary_fwd", "ppo_qk_rotary_bwd"):
         with pytest.raises(ValueError, match="tokens"):
-            _qk(entry, tokens=1 << 28)
+            _qk(entry, tokens=(1 << 28) - 16)
     rows, vocab, dim = (1 << 22) - 1, 1 << 29, 63  # 2^14 tiles of rows, so that 2^8 tiles of columns are 2^22 blocks
     args = ctypes.byref(L.LinearLossArgs(hidden=M, ld_hidden=dim, weight=2 * M, ld_weight=dim, rows=rows, vocab=vocab, dim=dim, temperature=1.0, type=1))
     sums, hidden = 3 * (vocab >> 8) * (rows + 1) * 4, (rows + 1) * 64 * 2

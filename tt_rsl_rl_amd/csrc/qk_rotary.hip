@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kJoinThreads) void qk_rotary_join_kernel(const QkAr
   out[head * dim + i] = static_cast<W>(static_cast<float>(sum));
 }
 
-constexpr int64_t kMostTokens = int64_t{1} << 28;  // 16 a block: a launch holds fewer than 2^32 threads
+constexpr int64_t kMostTokens = (int64_t{1} << 28) - 16;  // 16 a block: a launch holds fewer than 2^32 threads
 
 struct Plan {
   int vec, units, lanes_log2, tile, group;
