@@ -655,7 +655,9 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
                   Piece16 o;
 #pragma unroll
                   for (int f = 0; f < PER; ++f) o[f] = static_cast<T>(acc[i][(e + f) / 4][(e + f) % 4]);
-                  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, o), buffer, off, e * static_cast<int>(sizeof(T)), 0);
+                  // (of fp32's two pieces the first may be the head's last)
+                  const uint32_t piece = e == 0 || d + e < q.dc ? off + e * static_cast<uint32_t>(sizeof(T)) : 0x80000000u;
+                  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, o), buffer, piece, 0, 0);
                 }
               } else {
                 typedef uint32_t Pair __attribute__((ext_vector_type(2)));
