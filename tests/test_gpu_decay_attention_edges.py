@@ -5,8 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_decay_attention import _case, _check_backward, _check_forward, _ops, _to
-from tests.test_gpu_token_ops import F32
+from tests.test_gpu_decay_attention import _backward, _case, _check_backward, _check_forward, _forward, _ops, _to
+from tests.test_gpu_token_ops import BF16, F16, F32
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,66 @@ def test_fp32_heads_of_an_odd_number_of_pieces(cuda, dk, dv, states):
         assert bool((store[between] == 9).all())
     _check_forward(s, out, last, 0.2)
     _check_backward(s, (*grads, first), 0.2)
+
+
+def _rows_equal(got, want, rows, what):
+    """The same bits (but for a zero's sign) in the rows named."""
+    for name, x, y in zip(("d_q", "d_k", "d_v") if len(got) == 3 else ("out",), got, want):
+        assert torch.equal(x[rows], y[rows]), f"{what}: {name}"
+
+
+@pytest.mark.parametrize("states", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dk,dv", [(16, 16), (128, 128), (24, 40), (20, 36)])
+def test_what_lies_outside_the_sequences_is_not_seen(cuda, dk, dv, dtype, states):
+    """NaN before the first sequence and behind the last one, in tokens that share a piece with theirs."""
+    ops = _ops()
+    for before, lengths, behind in ((0, [120], 5), (5, [40, 23], 0), (3, [30], 30), (40, [100, 1, 60], 77)):
+        s = _case(dk + before, [before] + lengths + [behind], 4, 2, dk, dv, dtype, False)
+        s["cu"] = s["cu"][1:-1]
+        if states:
+            s["s0"], s["g1"] = torch.randn(2, len(lengths), 2, dk, dv, generator=torch.Generator().manual_seed(3))
+        clean = _to(s, cuda)
+        lo, hi = before, before + sum(lengths)
+        nan = {k: v.clone() for k, v in clean.items()}
+        for x in ("q", "k", "v", "g"):
+            nan[x][:lo], nan[x][hi:] = float("nan"), float("nan")
+        want, want_last = _forward(ops, clean, 0.4)
+        out, last = _forward(ops, nan, 0.4)
+        _rows_equal((out,), (want,), slice(lo, hi), f"{before}, {lengths}, {behind}")
+        *wants, want_first = _backward(ops, clean, 0.4)
+        *grads, first = _backward(ops, nan, 0.4)
+        _rows_equal(grads, wants, slice(lo, hi), f"{before}, {lengths}, {behind}")
+        if states:
+            assert torch.equal(last, want_last) and torch.equal(first, want_first)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("states", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dk,dv", [(16, 16), (128, 128), (20, 36)])
+def test_a_value_that_is_not_finite_at_a_pieces_end(cuda, dk, dv, dtype, states, value):
+    """In a sequence's last token a key or value is seen by that token alone, in its first one a query or a gradient of an output by that one's going back."""
+    ops = _ops()
+    for lengths in ([1], [33], [40, 23], [3, 60, 200], [100, 27, 500]):
+        s = _case(sum(lengths), lengths, 2, 1, dk, dv, dtype, states)
+        clean = _to(s, cuda)
+        want, want_last = _forward(ops, clean, 0.4)
+        *wants, want_first = _backward(ops, clean, 0.4)
+        starts = s["cu"].tolist()
+        for b in range(len(lengths)):
+            for which, token in (("k", starts[b + 1] - 1), ("v", starts[b + 1] - 1), ("q", starts[b]), ("g", starts[b])):
+                d = {k: v.clone() for k, v in clean.items()}
+                d[which][token, 0, 5] = value
+                what = f"{lengths}, {which} of token {token}"
+                others = torch.ones(sum(lengths), dtype=torch.bool, device=cuda)
+                others[token] = False
+                out, last = _forward(ops, d, 0.4)
+                *grads, first = _backward(ops, d, 0.4)
+                _rows_equal((out,), (want,), others, what)
+                _rows_equal(grads, wants, others, what)
+                if which in "kv":
+                    assert not bool(out[token].isfinite().all()), what
+                if states:
+                    apart = [i for i in range(len(lengths)) if i != b]
+                    assert torch.equal(last[apart], want_last[apart]) and torch.equal(first[apart], want_first[apart]), what

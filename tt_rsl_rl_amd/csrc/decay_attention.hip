@@ -504,8 +504,8 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     wait_memory();  // (the spans, as the compiler sees it, on the path that did not load them)
     lds_barrier();
     const bool poisoned = __builtin_amdgcn_readfirstlane(bad_any) != 0;
-    if (poisoned) {  // zeros where a token is not finite
-      for (int j = 0; j < n; ++j)
+    if (poisoned) {  // zeros where a token is not finite, and in the places behind the last one, which hold it too
+      for (int j = 0; j < C; ++j)
         if (bad[j / 32] >> (j % 32) & 1) {
           for (int d = thread; d < DB; d += kThreads) {
             if (!STATE_ONLY) b_rows[Rows_::at(j, d / Rows_::PIECE) + d % Rows_::PIECE] = static_cast<M>(0.0f);
