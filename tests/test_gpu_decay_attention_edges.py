@@ -100,3 +100,27 @@ def test_a_value_that_is_not_finite_at_a_pieces_end(cuda, dk, dv, dtype, states,
                 if states:
                     apart = [i for i in range(len(lengths)) if i != b]
                     assert torch.equal(last[apart], want_last[apart]) and torch.equal(first[apart], want_first[apart]), what
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kv_heads,dk,dv,lengths,huge", [(520, 16, 16, [150, 30, 170], [1]), (520, 12, 20, [100, 150], [0]), (2, 16, 16, [10, 10, 160, 10, 7], [0, 1, 3, 4]),
+                                                         (520, 32, 128, [9, 200], [0])])
+def test_a_sequence_whose_state_overflows(cuda, kv_heads, dk, dv, lengths, huge, dtype):
+    """Its products leave fp32's range: the sequences before and behind it are as they are without it.  (Heads enough for one block to go through all tokens.)"""
+    ops = _ops()
+    s = _case(11, lengths, kv_heads, kv_heads, dk, dv, dtype, False)
+    s["ld"] = s["ld"].clamp(max=-0.01)
+    d = _to(s, cuda)
+    starts, overflown = s["cu"].tolist(), torch.zeros(sum(lengths), dtype=torch.bool)
+    for b in huge:
+        overflown[starts[b] : starts[b + 1]] = True
+    for x in ("q", "k", "v", "g"):
+        d[x][overflown] *= 1e25
+        s[x][overflown] = 0
+    out, _ = _forward(ops, d, 0.5)
+    grads = _backward(ops, d, 0.5)
+    assert not bool(out[overflown].isfinite().all())
+    for x in (out, *grads[:3]):
+        x[overflown] = 0
+    _check_forward(s, out, None, 0.5)
+    _check_backward(s, grads, 0.5)

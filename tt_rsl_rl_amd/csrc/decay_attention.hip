@@ -139,7 +139,6 @@ struct MixArgs {
   int32_t spread;         // blocks that share a's heads of a head
   int32_t db, dc;
   int32_t reverse, w, cut;  // cut: chunks end with their sequence
-  int32_t lost;             // states come in, which need not be finite
   int32_t near;             // the outputs' rows too, and aligned to four bytes
   int32_t whole;            // rows are whole 16-byte pieces, not far apart
   float x, y, z;
@@ -406,7 +405,6 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     put_span(0, seg_begin + threadIdx.x, span_of(q, token_at_place(seg_begin + threadIdx.x)));
   lds_barrier();
   bool fresh = true;  // S is zeros
-  bool lost = q.lost != 0;  // S may be not finite
   each_state([](float, int, int) { return 0.0f; });
   if (!STATE_ONLY && first[0][0] < seg_begin) {  // goes on from the segment before
     const float* from = q.carry + (static_cast<int64_t>(seg - 1) * q.heads + head) * q.state_size;
@@ -686,14 +684,14 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
       // ---- the state ----
       if (ab >= q.ga - 1) {
         if (ab == q.ga - 1) {
-          const float f = first_last == first0 ? fades[n] : 0.0f;
+          const float f = fades[n];
 #pragma unroll
           for (int mb = 0; mb < DBT; ++mb)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int r4 = 0; r4 < 4; ++r4) S[mb][nt][r4] *= f;
-          if (first_last != first0 && lost) each_state([](float, int, int) { return 0.0f; }), lost = false;
+          if (first_last != first0) each_state([](float, int, int) { return 0.0f; });  // another sequence's, which may have left fp32's range
         }
 #pragma unroll
         for (int kj = 0; kj < C / K; ++kj) {
@@ -727,7 +725,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     if (poisoned && ab >= q.ga - 1) {
       bool hit = false;
       for (int j = 0; j < n; ++j) hit |= (bad[j / 32] >> (j % 32) & 1) && from_first[j] == first_last;
-      if (hit) each_state([](float, int, int) { return __builtin_nanf(""); }), lost = true;
+      if (hit) each_state([](float, int, int) { return __builtin_nanf(""); });
       lds_barrier();
       if (threadIdx.x == 0) bad_any = 0;
       if (threadIdx.x < (C + 31) / 32) bad[threadIdx.x] = 0;
@@ -922,7 +920,6 @@ int prepare(const char* who, const ppo_decay_attention_args& a, const float*& fr
 
 int mix(const ppo_decay_attention_args& a, MixArgs q, hipStream_t st) {
   const int piece = 16 / type_size(a.type);
-  q.lost = q.s_in != nullptr || q.segments > 1;
   if (q.carried == 0) q.ci = q.dc, q.cj = 1;
   else q.ci = 1, q.cj = q.db;  // as the pass before left it, turned over
   q.whole = a.key_dim % piece == 0 && a.value_dim % piece == 0;
