@@ -917,8 +917,8 @@ int ppo_qk_rotary_bwd(const ppo_qk_rotary_args* args, void* workspace, size_t wo
  * States, sums and the powers of f are fp32 or more.  Of bf16 inputs the matrix cores' operands that the call makes itself (S, R,
  * the chunks' matrices, weighted rows) are held as sums of two bf16 parts, where a state comes out its own as three; fp16 and fp32
  * inputs go through fp32 products.  Everything is summed in a fixed order.  What sees a token with an infinity or NaN
- * becomes infinite or NaN (a row's other elements may too); other sequences, what lies before it (behind it, going back) and rows
- * of no sequence do not.
+ * becomes infinite or NaN (a row's other elements may too), also where f's powers have vanished: 0 times it is NaN; other sequences,
+ * what lies before it (behind it, going back) and rows of no sequence do not.
  * key_dim, value_dim <= PPO_DECAY_MAX_DIM; q_heads <= 65535; the outputs' token_stride < 2^31.  No output may lie on an input or
  * another output, but d_initial_state may be d_final_state and final_state may be initial_state. */
 #define PPO_DECAY_MAX_DIM 128

@@ -124,3 +124,24 @@ def test_a_sequence_whose_state_overflows(cuda, kv_heads, dk, dv, lengths, huge,
         x[overflown] = 0
     _check_forward(s, out, None, 0.5)
     _check_backward(s, grads, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_value_that_is_not_finite_where_the_decays_powers_vanish(cuda, dtype):
+    """It reaches its sequence's end all the same, as 0 times what is not finite does: nowhere between does an output look right."""
+    ops = _ops()
+    s = _case(14, [300, 20], 2, 2, 16, 16, dtype, False)
+    clean = _to(s, cuda)
+    clean["ld"].copy_(torch.tensor([-4.0, -float("inf")]))
+    want, _ = _forward(ops, clean, 0.5)
+    *wants, _ = _backward(ops, clean, 0.5)
+    d = {k: v.clone() for k, v in clean.items()}
+    d["k"][10, :, 3] = float("inf")
+    out, _ = _forward(ops, d, 0.5)
+    assert torch.equal(out[:10], want[:10]) and torch.equal(out[300:], want[300:])
+    assert not bool(out[10:300].isfinite().any())
+    d = {k: v.clone() for k, v in clean.items()}
+    d["g"][290, :, 3] = float("inf")
+    _, d_k, d_v, _ = _backward(ops, d, 0.5)
+    assert torch.equal(d_k[291:], wants[1][291:]) and torch.equal(d_v[291:], wants[2][291:])
+    assert not bool(d_k[:291].isfinite().any()) and not bool(d_v[:291, :, 3].isfinite().any())

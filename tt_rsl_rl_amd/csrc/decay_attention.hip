@@ -496,7 +496,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
     if (thread < C) {
       const int i = min(thread, n - 1);
       weights[thread] = thread < n && from_first[i] == first_last ? q.z * fades[n - q.w - i] : 0.0f;
-      sights[thread] = thread < n && from_first[i] == first0 ? q.y * fades[i + q.w] : 0.0f;
+      sights[thread] = thread < n && from_first[i] == first0 ? q.y * fades[i + q.w] : __builtin_nanf("");  // (NaN: not at all)
     }
     if (ahead) put_span(buffer ^ 1, c0 + C + threadIdx.x, next_span);
     wait_memory();  // (the spans, as the compiler sees it, on the path that did not load them)
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(kThreads, 2) void decay_mix_kernel(const MixArgs q)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int r4 = 0; r4 < 4; ++r4) acc[i][nt][r4] = f != 0.0f ? acc[i][nt][r4] * f : 0.0f;
+              for (int r4 = 0; r4 < 4; ++r4) acc[i][nt][r4] = f == f ? acc[i][nt][r4] * f : 0.0f;  // (0 times what is not finite is not finite)
           }
         }
       }
