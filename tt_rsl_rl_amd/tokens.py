@@ -98,7 +98,8 @@ class QkNormRotary(nn.Module):
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale: float, cu_seqlens, initial_state, want_state: bool):
-        out = q.new_empty(*q.shape[:2], v.shape[2])
+        # (tokens of no sequence are 0: what goes on from here multiplies them by gradients of 0)
+        out = (q.new_empty if cu_seqlens is None else q.new_zeros)(*q.shape[:2], v.shape[2])
         sequences = 1 if cu_seqlens is None else cu_seqlens.numel() - 1
         final = q.new_empty(sequences, k.shape[1], k.shape[2], v.shape[2], dtype=torch.float32) if want_state else None
         ops.decay_attention_fwd(q, k, v, log_decay, out, scale=scale, cu_seqlens=cu_seqlens, initial_state=initial_state, final_state=final)
@@ -124,7 +125,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
                     cu_seqlens: torch.Tensor | None = None, initial_state: torch.Tensor | None = None,
                     want_state: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
     """``ops.decay_attention_fwd`` with its gradient: the output, and the state that each sequence ends with (None unless wanted).
-    log_decay is a constant; tokens of no sequence (cu_seqlens) get an output that means nothing and no gradient."""
+    log_decay is a constant; tokens of no sequence (cu_seqlens) get an output of 0 and no gradient."""
     if log_decay.requires_grad:
         raise ValueError("decay_attention: log_decay is a constant, it gets no gradient")
     return _DecayAttention.apply(q, k, v, log_decay, float(scale), cu_seqlens, initial_state, want_state)
