@@ -182,9 +182,10 @@ class DecayMixer(nn.Module):
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, tokens, mask, temperature: float, denom):
-        d_hidden = hidden.new_empty(hidden.shape) if ctx.needs_input_grad[0] else None
-        d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+    def forward(ctx, hidden, weight, tokens, mask, temperature: float, denom, recorded: bool):
+        # (needs_input_grad is a parameter's requires_grad, also where no graph is recorded)
+        d_hidden = hidden.new_empty(hidden.shape) if recorded and ctx.needs_input_grad[0] else None
+        d_weight = torch.empty_like(weight) if recorded and ctx.needs_input_grad[1] else None
         stats = torch.empty(4, device=hidden.device)
         ops.linear_cross_entropy(hidden, weight, tokens, d_hidden, d_weight, stats, mask=mask, temperature=temperature, denom=denom)
         ctx.save_for_backward(d_hidden, d_weight)
@@ -196,16 +197,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
         d_hidden, d_weight = ctx.saved_tensors
         # (in float32: the loss' factor need not be one of the operands' type)
         scaled = [None if d is None else (d.float() * d_loss).to(d.dtype) for d in (d_hidden, d_weight)]
-        return *scaled, None, None, None, None
+        return *scaled, None, None, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
                          temperature: float = 1.0, denom: float | None = None) -> torch.Tensor:
     """The mean cross entropy of tokens under softmax(hidden weight^T / temperature), hidden [..., dim], without the logits: a float32 scalar
-    whose gradients are made with it (``ops.linear_cross_entropy``)."""
+    whose gradients are made with it (``ops.linear_cross_entropy``; not under ``torch.no_grad()``), rounded to their operands' type before the
+    factor that the loss is multiplied by: float16 wants a loss scale as denom = N / scale."""
     hidden = hidden.reshape(-1, hidden.shape[-1])
     mask = None if mask is None else mask.reshape(-1).contiguous()
-    return _LinearCrossEntropy.apply(_rows(hidden), weight, tokens.reshape(-1).contiguous(), mask, float(temperature), denom)
+    return _LinearCrossEntropy.apply(_rows(hidden), weight, tokens.reshape(-1).contiguous(), mask, float(temperature), denom, torch.is_grad_enabled())
 
 
 class AdamW(torch.optim.Optimizer):
