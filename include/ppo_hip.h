@@ -873,7 +873,7 @@ typedef struct ppo_head_view {
  * error is some 2^-52 of the angle).  The weight is [D] for all heads, or [heads, D] (weight_per_head).
  * The backward pass takes the gradients of the results (q_out, k_out), turns them back (g) and gives
  *   d_weight = sum g n (over tokens, and heads where they share it);   d_x = (weight g - n mean(weight g n)) / sqrt(mean(x^2) + eps).
- * Sums over tokens are fp32 over up to some hundred rows and fp64 over those, in a fixed order: the same call gives the same bits.
+ * Sums over rows are fp32 over up to 512 one after another and fp64 over blocks of those, in a fixed order: the same call gives the same bits.
  * D and R are even, D <= PPO_QK_MAX_DIM, 2 <= R <= D; tokens < 2^28 - 16.  q_out and k_out (d_q and d_k) may be the very views that the call reads in
  * their place (q and k; going back also q_out and k_out); no other output may lie on an input or another output. */
 #define PPO_QK_MAX_DIM 512

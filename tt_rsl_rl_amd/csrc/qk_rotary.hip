@@ -22,6 +22,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kTurns = 4096;  // sines and cosines that a block holds at most: 32 KB of LDS
 constexpr int kMaxTile = 64;  // tokens of a block at most
+constexpr int kMostSummed = 512;  // rows of a sum in fp32
 
 struct QkArgs {
   ppo_qk_rotary_args a;
@@ -327,6 +328,8 @@ Plan plan_of(const ppo_qk_rotary_args& a, bool backward) {
   // rows for, or going back
   p.group = heads;
   while (p.group > 1 && p.tiles * ceil_div(heads, p.group) < 4 * cus && (backward || p.group * p.tile > at_once)) p.group = (p.group + 1) / 2;
+  // (going back a lane adds up every at_once-th row of its block before they go on in fp64)
+  if (backward && a.weight_per_head == 0) p.group = std::min(p.group, std::max(1, kMostSummed * at_once / p.tile));
   p.groups = ceil_div(heads, p.group);
   p.rows = a.weight_per_head != 0 ? p.tiles : p.tiles * p.groups;
   p.slots = a.weight_per_head != 0 ? heads : 2;
