@@ -910,7 +910,8 @@ int ppo_qk_rotary_bwd(const ppo_qk_rotary_args* args, void* workspace, size_t wo
  * cut; NULL: one sequence of all tokens).  Tokens before the first sequence and behind the last one are left as they are, in inputs
  * and outputs.  S starts at initial_state[b] (NULL: zeros) and ends in final_state[b] (NULL: not wanted), both
  * [sequences, kv_heads, key_dim, value_dim]; a sequence without tokens hands the one to the other.  A log_decay of -inf leaves each
- * token alone with itself; above 0 the past grows.  log_decay is a constant: it gets no gradient.
+ * token alone with itself; above 0 the past grows: exp(n log_decay) has to be in fp32's range for a sequence of n tokens (beyond it also
+ * zeros become NaN).  log_decay is a constant: it gets no gradient.
  * Backward, with R_t = f R_{t+1} + scale q_t d_out_t^T from d_final_state[b] (NULL: zeros) on:
  *   d_q_t = scale S_t d_out_t;   d_k_t = R_t v_t;   d_v_t = R_t^T k_t   (summed over the queries that share a head);
  *   d_initial_state[b] = f R_first (NULL: not wanted).
@@ -968,7 +969,8 @@ int ppo_decay_attention_step(const ppo_decay_step_args* args, ppo_stream_t strea
  *   lp = z_t - log sum_j exp(z_j);   p_j = exp(z_j - log sum exp z);   H = -sum_j p_j log p_j;   loss = -sum_r lp / N;
  *   d_z[r, j] = (p_j - [j = t]) / (N temperature);   d_hidden = d_z weight;   d_weight = d_z^T hidden.
  * Rows count, and N is, as in ppo_token_ppo_loss; a row that does not count gives lp = H = 0 and d_hidden 0.  Rows whose hidden or
- * products are not finite give what the formulas give.  If no row counts, every result is 0 (but stats[2], which is N).
+ * products are not finite give what the formulas give, but that an infinite fp32 operand (or one that rounds to infinity in bf16) makes
+ * NaN of what it is multiplied with.  If no row counts, every result is 0 (but stats[2], which is N).
  * ppo_linear_log_probs writes logp and entropy (either may be NULL).  ppo_linear_cross_entropy writes also stats[4] = loss, mean H,
  * N, 0 and d_hidden and d_weight, of their operands' type (either may be NULL: not wanted); logp and entropy as before.
  * Products are exact in fp32 sums (fp32 operands as three bf16 parts, six products); d_z is rounded to the operands' type for the
