@@ -46,3 +46,33 @@ def test_gradients_are_made_of_what_needs_them(asked):
     assert torch.equal(leaf.grad, torch.ones(3, 4))
     tokens.linear_cross_entropy(leaf, weight, tok)
     assert asked == [(False, True), (True, False), (True, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradients_are_multiplied_by_the_losses_factor_in_float32(monkeypatch, dtype):
+    """And rounded once: 0.1 is none of the 16-bit types' values."""
+    g = torch.Generator().manual_seed(0)
+    made = torch.randn(7, 4, generator=g).to(dtype), torch.randn(50, 4, generator=g).to(dtype)
+
+    def stand_in(hidden, weight, tok, d_hidden, d_weight, stats, mask=None, temperature=1.0, denom=None):
+        stats.fill_(2.0), d_hidden.copy_(made[0]), d_weight.copy_(made[1])
+
+    monkeypatch.setattr(ops, "linear_cross_entropy", stand_in)
+    hidden, weight = (torch.zeros_like(m).requires_grad_() for m in made)
+    (tokens.linear_cross_entropy(hidden, weight, torch.zeros(7, dtype=torch.int64)) * 0.1).backward()
+    for x, m in zip((hidden, weight), made):
+        assert x.grad.dtype is dtype and torch.equal(x.grad, (m.float() * torch.tensor(0.1)).to(dtype))
+
+
+@pytest.mark.gpu
+def test_the_backward_pass_makes_no_copies(cuda):
+    """What it allocates at its height is the gradients themselves (and what the allocator rounds up)."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    hidden = torch.randn(64, 512, generator=g, device=cuda).to(torch.bfloat16).requires_grad_()
+    weight = torch.randn(20000, 512, generator=g, device=cuda).to(torch.bfloat16).requires_grad_()
+    loss = tokens.linear_cross_entropy(hidden, weight, torch.randint(0, 20000, (64,), generator=g, device=cuda)) * 3.0
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    loss.backward()
+    assert torch.cuda.max_memory_allocated() - before <= 2 * (hidden.numel() + weight.numel()) + (4 << 20)

@@ -195,8 +195,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_loss):
         d_hidden, d_weight = ctx.saved_tensors
-        # (in float32: the loss' factor need not be one of the operands' type)
-        scaled = [None if d is None else (d.float() * d_loss).to(d.dtype) for d in (d_hidden, d_weight)]
+        # (in float32, since the loss' factor need not be one of the operands' type: as a vector it makes the product float32, rounded as it is stored, without
+        # copies of the gradients between)
+        scaled = [None if d is None else torch.mul(d, d_loss.reshape(1), out=torch.empty_like(d)) for d in (d_hidden, d_weight)]
         return *scaled, None, None, None, None, None
 
 
