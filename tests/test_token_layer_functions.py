@@ -76,3 +76,17 @@ def test_the_backward_pass_makes_no_copies(cuda):
     before = torch.cuda.memory_allocated()
     loss.backward()
     assert torch.cuda.max_memory_allocated() - before <= 2 * (hidden.numel() + weight.numel()) + (4 << 20)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_only_tokens_of_no_sequence_are_cleared(monkeypatch, packed):
+    """One sequence of all tokens has none: its outputs and gradients are all written by the operators."""
+    cleared = []
+    zeros = torch.Tensor.new_zeros
+    monkeypatch.setattr(torch.Tensor, "new_zeros", lambda self, *shape, **more: cleared.append(shape) or zeros(self, *shape, **more))
+    monkeypatch.setattr(ops, "decay_attention_fwd", lambda q, k, v, log_decay, out, **more: out.fill_(1.0))
+    monkeypatch.setattr(ops, "decay_attention_bwd", lambda g, q, k, v, log_decay, *grads, **more: [x.fill_(1.0) for x in grads] and None)
+    q, k, v = (torch.zeros(6, heads, 4, requires_grad=True) for heads in (2, 1, 1))
+    out, _ = tokens.decay_attention(q, k, v, torch.zeros(1), cu_seqlens=torch.tensor([0, 5]) if packed else None)
+    out.sum().backward()
+    assert len(cleared) == (4 if packed else 0) and all(bool((x.grad == 1).all()) for x in (q, k, v))

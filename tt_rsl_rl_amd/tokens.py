@@ -114,7 +114,8 @@ class _DecayAttention(torch.autograd.Function):
         q, k, v, log_decay, cu_seqlens, initial_state = ctx.saved_tensors
         if d_out is None:
             d_out = q.new_zeros(*q.shape[:2], v.shape[2])
-        grads = q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)  # (tokens of no sequence stay 0)
+        # (tokens of no sequence stay 0; without cu_seqlens there are none)
+        grads = tuple((x.new_empty if cu_seqlens is None else x.new_zeros)(x.shape) for x in (q, k, v))
         d_initial = torch.empty_like(initial_state) if initial_state is not None and ctx.needs_input_grad[6] else None
         ops.decay_attention_bwd(_rows(d_out), q, k, v, log_decay, *grads, scale=ctx.scale, cu_seqlens=cu_seqlens, initial_state=initial_state,
                                 d_final_state=None if d_final is None else d_final.contiguous(), d_initial_state=d_initial)
